@@ -27,3 +27,13 @@ from .engine import (  # noqa: F401
     synth_tokens,
     synth_uniform,
 )
+
+_DEVICE_OPS = ("delta_prefill", "delta_step")
+
+
+def __getattr__(name: str):
+    """The operators on torch tensors, imported (with torch) at first use."""
+    if name in _DEVICE_OPS:
+        from . import device_ops
+        return getattr(device_ops, name)
+    raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

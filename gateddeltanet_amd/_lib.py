@@ -8,7 +8,7 @@ from __future__ import annotations
 
 import ctypes
 import os
-from ctypes import POINTER, c_char, c_float, c_int, c_int32, c_size_t, c_uint16, c_uint32, c_uint64, c_void_p
+from ctypes import POINTER, c_char, c_float, c_int, c_int32, c_int64, c_size_t, c_uint16, c_uint32, c_uint64, c_void_p
 
 LIB_PATH = os.path.join(os.path.dirname(os.path.abspath(__file__)), "libgdn_amd.so")
 
@@ -146,6 +146,22 @@ class GDNBatchState(ctypes.Structure):
     ]
 
 
+DTYPE_BF16, DTYPE_FP16, DTYPE_FP32 = 0, 1, 2  # GDN_DTYPE_*
+
+
+class GDNDelta(ctypes.Structure):
+    """Arguments of gdn_delta_prefill and gdn_delta_step (device pointers)."""
+    _fields_ = [
+        ("dtype", c_int32), ("n_tokens", c_uint32), ("n_seqs", c_uint32),
+        ("n_qk_heads", c_uint32), ("n_v_heads", c_uint32), ("key_dim", c_uint32), ("value_dim", c_uint32),
+        ("l2norm", c_int32), ("scale", c_float), ("n_slots", c_uint32),
+        ("q_stride", c_int64), ("k_stride", c_int64), ("v_stride", c_int64), ("o_stride", c_int64),
+        ("g_stride", c_int64),
+        ("q", c_void_p), ("k", c_void_p), ("v", c_void_p), ("o", c_void_p), ("g", c_void_p), ("beta", c_void_p),
+        ("cu_seqlens", c_void_p), ("slots", c_void_p), ("state_in", c_void_p), ("state_out", c_void_p),
+    ]
+
+
 FP = POINTER(c_float)
 IP = POINTER(c_int32)
 LP = POINTER(GDNLogitsParity)
@@ -153,6 +169,9 @@ BP = POINTER(GDNBatchState)
 
 # name -> (restype, argtypes).  Every symbol include/gdn_amd.h declares.
 SIGNATURES = {
+    "gdn_delta_prefill_workspace": (c_size_t, [POINTER(GDNDelta)]),
+    "gdn_delta_prefill": (c_int, [POINTER(GDNDelta), c_void_p, c_size_t, c_void_p]),
+    "gdn_delta_step": (c_int, [POINTER(GDNDelta), c_void_p]),
     "gdn_model_load": (c_int, [POINTER(GDNModel), ctypes.c_char_p]),
     "gdn_model_load_fp32": (c_int, [POINTER(GDNModel), ctypes.c_char_p]),
     "gdn_model_free": (None, [POINTER(GDNModel)]),

@@ -50,6 +50,7 @@
 #include "gdn_device.h"
 #include "gdn_internal.h"
 #include "gdn_scan.h"
+#include "gdn_wy.h"
 
 namespace gdn {
 namespace bt {
@@ -65,8 +66,6 @@ constexpr int kKtH = kH / 32;           // k tiles of a K = 2048 projection
 constexpr int kKtI = kI / 32;           // k tiles of the down projection
 constexpr size_t kLayerState = (size_t)kNH * kHD * kHD;  // floats per (layer, stream)
 constexpr size_t kStreamTails = (size_t)3 * 3 * kH;      // floats per (layer, stream)
-
-typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
 
 enum { EPI_RAW = 0, EPI_QKVG = 2, EPI_LM = 4 };
 
@@ -1149,56 +1148,12 @@ __global__ __launch_bounds__(kT) void k_pscan(const float *__restrict__ qkv, con
 // S_m^T q / 16).  The sums are associated differently from the step's
 // sequential chains, so this mode matches the scan within a tolerance, not
 // bit for bit; o is rounded to BF16 as the step rounds it.
-
 //
 // q and k are BF16 values before their normalisation, so every product with
-// them runs on the BF16 matrix cores without loss: k_m . k_s and q_m . k_s
-// as they are, with the two inverse norms as factors of the sum, and
-// products with an FP32 operand (the state, the deltas) after that operand
-// is split into three BF16 terms whose sum it is (8 + 8 + 8 significand
-// bits).  v_mfma_f32_16x16x32_bf16 forms exact products and FP32 sums at
-// 16 times the rate of v_mfma_f32_16x16x4_f32, so three (or, between two
-// split operands, six) of them still take a fifth (three eighths) of its
-// time.
-
-__device__ __forceinline__ f32x4 mfma_bf16(u32x4 a, u32x4 b, f32x4 c) {
-    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c,
-                                                   0, 0, 0);
-}
-
-// x as three BF16 terms: p[0] + p[1] + p[2] = x (each rounded to nearest, the
-// differences exact), four values packed in two words.  The first term is
-// held to the largest finite BF16 value, so every finite x of 2^-110 and more
-// is its terms' sum (rounded up to an infinity, that term would leave
-// infinity - infinity behind); below, the last terms are BF16 subnormals.  An
-// infinite or NaN x has a NaN term.
-__device__ __forceinline__ void split3(const f32x4 x, u32x2 (&p)[3]) {
-    constexpr float kMax = 0x1.fep127f;
-    auto held = [](float v) { return __builtin_amdgcn_fmed3f(v, -kMax, kMax); };
-    f32x4 r = x;
-#pragma unroll
-    for (int i = 0; i < 3; ++i) {
-        p[i].x = i == 0 ? cvt_pk(held(r.x), held(r.y)) : cvt_pk(r.x, r.y);
-        p[i].y = i == 0 ? cvt_pk(held(r.z), held(r.w)) : cvt_pk(r.z, r.w);
-        if (i < 2) {
-            r.x = r.x - u2f(p[i].x << 16);
-            r.y = r.y - u2f(p[i].x & 0xffff0000u);
-            r.z = r.z - u2f(p[i].y << 16);
-            r.w = r.w - u2f(p[i].y & 0xffff0000u);
-        }
-    }
-}
-
-// The product of two split operands over one 32-wide k step, smallest terms
-// first (the three terms below 2^-24 of the product are left out).
-__device__ __forceinline__ f32x4 mfma_split(const u32x4 (&a)[3], const u32x4 (&b)[3], f32x4 c) {
-    c = mfma_bf16(a[2], b[0], c);
-    c = mfma_bf16(a[0], b[2], c);
-    c = mfma_bf16(a[1], b[1], c);
-    c = mfma_bf16(a[1], b[0], c);
-    c = mfma_bf16(a[0], b[1], c);
-    return mfma_bf16(a[0], b[0], c);
-}
+// them runs on the BF16 matrix cores without loss (gdn_wy.h): k_m . k_s and
+// q_m . k_s as they are, with the two inverse norms as factors of the sum, and
+// products with an FP32 operand (the state, the deltas) after that operand is
+// split into three BF16 terms.
 
 // One (chunk, head)'s operands of k_wy_seq, written by k_wy_prep: MFMA A
 // fragments (64 lanes x 8 BF16 values, 1 KB), grouped by the wave that reads

@@ -584,6 +584,77 @@ int gdn_test_batch_gemm(const float *W, const float *X, uint32_t N, uint32_t K, 
 int gdn_test_prefill_gemm(int kind, const float *W, const float *X, uint32_t N, uint32_t T, float *Y,
                           float *Y_step);
 
+/* ===== operators on the caller's device buffers =====
+ * No counterparts in the reference, whose recurrence and argmax live inside
+ * its decode step.  For a serving program that keeps its own batch: every
+ * pointer in the structs below is device memory, work is enqueued on `stream`
+ * (a hipStream_t of the current device; NULL = the null stream) and not waited
+ * for, nothing is allocated, and the host reads no device value, so every call
+ * can be captured into a graph.  What the host can see is checked (-1 and one
+ * line on stderr, nothing enqueued); indices that only the device sees
+ * (sequence ends, slots, token ids, lengths) are held to the buffers' sizes by
+ * the kernels.  Calls that may run at the same time need workspaces of their
+ * own.  Clear a struct before filling it. */
+
+/* Types of the activations and logits. */
+#define GDN_DTYPE_BF16 0
+#define GDN_DTYPE_FP16 1
+#define GDN_DTYPE_FP32 2
+
+/* The gated delta rule over a batch.  Per value head, with the FP32 state S
+ * [key_dim][value_dim] of its sequence and the query/key head
+ * (value head) / (n_v_heads / n_qk_heads), for each of the sequence's tokens:
+ *   S = exp(g) S;  d = beta (v - S^T k);  S = S + k d^T;  o = scale S^T q
+ * where l2norm != 0 puts q / sqrt(|q|^2 + 1e-6) and k / sqrt(|k|^2 + 1e-6) in
+ * the places of q and k.
+ *   n_tokens   rows of q, k, v, g, beta and o
+ *   n_seqs     sequences.  gdn_delta_prefill: sequence i is the rows
+ *              cu_seqlens[i] .. cu_seqlens[i + 1] - 1 (n_seqs + 1 values from
+ *              0 up; an empty one keeps its state); rows of no sequence are
+ *              not read and their o is left as it was.  gdn_delta_step:
+ *              n_tokens = n_seqs, row i is sequence i's token, cu_seqlens is
+ *              not read.
+ *   *_dim      64, 128 or 256, heads contiguous in a row
+ *   *_stride   elements between rows (g and beta: one stride).  q, k, v and o
+ *              rows start at multiples of 16 bytes
+ *   g, beta    FP32; g is the log of the decay (<= 0 in a stable model;
+ *              -inf clears the state)
+ *   state_in, state_out   [n_slots][n_v_heads][key_dim][value_dim] FP32, at
+ *              multiples of 16 bytes; the same buffer, or two that do not
+ *              overlap.  state_in NULL: every sequence starts from zero;
+ *              state_out NULL: the states are not kept.
+ *   slots      [n_seqs] the sequences' slots (NULL: slot i).  A sequence with
+ *              a slot outside 0 .. n_slots - 1 is left out (a padded row):
+ *              its o is left as it was.  No slot may occur twice.
+ * A value that is not finite reaches its own sequence and head only, there
+ * also the tokens up to 63 before it. */
+typedef struct {
+    int32_t dtype;              /* GDN_DTYPE_* of q, k, v and o */
+    uint32_t n_tokens, n_seqs;
+    uint32_t n_qk_heads, n_v_heads;
+    uint32_t key_dim, value_dim;
+    int32_t l2norm;
+    float scale;
+    uint32_t n_slots;
+    int64_t q_stride, k_stride, v_stride, o_stride, g_stride;
+    const void *q, *k, *v;
+    void *o;
+    const float *g, *beta;
+    const int32_t *cu_seqlens;
+    const int32_t *slots;
+    const float *state_in;
+    float *state_out;
+} GDNDelta;
+
+/* Packed sequences in the chunk-parallel form (as GDN_PREFILL_CHUNKED, products
+ * exact to FP32 rounding).  `workspace`: gdn_delta_prefill_workspace(args)
+ * bytes of device memory at a multiple of 16 bytes, needed until the work is
+ * done. */
+size_t gdn_delta_prefill_workspace(const GDNDelta *args);
+int gdn_delta_prefill(const GDNDelta *args, void *workspace, size_t workspace_bytes, void *stream);
+/* One token of every sequence. */
+int gdn_delta_step(const GDNDelta *args, void *stream);
+
 #ifdef __cplusplus
 }
 #endif
