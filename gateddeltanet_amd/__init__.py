@@ -28,7 +28,7 @@ from .engine import (  # noqa: F401
     synth_uniform,
 )
 
-_DEVICE_OPS = ("delta_prefill", "delta_step")
+_DEVICE_OPS = ("delta_prefill", "delta_step", "logits_process", "sample_tokens")
 
 
 def __getattr__(name: str):

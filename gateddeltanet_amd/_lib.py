@@ -162,6 +162,37 @@ class GDNDelta(ctypes.Structure):
     ]
 
 
+class GDNLogits(ctypes.Structure):
+    """Arguments of gdn_logits_process (device pointers)."""
+    _fields_ = [
+        ("dtype", c_int32), ("rows", c_uint32), ("vocab", c_uint32),
+        ("history_width", c_uint32), ("n_bias", c_uint32), ("n_masks", c_uint32),
+        ("logits_stride", c_int64), ("out_stride", c_int64), ("history_stride", c_int64), ("mask_stride", c_int64),
+        ("logits", c_void_p), ("out", c_void_p),
+        ("history", c_void_p), ("history_len", c_void_p), ("prompt_len", c_void_p),
+        ("repetition", c_void_p), ("presence", c_void_p), ("frequency", c_void_p),
+        ("bias_offsets", c_void_p), ("bias_ids", c_void_p), ("bias_values", c_void_p),
+        ("mask", c_void_p), ("mask_index", c_void_p),
+    ]
+
+
+class GDNSample(ctypes.Structure):
+    """Arguments of gdn_sample_tokens (device pointers)."""
+    _fields_ = [
+        ("dtype", c_int32), ("rows", c_uint32), ("vocab", c_uint32), ("reserved", c_uint32),
+        ("logits_stride", c_int64),
+        ("logits", c_void_p), ("uniform", c_void_p), ("temperature", c_void_p), ("top_k", c_void_p),
+        ("top_p", c_void_p), ("min_p", c_void_p), ("tokens", c_void_p), ("logprobs", c_void_p),
+    ]
+
+
+class GDNBatchSampling(ctypes.Structure):
+    """Host arrays of gdn_batch_sample, a row a stream."""
+    _fields_ = [(name, c_void_p) for name in (
+        "uniform", "temperature", "top_k", "top_p", "min_p", "repetition", "presence", "frequency", "history",
+        "history_offsets", "prompt_len", "bias_ids", "bias_offsets", "bias_values", "mask")]
+
+
 FP = POINTER(c_float)
 IP = POINTER(c_int32)
 LP = POINTER(GDNLogitsParity)
@@ -169,9 +200,12 @@ BP = POINTER(GDNBatchState)
 
 # name -> (restype, argtypes).  Every symbol include/gdn_amd.h declares.
 SIGNATURES = {
+    "gdn_batch_sample": (c_int, [POINTER(GDNBatchState), POINTER(GDNBatchSampling), IP, FP]),
     "gdn_delta_prefill_workspace": (c_size_t, [POINTER(GDNDelta)]),
     "gdn_delta_prefill": (c_int, [POINTER(GDNDelta), c_void_p, c_size_t, c_void_p]),
     "gdn_delta_step": (c_int, [POINTER(GDNDelta), c_void_p]),
+    "gdn_logits_process": (c_int, [POINTER(GDNLogits), c_void_p]),
+    "gdn_sample_tokens": (c_int, [POINTER(GDNSample), c_void_p]),
     "gdn_model_load": (c_int, [POINTER(GDNModel), ctypes.c_char_p]),
     "gdn_model_load_fp32": (c_int, [POINTER(GDNModel), ctypes.c_char_p]),
     "gdn_model_free": (None, [POINTER(GDNModel)]),

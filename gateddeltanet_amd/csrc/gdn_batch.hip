@@ -43,6 +43,7 @@
 #include <cmath>
 #include <cstdio>
 #include <cstring>
+#include <exception>
 #include <type_traits>
 #include <vector>
 
@@ -2140,6 +2141,10 @@ struct GDNBatchEngine {
     // their own, so a prefill leaves the other streams' last step readable)
     float *p_logits = nullptr;
     int *p_tok = nullptr;
+    // gdn_batch_sample: the processed logits, and the call's host arrays
+    float *c_logits = nullptr;
+    unsigned char *c_args = nullptr;
+    size_t c_args_cap = 0;
     int prefill_mode = GDN_PREFILL_SCAN;
     // prefill segment buffers, allocated at the first prefill for seg_cap
     // tokens (per token: residual ping-pong, projection sums, q/k/v,
@@ -2822,6 +2827,8 @@ void b_destroy(GDNBatchEngine *e) {
     (void)hipFree(e->x_d);
     (void)hipFree(e->p_logits);
     (void)hipFree(e->p_tok);
+    (void)hipFree(e->c_logits);
+    (void)hipFree(e->c_args);
     (void)hipFree(e->seg_mem);
     if (e->tok_host) (void)hipHostFree(e->tok_host);
     delete e;
@@ -2870,6 +2877,122 @@ int tails_copy(uint16_t *dev, int streams, int layers, uint32_t stream, float *h
             std::memcpy(host + i, &u, 4);
         }
     }
+    return 0;
+}
+
+// One device block of a call's host arrays, each at a multiple of 16 bytes.
+struct HostBlock {
+    std::vector<unsigned char> bytes;
+    template <class T>
+    size_t add(const T *src, size_t n) {
+        const size_t at = (bytes.size() + 15) / 16 * 16;
+        bytes.resize(at + n * sizeof(T));
+        if (n) std::memcpy(bytes.data() + at, src, n * sizeof(T));
+        return at;
+    }
+};
+
+// Whether the n + 1 offsets rise from zero or more.
+bool offsets_ok(const int32_t *offsets, int n) {
+    if (offsets[0] < 0) return false;
+    for (int i = 0; i < n; ++i)
+        if (offsets[i + 1] < offsets[i]) return false;
+    return true;
+}
+
+int b_sample(GDNBatchEngine *e, const GDNBatchSampling &h, int32_t *tokens, float *logprobs) {
+    const int n = e->streams;
+    if ((h.history_offsets && !offsets_ok(h.history_offsets, n)) || (h.bias_offsets && !offsets_ok(h.bias_offsets, n))) {
+        gdn_error("gdn_batch_sample: offsets must rise from zero");
+        return -1;
+    }
+    const int32_t n_hist = h.history_offsets ? h.history_offsets[n] : 0, n_bias = h.bias_offsets ? h.bias_offsets[n] : 0;
+    if ((n_hist && !h.history) || (n_bias && (!h.bias_ids || !h.bias_values)) || (h.temperature && !h.uniform)) {
+        gdn_error("gdn_batch_sample: an array is missing");
+        return -1;
+    }
+    if (!h.history_offsets && (h.repetition || h.presence || h.frequency || h.prompt_len)) {
+        gdn_error("gdn_batch_sample: penalties need a history");
+        return -1;
+    }
+    // rows of the histories, one width
+    int32_t width = 0;
+    for (int i = 0; i < n && h.history_offsets; ++i)
+        width = std::max(width, h.history_offsets[i + 1] - h.history_offsets[i]);
+    std::vector<int32_t> rows((size_t)n * width), lens(n);
+    for (int i = 0; i < n && h.history_offsets; ++i) {
+        lens[i] = h.history_offsets[i + 1] - h.history_offsets[i];
+        if (lens[i]) std::memcpy(&rows[(size_t)i * width], h.history + h.history_offsets[i], lens[i] * sizeof(int32_t));
+    }
+    const int words = (e->vocab + 31) / 32;
+    HostBlock blk;
+    auto add = [&](const auto *src, size_t count) { return src ? blk.add(src, count) : (size_t)-1; };
+    const size_t hist = add(h.history_offsets ? rows.data() : (const int32_t *)nullptr, rows.size()),
+                 len = add(h.history_offsets ? lens.data() : (const int32_t *)nullptr, n), pl = add(h.prompt_len, n),
+                 rep = add(h.repetition, n), pres = add(h.presence, n), freq = add(h.frequency, n),
+                 boff = add(n_bias ? h.bias_offsets : nullptr, n + 1), bid = add(n_bias ? h.bias_ids : nullptr, n_bias),
+                 bval = add(n_bias ? h.bias_values : nullptr, n_bias), mask = add(h.mask, (size_t)n * words),
+                 uni = add(h.uniform, n), temp = add(h.temperature, n), tk = add(h.top_k, n), tp = add(h.top_p, n),
+                 mp = add(h.min_p, n), out = (blk.bytes.size() + 15) / 16 * 16, need = out + (size_t)n * 8;
+    if (need > e->c_args_cap) {
+        (void)hipFree(e->c_args);
+        e->c_args = nullptr;
+        e->c_args_cap = 0;
+        GDN_HIP(hipMalloc(&e->c_args, need));
+        e->c_args_cap = need;
+    }
+    if (!e->c_logits) GDN_HIP(hipMalloc(&e->c_logits, (size_t)n * e->vocab * 4));
+    // the copy's source outlives it on every way out
+    struct Wait {
+        hipStream_t s;
+        ~Wait() { (void)hipStreamSynchronize(s); }
+    } wait{e->stream};
+    if (!blk.bytes.empty())
+        GDN_HIP(hipMemcpyAsync(e->c_args, blk.bytes.data(), blk.bytes.size(), hipMemcpyHostToDevice, e->stream));
+    auto at = [&](size_t o) -> const void * { return o == (size_t)-1 ? nullptr : e->c_args + o; };
+    const bool any = h.history_offsets || n_bias || h.mask;
+    if (any) {
+        GDNLogits a = {};
+        a.dtype = GDN_DTYPE_FP32;
+        a.rows = n;
+        a.vocab = e->vocab;
+        a.history_width = width;
+        a.n_bias = n_bias;
+        a.n_masks = n;
+        a.logits_stride = a.out_stride = e->vocab;
+        a.history_stride = width;
+        a.mask_stride = words;
+        a.logits = e->logits;
+        a.out = e->c_logits;
+        a.history = static_cast<const int32_t *>(at(hist));
+        a.history_len = static_cast<const int32_t *>(at(len));
+        a.prompt_len = static_cast<const int32_t *>(at(pl));
+        a.repetition = static_cast<const float *>(at(rep));
+        a.presence = static_cast<const float *>(at(pres));
+        a.frequency = static_cast<const float *>(at(freq));
+        a.bias_offsets = static_cast<const int32_t *>(at(boff));
+        a.bias_ids = static_cast<const int32_t *>(at(bid));
+        a.bias_values = static_cast<const float *>(at(bval));
+        a.mask = static_cast<const uint32_t *>(at(mask));
+        if (gdn_logits_process(&a, e->stream) != 0) return -1;
+    }
+    GDNSample s = {};
+    s.dtype = GDN_DTYPE_FP32;
+    s.rows = n;
+    s.vocab = e->vocab;
+    s.logits_stride = e->vocab;
+    s.logits = any ? e->c_logits : e->logits;
+    s.uniform = static_cast<const float *>(at(uni));
+    s.temperature = static_cast<const float *>(at(temp));
+    s.top_k = static_cast<const int32_t *>(at(tk));
+    s.top_p = static_cast<const float *>(at(tp));
+    s.min_p = static_cast<const float *>(at(mp));
+    s.tokens = reinterpret_cast<int32_t *>(e->c_args + out);
+    s.logprobs = reinterpret_cast<float *>(e->c_args + out + (size_t)n * 4);
+    if (gdn_sample_tokens(&s, e->stream) != 0) return -1;
+    GDN_HIP(hipMemcpyAsync(tokens, s.tokens, (size_t)n * 4, hipMemcpyDeviceToHost, e->stream));
+    if (logprobs) GDN_HIP(hipMemcpyAsync(logprobs, s.logprobs, (size_t)n * 4, hipMemcpyDeviceToHost, e->stream));
+    GDN_HIP(hipStreamSynchronize(e->stream));
     return 0;
 }
 
@@ -2924,6 +3047,22 @@ int gdn_batch_decode_step(GDNBatchState *state, const int32_t *tokens, int32_t *
         return -1;
     }
     return b_run_step(e, tokens, next_tokens, nullptr);
+}
+
+int gdn_batch_sample(GDNBatchState *state, const GDNBatchSampling *settings, int32_t *tokens, float *logprobs) {
+    GDNBatchEngine *e = engine_of(state);
+    if (!e) return -1;
+    if (tokens == nullptr) {
+        gdn_error("gdn_batch_sample: tokens is required");
+        return -1;
+    }
+    try {
+        const GDNBatchSampling none = {};
+        return b_sample(e, settings ? *settings : none, tokens, logprobs);
+    } catch (const std::exception &) {  // no host memory for the call's arrays
+        gdn_error("gdn_batch_sample: out of host memory");
+        return -1;
+    }
 }
 
 int gdn_batch_read_tokens(const GDNBatchState *state, int32_t *tokens) {

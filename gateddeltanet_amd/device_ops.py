@@ -1,6 +1,6 @@
 """The operators on the caller's device tensors (include/gdn_amd.h, "operators
 on the caller's device buffers"): the gated delta rule over a batch of
-sequences.
+sequences, and the way from a batch's logits to its tokens.
 
 Arguments are torch tensors on one GPU; work goes to that GPU's current stream
 and is not waited for, and every call can be captured into a graph.  Where a
@@ -10,7 +10,7 @@ that stream.  Errors raise ``GDNError``, before anything is enqueued.
 from __future__ import annotations
 
 import ctypes
-from typing import Optional
+from typing import Optional, Tuple
 
 import torch
 
@@ -125,3 +125,100 @@ def delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tenso
                   l2norm)
     _launch(q.device, "gdn_delta_step", L.load().gdn_delta_step, ctypes.byref(args))
     return out
+
+
+def _logits(x: torch.Tensor, name: str = "logits") -> int:
+    dtype = _DTYPES.get(x.dtype)
+    if dtype is None or not x.is_cuda or x.dim() != 2 or (x.shape[1] > 1 and x.stride(1) != 1):
+        _fail(f"{name}: expected a bfloat16, float16 or float32 [rows][vocabulary] on a GPU with contiguous rows, got "
+              f"{x.dtype} {tuple(x.shape)} on {x.device}")
+    return dtype
+
+
+def _matrix(device, name: str, x, dtype, rows: int) -> int:
+    if x.device != device or x.dtype != dtype or x.dim() != 2 or (rows >= 0 and x.shape[0] != rows) or (
+            x.shape[1] > 1 and x.stride(1) != 1):
+        _fail(f"{name}: expected {dtype} [{rows if rows >= 0 else 'n'}][n] on {device} with contiguous rows, got "
+              f"{x.dtype} {tuple(x.shape)} on {x.device}")
+    return x.data_ptr()
+
+
+def logits_process(logits: torch.Tensor, *, history: Optional[torch.Tensor] = None,
+                   history_len: Optional[torch.Tensor] = None, prompt_len: Optional[torch.Tensor] = None,
+                   repetition: Optional[torch.Tensor] = None, presence: Optional[torch.Tensor] = None,
+                   frequency: Optional[torch.Tensor] = None,
+                   bias: Optional[Tuple[torch.Tensor, torch.Tensor, torch.Tensor]] = None,
+                   mask: Optional[torch.Tensor] = None, mask_index: Optional[torch.Tensor] = None,
+                   out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """gdn_logits_process: penalties for repeated tokens, biases and masks.
+
+    logits [rows][vocab]; history int32 [rows][width] with history_len and
+    prompt_len int32 [rows]; repetition, presence, frequency FP32 [rows]; bias
+    (offsets int32 [rows + 1], ids int32, values FP32); mask int32 words
+    [masks][>= vocab / 32] with a set bit for every allowed token, mask_index
+    int32 [rows].  out may be logits itself.  Returns out.
+    """
+    dtype, device, rows = _logits(logits), logits.device, logits.shape[0]
+    if out is None:
+        out = torch.empty(logits.shape, dtype=logits.dtype, device=device)
+    elif _logits(out, "out") != dtype or out.shape != logits.shape or out.device != device:
+        _fail(f"out: expected {logits.dtype} {tuple(logits.shape)} on {device}, got {out.dtype} {tuple(out.shape)}")
+    a = L.GDNLogits(dtype, rows, logits.shape[1], 0, 0, 0, logits.stride(0), out.stride(0), 0, 0, logits.data_ptr(),
+                    out.data_ptr())
+    if history is not None:
+        if history_len is None:
+            _fail("history needs history_len")
+        a.history = _matrix(device, "history", history, torch.int32, rows)
+        a.history_width, a.history_stride = history.shape[1], history.stride(0)
+        a.history_len = _on(device, "history_len", history_len, torch.int32, (rows,))
+        a.prompt_len = _on(device, "prompt_len", prompt_len, torch.int32, (rows,))
+        a.repetition = _on(device, "repetition", repetition, torch.float32, (rows,))
+        a.presence = _on(device, "presence", presence, torch.float32, (rows,))
+        a.frequency = _on(device, "frequency", frequency, torch.float32, (rows,))
+    elif not (history_len is prompt_len is repetition is presence is frequency is None):
+        _fail("penalties need a history")
+    if bias is not None:
+        offsets, ids, values = bias
+        a.bias_offsets = _on(device, "bias offsets", offsets, torch.int32, (rows + 1,))
+        a.bias_ids = _on(device, "bias ids", ids, torch.int32, (-1,))
+        a.bias_values = _on(device, "bias values", values, torch.float32, (ids.shape[0],))
+        a.n_bias = ids.shape[0]
+    if mask is not None:
+        a.mask = _matrix(device, "mask", mask, torch.int32, -1)
+        a.n_masks, a.mask_stride = mask.shape[0], mask.stride(0) if mask.shape[0] > 1 else mask.shape[1]
+        if mask.shape[1] * 32 < logits.shape[1]:
+            _fail(f"mask: {mask.shape[1]} words are fewer than {logits.shape[1]} tokens")
+        a.mask_index = _on(device, "mask_index", mask_index, torch.int32, (rows,))
+    elif mask_index is not None:
+        _fail("mask_index needs a mask")
+    _launch(device, "gdn_logits_process", L.load().gdn_logits_process, ctypes.byref(a))
+    return out
+
+
+def sample_tokens(logits: torch.Tensor, uniform: Optional[torch.Tensor] = None, *,
+                  temperature: Optional[torch.Tensor] = None, top_k: Optional[torch.Tensor] = None,
+                  top_p: Optional[torch.Tensor] = None, min_p: Optional[torch.Tensor] = None,
+                  tokens: Optional[torch.Tensor] = None,
+                  logprobs: Optional[torch.Tensor] = None) -> Tuple[torch.Tensor, torch.Tensor]:
+    """gdn_sample_tokens: a token of every row and its log-probability.
+
+    logits [rows][vocab]; uniform (in [0, 1)), temperature, top_p and min_p
+    FP32 [rows], top_k int32 [rows].  Without a temperature, or where it is not
+    positive: the first of the highest logits.  Returns (tokens int32 [rows],
+    logprobs FP32 [rows]); -1 where no logit is above -infinity.
+    """
+    dtype, device, rows = _logits(logits), logits.device, logits.shape[0]
+    if tokens is None:
+        tokens = torch.empty(rows, dtype=torch.int32, device=device)
+    if logprobs is None:
+        logprobs = torch.empty(rows, dtype=torch.float32, device=device)
+    a = L.GDNSample(dtype, rows, logits.shape[1], 0, logits.stride(0), logits.data_ptr(),
+                    _on(device, "uniform", uniform, torch.float32, (rows,)),
+                    _on(device, "temperature", temperature, torch.float32, (rows,)),
+                    _on(device, "top_k", top_k, torch.int32, (rows,)),
+                    _on(device, "top_p", top_p, torch.float32, (rows,)),
+                    _on(device, "min_p", min_p, torch.float32, (rows,)),
+                    _on(device, "tokens", tokens, torch.int32, (rows,)),
+                    _on(device, "logprobs", logprobs, torch.float32, (rows,)))
+    _launch(device, "gdn_sample_tokens", L.load().gdn_sample_tokens, ctypes.byref(a))
+    return tokens, logprobs

@@ -341,6 +341,50 @@ class BatchState:
         _check(L.load().gdn_batch_decode_step(self.ptr, iptr(t), iptr(out)), "gdn_batch_decode_step")
         return out
 
+    def sample(self, uniform: Optional[Sequence[float]] = None, *, temperature=None, top_k=None, top_p=None,
+               min_p=None, repetition=None, presence=None, frequency=None,
+               histories: Optional[Sequence[Sequence[int]]] = None, prompt_len=None,
+               biases: Optional[Sequence[Dict[int, float]]] = None, mask: Optional[np.ndarray] = None):
+        """gdn_batch_sample: the streams' next tokens drawn from the last
+        step's logits, and their log-probabilities.  Settings are a value a
+        stream, or one for all; histories a token sequence a stream (prompt
+        first); biases a dict a stream; mask bool [n_streams][vocab], True
+        where a token is allowed."""
+        n, vocab = self.n_streams, self.model.config.vocab_size
+        keep, a = [], L.GDNBatchSampling()
+
+        def put(name, value, dtype, shape=(n,)):
+            if value is not None:
+                keep.append(np.ascontiguousarray(np.broadcast_to(np.asarray(value, dtype), shape)))
+                setattr(a, name, keep[-1].ctypes.data)
+
+        def ragged(lists):
+            if len(lists) != n:
+                raise GDNError(f"expected one entry for each of {n} streams, got {len(lists)}")
+            return np.cumsum([0] + [len(x) for x in lists])
+
+        for name, value in (("uniform", uniform), ("temperature", temperature), ("top_p", top_p), ("min_p", min_p),
+                            ("repetition", repetition), ("presence", presence), ("frequency", frequency)):
+            put(name, value, np.float32)
+        put("top_k", top_k, np.int32)
+        put("prompt_len", prompt_len, np.int32)
+        if histories is not None:
+            at = ragged(histories)
+            put("history_offsets", at, np.int32, (n + 1,))
+            put("history", np.concatenate([np.asarray(x, np.int32) for x in histories]), np.int32, (at[-1],))
+        if biases is not None:
+            at = ragged(biases)
+            put("bias_offsets", at, np.int32, (n + 1,))
+            put("bias_ids", [t for b in biases for t in b], np.int32, (at[-1],))
+            put("bias_values", [v for b in biases for v in b.values()], np.float32, (at[-1],))
+        if mask is not None:
+            bits = np.zeros((n, (vocab + 31) // 32 * 32), bool)
+            bits[:, :vocab] = np.broadcast_to(np.asarray(mask, bool), (n, vocab))
+            put("mask", np.packbits(bits, axis=1, bitorder="little").view(np.uint32), np.uint32, (n, bits.shape[1] // 32))
+        tokens, logprobs = np.empty(n, np.int32), np.empty(n, np.float32)
+        _check(L.load().gdn_batch_sample(self.ptr, ctypes.byref(a), iptr(tokens), fptr(logprobs)), "gdn_batch_sample")
+        return tokens, logprobs
+
     def prefill(self, stream: int, prompt: Sequence[int]) -> int:
         """gdn_batch_prefill: the prompt through one stream's state; returns
         the argmax of the last position (the .gdnstate seed token)."""

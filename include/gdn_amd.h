@@ -512,6 +512,29 @@ void gdn_batch_free(GDNBatchState *state);
 /* One step of every stream: tokens[n_streams] in; the greedy next tokens
  * out (next_tokens may be NULL).  -1 for a token outside [0, vocab). */
 int gdn_batch_decode_step(GDNBatchState *state, const int32_t *tokens, int32_t *next_tokens);
+/* Draws the streams' next tokens from the last step's (or, for a stream that
+ * was prefilled since, its prompt's) logits, which stay as they are: the
+ * processing of gdn_logits_process and the draw of gdn_sample_tokens, with every
+ * array on the HOST and a row a stream.
+ *   history    stream s's token ids are history[history_offsets[s] ..
+ *              history_offsets[s + 1] - 1], the first prompt_len[s] of them the
+ *              prompt's; history_offsets NULL: none, and no penalties
+ *   mask       [n_streams][(vocab + 31) / 32] words; NULL: none
+ * tokens[n_streams] and logprobs[n_streams] (may be NULL) out; the
+ * log-probability is over the processed logits.  Any other array may be NULL
+ * as there, and settings itself: the argmax.  -1 for offsets that fall or
+ * start below zero.  The first call allocates a second set of logits. */
+typedef struct {
+    const float *uniform, *temperature;
+    const int32_t *top_k;
+    const float *top_p, *min_p;
+    const float *repetition, *presence, *frequency;
+    const int32_t *history, *history_offsets, *prompt_len;
+    const int32_t *bias_ids, *bias_offsets;
+    const float *bias_values;
+    const uint32_t *mask;
+} GDNBatchSampling;
+int gdn_batch_sample(GDNBatchState *state, const GDNBatchSampling *settings, int32_t *tokens, float *logprobs);
 int gdn_batch_read_tokens(const GDNBatchState *state, int32_t *tokens);
 int gdn_batch_read_logits(const GDNBatchState *state, uint32_t stream, float *logits, size_t count);
 int gdn_batch_read_final_hidden(const GDNBatchState *state, uint32_t stream, float *hidden, size_t count);
@@ -654,6 +677,73 @@ size_t gdn_delta_prefill_workspace(const GDNDelta *args);
 int gdn_delta_prefill(const GDNDelta *args, void *workspace, size_t workspace_bytes, void *stream);
 /* One token of every sequence. */
 int gdn_delta_step(const GDNDelta *args, void *stream);
+
+/* Penalties, biases and masks on a batch of logits, each row on its own.  For
+ * token t of row r, in FP32, rounded once to dtype:
+ *   x = logits[r][t]
+ *   t in history[r]:         x = x > 0 ? x / repetition[r] : x * repetition[r]
+ *   t in it after the prompt, n times:  x = x - frequency[r] n - presence[r]
+ *   t among row r's biases:  x = x + the value (of its last entry there)
+ *   t's mask bit clear:      x = -infinity, whatever it was
+ *   out         may be logits (of equal strides); rows that overlap otherwise
+ *               are not allowed
+ *   history     [rows][history_stride] token ids, the first
+ *               history_len[r] of a row; those before prompt_len[r] are the
+ *               prompt's (prompt_len NULL: none are).  Lengths are held to
+ *               0 .. history_width; ids outside the vocabulary are skipped.
+ *               history NULL: no penalties
+ *   repetition, presence, frequency   [rows], NULL: 1, 0, 0
+ *   bias_*      row r's entries are bias_offsets[r] .. bias_offsets[r + 1] - 1
+ *               of the n_bias ids and values; bias_offsets NULL: none
+ *   mask        [n_masks][mask_stride] words, bit t % 32 of word t / 32 set for
+ *               an allowed token; row r uses mask mask_index[r] (NULL: r; an
+ *               index outside 0 .. n_masks - 1: none).  mask NULL: none
+ * vocab is at most 2^24. */
+typedef struct {
+    int32_t dtype;              /* GDN_DTYPE_* of logits and out */
+    uint32_t rows, vocab;
+    uint32_t history_width, n_bias, n_masks;
+    int64_t logits_stride, out_stride, history_stride, mask_stride;
+    const void *logits;
+    void *out;
+    const int32_t *history, *history_len, *prompt_len;
+    const float *repetition, *presence, *frequency;
+    const int32_t *bias_offsets, *bias_ids;
+    const float *bias_values;
+    const uint32_t *mask;
+    const int32_t *mask_index;
+} GDNLogits;
+int gdn_logits_process(const GDNLogits *args, void *stream);
+
+/* A token from each row of logits.  With the tokens ranked by logit, equal ones
+ * by index, and weights w = exp((x - max) / temperature[r]):
+ *   top_k[r] > 0      keeps the first top_k[r]
+ *   top_p[r] < 1      of those, keeps the ones that less than top_p[r] of their
+ *                     weight ranks before (the first in any case)
+ *   min_p[r] > 0      of those, keeps the ones of weight >= min_p[r] (the
+ *                     first in any case)
+ * and the token is the first, by index, up to which the kept weights add up to
+ * more than uniform[r] (in [0, 1)) of their sum.  temperature[r] <= 0, or
+ * temperature NULL: the first of the highest logits.  Any other array
+ * may be NULL: off (uniform NULL is refused with a temperature).
+ * logprobs[r] (NULL: not wanted) is the token's log softmax over the row as it
+ * is, at temperature 1 with no token left out.
+ * NaN logits are never chosen and carry no weight; a row without a logit above
+ * -infinity gives token -1 and log-probability -infinity.  Weights are held in
+ * 64-bit fixed point, 45 bits behind the point (fewer from 2^18 tokens on), so
+ * their sums do not depend on an order.  vocab is at most 2^20. */
+typedef struct {
+    int32_t dtype;              /* GDN_DTYPE_* of logits */
+    uint32_t rows, vocab, reserved;
+    int64_t logits_stride;
+    const void *logits;
+    const float *uniform, *temperature;
+    const int32_t *top_k;
+    const float *top_p, *min_p;
+    int32_t *tokens;
+    float *logprobs;
+} GDNSample;
+int gdn_sample_tokens(const GDNSample *args, void *stream);
 
 #ifdef __cplusplus
 }

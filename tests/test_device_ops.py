@@ -1,0 +1,149 @@
+"""Refusals of the operators on device buffers (gdn_delta_*, gdn_logits_process,
+gdn_sample_tokens), without a GPU: what the host can see is refused before
+anything touches a device, so the addresses here are never read."""
+import ctypes
+
+import pytest
+import torch
+
+import gateddeltanet_amd as g
+from gateddeltanet_amd import _lib
+
+AT = 1 << 20  # an address, 16-byte aligned, never read
+
+
+def delta(**change):
+    a = _lib.GDNDelta(_lib.DTYPE_BF16, 10, 2, 4, 8, 128, 128, 1, 0.1, 4, 512, 512, 1024, 1024, 8,
+                      AT, AT, AT, AT, AT, AT, AT, AT, AT, AT)
+    if change.pop("step", False):
+        a.n_tokens = a.n_seqs
+    for k, v in change.items():
+        setattr(a, k, v)
+    return a
+
+
+BAD_DELTA = [dict(dtype=3), dict(dtype=-1), dict(key_dim=96), dict(value_dim=512), dict(value_dim=0),
+             dict(n_qk_heads=0), dict(n_v_heads=0), dict(n_qk_heads=3), dict(n_v_heads=65536, n_qk_heads=1),
+             dict(n_seqs=65536), dict(n_tokens=1 << 31), dict(n_slots=1 << 31), dict(q=0), dict(k=0), dict(v=0),
+             dict(o=0), dict(g=0), dict(beta=0), dict(q=AT + 2), dict(k=AT + 8), dict(v=AT + 4), dict(o=AT + 2),
+             dict(state_in=AT + 4), dict(state_out=AT + 8), dict(q_stride=516), dict(v_stride=1028),
+             dict(k_stride=504), dict(o_stride=1016), dict(g_stride=7)]
+
+
+@pytest.mark.parametrize("change", BAD_DELTA, ids=lambda c: "-".join(f"{k}={v}" for k, v in c.items()))
+def test_delta_refuses(change, capfd):
+    lib = _lib.load()
+    a = delta(**change)
+    assert lib.gdn_delta_prefill(ctypes.byref(a), AT, 1 << 40, None) == -1
+    assert "gdn_delta_prefill: " in capfd.readouterr().err
+    a = delta(step=True, **{k: v for k, v in change.items() if k not in ("n_seqs", "n_tokens")})
+    for k in ("n_seqs", "n_tokens"):
+        if k in change:
+            a.n_seqs = a.n_tokens = change[k]
+    assert lib.gdn_delta_step(ctypes.byref(a), None) == -1
+    assert "gdn_delta_step: " in capfd.readouterr().err
+
+
+def test_delta_refuses_null_and_workspace():
+    lib = _lib.load()
+    a = delta()
+    ref = ctypes.byref(a)
+    need = lib.gdn_delta_prefill_workspace(ref)
+    assert need > 0
+    assert lib.gdn_delta_prefill(None, AT, need, None) == -1
+    assert lib.gdn_delta_step(None, None) == -1
+    assert lib.gdn_delta_prefill(ref, None, need, None) == -1
+    assert lib.gdn_delta_prefill(ref, AT + 8, need, None) == -1
+    assert lib.gdn_delta_prefill(ref, AT, need - 1, None) == -1
+    assert lib.gdn_delta_prefill(ctypes.byref(delta(cu_seqlens=0)), AT, need, None) == -1
+    assert lib.gdn_delta_step(ref, None) == -1  # 10 tokens of two sequences
+    assert lib.gdn_delta_prefill_workspace(None) == 0
+
+
+def test_delta_nothing_to_do():
+    lib = _lib.load()
+    assert lib.gdn_delta_prefill(ctypes.byref(delta(n_seqs=0)), None, 0, None) == 0
+    assert lib.gdn_delta_step(ctypes.byref(delta(n_seqs=0, n_tokens=0)), None) == 0
+
+
+@pytest.mark.parametrize("dtype,chunk", [(_lib.DTYPE_BF16, 64), (_lib.DTYPE_FP16, 32), (_lib.DTYPE_FP32, 32)])
+def test_delta_places_hold_every_chunk(dtype, chunk):
+    """The chunks of a sequence have places first / C + number + chunk: none is
+    shared, all lie inside the workspace (the kernels' indexing, restated)."""
+    import random
+
+    rng = random.Random(3)
+    lib = _lib.load()
+    one = lib.gdn_delta_prefill_workspace(ctypes.byref(delta(dtype=dtype, n_tokens=0, n_seqs=1)))
+    for _ in range(200):
+        lens = [rng.choice([0, 1, chunk - 1, chunk, chunk + 1, rng.randint(0, 5 * chunk)]) for _ in range(rng.randint(1, 9))]
+        start = rng.randint(0, chunk)
+        total = start + sum(lens) + rng.randint(0, 70)
+        places = lib.gdn_delta_prefill_workspace(
+            ctypes.byref(delta(dtype=dtype, n_tokens=total, n_seqs=len(lens)))) // one
+        used, first = [], start
+        for i, n in enumerate(lens):
+            used += [first // chunk + i + c for c in range(-(-n // chunk))]
+            first += n
+        assert len(set(used)) == len(used) and all(0 <= p < places for p in used), (lens, start, total)
+
+
+def logits(**change):
+    a = _lib.GDNLogits(_lib.DTYPE_FP32, 4, 1000, 50, 6, 4, 1000, 1000, 64, 32, AT, AT, AT, AT, AT, AT, AT, AT, AT, AT,
+                       AT, AT, AT)
+    for k, v in change.items():
+        setattr(a, k, v)
+    return a
+
+
+@pytest.mark.parametrize("change", [
+    dict(dtype=5), dict(vocab=(1 << 24) + 1), dict(rows=65536), dict(logits=0), dict(out=0), dict(history_len=0),
+    dict(bias_ids=0), dict(bias_values=0), dict(logits=AT + 2), dict(out=AT + 1), dict(logits_stride=999),
+    dict(out_stride=10), dict(history_stride=49), dict(history_width=1 << 31), dict(n_bias=1 << 31),
+    dict(n_masks=1 << 31), dict(mask_stride=31), dict(mask_index=0, n_masks=3),
+], ids=lambda c: "-".join(f"{k}={v}" for k, v in c.items()))
+def test_logits_process_refuses(change, capfd):
+    assert _lib.load().gdn_logits_process(ctypes.byref(logits(**change)), None) == -1
+    assert "gdn_logits_process: " in capfd.readouterr().err
+
+
+def sample(**change):
+    a = _lib.GDNSample(_lib.DTYPE_FP32, 4, 1000, 0, 1000, AT, AT, AT, AT, AT, AT, AT, AT)
+    for k, v in change.items():
+        setattr(a, k, v)
+    return a
+
+
+@pytest.mark.parametrize("change", [
+    dict(dtype=-2), dict(vocab=(1 << 20) + 1), dict(vocab=0), dict(rows=1 << 31), dict(logits=0), dict(tokens=0),
+    dict(uniform=0), dict(logits=AT + 2), dict(logits_stride=999),
+], ids=lambda c: "-".join(f"{k}={v}" for k, v in c.items()))
+def test_sample_refuses(change, capfd):
+    assert _lib.load().gdn_sample_tokens(ctypes.byref(sample(**change)), None) == -1
+    assert "gdn_sample_tokens: " in capfd.readouterr().err
+
+
+def test_nothing_to_do_and_null():
+    lib = _lib.load()
+    assert lib.gdn_logits_process(None, None) == -1 and lib.gdn_sample_tokens(None, None) == -1
+    assert lib.gdn_logits_process(ctypes.byref(logits(rows=0)), None) == 0
+    assert lib.gdn_logits_process(ctypes.byref(logits(vocab=0)), None) == 0
+    assert lib.gdn_sample_tokens(ctypes.byref(sample(rows=0)), None) == 0
+
+
+def test_tensors_must_be_on_a_gpu():
+    x = torch.zeros((4, 2, 64))
+    s, cu = torch.zeros((4, 2)), torch.zeros(2, dtype=torch.int32)
+    with pytest.raises(g.GDNError, match="on a GPU"):
+        g.delta_prefill(x, x, x, s, s, cu)
+    with pytest.raises(g.GDNError, match="on a GPU"):
+        g.delta_step(x, x, x, s, s, torch.zeros((4, 2, 64, 64)))
+    with pytest.raises(g.GDNError, match="on a GPU"):
+        g.logits_process(torch.zeros((2, 10)))
+    with pytest.raises(g.GDNError, match="on a GPU"):
+        g.sample_tokens(torch.zeros((2, 10)))
+
+
+def test_batch_sample_refuses_without_an_engine():
+    state, tokens = _lib.GDNBatchState(), (ctypes.c_int32 * 4)()
+    assert _lib.load().gdn_batch_sample(ctypes.byref(state), None, tokens, None) == -1
