@@ -4,6 +4,7 @@
 #include <hip/hip_runtime.h>
 
 #include <cstdio>
+#include <type_traits>
 
 #include "gdn_amd.h"
 #include "gdn_device.h"
@@ -143,11 +144,15 @@ __global__ __launch_bounds__(kPT) void k_process(GDNLogits p) {
 
 // A workgroup a row.  Weights are whole numbers of 2^-shift, so counts and
 // sums over the row are the same in any order.  The kept tokens are the first
-// ones of the ranking up to a border (key, index), found by histograms: first
-// over 2048 equal steps of (max - x) / temperature up to 32 -- what lies past
-// them has no weight -- then over 11, 11 and 10 bits of the border step's keys.
-constexpr int kST = 1024, kVals = 32, kBins = 2048;
-constexpr int kCells = (1 << 20) / 256;  // waves' pieces of the longest row
+// ones of the ranking up to a border (key, index): one histogram over kBins
+// steps of 1 / 32 in (max - x) / temperature -- what lies past them has no
+// weight -- gives the step the border is in, and the step's tokens, usually
+// some tens, are ranked against each other in LDS.  More than fit there go
+// through histograms of 11, 11 and 10 bits of their keys.
+constexpr int kST = 1024, kBins = kST, kWaves = kST / 64;
+constexpr int kList = 1024;           // tokens of a step that are ranked directly
+constexpr int kRadix = 2048;          // bins of a key histogram
+constexpr int kCells = (1 << 20) / 256;  // pieces of the longest row
 
 // The 32-bit key of x that grows as x falls (x not NaN; the zeros are equal).
 __device__ __forceinline__ uint32_t fall_key(float x) {
@@ -155,33 +160,14 @@ __device__ __forceinline__ uint32_t fall_key(float x) {
     return u & 0x80000000u ? u : ~u & 0x7fffffffu;
 }
 
-// exp(-d k ln 2) in steps of 2^-shift, d >= 0 (infinity: 0), from the Taylor
-// series of the exponential about the nearest power of two (12 terms:
-// 2e-16), k = log2(e) / temperature.
-struct Weights {
-    double k, unit, half;  // 2^shift
-    __device__ __forceinline__ uint64_t of(float d) const {
-        const double z = (double)d * k;
-        if (!(z < 64.0)) return 0;
-        const double e = __builtin_rint(z), t = (e - z) * 0.69314718055994530942;
-        double y = 1.0 / 479001600.0;
-        y = __builtin_fma(y, t, 1.0 / 39916800.0);
-        y = __builtin_fma(y, t, 1.0 / 3628800.0);
-        y = __builtin_fma(y, t, 1.0 / 362880.0);
-        y = __builtin_fma(y, t, 1.0 / 40320.0);
-        y = __builtin_fma(y, t, 1.0 / 5040.0);
-        y = __builtin_fma(y, t, 1.0 / 720.0);
-        y = __builtin_fma(y, t, 1.0 / 120.0);
-        y = __builtin_fma(y, t, 1.0 / 24.0);
-        y = __builtin_fma(y, t, 1.0 / 6.0);
-        y = __builtin_fma(y, t, 0.5);
-        y = __builtin_fma(y, t, 1.0);
-        y = __builtin_fma(y, t, 1.0);
-        // the sum's low bits are the rounded number of steps
-        const double s = __builtin_fma(__builtin_ldexp(y, -(int)e), unit, 0x1p52);
-        return __builtin_bit_cast(uint64_t, s) & 0xfffffffffffffull;
-    }
-};
+// exp(-x), x >= 0, to 2 units of 2^-24 (0 for infinity and NaN): the base-2
+// exponential with the rounding error of its argument made good.
+__device__ __forceinline__ float exp_neg(float x) {
+    constexpr float kL = 1.44269502f, kLo = 1.92596299e-8f;  // log2(e)
+    const float y = x * kL, e = __builtin_fmaf(x, kLo, __builtin_fmaf(x, kL, -y));
+    const float p = __builtin_amdgcn_exp2f(-y);
+    return y < 126.0f ? __builtin_fmaf(p, -0.693147181f * e, p) : 0.0f;
+}
 
 __device__ __forceinline__ uint64_t shfl_up64(uint64_t v, int d) {
     return ((uint64_t)(uint32_t)__shfl_up((int)(v >> 32), d) << 32) | (uint32_t)__shfl_up((int)v, d);
@@ -195,17 +181,30 @@ __device__ __forceinline__ uint64_t wave_scan(uint64_t v, int lane) {
     return v;
 }
 
+struct Ranked {
+    uint32_t key;
+    int at;
+    uint64_t w;
+};
 struct SampleLds {
-    uint32_t count[kBins];
-    unsigned long long mass[kBins];
-    uint64_t cell[kCells];
-    uint64_t wsum[kST / 64];
-    float wmax[kST / 64];
-    uint32_t warg[kST / 64];
-    double wexp[kST / 64];
-    uint64_t before, inside;  // of the bin found: weight (or count) ranked before it, and in it
-    uint64_t base;            // weight before it where counts decide
-    uint32_t bin;
+    double power[kBins];  // exp(-b / 32) 2^shift
+    union {
+        struct {
+            unsigned long long mass[kRadix];
+            uint32_t count[kRadix];
+        };
+        Ranked list[kList];
+        uint64_t cell[kCells];
+    };
+    uint64_t wsum[kWaves];
+    float wmax[kWaves];
+    int warg[kWaves];
+    double wexp[kWaves];
+    uint64_t base;    // weight ranked before a bin found
+    double left;      // of the goal, in it
+    uint32_t key;     // a border
+    int at;
+    uint32_t bin, n;
 };
 
 // The sum over the workgroup before each thread, and the whole sum.
@@ -217,7 +216,7 @@ __device__ __forceinline__ uint64_t block_scan(uint64_t v, uint64_t *wsum, uint6
     __syncthreads();
     uint64_t at = 0, all = 0;
 #pragma unroll
-    for (int i = 0; i < kST / 64; ++i) {
+    for (int i = 0; i < kWaves; ++i) {
         at += i < w ? wsum[i] : 0;
         all += wsum[i];
     }
@@ -225,41 +224,187 @@ __device__ __forceinline__ uint64_t block_scan(uint64_t v, uint64_t *wsum, uint6
     return at + s - v;
 }
 
-template <class T, bool ONE>
-__global__ __launch_bounds__(kST) void k_sample(GDNSample p, int shift) {
-    constexpr int V = T::kVec, NV = kVals / V, kPage = kST * kVals;
-    __shared__ SampleLds lds;
-    const int r = blockIdx.x, t = threadIdx.x, lane = t & 63, w = t >> 6, n = (int)p.vocab;
-    const typename T::E *row = static_cast<const typename T::E *>(p.logits) + (size_t)r * p.logits_stride;
-    const float nan = __builtin_nanf("");
-    float x[NV][V];
-    // f(value, index) over the row, a page of it in registers at a time; index
-    // = page + (i kST + thread) V + j, so a wave's 64 V are consecutive
-    auto load = [&](int page) {
+// A row and how its tokens fall and weigh.
+template <class T>
+struct Row {
+    static constexpr int V = T::kVec;
+    const typename T::E *row;
+    const double *power;
+    int n;
+    float top;
+    double top_d, inv_temp, step;  // step: 32 / temperature
+
+    // f(value, index), a wave's 64 V tokens consecutive
+    template <class F>
+    __device__ __forceinline__ void each(F &&f) const {
+#pragma unroll 2
+        for (int at = (int)threadIdx.x * V; at < n; at += kST * V) {
+            float x[V];
+            load_vec<T>(row, at, n, __builtin_nanf(""), x);
 #pragma unroll
-        for (int i = 0; i < NV; ++i) load_vec<T>(row, page + (i * kST + t) * V, n, nan, x[i]);
-    };
-    if (ONE) load(0);
-    auto each = [&](auto &&f) __attribute__((always_inline)) {
-        for (int page = 0; page < (ONE ? 1 : n); page += kPage) {
-            if (!ONE) load(page);
-#pragma unroll
-            for (int i = 0; i < NV; ++i)
-#pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    // a value of its own in every pass: what the passes form
-                    // from it is cheaper again than kept (32 values a thread)
-                    float v = x[i][j];
-                    asm volatile("" : "+v"(v));
-                    f(v, page + (i * kST + t) * V + j);
-                }
+            for (int j = 0; j < V; ++j) f(x[j], at + j);
         }
-    };
+    }
+    // how far below the highest; NaN for NaN, whose bin and exponential are
+    // those of infinity
+    __device__ __forceinline__ double fall(float v) const { return v == top ? 0.0 : top_d - (double)v; }
+    // kBins where the weight is 0: exp(-32) is half a unit of 2^-45
+    __device__ __forceinline__ int bin(double d) const { return (int)__builtin_fmin(d * step, (double)kBins); }
+    // exp(-d / temperature) 2^shift, rounded to a whole number: from the
+    // step's power and the Taylor series of what is left (1 / 32 at most: the
+    // first term left out is 6e-15)
+    __device__ __forceinline__ uint64_t weight(double d, int b) const {
+        if (b >= kBins) return 0;
+        const double t = __builtin_fma(-d, inv_temp, (double)b * (1.0 / 32.0));
+        double y = 1.0 / 720.0;
+        y = __builtin_fma(y, t, 1.0 / 120.0);
+        y = __builtin_fma(y, t, 1.0 / 24.0);
+        y = __builtin_fma(y, t, 1.0 / 6.0);
+        y = __builtin_fma(y, t, 0.5);
+        y = __builtin_fma(y, t, 1.0);
+        y = __builtin_fma(y, t, 1.0);
+        // the sum's low bits are the rounded number
+        return __builtin_bit_cast(uint64_t, __builtin_fma(power[b], y, 0x1p52)) & 0xfffffffffffffull;
+    }
+    __device__ __forceinline__ uint64_t weight(double d) const { return weight(d, bin(d)); }
+};
+
+// The border of the tokens of step `b` whose ranked counts (by_mass: weights)
+// first reach `left`, into lds.key and lds.at; their weight is the result.
+template <class T>
+__device__ uint64_t border_in(const Row<T> &r, SampleLds &lds, int b, bool by_mass, double left) {
+    const int t = threadIdx.x;
+    __syncthreads();
+    if (t == 0) lds.n = 0;
+    __syncthreads();
+    r.each([&](float v, int at) __attribute__((always_inline)) {
+        const double d = r.fall(v);
+        if (r.bin(d) == b) {
+            const uint32_t i = atomicAdd(&lds.n, 1u);
+            if (i < (uint32_t)kList) lds.list[i] = Ranked{fall_key(v), at, r.weight(d, b)};
+        }
+    });
+    __syncthreads();
+    const int n = (int)lds.n;
+    if (n <= kList) {
+        // the tokens' own ranks
+        if (t < n) {
+            const Ranked me = lds.list[t];
+            int rank = 0;
+            uint64_t before = 0;
+            for (int i = 0; i < n; ++i) {
+                const Ranked o = lds.list[i];
+                if (o.key < me.key || (o.key == me.key && o.at < me.at)) {
+                    ++rank;
+                    before += o.w;
+                }
+            }
+            const double from = by_mass ? (double)before : (double)rank,
+                         to = by_mass ? (double)(before + me.w) : (double)(rank + 1);
+            // rounding in `left` past the step's end: its last token
+            if ((from < left && to >= left) || (rank == n - 1 && to < left)) {
+                lds.key = me.key;
+                lds.at = me.at;
+                lds.base = before + me.w;
+            }
+        }
+        __syncthreads();
+        return lds.base;
+    }
+    uint64_t base = 0;
+    uint32_t prefix = 0, have = 0;
+    uint64_t each_w = 0;
+    for (int level = 0; level < 3; ++level) {
+        const int sh = level == 0 ? 21 : level == 1 ? 10 : 0;
+        const uint32_t bits = level == 2 ? 0x3ffu : 0x7ffu;
+        const uint32_t above = level == 0 ? 0u : ~0u << (level == 1 ? 21 : 10);
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < kRadix / kST; ++i) {
+            lds.count[t + i * kST] = 0;
+            lds.mass[t + i * kST] = 0;
+        }
+        __syncthreads();
+        r.each([&](float v, int) __attribute__((always_inline)) {
+            const double d = r.fall(v);
+            const uint32_t key = fall_key(v);
+            if (r.bin(d) == b && (key & above) == prefix) {
+                atomicAdd(&lds.count[(key >> sh) & bits], 1u);
+                atomicAdd(&lds.mass[(key >> sh) & bits], (unsigned long long)r.weight(d, b));
+            }
+        });
+        __syncthreads();
+        const int at = 2 * t;
+        const uint64_t m0 = lds.mass[at], m1 = lds.mass[at + 1], c0 = lds.count[at], c1 = lds.count[at + 1];
+        uint64_t all_m, all_c;
+        const uint64_t mb = block_scan(m0 + m1, lds.wsum, all_m), cb = block_scan(c0 + c1, lds.wsum, all_c);
+        const uint64_t v0 = by_mass ? m0 : c0, v1 = by_mass ? m1 : c1, vb = by_mass ? mb : cb;
+        // what the bin above holds is all here: rounding past it ends there
+        const double goal = __builtin_fmin(left, (double)(by_mass ? all_m : all_c));
+        if (v0 + v1 != 0 && (double)vb < goal && (double)(vb + v0 + v1) >= goal) {
+            const bool second = !((double)(vb + v0) >= goal);
+            lds.bin = at + second;
+            lds.left = goal - (double)(vb + (second ? v0 : 0));
+            lds.base = mb + (second ? m0 : 0);
+        }
+        __syncthreads();
+        prefix |= lds.bin << sh;
+        left = lds.left;
+        base += lds.base;
+        have = lds.count[lds.bin];
+        each_w = lds.mass[lds.bin] / have;
+    }
+    // of the border key's tokens (one weight all), the first `need` are kept
+    uint64_t need = by_mass ? (uint64_t)__builtin_ceil(left / (double)each_w) : (uint64_t)left;
+    need = need < 1 ? 1 : (need < have ? need : have);
+    // the place of the last of these: the pieces' counts, then the piece's own
+    constexpr int V = T::kVec;
+    const int n_cells = (r.n + 64 * V - 1) / (64 * V), lane = t & 63, w = t >> 6;
+    __syncthreads();
+    for (int c = w; c < n_cells; c += kWaves) {
+        float x[V];
+        load_vec<T>(r.row, (c * 64 + lane) * V, r.n, __builtin_nanf(""), x);
+        uint64_t k = 0;
+#pragma unroll
+        for (int j = 0; j < V; ++j) k += x[j] == x[j] && fall_key(x[j]) == prefix;
+        k = wave_scan(k, lane);
+        if (lane == 63) lds.cell[c] = k;
+    }
+    __syncthreads();
+    const int per = (n_cells + kST - 1) / kST;
+    uint64_t mine = 0, all;
+    for (int i = 0; i < per; ++i) mine += t * per + i < n_cells ? lds.cell[t * per + i] : 0;
+    uint64_t at = block_scan(mine, lds.wsum, all);
+    if (at < need && at + mine >= need) {
+        int c = t * per;
+        while (at + lds.cell[c] < need) at += lds.cell[c++];
+        for (int i = c * 64 * V; i < r.n; ++i) {
+            const float v = T::get(r.row[i]);
+            if (v == v && fall_key(v) == prefix && ++at == need) {
+                lds.key = prefix;
+                lds.at = i;
+                break;
+            }
+        }
+    }
+    __syncthreads();
+    return base + need * each_w;
+}
+
+template <class T>
+__global__ __launch_bounds__(kST) void k_sample(GDNSample p, int shift) {
+    constexpr int V = T::kVec;
+    __shared__ SampleLds lds;
+    const int ri = blockIdx.x, t = threadIdx.x, lane = t & 63, w = t >> 6;
+    Row<T> r;
+    r.row = static_cast<const typename T::E *>(p.logits) + (size_t)ri * p.logits_stride;
+    r.n = (int)p.vocab;
+    r.power = lds.power;
 
     // the highest logit, and its first place
     float top = -kInf;
     int arg = 0x7fffffff;
-    each([&](float v, int at) __attribute__((always_inline)) {
+    r.each([&](float v, int at) __attribute__((always_inline)) {
         if (v > top) {
             top = v;
             arg = at;
@@ -276,250 +421,168 @@ __global__ __launch_bounds__(kST) void k_sample(GDNSample p, int shift) {
     }
     if (lane == 0) {
         lds.wmax[w] = top;
-        lds.warg[w] = (uint32_t)arg;
+        lds.warg[w] = arg;
     }
+    const float temp = p.temperature ? p.temperature[ri] : 0.0f;
+    const bool greedy = !(temp > 0.0f);
+    const int k = p.top_k ? p.top_k[ri] : 0;
+    const float tp = p.top_p ? p.top_p[ri] : 1.0f;
+    const bool first_only = tp <= 0.0f;
+    const bool by_k = !greedy && !first_only && k > 0 && k < r.n, by_p = !greedy && !first_only && tp < 1.0f;
+    lds.power[t] = __builtin_ldexp(exp(-(double)t / 32.0), shift);
+    lds.count[t] = 0;
+    lds.mass[t] = 0;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < kST / 64; ++i)
-        if (lds.wmax[i] > top || (lds.wmax[i] == top && (int)lds.warg[i] < arg)) {
+    for (int i = 0; i < kWaves; ++i)
+        if (lds.wmax[i] > top || (lds.wmax[i] == top && lds.warg[i] < arg)) {
             top = lds.wmax[i];
-            arg = (int)lds.warg[i];
+            arg = lds.warg[i];
         }
     if (arg == 0x7fffffff) {  // nothing above -infinity
         if (t == 0) {
-            p.tokens[r] = -1;
-            if (p.logprobs) p.logprobs[r] = -kInf;
+            p.tokens[ri] = -1;
+            if (p.logprobs) p.logprobs[ri] = -kInf;
         }
         return;
     }
-    // how far below the highest, infinity for what carries no weight
-    auto fall = [&](float v) __attribute__((always_inline)) {
-        const float d = top - v;
-        return v == top ? 0.0f : (d >= 0.0f ? d : kInf);
+    r.top = top;
+    r.top_d = (double)top;
+    r.inv_temp = 1.0 / (double)temp;
+    r.step = 32.0 * r.inv_temp;
+
+    // the sum of exponentials, and the steps' counts and weights
+    double sum = 0.0;
+    auto pass = [&](auto sum_on, auto count_on, auto mass_on) __attribute__((always_inline)) {
+        r.each([&](float v, int) __attribute__((always_inline)) {
+            const double d = r.fall(v);
+            if (sum_on) sum += (double)exp_neg((float)d);
+            if (count_on || mass_on) {
+                const int b = r.bin(d);
+                if (b < kBins) {
+                    if (count_on) atomicAdd(&lds.count[b], 1u);
+                    if (mass_on) atomicAdd(&lds.mass[b], (unsigned long long)r.weight(d, b));
+                }
+            }
+        });
     };
+    constexpr std::true_type on;
+    constexpr std::false_type off;
+    if (by_k && by_p) pass(on, on, on);
+    else if (by_k) pass(on, on, off);
+    else if (by_p) pass(on, off, on);
+    else if (p.logprobs) pass(on, off, off);
     double log_sum = 0.0;
     if (p.logprobs) {
-        double s = 0.0;
-        each([&](float v, int) __attribute__((always_inline)) { s += (double)expf(-fall(v)); });
 #pragma unroll
-        for (int d = 1; d < 64; d <<= 1) s += __shfl_xor(s, d);
-        if (lane == 0) lds.wexp[w] = s;
+        for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d);
+        if (lane == 0) lds.wexp[w] = sum;
         __syncthreads();
-        s = 0.0;
+        sum = 0.0;
 #pragma unroll
-        for (int i = 0; i < kST / 64; ++i) s += lds.wexp[i];
-        log_sum = log(s);
+        for (int i = 0; i < kWaves; ++i) sum += lds.wexp[i];
+        log_sum = log(sum);
     }
-    const float temp = p.temperature ? p.temperature[r] : 0.0f;
-    if (!(temp > 0.0f)) {
+    if (greedy) {
         if (t == 0) {
-            p.tokens[r] = arg;
-            if (p.logprobs) p.logprobs[r] = (float)-log_sum;
+            p.tokens[ri] = arg;
+            if (p.logprobs) p.logprobs[ri] = (float)-log_sum;
         }
         return;
     }
-    Weights wt;
-    wt.k = 1.44269504088896340736 / (double)temp;
-    wt.unit = __builtin_ldexp(1.0, shift);
-    const float step = __builtin_fminf((float)(kBins - 1) / (32.0f * temp), 3.0e38f);
-    auto bin_of = [&](float d) __attribute__((always_inline)) {
-        return (int)__builtin_fminf(d * step, (float)(kBins - 1));
-    };
-    const int k = p.top_k ? p.top_k[r] : 0;
-    const float tp = p.top_p ? p.top_p[r] : 1.0f;
+
     // the border: tokens of a key below it are kept, of its key those up to
     // place edge_at
     uint32_t edge = 0xffffffffu;
     int edge_at = 0x7fffffff;
-
-    // the first bin up to which the counts (by_mass: the weights) reach `goal`;
-    // false if they never do
-    auto find = [&](bool by_mass, double goal) __attribute__((always_inline)) {
+    if (by_k || by_p) {
         __syncthreads();
-        const int b = 2 * t;
-        const uint64_t m0 = lds.mass[b], m1 = lds.mass[b + 1], c0 = lds.count[b], c1 = lds.count[b + 1];
-        uint64_t all;
-        const uint64_t mb = block_scan(m0 + m1, lds.wsum, all), cb = block_scan(c0 + c1, lds.wsum, all);
-        const uint64_t v0 = by_mass ? m0 : c0, v1 = by_mass ? m1 : c1, vb = by_mass ? mb : cb;
-        if (t == 0) lds.bin = kBins;
-        __syncthreads();
-        if (v0 + v1 != 0 && (double)vb < goal && (double)(vb + v0 + v1) >= goal) {
-            const bool second = !((double)(vb + v0) >= goal);
-            lds.bin = b + second;
-            lds.before = vb + (second ? v0 : 0);
-            lds.inside = second ? v1 : v0;
-            lds.base = mb + (second ? m0 : 0);
-        }
-        __syncthreads();
-        return lds.bin;
-    };
-    // moves the border to where the ranking's counts or weights reach `goal`,
-    // and gives the weight up to it (~0: it stays)
-    auto cut = [&](bool by_mass, double goal) -> uint64_t {
-        auto clear = [&]() __attribute__((always_inline)) {
-            __syncthreads();
-#pragma unroll
-            for (int i = 0; i < kBins / kST; ++i) {
-                lds.count[t + i * kST] = 0;
-                lds.mass[t + i * kST] = 0;
+        const uint64_t count = lds.count[t], mass = lds.mass[t];
+        uint64_t n_all = 0, kept = 0, n_before = 0, m_before = 0;
+        if (by_k) n_before = block_scan(count, lds.wsum, n_all);
+        if (by_p) m_before = block_scan(mass, lds.wsum, kept);
+        if (by_k && (uint64_t)k <= n_all) {
+            if (n_before < (uint64_t)k && n_before + count >= (uint64_t)k) {
+                lds.bin = t;
+                lds.left = (double)((uint64_t)k - n_before);
+                lds.base = m_before;
             }
             __syncthreads();
-        };
-        auto put = [&](int bin, float d) __attribute__((always_inline)) {
-            atomicAdd(&lds.count[bin], 1u);
-            atomicAdd(&lds.mass[bin], (unsigned long long)wt.of(d));
-        };
-        clear();
-        each([&](float v, int at) __attribute__((always_inline)) {
-            const float d = fall(v);
-            const int b = bin_of(d);
-            const uint32_t key = fall_key(v);
-            if (b < kBins - 1 && (key < edge || (key == edge && at <= edge_at))) put(b, d);
-        });
-        const uint32_t b0 = find(by_mass, goal);
-        if (b0 >= kBins) return ~0ull;  // past the weights' end
-        uint64_t base = lds.base;
-        double left = goal - (double)lds.before;
-        uint32_t prefix = 0;
-        for (int level = 0; level < 3; ++level) {
-            const int sh = level == 0 ? 21 : level == 1 ? 10 : 0;
-            const uint32_t bits = level == 2 ? 0x3ffu : 0x7ffu;
-            const uint32_t above = level == 0 ? 0u : ~0u << (level == 1 ? 21 : 10);
-            clear();
-            each([&](float v, int at) __attribute__((always_inline)) {
-                const float d = fall(v);
-                const uint32_t key = fall_key(v);
-                if (bin_of(d) == (int)b0 && d < kInf && (key & above) == prefix &&
-                    (key < edge || (key == edge && at <= edge_at)))
-                    put((int)((key >> sh) & bits), d);
-            });
-            // what the bin above holds is all here: rounding past it ends there
-            left = __builtin_fmin(left, (double)lds.inside);
-            const uint32_t b = find(by_mass, left);
-            prefix |= b << sh;
-            left -= (double)lds.before;
-            base += lds.base;
+            const uint64_t base = lds.base;
+            kept = base + border_in(r, lds, (int)lds.bin, false, lds.left);
+            edge = lds.key;
+            edge_at = lds.at;
         }
-        // of the border key's tokens (one weight all), the first `need` are kept
-        const uint32_t have = lds.count[prefix & 0x3ffu];
-        const uint64_t each_w = lds.mass[prefix & 0x3ffu] / have;
-        uint64_t need;
-        if (by_mass) {
-            need = each_w ? (uint64_t)__builtin_ceil(left / (double)each_w) : have;
-        } else {
-            need = (uint64_t)left;
-        }
-        need = need < 1 ? 1 : need;
-        if (need < have) {
-            // its place: the pieces' counts, then the piece's own tokens
+        if (by_p) {
+            const double goal = (double)tp * (double)kept;
             __syncthreads();
-            const int cells = (n + 64 * V - 1) / (64 * V);
-            for (int page = 0; page < n; page += kPage) {
-                if (!ONE) load(page);
-#pragma unroll
-                for (int i = 0; i < NV; ++i) {
-                    uint32_t c = 0;
-#pragma unroll
-                    for (int j = 0; j < V; ++j) c += fall_key(x[i][j]) == prefix && x[i][j] == x[i][j];
-#pragma unroll
-                    for (int d = 1; d < 64; d <<= 1) c += __shfl_xor((int)c, d);
-                    const int at = page / (64 * V) + i * (kST / 64) + w;
-                    if (lane == 0 && at < cells) lds.cell[at] = c;
-                }
+            // a goal that rounds past the last step's end ends there
+            if (mass != 0 && (double)m_before < goal && (double)(m_before + mass) >= goal) {
+                lds.bin = t;
+                lds.left = goal - (double)m_before;
             }
             __syncthreads();
-            uint64_t mine = 0, all;
-            const int per = (cells + kST - 1) / kST;
-            for (int i = 0; i < per; ++i) mine += t * per + i < cells ? lds.cell[t * per + i] : 0;
-            uint64_t at = block_scan(mine, lds.wsum, all);
-            if (at < need && at + mine >= need) {
-                int c = t * per;
-                while (at + lds.cell[c] < need) at += lds.cell[c++];
-                for (int i = c * 64 * V; i < n; ++i) {
-                    const float v = T::get(row[i]);
-                    if (v == v && fall_key(v) == prefix && ++at == need) {
-                        lds.bin = (uint32_t)i;
-                        break;
-                    }
-                }
+            // tokens past the first border rank behind all that reach the goal
+            border_in(r, lds, (int)lds.bin, true, lds.left);
+            if (lds.key < edge || (lds.key == edge && lds.at < edge_at)) {
+                edge = lds.key;
+                edge_at = lds.at;
             }
-            __syncthreads();
-            edge_at = (int)lds.bin;
-        } else {
-            need = have;
-            if (prefix != edge) edge_at = 0x7fffffff;
         }
-        edge = prefix;
-        return base + need * each_w;
-    };
-
-    uint64_t kept_mass = ~0ull;
-    if (k > 0 && k < n) kept_mass = cut(false, (double)k);
-    if (tp < 1.0f) {
-        if (!(tp > 0.0f)) {
-            edge = fall_key(top);
-            edge_at = arg;
-        } else {
-            if (kept_mass == ~0ull) {
-                uint64_t s = 0;
-                each([&](float v, int) __attribute__((always_inline)) { s += wt.of(fall(v)); });
-                block_scan(s, lds.wsum, kept_mass);
-            }
-            cut(true, (double)tp * (double)kept_mass);
-        }
+    } else if (first_only) {
+        edge = fall_key(top);
+        edge_at = arg;
     }
-    const float mp = p.min_p ? p.min_p[r] : 0.0f;
-    const double least = mp > 0.0f ? (double)__builtin_fminf(mp, 1.0f) * wt.unit : 0.0;
+    const float mp = p.min_p ? p.min_p[ri] : 0.0f;
+    const double least = mp > 0.0f ? __builtin_ldexp((double)__builtin_fminf(mp, 1.0f), shift) : 0.0;
     auto weight = [&](float v, int at) __attribute__((always_inline)) -> uint64_t {
         const uint32_t key = fall_key(v);
         if (!(key < edge || (key == edge && at <= edge_at))) return 0;
-        const uint64_t s = wt.of(fall(v));
+        const uint64_t s = r.weight(r.fall(v));
         return (double)s >= least ? s : 0;
     };
 
     // the kept weights by pieces of 64 V tokens, the piece the draw falls in,
     // the token in it
-    const int cells = (n + 64 * V - 1) / (64 * V);
+    const int cells = (r.n + 64 * V - 1) / (64 * V);
     __syncthreads();
-    for (int page = 0; page < n; page += kPage) {
-        if (!ONE) load(page);
+    for (int c = w; c < cells; c += kWaves) {
+        const int at = (c * 64 + lane) * V;
+        float x[V];
+        load_vec<T>(r.row, at, r.n, __builtin_nanf(""), x);
+        uint64_t s = 0;
 #pragma unroll
-        for (int i = 0; i < NV; ++i) {
-            uint64_t s = 0;
-#pragma unroll
-            for (int j = 0; j < V; ++j) s += weight(x[i][j], page + (i * kST + t) * V + j);
-            s = wave_scan(s, lane);
-            const int at = page / (64 * V) + i * (kST / 64) + w;
-            if (lane == 63 && at < cells) lds.cell[at] = s;
-        }
+        for (int j = 0; j < V; ++j) s += weight(x[j], at + j);
+        if (__ballot(s != 0) != 0) s = wave_scan(s, lane);
+        if (lane == 63) lds.cell[c] = s;
     }
     __syncthreads();
     uint64_t mine = 0, all;
     const int per = (cells + kST - 1) / kST;
     for (int i = 0; i < per; ++i) mine += t * per + i < cells ? lds.cell[t * per + i] : 0;
     uint64_t at = block_scan(mine, lds.wsum, all);
-    const double u = (double)p.uniform[r];
+    const double u = (double)p.uniform[ri];
     uint64_t goal = u > 0.0 ? (uint64_t)__builtin_fmin(u * (double)all, 9.2e18) : 0;
     goal = goal < all ? goal : all - 1;
     if (at <= goal && at + mine > goal) {
         int c = t * per;
         while (at + lds.cell[c] <= goal) at += lds.cell[c++];
         lds.bin = (uint32_t)c;
-        lds.before = at;
+        lds.base = at;
     }
     __syncthreads();
     if (w == 0) {
         const int c0 = (int)lds.bin * 64 * V + lane * V;
         float y[V];
-        load_vec<T>(row, c0, n, nan, y);
-        uint64_t s[V], sum = 0;
+        load_vec<T>(r.row, c0, r.n, __builtin_nanf(""), y);
+        uint64_t s[V], own = 0;
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             s[j] = weight(y[j], c0 + j);
-            sum += s[j];
+            own += s[j];
         }
-        uint64_t run = lds.before + wave_scan(sum, lane) - sum;
-        if (run <= goal && run + sum > goal) {
+        uint64_t run = lds.base + wave_scan(own, lane) - own;
+        if (run <= goal && run + own > goal) {
             int j = 0;
 #pragma unroll
             for (int i = 0; i < V; ++i) {
@@ -530,8 +593,8 @@ __global__ __launch_bounds__(kST) void k_sample(GDNSample p, int shift) {
                     break;
                 }
             }
-            p.tokens[r] = c0 + j;
-            if (p.logprobs) p.logprobs[r] = (float)(-(double)fall(T::get(row[c0 + j])) - log_sum);
+            p.tokens[ri] = c0 + j;
+            if (p.logprobs) p.logprobs[ri] = (float)(-r.fall(T::get(r.row[c0 + j])) - log_sum);
         }
     }
 }
@@ -599,18 +662,9 @@ extern "C" int gdn_sample_tokens(const GDNSample *args, void *stream) {
     // 2^shift times the vocabulary stays below 2^63
     const int shift = a.vocab <= (1u << 18) ? 45 : 43;
     const dim3 grid(a.rows), block(kST);
-    const bool one = a.vocab <= (uint32_t)(kST * kVals);
     hipStream_t s = static_cast<hipStream_t>(stream);
-#define GDN_LAUNCH_SAMPLE(T)                                                                  \
-    if (one) hipLaunchKernelGGL((k_sample<T, true>), grid, block, 0, s, a, shift);            \
-    else hipLaunchKernelGGL((k_sample<T, false>), grid, block, 0, s, a, shift)
-    if (a.dtype == GDN_DTYPE_BF16) {
-        GDN_LAUNCH_SAMPLE(Bf16);
-    } else if (a.dtype == GDN_DTYPE_FP16) {
-        GDN_LAUNCH_SAMPLE(Fp16);
-    } else {
-        GDN_LAUNCH_SAMPLE(Fp32);
-    }
-#undef GDN_LAUNCH_SAMPLE
+    if (a.dtype == GDN_DTYPE_BF16) hipLaunchKernelGGL(k_sample<Bf16>, grid, block, 0, s, a, shift);
+    else if (a.dtype == GDN_DTYPE_FP16) hipLaunchKernelGGL(k_sample<Fp16>, grid, block, 0, s, a, shift);
+    else hipLaunchKernelGGL(k_sample<Fp32>, grid, block, 0, s, a, shift);
     return launched(who);
 }
