@@ -35,5 +35,7 @@ def __getattr__(name: str):
     """The operators on torch tensors, imported (with torch) at first use."""
     if name in _DEVICE_OPS:
         from . import device_ops
-        return getattr(device_ops, name)
+        for op in _DEVICE_OPS:
+            globals()[op] = getattr(device_ops, op)
+        return globals()[name]
     raise AttributeError(f"module {__name__!r} has no attribute {name!r}")

@@ -20,63 +20,69 @@ from .engine import GDNError
 _DTYPES = {torch.bfloat16: L.DTYPE_BF16, torch.float16: L.DTYPE_FP16, torch.float32: L.DTYPE_FP32}
 
 
+_raw_stream = torch._C._cuda_getCurrentRawStream  # current_stream().cuda_stream without the objects, 2.7 us less
+_F32, _I32 = torch.float32, torch.int32
+
+
 def _fail(what: str) -> None:
     raise GDNError(what)
 
 
-def _on(device: torch.device, name: str, x, dtype, shape) -> int:
-    """The address of contiguous tensor x, or None's; shape with -1 = any."""
+def _on(dev: int, name: str, x, dtype, shape) -> int:
+    """The address of x, contiguous, of this type and shape on GPU dev (None: 0)."""
     if x is None:
         return 0
-    if x.device != device or x.dtype != dtype or len(x.shape) != len(shape) or not x.is_contiguous() or any(
-            a != b for a, b in zip(x.shape, shape) if b >= 0):
-        _fail(f"{name}: expected a contiguous {dtype} tensor of shape {tuple(shape)} on {device}, got "
-              f"{x.dtype} {tuple(x.shape)} on {x.device}")
-    return x.data_ptr()
+    if x.dtype is dtype and x.shape == shape and x.get_device() == dev and x.is_contiguous():
+        return x.data_ptr()
+    _fail(f"{name}: expected a contiguous {dtype} tensor of shape {tuple(shape)} on GPU {dev}, got {x.dtype} "
+          f"{tuple(x.shape)} strides {x.stride()} on {x.device}")
 
 
-def _launch(device: torch.device, what: str, fn, *args) -> None:
-    """fn(*args, stream) with the tensors' device as the current one."""
-    if torch.cuda.current_device() == device.index:
-        rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+def _launch(dev: int, what: str, fn, *args) -> None:
+    """fn(*args, stream) with GPU dev as the current one."""
+    if torch.cuda.current_device() == dev:
+        rc = fn(*args, _raw_stream(dev))
     else:
-        with torch.cuda.device(device):
-            rc = fn(*args, torch.cuda.current_stream().cuda_stream)
+        with torch.cuda.device(dev):
+            rc = fn(*args, _raw_stream(dev))
     if rc != 0:
         _fail(f"{what} failed (rc={rc})")
 
 
-def _heads(name: str, x: torch.Tensor, like: torch.Tensor) -> None:
-    if x.device != like.device or x.dtype != like.dtype or x.dim() != 3 or (
-            x.shape[0] > 0 and (x.stride(2) != 1 or x.stride(1) != x.shape[2])):
-        _fail(f"{name}: expected {like.dtype} [rows][heads][dim] on {like.device} with contiguous heads, got {x.dtype} "
-              f"{tuple(x.shape)} strides {x.stride()} on {x.device}")
-
-
-def _delta(q, k, v, g, beta, out, state_in, state_out, slots, n_seqs, scale, l2norm):
-    dtype = _DTYPES.get(q.dtype)
-    if dtype is None or not q.is_cuda:
-        _fail(f"q: expected a bfloat16, float16 or float32 tensor on a GPU, got {q.dtype} on {q.device}")
+def _delta(q, k, v, g, beta, out, state_in, state_out, slots, n_seqs, cu, scale, l2norm):
+    """(GPU, GDNDelta) of a call, checked."""
+    qt, dev = q.dtype, q.get_device()
+    dtype = _DTYPES.get(qt)
+    if dtype is None or dev < 0:
+        _fail(f"q: expected a bfloat16, float16 or float32 tensor on a GPU, got {qt} on {q.device}")
     for name, x in (("q", q), ("k", k), ("v", v), ("out", out)):
-        _heads(name, x, q)
-    n, hq, dk = q.shape
-    hv, dv = v.shape[1:]
-    if k.shape != q.shape or v.shape[0] != n or out.shape != v.shape:
-        _fail(f"shapes do not agree: q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}, out {tuple(out.shape)}")
-    if g.shape != (n, hv) or beta.shape != (n, hv) or g.dtype != torch.float32 or beta.dtype != torch.float32 or (
-            g.device != q.device or beta.device != q.device) or (
-            n > 0 and hv > 1 and (g.stride(1) != 1 or beta.stride(1) != 1)) or (n > 1 and g.stride(0) != beta.stride(0)):
+        if x.dtype is not qt or x.dim() != 3 or x.get_device() != dev:
+            _fail(f"{name}: expected {qt} [rows][heads][dim] on {q.device}, got {x.dtype} {tuple(x.shape)} on {x.device}")
+    n, hq, dk = qs = q.shape
+    _, hv, dv = vs = v.shape
+    if k.shape != qs or vs[0] != n or out.shape != vs:
+        _fail(f"shapes do not agree: q {tuple(qs)}, k {tuple(k.shape)}, v {tuple(vs)}, out {tuple(out.shape)}")
+    sq, sk, sv, so = q.stride(), k.stride(), v.stride(), out.stride()
+    heads, values = (dk, 1), (dv, 1)
+    if n and (sq[1:] != heads or sk[1:] != heads or sv[1:] != values or so[1:] != values):
+        _fail(f"heads must be contiguous in a row: strides q {sq}, k {sk}, v {sv}, out {so}")
+    gates, sg, sb = (n, hv), g.stride(), beta.stride()
+    if g.shape != gates or beta.shape != gates or g.dtype is not _F32 or beta.dtype is not _F32 or (
+            g.get_device() != dev or beta.get_device() != dev) or (
+            n > 0 and hv > 1 and (sg[1] != 1 or sb[1] != 1)) or (n > 1 and sg[0] != sb[0]):
         _fail(f"g and beta: expected float32 [{n}][{hv}] of equal row strides on {q.device}")
-    pool = state_out if state_out is not None else state_in
-    n_slots = pool.shape[0] if pool is not None else n_seqs
-    states = [_on(q.device, name, x, torch.float32, (n_slots, hv, dk, dv))
-              for name, x in (("state_in", state_in), ("state_out", state_out))]
-    where = _on(q.device, "slots", slots, torch.int32, (n_seqs,))
+    pool = state_in if state_out is None else state_out
+    n_slots = n_seqs if pool is None else pool.shape[0] if pool.dim() else -1
+    states = (n_slots, hv, dk, dv)
+    at_in = _on(dev, "state_in", state_in, _F32, states)
+    at_out = at_in if state_out is state_in else _on(dev, "state_out", state_out, _F32, states)
     if slots is None and n_slots < n_seqs:
         _fail(f"{n_seqs} sequences without slots need as many states, got {n_slots}")
-    return L.GDNDelta(dtype, n, n_seqs, hq, hv, dk, dv, 1 if l2norm else 0, dk**-0.5 if scale is None else scale,
-                      n_slots, q.stride(0), k.stride(0), v.stride(0), out.stride(0), g.stride(0), q.data_ptr(),
-                      k.data_ptr(), v.data_ptr(), out.data_ptr(), g.data_ptr(), beta.data_ptr(), 0, where, *states)
+    return dev, L.GDNDelta(
+        dtype, n, n_seqs, hq, hv, dk, dv, 1 if l2norm else 0, dk**-0.5 if scale is None else scale, n_slots, sq[0],
+        sk[0], sv[0], so[0], sg[0], q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), g.data_ptr(),
+        beta.data_ptr(), _on(dev, "cu_seqlens", cu, _I32, (n_seqs + 1,)), _on(dev, "slots", slots, _I32, (n_seqs,)),
+        at_in, at_out)
 
 
 def delta_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tensor, beta: torch.Tensor,
@@ -98,17 +104,17 @@ def delta_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Te
     workspace: uint8, gdn_delta_prefill_workspace bytes (None: allocated).
     """
     if out is None:
-        out = torch.empty(v.shape, dtype=v.dtype, device=v.device)
+        out = torch.empty_like(v, memory_format=torch.contiguous_format)
     n_seqs = cu_seqlens.shape[0] - 1 if cu_seqlens.dim() == 1 else -1
     if n_seqs < 0:
         _fail("cu_seqlens: expected int32 [sequences + 1]")
-    args = _delta(q, k, v, g, beta, out, state_in, state_out, slots, n_seqs, scale, l2norm)
-    args.cu_seqlens = _on(q.device, "cu_seqlens", cu_seqlens, torch.int32, (n_seqs + 1,))
+    dev, args = _delta(q, k, v, g, beta, out, state_in, state_out, slots, n_seqs, cu_seqlens, scale, l2norm)
     lib, ref = L.load(), ctypes.byref(args)
     if workspace is None:
         workspace = torch.empty(lib.gdn_delta_prefill_workspace(ref), dtype=torch.uint8, device=q.device)
-    ws = _on(q.device, "workspace", workspace, torch.uint8, (-1,))
-    _launch(q.device, "gdn_delta_prefill", lib.gdn_delta_prefill, ref, ws, workspace.numel())
+    size = workspace.numel()
+    _launch(dev, "gdn_delta_prefill", lib.gdn_delta_prefill, ref,
+            _on(dev, "workspace", workspace, torch.uint8, (size,)), size)
     return out
 
 
@@ -120,27 +126,30 @@ def delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tenso
     is sequence i's, its state slot slots[i] of ``state``, updated in place (or
     written to state_out).  Shapes and the rest as delta_prefill's."""
     if out is None:
-        out = torch.empty(v.shape, dtype=v.dtype, device=v.device)
-    args = _delta(q, k, v, g, beta, out, state, state if state_out is None else state_out, slots, q.shape[0], scale,
-                  l2norm)
-    _launch(q.device, "gdn_delta_step", L.load().gdn_delta_step, ctypes.byref(args))
+        out = torch.empty_like(v, memory_format=torch.contiguous_format)
+    dev, args = _delta(q, k, v, g, beta, out, state, state if state_out is None else state_out, slots, q.shape[0], None,
+                       scale, l2norm)
+    _launch(dev, "gdn_delta_step", L.load().gdn_delta_step, ctypes.byref(args))
     return out
 
 
-def _logits(x: torch.Tensor, name: str = "logits") -> int:
-    dtype = _DTYPES.get(x.dtype)
-    if dtype is None or not x.is_cuda or x.dim() != 2 or (x.shape[1] > 1 and x.stride(1) != 1):
+def _logits(x: torch.Tensor, name: str = "logits"):
+    """(GPU, type, rows, vocabulary, row stride) of a batch of logits."""
+    dtype, dev = _DTYPES.get(x.dtype), x.get_device()
+    if dtype is None or dev < 0 or x.dim() != 2 or (x.shape[1] > 1 and x.stride(1) != 1):
         _fail(f"{name}: expected a bfloat16, float16 or float32 [rows][vocabulary] on a GPU with contiguous rows, got "
-              f"{x.dtype} {tuple(x.shape)} on {x.device}")
-    return dtype
+              f"{x.dtype} {tuple(x.shape)} strides {x.stride()} on {x.device}")
+    rows, vocab = x.shape
+    return dev, dtype, rows, vocab, x.stride(0)
 
 
-def _matrix(device, name: str, x, dtype, rows: int) -> int:
-    if x.device != device or x.dtype != dtype or x.dim() != 2 or (rows >= 0 and x.shape[0] != rows) or (
+def _matrix(dev: int, name: str, x, rows: int):
+    """(address, columns, row stride) of an int32 matrix (rows < 0: any)."""
+    if x.dtype is not _I32 or x.dim() != 2 or x.get_device() != dev or (rows >= 0 and x.shape[0] != rows) or (
             x.shape[1] > 1 and x.stride(1) != 1):
-        _fail(f"{name}: expected {dtype} [{rows if rows >= 0 else 'n'}][n] on {device} with contiguous rows, got "
-              f"{x.dtype} {tuple(x.shape)} on {x.device}")
-    return x.data_ptr()
+        _fail(f"{name}: expected int32 [{rows if rows >= 0 else 'n'}][n] on GPU {dev} with contiguous rows, got "
+              f"{x.dtype} {tuple(x.shape)} strides {x.stride()} on {x.device}")
+    return x.data_ptr(), x.shape[1], x.stride(0) if x.shape[0] > 1 else x.shape[1]
 
 
 def logits_process(logits: torch.Tensor, *, history: Optional[torch.Tensor] = None,
@@ -158,40 +167,44 @@ def logits_process(logits: torch.Tensor, *, history: Optional[torch.Tensor] = No
     [masks][>= vocab / 32] with a set bit for every allowed token, mask_index
     int32 [rows].  out may be logits itself.  Returns out.
     """
-    dtype, device, rows = _logits(logits), logits.device, logits.shape[0]
+    dev, dtype, rows, vocab, stride = _logits(logits)
     if out is None:
-        out = torch.empty(logits.shape, dtype=logits.dtype, device=device)
-    elif _logits(out, "out") != dtype or out.shape != logits.shape or out.device != device:
-        _fail(f"out: expected {logits.dtype} {tuple(logits.shape)} on {device}, got {out.dtype} {tuple(out.shape)}")
-    a = L.GDNLogits(dtype, rows, logits.shape[1], 0, 0, 0, logits.stride(0), out.stride(0), 0, 0, logits.data_ptr(),
-                    out.data_ptr())
+        out = torch.empty_like(logits, memory_format=torch.contiguous_format)
+        into = vocab
+    else:
+        to_dev, to_type, _, _, into = _logits(out, "out")
+        if to_dev != dev or to_type != dtype or out.shape != logits.shape:
+            _fail(f"out: expected {logits.dtype} {tuple(logits.shape)} on {logits.device}, got {out.dtype} "
+                  f"{tuple(out.shape)} on {out.device}")
+    one, hist, length, prompt, width, h_stride = (rows,), 0, 0, 0, 0, 0
+    rep = pres = freq = 0
     if history is not None:
         if history_len is None:
             _fail("history needs history_len")
-        a.history = _matrix(device, "history", history, torch.int32, rows)
-        a.history_width, a.history_stride = history.shape[1], history.stride(0)
-        a.history_len = _on(device, "history_len", history_len, torch.int32, (rows,))
-        a.prompt_len = _on(device, "prompt_len", prompt_len, torch.int32, (rows,))
-        a.repetition = _on(device, "repetition", repetition, torch.float32, (rows,))
-        a.presence = _on(device, "presence", presence, torch.float32, (rows,))
-        a.frequency = _on(device, "frequency", frequency, torch.float32, (rows,))
+        hist, width, h_stride = _matrix(dev, "history", history, rows)
+        length, prompt = _on(dev, "history_len", history_len, _I32, one), _on(dev, "prompt_len", prompt_len, _I32, one)
+        rep, pres = _on(dev, "repetition", repetition, _F32, one), _on(dev, "presence", presence, _F32, one)
+        freq = _on(dev, "frequency", frequency, _F32, one)
     elif not (history_len is prompt_len is repetition is presence is frequency is None):
         _fail("penalties need a history")
+    b_at = b_ids = b_values = n_bias = 0
     if bias is not None:
         offsets, ids, values = bias
-        a.bias_offsets = _on(device, "bias offsets", offsets, torch.int32, (rows + 1,))
-        a.bias_ids = _on(device, "bias ids", ids, torch.int32, (-1,))
-        a.bias_values = _on(device, "bias values", values, torch.float32, (ids.shape[0],))
-        a.n_bias = ids.shape[0]
+        entries = (ids.numel(),)
+        b_at = _on(dev, "bias offsets", offsets, _I32, (rows + 1,))
+        b_ids, b_values = _on(dev, "bias ids", ids, _I32, entries), _on(dev, "bias values", values, _F32, entries)
+        n_bias = entries[0]
+    m_at = m_index = n_masks = m_stride = 0
     if mask is not None:
-        a.mask = _matrix(device, "mask", mask, torch.int32, -1)
-        a.n_masks, a.mask_stride = mask.shape[0], mask.stride(0) if mask.shape[0] > 1 else mask.shape[1]
-        if mask.shape[1] * 32 < logits.shape[1]:
-            _fail(f"mask: {mask.shape[1]} words are fewer than {logits.shape[1]} tokens")
-        a.mask_index = _on(device, "mask_index", mask_index, torch.int32, (rows,))
+        m_at, words, m_stride = _matrix(dev, "mask", mask, -1)
+        if words * 32 < vocab:
+            _fail(f"mask: {words} words are fewer than {vocab} tokens")
+        n_masks, m_index = mask.shape[0], _on(dev, "mask_index", mask_index, _I32, one)
     elif mask_index is not None:
         _fail("mask_index needs a mask")
-    _launch(device, "gdn_logits_process", L.load().gdn_logits_process, ctypes.byref(a))
+    a = L.GDNLogits(dtype, rows, vocab, width, n_bias, n_masks, stride, into, h_stride, m_stride, logits.data_ptr(),
+                    out.data_ptr(), hist, length, prompt, rep, pres, freq, b_at, b_ids, b_values, m_at, m_index)
+    _launch(dev, "gdn_logits_process", L.load().gdn_logits_process, ctypes.byref(a))
     return out
 
 
@@ -207,18 +220,15 @@ def sample_tokens(logits: torch.Tensor, uniform: Optional[torch.Tensor] = None, 
     positive: the first of the highest logits.  Returns (tokens int32 [rows],
     logprobs FP32 [rows]); -1 where no logit is above -infinity.
     """
-    dtype, device, rows = _logits(logits), logits.device, logits.shape[0]
+    dev, dtype, rows, vocab, stride = _logits(logits)
+    one = (rows,)
     if tokens is None:
-        tokens = torch.empty(rows, dtype=torch.int32, device=device)
+        tokens = torch.empty(one, dtype=_I32, device=logits.device)
     if logprobs is None:
-        logprobs = torch.empty(rows, dtype=torch.float32, device=device)
-    a = L.GDNSample(dtype, rows, logits.shape[1], 0, logits.stride(0), logits.data_ptr(),
-                    _on(device, "uniform", uniform, torch.float32, (rows,)),
-                    _on(device, "temperature", temperature, torch.float32, (rows,)),
-                    _on(device, "top_k", top_k, torch.int32, (rows,)),
-                    _on(device, "top_p", top_p, torch.float32, (rows,)),
-                    _on(device, "min_p", min_p, torch.float32, (rows,)),
-                    _on(device, "tokens", tokens, torch.int32, (rows,)),
-                    _on(device, "logprobs", logprobs, torch.float32, (rows,)))
-    _launch(device, "gdn_sample_tokens", L.load().gdn_sample_tokens, ctypes.byref(a))
+        logprobs = torch.empty(one, dtype=_F32, device=logits.device)
+    a = L.GDNSample(dtype, rows, vocab, 0, stride, logits.data_ptr(), _on(dev, "uniform", uniform, _F32, one),
+                    _on(dev, "temperature", temperature, _F32, one), _on(dev, "top_k", top_k, _I32, one),
+                    _on(dev, "top_p", top_p, _F32, one), _on(dev, "min_p", min_p, _F32, one),
+                    _on(dev, "tokens", tokens, _I32, one), _on(dev, "logprobs", logprobs, _F32, one))
+    _launch(dev, "gdn_sample_tokens", L.load().gdn_sample_tokens, ctypes.byref(a))
     return tokens, logprobs
