@@ -82,15 +82,20 @@ struct Raw8 {
     }
 };
 
-// A product of operands of NA and NB terms over one 32-wide k step, smallest
-// terms first; terms below 2^-24 of the product are left out.
-template <int NA, int NB>
-__device__ __forceinline__ f32x4 mfma_terms(const u32x4 (&a)[NA], const u32x4 (&b)[NB], f32x4 c) {
+// f(a, b) for the terms a, b of two operands, of NA and NB terms, whose
+// products count, smallest first; products below 2^-24 of the whole are left
+// out.
+template <int NA, int NB, class F>
+__device__ __forceinline__ void for_terms(F &&f) {
 #pragma unroll
     for (int s = 2; s >= 0; --s)
 #pragma unroll
         for (int i = NA - 1; i >= 0; --i)
-            if (s - i >= 0 && s - i < NB) c = mfma_bf16(a[i], b[s - i], c);
+            if (s - i >= 0 && s - i < NB) f(i, s - i);
+}
+template <int NA, int NB>
+__device__ __forceinline__ f32x4 mfma_terms(const u32x4 (&a)[NA], const u32x4 (&b)[NB], f32x4 c) {
+    for_terms<NA, NB>([&](int i, int j) __attribute__((always_inline)) { c = mfma_bf16(a[i], b[j], c); });
     return c;
 }
 
@@ -98,17 +103,24 @@ __device__ __forceinline__ f32x4 mfma_terms(const u32x4 (&a)[NA], const u32x4 (&
 template <class T>
 constexpr int kChunk = T::kTerms == 1 ? 64 : 32;
 
+// Four values of 16-bit columns l % 16: of each 16 lanes, lane l names the
+// 8 bytes of row l / 4, columns 4 (l % 4) .. + 3, and gets its column's four rows.
+__device__ __forceinline__ u32x2 read_transposed(const u32x2 *lds) {
+    typedef short s16x4 __attribute__((ext_vector_type(4)));
+    typedef __attribute__((address_space(3))) s16x4 *Ptr;
+    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Ptr)(const_cast<u32x2 *>(lds))));
+}
+
 // Where a 16 x 32 tile (row tile i, column step j) of a chunk's lower
 // triangular matrix is kept: tiles above the diagonal are zero and left out.
 template <int C>
 constexpr int kTriTiles = C == 64 ? 6 : 2;
 __device__ __forceinline__ constexpr int tri_tile(int i, int j) { return i < 2 ? i : 2 * i - 2 + j; }
 
-// What k_delta_seq needs of one (chunk, value head), as it lies in its LDS.
-// Matrices as MFMA A fragments of the three BF16 terms: lane l carries row
-// 16 i + l % 16 and columns 32 j + 4 (l / 16) + {0..3, 16..19}, the tokens that
-// lane holds of a 32-token step in the accumulator layout, so that results
-// become the next product's B operand where they lie.
+// What k_delta_seq needs of one (chunk, value head).  Matrices as MFMA A
+// fragments of the three BF16 terms: lane l carries row 16 i + l % 16 and
+// columns 32 j + 4 (l / 16) + {0..3, 16..19}, the tokens that lane holds of a
+// 32-token step in the accumulator layout.
 //   sc[m]  exp(G_m) |k_m|^-1, beta_m, scale exp(G_m) |q_m|^-1,
 //          exp(G_{n-1} - G_m) |k_m|^-1; zeros past the chunk's n tokens
 //   dn     exp(G_{n-1})
@@ -117,6 +129,13 @@ struct ChunkOps {
     u32x4 tf[kTriTiles<C>][3][64], mf[kTriTiles<C>][3][64];
     f32x4 sc[C];
     f32x4 dn;
+};
+
+// k and q of one (chunk, query/key head) as BF16 terms, rows past the chunk's
+// end zero: for the types that do not enter the products as they are.
+template <class T, int DK>
+struct Planes {
+    uint16_t k[T::kTerms][kChunk<T>][DK], q[T::kTerms][kChunk<T>][DK];
 };
 
 // One sequence's rows.
@@ -152,7 +171,8 @@ __device__ __forceinline__ int place_of(int first, int i) {
 // from the diagonal on FP32 MFMAs.  G is summed in 64 bits: the weights are
 // exponentials of its differences.
 template <class T, int DK>
-__global__ __launch_bounds__(4 * kChunk<T>) void k_delta_prep(GDNDelta p, ChunkOps<kChunk<T>> *__restrict__ ops_all) {
+__global__ __launch_bounds__(4 * kChunk<T>) void k_delta_prep(GDNDelta p, ChunkOps<kChunk<T>> *__restrict__ ops_all,
+                                                                Planes<T, DK> *__restrict__ planes) {
     constexpr int C = kChunk<T>, NW = C / 16, NT = T::kTerms, KS = DK / 32, LD = C + 4;
     constexpr int kFrag = NW * KS * NT * 64 * 16, kMat = C * LD * 4;
     __shared__ __attribute__((aligned(16))) unsigned char mem[kFrag > kMat ? kFrag : kMat];
@@ -222,6 +242,16 @@ __global__ __launch_bounds__(4 * kChunk<T>) void k_delta_prep(GDNDelta p, ChunkO
         qr[s].terms(qa[s]);
 #pragma unroll
         for (int j = 0; j < NT; ++j) kb[w][s][j][lane] = ka[j];
+        if constexpr (NT > 1) {
+            if (hv % (int)(p.n_v_heads / p.n_qk_heads) == 0) {
+                Planes<T, DK> &pl = planes[(size_t)place * p.n_qk_heads + hk];
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    *reinterpret_cast<u32x4 *>(&pl.k[j][mine][32 * s + 8 * kk]) = ka[j];
+                    *reinterpret_cast<u32x4 *>(&pl.q[j][mine][32 * s + 8 * kk]) = qa[s][j];
+                }
+            }
+        }
     }
     kn += __shfl_xor(kn, 16);
     qn += __shfl_xor(qn, 16);
@@ -338,35 +368,58 @@ __global__ __launch_bounds__(4 * kChunk<T>) void k_delta_prep(GDNDelta p, ChunkO
 
 // ------------------------------------------------------------ the sequences
 
-// One (sequence, value head)'s chunks in order for 16 NW value columns, a wave
-// 16 of them with all keys: its state is the accumulator tiles of its updates
-// (lane l: key 16 tile + 4 (l / 16) + r, column l % 16), and every product of a
-// chunk has its B operand in the wave's own registers:
+// One (sequence, value head)'s chunks in order:
 //   d = T (beta (v - exp(G) K S));  o = exp(G) Q S + M d;
 //   S' = exp(G_{n-1}) S + K^T (exp(G_{n-1} - G) d)
-// so the waves meet only where the chunk's A operands change in LDS: K and Q by
-// rows, K by keys, T and M.  The next chunk's are on their way in registers
-// meanwhile.  16-byte units of a row are XORed with the row's low bits, which
-// spreads both the fragments' reads and the transposed writes over the banks.
-template <class T, int DK>
+// A workgroup of eight waves has CT = 8 / KP tiles of 16 value columns, KP waves
+// a tile, a KP-th of the keys each.  A wave's state is the accumulator tiles of
+// its updates, and lies so that it is also the B operand of its K S and Q S: of
+// a 32-key step, lane l holds keys 8 (l / 16) .. + 7 of column l % 16, the first
+// four in one tile, the others in the next.  The KP waves' shares of K S and Q S
+// meet in LDS where the wave that owns a 16-token tile adds them; it forms b, its
+// rows of d and of o, and leaves the BF16 terms of b, d and the scaled d in LDS
+// as the B operands that the tile's waves read.  K and Q lie in LDS by rows, the
+// 16-byte units XORed with the row's low bits (no two of eight rows on one
+// bank); the update reads K transposed (ds_read_b64_tr_b16).  The next chunk's
+// operands are loaded into registers meanwhile.
+constexpr int kSeqWaves = 8, kSeqT = 64 * kSeqWaves;
+
+template <class T, int DK, int KP>
 struct SeqLds {
-    static constexpr int C = kChunk<T>, NT = T::kTerms;
-    u32x4 kr[NT][C][DK / 8], qr[NT][C][DK / 8], kt[NT][DK][C / 8];
-    ChunkOps<C> ops;
+    static constexpr int C = kChunk<T>, NT = T::kTerms, CT = kSeqWaves / KP, MT = C / 16, JT = C / 32;
+    // K of two chunks where the LDS holds it: the next one's is written while
+    // this one's is read, a barrier less
+    static constexpr int kBuf = NT * C * DK >= 3 * 32 * 256 ? 1 : 2;
+    u32x4 k[kBuf][NT][C][DK / 8];
+    // b's terms take q's place once Q S is formed
+    union {
+        u32x4 q[NT][C][DK / 8];
+        u32x4 b[CT][JT][3][64];
+    };
+    union {
+        f32x4 part[CT][MT][2][KP - 1][64];  // K S and Q S: [tile][token tile][which][wave but the owner]
+        u32x4 df[CT][2][JT][3][64];         // d and the scaled d: [tile][which][step][term]
+    };
+    f32x4 sc[2][C + 1];  // a chunk's sc and, last, dn
 };
 
-template <class T, int DK, int NW>
-__global__ __launch_bounds__(64 * NW) void k_delta_seq(GDNDelta p, const ChunkOps<kChunk<T>> *__restrict__ ops_all,
-                                                       int pairs) {
-    constexpr int C = kChunk<T>, NT = T::kTerms, TPB = 64 * NW, MT = C / 16, JT = C / 32, KS = DK / 32;
-    constexpr int kTasks = (C / 4) * (DK / 8), PT = (kTasks + TPB - 1) / TPB;
-    constexpr int kOps = sizeof(ChunkOps<C>) / 16, PO = (kOps + TPB - 1) / TPB;
-    __shared__ SeqLds<T, DK> lds;
+template <class T, int DK, int KP>
+__global__ __launch_bounds__(kSeqT, 2) void k_delta_seq(GDNDelta p, const ChunkOps<kChunk<T>> *__restrict__ ops_all,
+                                                        const Planes<T, DK> *__restrict__ planes, int pairs) {
+    using Lds = SeqLds<T, DK, KP>;
+    constexpr int C = Lds::C, NT = Lds::NT, CT = Lds::CT, MT = Lds::MT, JT = Lds::JT, kBuf = Lds::kBuf;
+    constexpr int KS = DK / 32 / KP;              // 32-key steps of a wave
+    constexpr int OT = MT >= KP ? MT / KP : 1;    // token tiles a wave owns
+    constexpr int kUnits = NT * C * DK / 8, PU = (kUnits + kSeqT - 1) / kSeqT;
+    constexpr int kSc = C + 1;
+    static_assert(KS >= 1 && MT >= KP, "whole steps and tiles");
+    __shared__ Lds lds;
     const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
     const int t = threadIdx.x, w = t >> 6, lane = t & 63, li = lane & 15, kk = lane >> 4;
+    const int ks = w % KP, ct = w / KP;
     // the column groups of a (sequence, head) share its operands: one XCD's
     // (workgroups go to the eight in turn)
-    const int groups = (int)p.value_dim / (16 * NW), x = blockIdx.x >> 3;
+    const int groups = (int)p.value_dim / (16 * CT), x = blockIdx.x >> 3;
     const int pair = (x / groups) * 8 + (blockIdx.x & 7), cg = x % groups;
     if (pair >= pairs) return;
     const int seq = pair / (int)p.n_v_heads, hv = pair % (int)p.n_v_heads;
@@ -374,204 +427,276 @@ __global__ __launch_bounds__(64 * NW) void k_delta_seq(GDNDelta p, const ChunkOp
     const int slot = slot_of(p, seq);
     if (slot < 0) return;
     const Span sp = span_of(p, seq);
-    const int chunks = (sp.n + C - 1) / C, col = 16 * (NW * cg + w) + li;
-    const size_t state_at = ((size_t)slot * p.n_v_heads + hv) * DK * p.value_dim + col;
-    const ChunkOps<C> *ops = ops_all + (size_t)place_of<C>(sp.first, seq) * p.n_v_heads + hv;
+    const int chunks = (sp.n + C - 1) / C, col = 16 * (CT * cg + ct) + li;
+    const size_t place = (size_t)place_of<C>(sp.first, seq);
+    const ChunkOps<C> *ops = ops_all + place * p.n_v_heads + hv;
+    // the state's key of tile a, register r of step s: key0 + 32 s + 4 a + r
+    const int key0 = ks * (DK / KP) + 8 * kk;
+    const size_t state_at = (((size_t)slot * p.n_v_heads + hv) * DK + key0) * p.value_dim + col;
 
-    f32x4 S[DK / 16];
+    f32x4 S[KS][2];
 #pragma unroll
-    for (int i = 0; i < DK / 16; ++i)
+    for (int s = 0; s < KS; ++s)
 #pragma unroll
-        for (int r = 0; r < 4; ++r)
-            S[i][r] = p.state_in ? p.state_in[state_at + (size_t)(16 * i + 4 * kk + r) * p.value_dim] : 0.0f;
+        for (int a = 0; a < 2; ++a)
+#pragma unroll
+            for (int r = 0; r < 4; ++r)
+                S[s][a][r] = p.state_in ? p.state_in[state_at + (size_t)(32 * s + 4 * a + r) * p.value_dim] : 0.0f;
 
-    Raw8<T> kreg[PT][4], qreg[PT][4];
-    u32x4 oreg[PO];
-    auto fetch = [&](int c) __attribute__((always_inline)) {
-        const int n = min(C, sp.n - C * c);
+    // the tiles this wave owns; tile i has column steps 0 .. i / 2
+    auto tile_of = [&](int o) { return o == 0 ? ks : MT - 1 - ks; };
+    constexpr int kTri = KP == 4 ? 2 : OT == 2 ? 3 : 1;  // their matrix tiles
+    u32x4 kreg[PU], qreg[PU], tf[kTri][3], mf[kTri][3];
+    f32x4 sreg;
+    auto fetch_rows = [&](int c) __attribute__((always_inline)) {
+        if constexpr (NT == 1) {
+            // rows past the sequence's end: its last one, whose products meet
+            // zero factors
+            const int n = sp.n - C * c;
+            const uint16_t *kp = static_cast<const uint16_t *>(p.k) + (size_t)(sp.first + C * c) * p.k_stride + hk * DK;
+            const uint16_t *qp = static_cast<const uint16_t *>(p.q) + (size_t)(sp.first + C * c) * p.q_stride + hk * DK;
 #pragma unroll
-        for (int i = 0; i < PT; ++i) {
-            const int task = min(t + i * TPB, kTasks - 1), g8 = task % (DK / 8), quad = task / (DK / 8);
+            for (int i = 0; i < PU; ++i) {
+                const int u = t + i * kSeqT, row = min(u / (DK / 8), n - 1), at = 8 * (u % (DK / 8));
+                static_assert(NT > 1 || kUnits % kSeqT == 0, "whole units a thread");
+                kreg[i] = *reinterpret_cast<const u32x4 *>(kp + (size_t)row * p.k_stride + at);
+                qreg[i] = *reinterpret_cast<const u32x4 *>(qp + (size_t)row * p.q_stride + at);
+            }
+        } else {
+            const Planes<T, DK> &pl = planes[(place + c) * p.n_qk_heads + hk];
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const size_t row = (size_t)(sp.first + C * c + min(4 * quad + e, n - 1));
-                kreg[i][e].load(p.k, row * p.k_stride + hk * DK + 8 * g8);
-                qreg[i][e].load(p.q, row * p.q_stride + hk * DK + 8 * g8);
+            for (int i = 0; i < PU; ++i) {
+                const int u = min(t + i * kSeqT, kUnits - 1);
+                kreg[i] = reinterpret_cast<const u32x4 *>(pl.k)[u];
+                qreg[i] = reinterpret_cast<const u32x4 *>(pl.q)[u];
             }
         }
-        const u32x4 *src = reinterpret_cast<const u32x4 *>(ops + (size_t)c * p.n_v_heads);
-#pragma unroll
-        for (int i = 0; i < PO; ++i) oreg[i] = src[min(t + i * TPB, kOps - 1)];
+        const ChunkOps<C> &o = ops[(size_t)c * p.n_v_heads];
+        sreg = t < C ? o.sc[min(t, C - 1)] : o.dn;
     };
-    auto place = [&](int c) __attribute__((always_inline)) {
-        const int n = min(C, sp.n - C * c);
+    auto fetch_tri = [&](const u32x4(&m)[kTriTiles<C>][3][64], u32x4(&f)[kTri][3]) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < PT; ++i) {
-            const int task = t + i * TPB, g8 = task % (DK / 8), quad = task / (DK / 8);
-            if (kTasks % TPB != 0 && task >= kTasks) break;
-            // keys 8 g8 .. + 7: two groups of four of the 32-key step g8 / 4
-            const int u0 = 4 * (g8 / 4) + 2 * (g8 & 1), half = (g8 >> 1) & 1;
-            u32x4 kt[4][NT], qt[NT];
-#pragma unroll
-            for (int e = 0; e < 4; ++e) {
-                const int m = 4 * quad + e;
-                if (m >= n) {
-                    kreg[i][e].zero();
-                    qreg[i][e].zero();
+        for (int q = 0; q < 3; ++q) {
+            if constexpr (KP == 4) {
+                // tile ks: one step or two (a second load of the first, unused)
+                f[0][q] = m[tri_tile(ks, 0)][q][lane];
+                f[1][q] = m[tri_tile(ks, ks / 2)][q][lane];
+            } else {
+                f[0][q] = m[ks][q][lane];
+                if constexpr (OT == 2) {
+                    f[1][q] = m[tri_tile(3 - ks, 0)][q][lane];
+                    f[2][q] = m[tri_tile(3 - ks, 1)][q][lane];
                 }
-                kreg[i][e].terms(kt[e]);
-                qreg[i][e].terms(qt);
-#pragma unroll
-                for (int j = 0; j < NT; ++j)
-#pragma unroll
-                    for (int h = 0; h < 2; ++h) {
-                        const int u = (u0 + h) ^ (m & 7);
-                        reinterpret_cast<u32x2 *>(&lds.kr[j][m][u])[half] = (u32x2){kt[e][j][2 * h], kt[e][j][2 * h + 1]};
-                        reinterpret_cast<u32x2 *>(&lds.qr[j][m][u])[half] = (u32x2){qt[j][2 * h], qt[j][2 * h + 1]};
-                    }
             }
-            // tokens 4 quad .. + 3 of each key
-            const int ut = 4 * (quad / 8) + (quad & 3), th = (quad >> 2) & 1;
-#pragma unroll
-            for (int j = 0; j < NT; ++j)
-#pragma unroll
-                for (int e = 0; e < 8; ++e) {
-                    const uint32_t sel = e & 1 ? 0x07060302u : 0x05040100u;
-                    u32x2 v;
-                    v.x = __builtin_amdgcn_perm(kt[1][j][e / 2], kt[0][j][e / 2], sel);
-                    v.y = __builtin_amdgcn_perm(kt[3][j][e / 2], kt[2][j][e / 2], sel);
-                    const int key = 8 * g8 + e;
-                    const int u = ut ^ (C == 64 ? (key ^ (key >> 3)) & 7 : ((key >> 1) ^ (key >> 3)) & 3);
-                    reinterpret_cast<u32x2 *>(&lds.kt[j][key][u])[th] = v;
-                }
         }
-        u32x4 *dst = reinterpret_cast<u32x4 *>(&lds.ops);
+    };
+    auto put_units = [&](u32x4 *dst, const u32x4(&src)[PU]) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < PO; ++i)
-            if (t + i * TPB < kOps) dst[t + i * TPB] = oreg[i];
+        for (int i = 0; i < PU; ++i) {
+            const int u = t + i * kSeqT;
+            if (kUnits % kSeqT == 0 || u < kUnits) dst[u ^ ((u / (DK / 8)) & 7)] = src[i];
+        }
+    };
+    auto put_sc = [&](int c) __attribute__((always_inline)) {
+        if (t < kSc) lds.sc[c & 1][t] = sreg;
+    };
+    // this wave's rows of a matrix times the terms in LDS
+    auto tri_product = [&](const u32x4(&f)[kTri][3], const u32x4(&b)[JT][3][64], f32x4(&y)[OT])
+                           __attribute__((always_inline)) {
+        u32x4 bo[JT][3];
+#pragma unroll
+        for (int j = 0; j < JT; ++j)
+#pragma unroll
+            for (int q = 0; q < 3; ++q) bo[j][q] = b[j][q][lane];
+        f32x4 acc[kTri];
+#pragma unroll
+        for (int i = 0; i < kTri; ++i) acc[i] = zero;
+        for_terms<3, 3>([&](int m, int q) __attribute__((always_inline)) {
+            if constexpr (KP == 4) {
+                acc[0] = mfma_bf16(f[0][m], bo[0][q], acc[0]);
+                acc[1] = mfma_bf16(f[1][m], bo[1][q], acc[1]);
+            } else {
+                acc[0] = mfma_bf16(f[0][m], bo[0][q], acc[0]);
+                if constexpr (OT == 2) {
+                    acc[1] = mfma_bf16(f[1][m], bo[0][q], acc[1]);
+                    acc[2] = mfma_bf16(f[2][m], bo[1][q], acc[2]);
+                }
+            }
+        });
+        if constexpr (KP == 4) {
+            y[0] = ks < 2 ? acc[0] : acc[0] + acc[1];
+        } else {
+            y[0] = acc[0];
+            if constexpr (OT == 2) y[1] = acc[1] + acc[2];
+        }
+    };
+    // the terms of a tile's values, as half a B operand
+    auto put_terms = [&](u32x4(&dst)[JT][3][64], int tile, const f32x4 v) __attribute__((always_inline)) {
+        u32x2 e[3];
+        split3(v, e);
+#pragma unroll
+        for (int q = 0; q < 3; ++q) reinterpret_cast<u32x2 *>(&dst[tile >> 1][q][lane])[tile & 1] = e[q];
     };
 
-    if (chunks > 0) fetch(0);
+    if (chunks > 0) {
+        fetch_rows(0);
+        fetch_tri(ops[0].tf, tf);
+        fetch_tri(ops[0].mf, mf);
+        put_units(&lds.k[0][0][0][0], kreg);
+        put_units(&lds.q[0][0][0], qreg);
+        put_sc(0);
+    }
     for (int c = 0; c < chunks; ++c) {
-        const int n = min(C, sp.n - C * c);
+        const int n = min(C, sp.n - C * c), cn = min(c + 1, chunks - 1);
         const size_t row0 = (size_t)sp.first + (size_t)C * c;
-        if (c > 0) __syncthreads();
-        place(c);
-        __syncthreads();
-        f32x4 v[MT];
+        const auto &kc = lds.k[kBuf == 2 ? c & 1 : 0];
+        const f32x4 *sc = lds.sc[c & 1];
+        __syncthreads();  // this chunk's K, Q and scalars
+        float v[OT][4];
 #pragma unroll
-        for (int i = 0; i < MT; ++i)
+        for (int o = 0; o < OT; ++o)
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
-                const int m = 16 * i + 4 * kk + r;
-                const float x = T::get(p.v, (row0 + min(m, n - 1)) * p.v_stride + (size_t)hv * p.value_dim + col);
-                v[i][r] = m < n ? x : 0.0f;
+                const int m = min(16 * tile_of(o) + 4 * kk + r, n - 1);
+                v[o][r] = T::get(p.v, (row0 + m) * p.v_stride + (size_t)hv * p.value_dim + col);
             }
-        if (c + 1 < chunks) fetch(c + 1);
-        // K S and Q S
-        f32x4 ks[MT], qs[MT];
+        fetch_rows(cn);  // (the last chunk's again, unused)
+        {
+            // this wave's share of K S and Q S
+            f32x4 y[MT][2];
 #pragma unroll
-        for (int i = 0; i < MT; ++i) ks[i] = qs[i] = zero;
+            for (int i = 0; i < MT; ++i) y[i][0] = y[i][1] = zero;
 #pragma unroll
-        for (int s = 0; s < KS; ++s) {
-            u32x2 a[3], b[3];
-            split3(S[2 * s], a);
-            split3(S[2 * s + 1], b);
-            u32x4 sb[3];
-#pragma unroll
-            for (int q = 0; q < 3; ++q) sb[q] = (u32x4){a[q].x, a[q].y, b[q].x, b[q].y};
-#pragma unroll
-            for (int i = 0; i < MT; ++i) {
-                const int u = (4 * s + kk) ^ (li & 7);
-                u32x4 ka[NT], qa[NT];
-#pragma unroll
-                for (int j = 0; j < NT; ++j) {
-                    ka[j] = lds.kr[j][16 * i + li][u];
-                    qa[j] = lds.qr[j][16 * i + li][u];
-                }
-                ks[i] = mfma_terms<NT, 3>(ka, sb, ks[i]);
-                qs[i] = mfma_terms<NT, 3>(qa, sb, qs[i]);
-            }
-        }
-        // a step's 32 tokens as a B operand's terms, from accumulator tiles
-        auto as_operand = [&](const f32x4 *x, u32x4(&b)[JT][3]) __attribute__((always_inline)) {
-#pragma unroll
-            for (int j = 0; j < JT; ++j) {
+            for (int s = 0; s < KS; ++s) {
                 u32x2 lo[3], hi[3];
-                split3(x[2 * j], lo);
-                split3(x[2 * j + 1], hi);
+                split3(S[s][0], lo);
+                split3(S[s][1], hi);
+                u32x4 sb[3];
 #pragma unroll
-                for (int q = 0; q < 3; ++q) b[j][q] = (u32x4){lo[q].x, lo[q].y, hi[q].x, hi[q].y};
+                for (int q = 0; q < 3; ++q) sb[q] = (u32x4){lo[q].x, lo[q].y, hi[q].x, hi[q].y};
+                u32x4 ka[MT][NT], qa[MT][NT];
+                const int u = (key0 / 8 + 4 * s) ^ (li & 7);
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+#pragma unroll
+                    for (int j = 0; j < NT; ++j) {
+                        ka[i][j] = kc[j][16 * i + li][u];
+                        qa[i][j] = lds.q[j][16 * i + li][u];
+                    }
+                // eight chains in turn: a product that waits for the one
+                // before it takes twice its time
+                for_terms<NT, 3>([&](int a, int b) __attribute__((always_inline)) {
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) {
+                        y[i][0] = mfma_bf16(ka[i][a], sb[b], y[i][0]);
+                        y[i][1] = mfma_bf16(qa[i][a], sb[b], y[i][1]);
+                    }
+                });
             }
-        };
-        f32x4 fs[MT], d[MT];
-        u32x4 ob[JT][3];
+            auto owner = [&](int i) { return i < KP ? i : MT - 1 - i; };
 #pragma unroll
-        for (int i = 0; i < MT; ++i) {
-            f32x4 b;
+            for (int i = 0; i < MT; ++i)
+                if (owner(i) != ks) {
+                    const int at = ks < owner(i) ? ks : ks - 1;
+                    lds.part[ct][i][0][at][lane] = y[i][0];
+                    lds.part[ct][i][1][at][lane] = y[i][1];
+                }
+            __syncthreads();
+            // b, and what stands of o, of the owned tiles
+            f32x4 qs[OT], sw[OT];
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const f32x4 sc = lds.ops.sc[16 * i + 4 * kk + r];
-                b[r] = sc.y * (v[i][r] - sc.x * ks[i][r]);
-                qs[i][r] *= sc.z;
-                fs[i][r] = sc.w;
+            for (int o = 0; o < OT; ++o) {
+                const int tile = tile_of(o);
+                f32x4 kv = zero, qv = zero;
+#pragma unroll
+                for (int i = 0; i < MT; ++i)
+                    if (i == tile) {
+                        kv = y[i][0];
+                        qv = y[i][1];
+                    }
+#pragma unroll
+                for (int a = 0; a < KP - 1; ++a) {
+                    kv += lds.part[ct][tile][0][a][lane];
+                    qv += lds.part[ct][tile][1][a][lane];
+                }
+                f32x4 b;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const f32x4 e = sc[16 * tile + 4 * kk + r];
+                    b[r] = e.y * (v[o][r] - e.x * kv[r]);
+                    qs[o][r] = e.z * qv[r];
+                    sw[o][r] = e.w;
+                }
+                put_terms(lds.b[ct], tile, b);
             }
-            ks[i] = b;
+            __syncthreads();
+            f32x4 d[OT];
+            tri_product(tf, lds.b[ct], d);
+            fetch_tri(ops[(size_t)cn * p.n_v_heads].tf, tf);
+#pragma unroll
+            for (int o = 0; o < OT; ++o) {
+                put_terms(lds.df[ct][1], tile_of(o), d[o] * sw[o]);
+                put_terms(lds.df[ct][0], tile_of(o), d[o]);
+            }
+            __syncthreads();
+            // the update, and the rows of o
+            u32x4 fo[JT][3];
+#pragma unroll
+            for (int j = 0; j < JT; ++j)
+#pragma unroll
+                for (int q = 0; q < 3; ++q) fo[j][q] = lds.df[ct][1][j][q][lane];
+            f32x4 om[OT];
+            tri_product(mf, lds.df[ct][0], om);
+            fetch_tri(ops[(size_t)cn * p.n_v_heads].mf, mf);
+            const float dn = sc[C].x;
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                u32x4 a[2][JT][NT];
+#pragma unroll
+                for (int h = 0; h < 2; ++h)
+#pragma unroll
+                    for (int j = 0; j < JT; ++j)
+#pragma unroll
+                        for (int q = 0; q < NT; ++q) {
+                            // this lane's address: token + l % 16 / 4 of each
+                            // group of four, keys of group l % 4
+                            const int m = 32 * j + 4 * kk + (li >> 2);
+                            const int u = (ks * (DK / KP) / 8 + 4 * s + (li & 3)) ^ (m & 7);
+                            const u32x2 lo = read_transposed(reinterpret_cast<const u32x2 *>(&kc[q][m][u]) + h);
+                            const u32x2 hi = read_transposed(reinterpret_cast<const u32x2 *>(&kc[q][m + 16][u]) + h);
+                            a[h][j][q] = (u32x4){lo.x, lo.y, hi.x, hi.y};
+                        }
+                S[s][0] *= dn;
+                S[s][1] *= dn;
+                for_terms<NT, 3>([&](int e, int f) __attribute__((always_inline)) {
+#pragma unroll
+                    for (int j = 0; j < JT; ++j)
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) S[s][h] = mfma_bf16(a[h][j][e], fo[j][f], S[s][h]);
+                });
+            }
+#pragma unroll
+            for (int o = 0; o < OT; ++o)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int m = 16 * tile_of(o) + 4 * kk + r;
+                    if (m < n)
+                        T::put(p.o, (row0 + m) * p.o_stride + (size_t)hv * p.value_dim + col, qs[o][r] + om[o][r]);
+                }
         }
-        as_operand(ks, ob);
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
-            d[i] = zero;
-#pragma unroll
-            for (int j = 0; j <= i / 2; ++j) {
-                u32x4 a[3];
-#pragma unroll
-                for (int q = 0; q < 3; ++q) a[q] = lds.ops.tf[tri_tile(i, j)][q][lane];
-                d[i] = mfma_split(a, ob[j], d[i]);
-            }
-        }
-        as_operand(d, ob);
-#pragma unroll
-        for (int i = 0; i < MT; ++i) {
-#pragma unroll
-            for (int j = 0; j <= i / 2; ++j) {
-                u32x4 a[3];
-#pragma unroll
-                for (int q = 0; q < 3; ++q) a[q] = lds.ops.mf[tri_tile(i, j)][q][lane];
-                qs[i] = mfma_split(a, ob[j], qs[i]);
-            }
-#pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int m = 16 * i + 4 * kk + r;
-                if (m < n) T::put(p.o, (row0 + m) * p.o_stride + (size_t)hv * p.value_dim + col, qs[i][r]);
-            }
-#pragma unroll
-            for (int r = 0; r < 4; ++r) d[i][r] *= fs[i][r];
-        }
-        as_operand(d, ob);
-        const float dn = lds.ops.dn.x;
-#pragma unroll
-        for (int i = 0; i < DK / 16; ++i) {
-            const int key = 16 * i + li;
-            const int sw = C == 64 ? (key ^ (key >> 3)) & 7 : ((key >> 1) ^ (key >> 3)) & 3;
-            f32x4 s = S[i];
-#pragma unroll
-            for (int r = 0; r < 4; ++r) s[r] *= dn;
-#pragma unroll
-            for (int j = 0; j < JT; ++j) {
-                u32x4 a[NT];
-#pragma unroll
-                for (int q = 0; q < NT; ++q) a[q] = lds.kt[q][key][(4 * j + kk) ^ sw];
-                s = mfma_terms<NT, 3>(a, ob[j], s);
-            }
-            S[i] = s;
-        }
+        if (kBuf == 1) __syncthreads();
+        put_units(&lds.k[kBuf == 2 ? (c + 1) & 1 : 0][0][0][0], kreg);
+        put_units(&lds.q[0][0][0], qreg);
+        put_sc(c + 1);
     }
     if (p.state_out) {
 #pragma unroll
-        for (int i = 0; i < DK / 16; ++i)
+        for (int s = 0; s < KS; ++s)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) p.state_out[state_at + (size_t)(16 * i + 4 * kk + r) * p.value_dim] = S[i][r];
+            for (int a = 0; a < 2; ++a)
+#pragma unroll
+                for (int r = 0; r < 4; ++r)
+                    p.state_out[state_at + (size_t)(32 * s + 4 * a + r) * p.value_dim] = S[s][a][r];
     }
 }
 
@@ -672,11 +797,21 @@ __global__ __launch_bounds__(kT) void k_delta_step(GDNDelta p) {
 
 // ------------------------------------------------------------ host
 
+#ifndef SEQ_WIDE_FROM
+#define SEQ_WIDE_FROM 256
+#endif
 int chunk_of(const GDNDelta *a) { return a->dtype == GDN_DTYPE_BF16 ? kChunk<Bf16> : kChunk<Fp32>; }
-size_t ops_bytes(const GDNDelta *a) {
-    return a->dtype == GDN_DTYPE_BF16 ? sizeof(ChunkOps<64>) : sizeof(ChunkOps<32>);
-}
 size_t places(const GDNDelta *a) { return (size_t)a->n_tokens / chunk_of(a) + a->n_seqs; }
+// The chunks' matrices, then k and q in terms.
+size_t ops_bytes(const GDNDelta *a) {
+    return places(a) * a->n_v_heads *
+           (a->dtype == GDN_DTYPE_BF16 ? sizeof(ChunkOps<kChunk<Bf16>>) : sizeof(ChunkOps<kChunk<Fp32>>));
+}
+size_t plane_bytes(const GDNDelta *a) {
+    if (a->dtype == GDN_DTYPE_BF16) return 0;
+    const int terms = a->dtype == GDN_DTYPE_FP16 ? Fp16::kTerms : Fp32::kTerms;
+    return places(a) * a->n_qk_heads * 2 * terms * kChunk<Fp32> * a->key_dim * sizeof(uint16_t);
+}
 
 bool dim_ok(uint32_t d) { return d == 64 || d == 128 || d == 256; }
 
@@ -721,15 +856,28 @@ int launched(const char *who) {
     return 0;
 }
 
+template <class T, int DK, int KP>
+void launch_seq(const GDNDelta &a, const ChunkOps<kChunk<T>> *ops, const Planes<T, DK> *planes, hipStream_t s) {
+    constexpr int CT = kSeqWaves / KP;
+    const int pairs = (int)(a.n_seqs * a.n_v_heads), groups = (int)a.value_dim / (16 * CT);
+    hipLaunchKernelGGL((k_delta_seq<T, DK, KP>), dim3((unsigned)((pairs + 7) / 8 * 8 * groups)), dim3(kSeqT), 0, s, a,
+                       ops, planes, pairs);
+}
 template <class T, int DK>
 void launch_prefill(const GDNDelta &a, void *ws, hipStream_t s) {
-    constexpr int C = kChunk<T>, NW = 4;
+    constexpr int C = kChunk<T>;
     auto *ops = static_cast<ChunkOps<C> *>(ws);
+    auto *planes = reinterpret_cast<Planes<T, DK> *>(static_cast<char *>(ws) + ops_bytes(&a));
     if (a.n_tokens != 0)
-        hipLaunchKernelGGL((k_delta_prep<T, DK>), dim3((unsigned)places(&a), a.n_v_heads), dim3(4 * C), 0, s, a, ops);
-    const int pairs = (int)(a.n_seqs * a.n_v_heads), groups = (int)a.value_dim / (16 * NW);
-    hipLaunchKernelGGL((k_delta_seq<T, DK, NW>), dim3((unsigned)((pairs + 7) / 8 * 8 * groups)), dim3(64 * NW), 0, s,
-                       a, ops, pairs);
+        hipLaunchKernelGGL((k_delta_prep<T, DK>), dim3((unsigned)places(&a), a.n_v_heads), dim3(4 * C), 0, s, a, ops,
+                           planes);
+    if constexpr (C == 64 && DK >= 128) {
+        if ((size_t)a.n_seqs * a.n_v_heads * (a.value_dim / 64) < SEQ_WIDE_FROM) {
+            launch_seq<T, DK, 4>(a, ops, planes, s);
+            return;
+        }
+    }
+    launch_seq<T, DK, 2>(a, ops, planes, s);
 }
 template <class T>
 void launch_prefill_dk(const GDNDelta &a, void *ws, hipStream_t s) {
@@ -761,7 +909,7 @@ void launch_step_dk(const GDNDelta &a, hipStream_t s) {
 extern "C" size_t gdn_delta_prefill_workspace(const GDNDelta *args) {
     using namespace gdn::delta;
     if (args == nullptr || args->dtype < GDN_DTYPE_BF16 || args->dtype > GDN_DTYPE_FP32) return 0;
-    return places(args) * args->n_v_heads * ops_bytes(args);
+    return ops_bytes(args) + plane_bytes(args);
 }
 
 extern "C" int gdn_delta_prefill(const GDNDelta *args, void *workspace, size_t workspace_bytes, void *stream) {
