@@ -382,11 +382,9 @@ __global__ __launch_bounds__(4 * kChunk<T>) void k_delta_prep(GDNDelta p, ChunkO
 // 16-byte units XORed with the row's low bits (no two of eight rows on one
 // bank); the update reads K transposed (ds_read_b64_tr_b16).  The next chunk's
 // operands are loaded into registers meanwhile.
-constexpr int kSeqWaves = 8, kSeqT = 64 * kSeqWaves;
-
-template <class T, int DK, int KP>
+template <class T, int DK, int KP, int NW>
 struct SeqLds {
-    static constexpr int C = kChunk<T>, NT = T::kTerms, CT = kSeqWaves / KP, MT = C / 16, JT = C / 32;
+    static constexpr int C = kChunk<T>, NT = T::kTerms, CT = NW / KP, MT = C / 16, JT = C / 32;
     // K of two chunks where the LDS holds it: the next one's is written while
     // this one's is read, a barrier less
     static constexpr int kBuf = NT * C * DK >= 3 * 32 * 256 ? 1 : 2;
@@ -403,10 +401,11 @@ struct SeqLds {
     f32x4 sc[2][C + 1];  // a chunk's sc and, last, dn
 };
 
-template <class T, int DK, int KP>
-__global__ __launch_bounds__(kSeqT, 2) void k_delta_seq(GDNDelta p, const ChunkOps<kChunk<T>> *__restrict__ ops_all,
+template <class T, int DK, int KP, int NW>
+__global__ __launch_bounds__(64 * NW) void k_delta_seq(GDNDelta p, const ChunkOps<kChunk<T>> *__restrict__ ops_all,
                                                         const Planes<T, DK> *__restrict__ planes, int pairs) {
-    using Lds = SeqLds<T, DK, KP>;
+    using Lds = SeqLds<T, DK, KP, NW>;
+    constexpr int kSeqT = 64 * NW;
     constexpr int C = Lds::C, NT = Lds::NT, CT = Lds::CT, MT = Lds::MT, JT = Lds::JT, kBuf = Lds::kBuf;
     constexpr int KS = DK / 32 / KP;              // 32-key steps of a wave
     constexpr int OT = MT >= KP ? MT / KP : 1;    // token tiles a wave owns
@@ -415,7 +414,7 @@ __global__ __launch_bounds__(kSeqT, 2) void k_delta_seq(GDNDelta p, const ChunkO
     static_assert(KS >= 1 && MT >= KP, "whole steps and tiles");
     __shared__ Lds lds;
     const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
-    const int t = threadIdx.x, w = t >> 6, lane = t & 63, li = lane & 15, kk = lane >> 4;
+    const int t = threadIdx.x, w = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63, li = lane & 15, kk = lane >> 4;
     const int ks = w % KP, ct = w / KP;
     // the column groups of a (sequence, head) share its operands: one XCD's
     // (workgroups go to the eight in turn)
@@ -424,9 +423,11 @@ __global__ __launch_bounds__(kSeqT, 2) void k_delta_seq(GDNDelta p, const ChunkO
     if (pair >= pairs) return;
     const int seq = pair / (int)p.n_v_heads, hv = pair % (int)p.n_v_heads;
     const int hk = hv / (int)(p.n_v_heads / p.n_qk_heads);
-    const int slot = slot_of(p, seq);
+    const int slot = __builtin_amdgcn_readfirstlane(slot_of(p, seq));
     if (slot < 0) return;
-    const Span sp = span_of(p, seq);
+    Span sp = span_of(p, seq);
+    sp.first = __builtin_amdgcn_readfirstlane(sp.first);
+    sp.n = __builtin_amdgcn_readfirstlane(sp.n);
     const int chunks = (sp.n + C - 1) / C, col = 16 * (CT * cg + ct) + li;
     const size_t place = (size_t)place_of<C>(sp.first, seq);
     const ChunkOps<C> *ops = ops_all + place * p.n_v_heads + hv;
@@ -446,21 +447,28 @@ __global__ __launch_bounds__(kSeqT, 2) void k_delta_seq(GDNDelta p, const ChunkO
     // the tiles this wave owns; tile i has column steps 0 .. i / 2
     auto tile_of = [&](int o) { return o == 0 ? ks : MT - 1 - ks; };
     constexpr int kTri = KP == 4 ? 2 : OT == 2 ? 3 : 1;  // their matrix tiles
-    u32x4 kreg[PU], qreg[PU], tf[kTri][3], mf[kTri][3];
+    // rows at a chunk's uniform address, their offsets in 32 bits
+    constexpr uint32_t kSize = T::kWords / 2;
+    const uint32_t k_row = (uint32_t)p.k_stride * kSize, q_row = (uint32_t)p.q_stride * kSize,
+                   v_row = (uint32_t)p.v_stride * kSize, o_row = (uint32_t)p.o_stride * kSize;
+    auto rows_at = [&](const void *x, int64_t stride, int row, int head) __attribute__((always_inline)) {
+        return static_cast<const char *>(x) + ((size_t)row * stride + head) * kSize;
+    };
+    u32x4 kreg[PU], qreg[PU], tri[kTri][3];
     f32x4 sreg;
     auto fetch_rows = [&](int c) __attribute__((always_inline)) {
         if constexpr (NT == 1) {
             // rows past the sequence's end: its last one, whose products meet
             // zero factors
             const int n = sp.n - C * c;
-            const uint16_t *kp = static_cast<const uint16_t *>(p.k) + (size_t)(sp.first + C * c) * p.k_stride + hk * DK;
-            const uint16_t *qp = static_cast<const uint16_t *>(p.q) + (size_t)(sp.first + C * c) * p.q_stride + hk * DK;
+            const char *kp = rows_at(p.k, p.k_stride, sp.first + C * c, hk * DK),
+                       *qp = rows_at(p.q, p.q_stride, sp.first + C * c, hk * DK);
 #pragma unroll
             for (int i = 0; i < PU; ++i) {
-                const int u = t + i * kSeqT, row = min(u / (DK / 8), n - 1), at = 8 * (u % (DK / 8));
-                static_assert(NT > 1 || kUnits % kSeqT == 0, "whole units a thread");
-                kreg[i] = *reinterpret_cast<const u32x4 *>(kp + (size_t)row * p.k_stride + at);
-                qreg[i] = *reinterpret_cast<const u32x4 *>(qp + (size_t)row * p.q_stride + at);
+                static_assert(kUnits % kSeqT == 0, "whole units a thread");
+                const int u = t + i * kSeqT, row = min(u / (DK / 8), n - 1), at = 16 * (u % (DK / 8));
+                kreg[i] = *reinterpret_cast<const u32x4 *>(kp + (__umul24(row, k_row) + at));
+                qreg[i] = *reinterpret_cast<const u32x4 *>(qp + (__umul24(row, q_row) + at));
             }
         } else {
             const Planes<T, DK> &pl = planes[(place + c) * p.n_qk_heads + hk];
@@ -474,7 +482,8 @@ __global__ __launch_bounds__(kSeqT, 2) void k_delta_seq(GDNDelta p, const ChunkO
         const ChunkOps<C> &o = ops[(size_t)c * p.n_v_heads];
         sreg = t < C ? o.sc[min(t, C - 1)] : o.dn;
     };
-    auto fetch_tri = [&](const u32x4(&m)[kTriTiles<C>][3][64], u32x4(&f)[kTri][3]) __attribute__((always_inline)) {
+    auto fetch_tri = [&](const u32x4(&m)[kTriTiles<C>][3][64]) __attribute__((always_inline)) {
+        auto &f = tri;
 #pragma unroll
         for (int q = 0; q < 3; ++q) {
             if constexpr (KP == 4) {
@@ -500,34 +509,34 @@ __global__ __launch_bounds__(kSeqT, 2) void k_delta_seq(GDNDelta p, const ChunkO
     auto put_sc = [&](int c) __attribute__((always_inline)) {
         if (t < kSc) lds.sc[c & 1][t] = sreg;
     };
-    // this wave's rows of a matrix times the terms in LDS
-    auto tri_product = [&](const u32x4(&f)[kTri][3], const u32x4(&b)[JT][3][64], f32x4(&y)[OT])
-                           __attribute__((always_inline)) {
+    // this wave's rows of the matrix in `tri` times the terms in LDS, in a
+    // chain for each order of the terms' products
+    auto tri_product = [&](const u32x4(&b)[JT][3][64], f32x4(&y)[OT]) __attribute__((always_inline)) {
         u32x4 bo[JT][3];
 #pragma unroll
         for (int j = 0; j < JT; ++j)
 #pragma unroll
             for (int q = 0; q < 3; ++q) bo[j][q] = b[j][q][lane];
-        f32x4 acc[kTri];
+        f32x4 acc[kTri][3];
 #pragma unroll
-        for (int i = 0; i < kTri; ++i) acc[i] = zero;
+        for (int i = 0; i < kTri; ++i)
+#pragma unroll
+            for (int q = 0; q < 3; ++q) acc[i][q] = zero;
         for_terms<3, 3>([&](int m, int q) __attribute__((always_inline)) {
-            if constexpr (KP == 4) {
-                acc[0] = mfma_bf16(f[0][m], bo[0][q], acc[0]);
-                acc[1] = mfma_bf16(f[1][m], bo[1][q], acc[1]);
-            } else {
-                acc[0] = mfma_bf16(f[0][m], bo[0][q], acc[0]);
-                if constexpr (OT == 2) {
-                    acc[1] = mfma_bf16(f[1][m], bo[0][q], acc[1]);
-                    acc[2] = mfma_bf16(f[2][m], bo[1][q], acc[2]);
-                }
+#pragma unroll
+            for (int i = 0; i < kTri; ++i) {
+                const int j = KP == 4 ? i : i == 2;
+                acc[i][m + q] = mfma_bf16(tri[i][m], bo[j][q], acc[i][m + q]);
             }
         });
+        f32x4 sum[kTri];
+#pragma unroll
+        for (int i = 0; i < kTri; ++i) sum[i] = (acc[i][2] + acc[i][1]) + acc[i][0];
         if constexpr (KP == 4) {
-            y[0] = ks < 2 ? acc[0] : acc[0] + acc[1];
+            y[0] = ks < 2 ? sum[0] : sum[0] + sum[1];
         } else {
-            y[0] = acc[0];
-            if constexpr (OT == 2) y[1] = acc[1] + acc[2];
+            y[0] = sum[0];
+            if constexpr (OT == 2) y[1] = sum[1] + sum[2];
         }
     };
     // the terms of a tile's values, as half a B operand
@@ -540,15 +549,14 @@ __global__ __launch_bounds__(kSeqT, 2) void k_delta_seq(GDNDelta p, const ChunkO
 
     if (chunks > 0) {
         fetch_rows(0);
-        fetch_tri(ops[0].tf, tf);
-        fetch_tri(ops[0].mf, mf);
+        fetch_tri(ops[0].tf);
         put_units(&lds.k[0][0][0][0], kreg);
         put_units(&lds.q[0][0][0], qreg);
         put_sc(0);
     }
     for (int c = 0; c < chunks; ++c) {
         const int n = min(C, sp.n - C * c), cn = min(c + 1, chunks - 1);
-        const size_t row0 = (size_t)sp.first + (size_t)C * c;
+        const char *vp = rows_at(p.v, p.v_stride, sp.first + C * c, hv * (int)p.value_dim);
         const auto &kc = lds.k[kBuf == 2 ? c & 1 : 0];
         const f32x4 *sc = lds.sc[c & 1];
         __syncthreads();  // this chunk's K, Q and scalars
@@ -558,7 +566,7 @@ __global__ __launch_bounds__(kSeqT, 2) void k_delta_seq(GDNDelta p, const ChunkO
 #pragma unroll
             for (int r = 0; r < 4; ++r) {
                 const int m = min(16 * tile_of(o) + 4 * kk + r, n - 1);
-                v[o][r] = T::get(p.v, (row0 + m) * p.v_stride + (size_t)hv * p.value_dim + col);
+                v[o][r] = T::get(vp + (__umul24(m, v_row) + col * kSize), 0);
             }
         fetch_rows(cn);  // (the last chunk's again, unused)
         {
@@ -631,8 +639,8 @@ __global__ __launch_bounds__(kSeqT, 2) void k_delta_seq(GDNDelta p, const ChunkO
             }
             __syncthreads();
             f32x4 d[OT];
-            tri_product(tf, lds.b[ct], d);
-            fetch_tri(ops[(size_t)cn * p.n_v_heads].tf, tf);
+            tri_product(lds.b[ct], d);
+            fetch_tri(ops[(size_t)c * p.n_v_heads].mf);
 #pragma unroll
             for (int o = 0; o < OT; ++o) {
                 put_terms(lds.df[ct][1], tile_of(o), d[o] * sw[o]);
@@ -645,9 +653,10 @@ __global__ __launch_bounds__(kSeqT, 2) void k_delta_seq(GDNDelta p, const ChunkO
             for (int j = 0; j < JT; ++j)
 #pragma unroll
                 for (int q = 0; q < 3; ++q) fo[j][q] = lds.df[ct][1][j][q][lane];
-            f32x4 om[OT];
-            tri_product(mf, lds.df[ct][0], om);
-            fetch_tri(ops[(size_t)cn * p.n_v_heads].mf, mf);
+            // the next chunk's rows (q's place, b's until here, is free)
+            if (kBuf == 2) put_units(&lds.k[(c + 1) & 1][0][0][0], kreg);
+            put_units(&lds.q[0][0][0], qreg);
+            put_sc(c + 1);
             const float dn = sc[C].x;
 #pragma unroll
             for (int s = 0; s < KS; ++s) {
@@ -675,19 +684,31 @@ __global__ __launch_bounds__(kSeqT, 2) void k_delta_seq(GDNDelta p, const ChunkO
                         for (int h = 0; h < 2; ++h) S[s][h] = mfma_bf16(a[h][j][e], fo[j][f], S[s][h]);
                 });
             }
+            f32x4 om[OT];
+            tri_product(lds.df[ct][0], om);
+            fetch_tri(ops[(size_t)cn * p.n_v_heads].tf);
+            char *op = const_cast<char *>(rows_at(p.o, p.o_stride, sp.first + C * c, hv * (int)p.value_dim));
+            auto put_o = [&](int o, int r) __attribute__((always_inline)) {
+                const int m = 16 * tile_of(o) + 4 * kk + r;
+                T::put(op + (__umul24(m, o_row) + col * kSize), 0, qs[o][r] + om[o][r]);
+            };
+            if (n == C) {
 #pragma unroll
-            for (int o = 0; o < OT; ++o)
+                for (int o = 0; o < OT; ++o)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int m = 16 * tile_of(o) + 4 * kk + r;
-                    if (m < n)
-                        T::put(p.o, (row0 + m) * p.o_stride + (size_t)hv * p.value_dim + col, qs[o][r] + om[o][r]);
-                }
+                    for (int r = 0; r < 4; ++r) put_o(o, r);
+            } else {
+#pragma unroll
+                for (int o = 0; o < OT; ++o)
+#pragma unroll
+                    for (int r = 0; r < 4; ++r)
+                        if (16 * tile_of(o) + 4 * kk + r < n) put_o(o, r);
+            }
         }
-        if (kBuf == 1) __syncthreads();
-        put_units(&lds.k[kBuf == 2 ? (c + 1) & 1 : 0][0][0][0], kreg);
-        put_units(&lds.q[0][0][0], qreg);
-        put_sc(c + 1);
+        if (kBuf == 1) {
+            __syncthreads();
+            put_units(&lds.k[0][0][0][0], kreg);
+        }
     }
     if (p.state_out) {
 #pragma unroll
@@ -797,8 +818,9 @@ __global__ __launch_bounds__(kT) void k_delta_step(GDNDelta p) {
 
 // ------------------------------------------------------------ host
 
-#ifndef SEQ_WIDE_FROM
-#define SEQ_WIDE_FROM 256
+#ifndef SEQ_ONE
+#define SEQ_ONE 256
+#define SEQ_TWO 1000000
 #endif
 int chunk_of(const GDNDelta *a) { return a->dtype == GDN_DTYPE_BF16 ? kChunk<Bf16> : kChunk<Fp32>; }
 size_t places(const GDNDelta *a) { return (size_t)a->n_tokens / chunk_of(a) + a->n_seqs; }
@@ -840,6 +862,9 @@ int check(const char *who, const GDNDelta *a, bool packed) {
                          reinterpret_cast<uintptr_t>(a->state_in) | reinterpret_cast<uintptr_t>(a->state_out);
     if ((at & 15) != 0 || ((a->q_stride | a->k_stride | a->v_stride | a->o_stride) % per16) != 0)
         return refuse(who, "rows of q, k, v and o and the states start at multiples of 16 bytes");
+    // rows' offsets inside a chunk are formed in 24 x 24 bits
+    if (((a->q_stride | a->k_stride | a->v_stride | a->o_stride) * size) >> 24 != 0)
+        return refuse(who, "a row stride is negative or larger than 16 MB");
     const int64_t dq = (int64_t)a->n_qk_heads * a->key_dim, dv = (int64_t)a->n_v_heads * a->value_dim;
     if (a->n_tokens > 1 && (a->q_stride < dq || a->k_stride < dq || a->v_stride < dv || a->o_stride < dv ||
                             a->g_stride < (int64_t)a->n_v_heads))
@@ -856,12 +881,11 @@ int launched(const char *who) {
     return 0;
 }
 
-template <class T, int DK, int KP>
+template <class T, int DK, int KP, int NW>
 void launch_seq(const GDNDelta &a, const ChunkOps<kChunk<T>> *ops, const Planes<T, DK> *planes, hipStream_t s) {
-    constexpr int CT = kSeqWaves / KP;
-    const int pairs = (int)(a.n_seqs * a.n_v_heads), groups = (int)a.value_dim / (16 * CT);
-    hipLaunchKernelGGL((k_delta_seq<T, DK, KP>), dim3((unsigned)((pairs + 7) / 8 * 8 * groups)), dim3(kSeqT), 0, s, a,
-                       ops, planes, pairs);
+    const int pairs = (int)(a.n_seqs * a.n_v_heads), groups = (int)a.value_dim / (16 * (NW / KP));
+    hipLaunchKernelGGL((k_delta_seq<T, DK, KP, NW>), dim3((unsigned)((pairs + 7) / 8 * 8 * groups)), dim3(64 * NW), 0, s,
+                       a, ops, planes, pairs);
 }
 template <class T, int DK>
 void launch_prefill(const GDNDelta &a, void *ws, hipStream_t s) {
@@ -871,13 +895,15 @@ void launch_prefill(const GDNDelta &a, void *ws, hipStream_t s) {
     if (a.n_tokens != 0)
         hipLaunchKernelGGL((k_delta_prep<T, DK>), dim3((unsigned)places(&a), a.n_v_heads), dim3(4 * C), 0, s, a, ops,
                            planes);
+    const size_t tiles = (size_t)a.n_seqs * a.n_v_heads * (a.value_dim / 16);
     if constexpr (C == 64 && DK >= 128) {
-        if ((size_t)a.n_seqs * a.n_v_heads * (a.value_dim / 64) < SEQ_WIDE_FROM) {
-            launch_seq<T, DK, 4>(a, ops, planes, s);
-            return;
-        }
+        if (tiles <= SEQ_ONE) launch_seq<T, DK, 4, 4>(a, ops, planes, s);
+        else if (tiles <= SEQ_TWO) launch_seq<T, DK, 4, 8>(a, ops, planes, s);
+        else launch_seq<T, DK, 2, 8>(a, ops, planes, s);
+    } else {
+        if (tiles <= SEQ_ONE) launch_seq<T, DK, 2, 4>(a, ops, planes, s);
+        else launch_seq<T, DK, 2, 8>(a, ops, planes, s);
     }
-    launch_seq<T, DK, 2>(a, ops, planes, s);
 }
 template <class T>
 void launch_prefill_dk(const GDNDelta &a, void *ws, hipStream_t s) {
