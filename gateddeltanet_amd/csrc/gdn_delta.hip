@@ -4,7 +4,8 @@
 #include <hip/hip_runtime.h>
 
 #include <cstdio>
-#include <mutex>
+#include <type_traits>
+#include <utility>
 
 #include "gdn_amd.h"
 #include "gdn_device.h"
@@ -161,28 +162,103 @@ __device__ __forceinline__ int place_of(int first, int i) {
 
 // ------------------------------------------------------------ chunk operands
 
-// The matrices of one (chunk, value head): grid (places, value heads), a wave
-// for every 16 tokens.  With G the cumulative log decay inside the chunk and
-// k, q normalised:
+// 2^y, to about 2^-23 of it: the whole powers apart from the rest, which is
+// small enough for FP32.
+__device__ __forceinline__ float exp2_of(double y) {
+    const double n = __builtin_rint(y);
+    return __builtin_ldexpf(__builtin_amdgcn_exp2f((float)(y - n)), (int)n);
+}
+
+// The sums of a wave's values up to each lane, by data-parallel moves.
+template <int CTRL, int ROWS>
+__device__ __forceinline__ double moved(double v) {
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)u, CTRL, ROWS, 0xf, false),
+                   hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(u >> 32), CTRL, ROWS, 0xf, false);
+    return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
+}
+__device__ __forceinline__ double wave_scan(double v) {
+    v += moved<0x111, 0xf>(v);  // row_shr 1, 2, 4, 8
+    v += moved<0x112, 0xf>(v);
+    v += moved<0x114, 0xf>(v);
+    v += moved<0x118, 0xf>(v);
+    v += moved<0x142, 0xa>(v);  // row_bcast 15 into rows 1 and 3, 31 into 2 and 3
+    v += moved<0x143, 0xc>(v);
+    return v;
+}
+
+// Column `col` of the inverse of a unit lower triangular 16 x 16 block whose
+// row r is lane r's `row`: forward substitution, row M's values broadcast
+// over its 16 lanes (row_newbcast).
+template <int M, int... S>
+__device__ __forceinline__ float subst_row(const float (&row)[16], const float (&col)[16], float unit,
+                                           std::integer_sequence<int, S...>) {
+    float acc[2] = {unit, 0.0f};
+    ((acc[S & 1] = __builtin_fmaf(
+          -__builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, row[S]), 0x150 + M, 0xf, 0xf, true)),
+          col[S], acc[S & 1])),
+     ...);
+    return acc[0] + acc[1];
+}
+template <int... M>
+__device__ __forceinline__ void subst(const float (&row)[16], int li, float (&col)[16], std::integer_sequence<int, M...>) {
+    ((col[M] = subst_row<M>(row, col, li == M ? 1.0f : 0.0f, std::make_integer_sequence<int, M>())), ...);
+}
+
+// The matrices of one (chunk, value head): grid (places + 1, value heads), a
+// wave for every 16 tokens.  With G the cumulative log decay inside the chunk
+// and k, q normalised:
 //   L[m][s] = beta_m exp(G_m - G_s) (k_m . k_s), s < m;  T = (I + L)^-1
 //   M[m][s] = scale exp(G_m - G_s) (q_m . k_s), s <= m
-// T by 16 x 16 blocks: the diagonal ones by forward substitution (a lane a
-// column), then T[I][J] = -T[I][I] sum_{J <= K < I} L[I][K] T[K][J] by distance
-// from the diagonal on FP32 MFMAs.  G is summed in 64 bits: the weights are
-// exponentials of its differences.
+// G is summed in 64 bits: the weights are exponentials of its differences.
+// Wave w forms the products of k's 16-token tile w and of q's tile NW - 1 - w
+// with the tiles before them, five each of four waves' twenty.  T by 16 x 16
+// blocks: the diagonal ones by substitution, all in wave 0 (a lane a column)
+// while the others write M; then T_21 = -T_22 L_21 T_11 for the 32 x 32 blocks'
+// and for the whole's halves on FP32 MFMAs.
+// The last place's workgroup orders the sequences for k_delta_seq, longest
+// first, by counting their chunks in 256 steps.
 template <class T, int DK>
-__global__ __launch_bounds__(4 * kChunk<T>) void k_delta_prep(GDNDelta p, ChunkOps<kChunk<T>> *__restrict__ ops_all,
-                                                                Planes<T, DK> *__restrict__ planes) {
+__global__ __launch_bounds__(4 * kChunk<T>) void k_delta_prep(GDNDelta p, int *__restrict__ order,
+                                                              ChunkOps<kChunk<T>> *__restrict__ ops_all,
+                                                              Planes<T, DK> *__restrict__ planes) {
     constexpr int C = kChunk<T>, NW = C / 16, NT = T::kTerms, KS = DK / 32, LD = C + 4;
-    constexpr int kFrag = NW * KS * NT * 64 * 16, kMat = C * LD * 4;
-    __shared__ __attribute__((aligned(16))) unsigned char mem[kFrag > kMat ? kFrag : kMat];
-    __shared__ __attribute__((aligned(16))) float lm[C][LD], mm[C][LD];
+    struct Mats {
+        float t[C][LD], m[C][LD];
+    };
+    __shared__ __attribute__((aligned(16))) union {
+        u32x4 kb[NW][KS][NT][64];
+        Mats mat;  // once the products are formed
+        uint32_t bucket[256];
+    } mem;
+    __shared__ __attribute__((aligned(16))) float lm[C][LD];
     __shared__ double glog[C];
     __shared__ float ikn[C], iqn[C], bet[C];
-    u32x4(*kb)[KS][NT][64] = reinterpret_cast<u32x4(*)[KS][NT][64]>(mem);
-    float(*tm)[LD] = reinterpret_cast<float(*)[LD]>(mem);  // once the products are formed
-    const int t = threadIdx.x, w = t >> 6, lane = t & 63, li = lane & 15, kk = lane >> 4;
+    const int t = threadIdx.x, w = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63, li = lane & 15, kk = lane >> 4;
     const int place = blockIdx.x, hv = blockIdx.y, hk = hv / (int)(p.n_v_heads / p.n_qk_heads);
+    if (place == (int)gridDim.x - 1) {
+        if (hv != 0) return;
+        for (int i = t; i < 256; i += 64 * NW) mem.bucket[i] = 0;
+        __syncthreads();
+        auto step = [&](int i) { return 255 - min((span_of(p, i).n + C - 1) / C, 255); };
+        for (int i = t; i < (int)p.n_seqs; i += 64 * NW) atomicAdd(&mem.bucket[step(i)], 1u);
+        __syncthreads();
+        if (w == 0) {
+            u32x4 &own = *reinterpret_cast<u32x4 *>(&mem.bucket[4 * lane]);
+            const u32x4 n = own;
+            uint32_t at = n.x + n.y + n.z + n.w;
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) {
+                const uint32_t o = (uint32_t)__shfl_up((int)at, d);
+                if (lane >= d) at += o;
+            }
+            at -= n.x + n.y + n.z + n.w;
+            own = (u32x4){at, at + n.x, at + n.x + n.y, at + n.x + n.y + n.z};
+        }
+        __syncthreads();
+        for (int i = t; i < (int)p.n_seqs; i += 64 * NW) order[atomicAdd(&mem.bucket[step(i)], 1u)] = i;
+        return;
+    }
     int lo = 0, hi = (int)p.n_seqs - 1;
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
@@ -195,175 +271,218 @@ __global__ __launch_bounds__(4 * kChunk<T>) void k_delta_prep(GDNDelta p, ChunkO
     const int n = min(C, sp.n - m0), row0 = sp.first + m0;
     ChunkOps<C> &ops = ops_all[(size_t)place * p.n_v_heads + hv];
 
-    // wave w's 16 tokens, as A and as B fragments the same
+    // the wave's 16 tokens of k and of q, as A and as B fragments the same
+    const int wq = NW - 1 - w, km = 16 * w + li, qm = 16 * wq + li;
     Raw8<T> kr[KS], qr[KS];
-    const int mine = 16 * w + li;
+    float gv, bv;
     {
-        const size_t r = (size_t)(row0 + min(mine, n - 1));
-#pragma unroll
-        for (int s = 0; s < KS; ++s) kr[s].load(p.k, r * p.k_stride + hk * DK + 32 * s + 8 * kk);
-#pragma unroll
-        for (int s = 0; s < KS; ++s) qr[s].load(p.q, r * p.q_stride + hk * DK + 32 * s + 8 * kk);
-    }
-    if (t < 64) {
+        // (loads return in order: the gates first)
         const size_t r = (size_t)(row0 + min(t, n - 1)) * p.g_stride + hv;
-        // a decay of zero is one too small for FP32, so that differences of G
-        // stay numbers
-        float gv = p.g[r];
-        gv = gv < -1e5f ? -1e5f : gv;
-        double v = t < n ? (double)gv : 0.0;
+        gv = p.g[r];
+        bv = p.beta[r];
+        const size_t rk = (size_t)(row0 + min(km, n - 1)), rq = (size_t)(row0 + min(qm, n - 1));
 #pragma unroll
-        for (int d = 1; d < C; d <<= 1) {
-            const double o = __shfl_up(v, d);
-            if (lane >= d) v += o;
-        }
+        for (int s = 0; s < KS; ++s) kr[s].load(p.k, rk * p.k_stride + hk * DK + 32 * s + 8 * kk);
+#pragma unroll
+        for (int s = 0; s < KS; ++s) qr[s].load(p.q, rq * p.q_stride + hk * DK + 32 * s + 8 * kk);
+    }
+    if (w == 0) {
+        // a decay of zero is one too small for FP32, so that differences of G
+        // stay numbers; G in powers of two
+        gv = gv < -1e5f ? -1e5f : gv;
+        const double sum = wave_scan(t < n ? (double)gv * 1.44269504088896340736 : 0.0);
         if (t < C) {
-            glog[t] = v;
-            bet[t] = t < n ? p.beta[r] : 0.0f;
+            glog[t] = sum;
+            bet[t] = t < n ? bv : 0.0f;
         }
     }
-    u32x4 qa[KS][NT];
-    float kn = 0.0f, qn = 0.0f;
+    u32x4 qa[KS][NT], ka[KS][NT];
+    float kn[2] = {0.0f, 0.0f}, qn[2] = {0.0f, 0.0f};
 #pragma unroll
     for (int s = 0; s < KS; ++s) {
-        if (mine >= n) {
-            kr[s].zero();
-            qr[s].zero();
-        }
+        if (km >= n) kr[s].zero();
         float x[8];
         T::get8(kr[s].w, x);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) kn = __builtin_fmaf(x[e], x[e], kn);
+        for (int e = 0; e < 8; ++e) kn[e & 1] = __builtin_fmaf(x[e], x[e], kn[e & 1]);
+        kr[s].terms(ka[s]);
+#pragma unroll
+        for (int j = 0; j < NT; ++j) mem.kb[w][s][j][lane] = ka[s][j];
+    }
+#pragma unroll
+    for (int s = 0; s < KS; ++s) {
+        if (qm >= n) qr[s].zero();
+        float x[8];
         T::get8(qr[s].w, x);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) qn = __builtin_fmaf(x[e], x[e], qn);
-        u32x4 ka[NT];
-        kr[s].terms(ka);
+        for (int e = 0; e < 8; ++e) qn[e & 1] = __builtin_fmaf(x[e], x[e], qn[e & 1]);
         qr[s].terms(qa[s]);
+    }
+    if constexpr (NT > 1) {
+        if (hv % (int)(p.n_v_heads / p.n_qk_heads) == 0) {
+            Planes<T, DK> &pl = planes[(size_t)place * p.n_qk_heads + hk];
 #pragma unroll
-        for (int j = 0; j < NT; ++j) kb[w][s][j][lane] = ka[j];
-        if constexpr (NT > 1) {
-            if (hv % (int)(p.n_v_heads / p.n_qk_heads) == 0) {
-                Planes<T, DK> &pl = planes[(size_t)place * p.n_qk_heads + hk];
+            for (int s = 0; s < KS; ++s)
 #pragma unroll
                 for (int j = 0; j < NT; ++j) {
-                    *reinterpret_cast<u32x4 *>(&pl.k[j][mine][32 * s + 8 * kk]) = ka[j];
-                    *reinterpret_cast<u32x4 *>(&pl.q[j][mine][32 * s + 8 * kk]) = qa[s][j];
+                    *reinterpret_cast<u32x4 *>(&pl.k[j][km][32 * s + 8 * kk]) = ka[s][j];
+                    *reinterpret_cast<u32x4 *>(&pl.q[j][qm][32 * s + 8 * kk]) = qa[s][j];
                 }
-            }
         }
     }
-    kn += __shfl_xor(kn, 16);
-    qn += __shfl_xor(qn, 16);
-    kn += __shfl_xor(kn, 32);
-    qn += __shfl_xor(qn, 32);
+    auto norm = [&](const float(&x)[2]) __attribute__((always_inline)) {
+        float v = x[0] + x[1];
+        v += __shfl_xor(v, 16);
+        v += __shfl_xor(v, 32);
+        return p.l2norm ? 1.0f / __builtin_sqrtf(v + 1e-6f) : 1.0f;
+    };
+    const float kv = norm(kn), qv = norm(qn);
     if (kk == 0) {
-        ikn[mine] = p.l2norm ? 1.0f / __builtin_sqrtf(kn + 1e-6f) : 1.0f;
-        iqn[mine] = p.l2norm ? 1.0f / __builtin_sqrtf(qn + 1e-6f) : 1.0f;
+        ikn[km] = kv;
+        iqn[qm] = qv;
     }
     __syncthreads();
     if (t < C) {
-        const float eg = expf((float)glog[t]);
+        const float eg = exp2_of(glog[t]);
         const bool in = t < n;
         ops.sc[t] = (f32x4){in ? eg * ikn[t] : 0.0f, bet[t], in ? p.scale * (eg * iqn[t]) : 0.0f,
-                            in ? expf((float)(glog[n - 1] - glog[t])) * ikn[t] : 0.0f};
-        if (t == 0) ops.dn = (f32x4){expf((float)glog[n - 1]), 0.0f, 0.0f, 0.0f};
+                            in ? exp2_of(glog[n - 1] - glog[t]) * ikn[t] : 0.0f};
+        if (t == 0) ops.dn = (f32x4){exp2_of(glog[n - 1]), 0.0f, 0.0f, 0.0f};
     }
-    f32x4 gk[NW], gq[NW];
+    // products of the wave's tiles with those before them, then the weights;
+    // W: the wave, known where it is compiled
+    auto products = [&](auto W) __attribute__((always_inline)) {
+        constexpr int kW = decltype(W)::value, kQ = NW - 1 - kW, kMost = kW > kQ ? kW : kQ;
+        f32x4 gk[kW + 1], gq[kQ + 1];
 #pragma unroll
-    for (int s = 0; s < NW; ++s) gk[s] = gq[s] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
+        for (int c = 0; c <= kW; ++c) gk[c] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int s = 0; s < KS; ++s) {
-        u32x4 ka[NT];
+        for (int c = 0; c <= kQ; ++c) gq[c] = (f32x4){0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int j = 0; j < NT; ++j) ka[j] = kb[w][s][j][lane];
+        for (int s = 0; s < KS; ++s) {
+            u32x4 b[kMost + 1][NT];
 #pragma unroll
-        for (int c = 0; c < NW; ++c)
-            if (c <= w) {
-                u32x4 b[NT];
+            for (int c = 0; c <= kMost; ++c)
 #pragma unroll
-                for (int j = 0; j < NT; ++j) b[j] = kb[c][s][j][lane];
-                gk[c] = mfma_terms<NT, NT>(ka, b, gk[c]);
-                gq[c] = mfma_terms<NT, NT>(qa[s], b, gq[c]);
-            }
-    }
-    __syncthreads();  // k's fragments are read; T takes their place
+                for (int j = 0; j < NT; ++j) b[c][j] = mem.kb[c][s][j][lane];
+            for_terms<NT, NT>([&](int x, int y) __attribute__((always_inline)) {
 #pragma unroll
-    for (int s = 0; s < NW; ++s) {
-        const int c = 16 * s + li;
+                for (int c = 0; c <= kMost; ++c) {
+                    if (c <= kW) gk[c] = mfma_bf16(ka[s][x], b[c][y], gk[c]);
+                    if (c <= kQ) gq[c] = mfma_bf16(qa[s][x], b[c][y], gq[c]);
+                }
+            });
+        }
+        __syncthreads();  // k's fragments are read; T and M take their place
+        double gm[2][4];
+        float fk[4], fq[4];
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
-            const int m = 16 * w + 4 * kk + r;
-            float lv = 0.0f, mv = 0.0f;
-            if (m < n && c <= m) {
-                const float ratio = expf((float)(glog[m] - glog[c])) * ikn[c];
-                if (c < m) lv = bet[m] * (ratio * ikn[m]) * gk[s][r];
-                mv = p.scale * ((ratio * iqn[m]) * gq[s][r]);
-            }
-            lm[m][c] = lv;
-            mm[m][c] = mv;
-            tm[m][c] = 0.0f;
+            const int mk = 16 * kW + 4 * kk + r, mq = 16 * kQ + 4 * kk + r;
+            gm[0][r] = glog[mk];
+            gm[1][r] = glog[mq];
+            fk[r] = mk < n ? bet[mk] * ikn[mk] : 0.0f;
+            fq[r] = mq < n ? p.scale * iqn[mq] : 0.0f;
         }
+#pragma unroll
+        for (int c = 0; c <= kMost; ++c) {
+            const int col = 16 * c + li;
+            const double gc = glog[col];
+            const float ic = ikn[col];
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                if (c <= kW) {
+                    const float e = exp2_of(gm[0][r] - gc) * ic;
+                    lm[16 * kW + 4 * kk + r][col] = c < kW || li < 4 * kk + r ? (e * fk[r]) * gk[c][r] : 0.0f;
+                }
+                if (c <= kQ) {
+                    const float e = exp2_of(gm[1][r] - gc) * ic;
+                    mem.mat.m[16 * kQ + 4 * kk + r][col] = c < kQ || li <= 4 * kk + r ? (e * fq[r]) * gq[c][r] : 0.0f;
+                }
+            }
+        }
+        // above the diagonal, the other half of a 32-column step
+        if constexpr (kW % 2 == 0) {
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                mem.mat.t[16 * kW + 4 * kk + r][16 * (kW + 1) + li] = 0.0f;
+                mem.mat.m[16 * kW + 4 * kk + r][16 * (kW + 1) + li] = 0.0f;
+            }
+        }
+    };
+    if (w == 0) products(std::integral_constant<int, 0>());
+    else if (w == 1) products(std::integral_constant<int, 1>());
+    if constexpr (NW == 4) {
+        if (w == 2) products(std::integral_constant<int, 2>());
+        else if (w == 3) products(std::integral_constant<int, 3>());
     }
     __syncthreads();
-    auto write_terms = [&](const float(*src)[LD], u32x4(&dst)[kTriTiles<C>][3][64], int i, int j) {
+    float(&tm)[C][LD] = mem.mat.t;
+    auto write_terms = [&](const float(&src)[C][LD], u32x4(&dst)[kTriTiles<C>][3][64], int f) __attribute__((always_inline)) {
+        const int i = f < 2 ? f : 2 + (f - 2) / 2, j = f < 2 ? 0 : f & 1;
         u32x2 a[3], b[3];
         split3(*reinterpret_cast<const f32x4 *>(&src[16 * i + li][32 * j + 4 * kk]), a);
         split3(*reinterpret_cast<const f32x4 *>(&src[16 * i + li][32 * j + 16 + 4 * kk]), b);
 #pragma unroll
-        for (int q = 0; q < 3; ++q) dst[tri_tile(i, j)][q][lane] = (u32x4){a[q].x, a[q].y, b[q].x, b[q].y};
+        for (int q = 0; q < 3; ++q) dst[f][q][lane] = (u32x4){a[q].x, a[q].y, b[q].x, b[q].y};
     };
     if (w == 0) {
-        // lane 16 B + j: column j of the inverse of diagonal block B
         const int b0 = 16 * (kk < NW ? kk : 0);
-        float tc[16];
+        float row[16], tc[16];
 #pragma unroll
-        for (int m = 0; m < 16; ++m) {
-            float acc = m == li ? 1.0f : 0.0f;
+        for (int q = 0; q < 4; ++q) {
+            const f32x4 v = *reinterpret_cast<const f32x4 *>(&lm[b0 + li][b0 + 4 * q]);
 #pragma unroll
-            for (int s4 = 0; s4 < (m + 3) / 4; ++s4) {
-                const f32x4 lv = *reinterpret_cast<const f32x4 *>(&lm[b0 + m][b0 + 4 * s4]);
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                    if (4 * s4 + e < m) acc = __builtin_fmaf(lv[e], -tc[4 * s4 + e], acc);
-            }
-            tc[m] = acc;
+            for (int e = 0; e < 4; ++e) row[4 * q + e] = v[e];
         }
+        subst(row, li, tc, std::make_integer_sequence<int, 16>());
         if (kk < NW) {
 #pragma unroll
             for (int m = 0; m < 16; ++m) tm[b0 + m][b0 + li] = tc[m];
         }
     } else {
-        for (int f = w - 1; f < kTriTiles<C>; f += NW - 1) {
-            const int i = f < 2 ? f : 2 + (f - 2) / 2, j = f < 2 ? 0 : f & 1;
-            write_terms(mm, ops.mf, i, j);
-        }
+        for (int f = w - 1; f < kTriTiles<C>; f += NW - 1) write_terms(mem.mat.m, ops.mf, f);
     }
     __syncthreads();
+    // a tile's product A B over 16 columns, A from LDS, B's rows 4 kk + q of
+    // column l % 16 in registers (as a product's result lies)
+    auto times = [&](const float(&A)[C][LD], int i, int k, const f32x4 b, f32x4 c) __attribute__((always_inline)) {
+        const f32x4 a = *reinterpret_cast<const f32x4 *>(&A[16 * i + li][16 * k + 4 * kk]);
 #pragma unroll
-    for (int d = 1; d < NW; ++d) {
-        if (w + d < NW) {
-            const int I = w + d, J = w;
-            f32x4 y = {0.0f, 0.0f, 0.0f, 0.0f}, z = y;
-            for (int K = J; K < I; ++K) {
-                const f32x4 a = *reinterpret_cast<const f32x4 *>(&lm[16 * I + li][16 * K + 4 * kk]);
+        for (int q = 0; q < 4; ++q) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[q], b[q], c, 0, 0, 0);
+        return c;
+    };
+    auto tile = [&](int k, int j) __attribute__((always_inline)) {
+        f32x4 b;
 #pragma unroll
-                for (int q = 0; q < 4; ++q)
-                    y = __builtin_amdgcn_mfma_f32_16x16x4f32(a[q], tm[16 * K + 4 * kk + q][16 * J + li], y, 0, 0, 0);
-            }
-            // y's rows 4 kk + r are the B operand's k = 4 kk + q as they lie
-            const f32x4 a = *reinterpret_cast<const f32x4 *>(&tm[16 * I + li][16 * I + 4 * kk]);
+        for (int q = 0; q < 4; ++q) b[q] = tm[16 * k + 4 * kk + q][16 * j + li];
+        return b;
+    };
+    auto put = [&](int i, int j, const f32x4 z) __attribute__((always_inline)) {
 #pragma unroll
-            for (int q = 0; q < 4; ++q) z = __builtin_amdgcn_mfma_f32_16x16x4f32(a[q], y[q], z, 0, 0, 0);
-#pragma unroll
-            for (int r = 0; r < 4; ++r) tm[16 * I + 4 * kk + r][16 * J + li] = -z[r];
+        for (int r = 0; r < 4; ++r) tm[16 * i + 4 * kk + r][16 * j + li] = -z[r];
+    };
+    const f32x4 none = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (w % 2 == 0) put(w + 1, w, times(tm, w + 1, w + 1, times(lm, w + 1, w, tile(w, w), none), none));
+    __syncthreads();
+    if constexpr (NW == 4) {
+        // wave w: tile (2 + w / 2, w % 2) of the lower left half
+        const int j = w % 2;
+        const f32x4 b0 = tile(0, 0), b1 = j ? tile(1, 1) : tile(1, 0);
+        f32x4 y2 = none, y3 = none, z;
+        if (j == 0) y2 = times(lm, 2, 0, b0, none);
+        y2 = times(lm, 2, 1, b1, y2);
+        if (w < 2) {
+            z = times(tm, 2, 2, y2, none);
+        } else {
+            if (j == 0) y3 = times(lm, 3, 0, b0, none);
+            y3 = times(lm, 3, 1, b1, y3);
+            z = times(tm, 3, 3, y3, times(tm, 3, 2, y2, none));
         }
+        put(2 + w / 2, j, z);
         __syncthreads();
     }
-    for (int f = w; f < kTriTiles<C>; f += NW) {
-        const int i = f < 2 ? f : 2 + (f - 2) / 2, j = f < 2 ? 0 : f & 1;
-        write_terms(tm, ops.tf, i, j);
-    }
+    for (int f = w; f < kTriTiles<C>; f += NW) write_terms(tm, ops.tf, f);
 }
 
 // ------------------------------------------------------------ the sequences
@@ -371,64 +490,63 @@ __global__ __launch_bounds__(4 * kChunk<T>) void k_delta_prep(GDNDelta p, ChunkO
 // One (sequence, value head)'s chunks in order:
 //   d = T (beta (v - exp(G) K S));  o = exp(G) Q S + M d;
 //   S' = exp(G_{n-1}) S + K^T (exp(G_{n-1} - G) d)
-// A workgroup of eight waves has CT = 8 / KP tiles of 16 value columns, KP waves
-// a tile, a KP-th of the keys each.  A wave's state is the accumulator tiles of
-// its updates, and lies so that it is also the B operand of its K S and Q S: of
-// a 32-key step, lane l holds keys 8 (l / 16) .. + 7 of column l % 16, the first
-// four in one tile, the others in the next.  The KP waves' shares of K S and Q S
-// meet in LDS where the wave that owns a 16-token tile adds them; it forms b, its
-// rows of d and of o, and leaves the BF16 terms of b, d and the scaled d in LDS
-// as the B operands that the tile's waves read.  K and Q lie in LDS by rows, the
-// 16-byte units XORed with the row's low bits (no two of eight rows on one
-// bank); the update reads K transposed (ds_read_b64_tr_b16).  The next chunk's
-// operands are loaded into registers meanwhile.
-template <class T, int DK, int KP, int NW>
+// A workgroup has a tile of 16 value columns, its KP waves a KP-th of the keys
+// each.  A wave's state is the accumulator tiles of its updates, and lies
+// so that it is also the B operand of its K S and Q S: of a 32-key step, lane l
+// holds keys 8 (l / 16) .. + 7 of column l % 16, the first four in one tile, the
+// others in the next.  A wave's K and Q go through LDS areas of its own, which
+// turn whole lines of memory into A fragments (16-byte units XORed with the
+// row's low bits); the update reads K transposed (ds_read_b64_tr_b16).  The KP
+// waves' shares of K S and Q S meet in LDS where the wave that owns a 16-token
+// tile adds them; it forms b, its rows of d and of o, and leaves the BF16 terms
+// of b, d and the scaled d in LDS as the B operands that the tile's waves read.
+// Three barriers a chunk; every operand of the next chunk is on its way into
+// registers meanwhile, in the order of its use.
+template <class T, int DK, int KP>
 struct SeqLds {
-    static constexpr int C = kChunk<T>, NT = T::kTerms, CT = NW / KP, MT = C / 16, JT = C / 32;
-    // K of two chunks where the LDS holds it: the next one's is written while
-    // this one's is read, a barrier less
-    static constexpr int kBuf = NT * C * DK >= 3 * 32 * 256 ? 1 : 2;
-    u32x4 k[kBuf][NT][C][DK / 8];
-    // b's terms take q's place once Q S is formed
-    union {
-        u32x4 q[NT][C][DK / 8];
-        u32x4 b[CT][JT][3][64];
+    static constexpr int C = kChunk<T>, NT = T::kTerms, MT = C / 16, JT = C / 32, UR = DK / KP / 8;
+    // tiles a wave does not own, blocks of b that its area holds
+    static constexpr int kFor = KP <= MT ? MT - MT / KP : MT, kB = (3 * JT + KP - 1) / KP;
+    // q's area takes the shares for other waves and b once Q S is formed
+    union Area {
+        u32x4 q[NT][C][UR];
+        struct {
+            f32x4 part[kFor][2][64];  // [tile][K S, Q S]
+            u32x4 b[kB][64];          // block 3 step + term is the KP-th part's
+        };
     };
-    union {
-        f32x4 part[CT][MT][2][KP - 1][64];  // K S and Q S: [tile][token tile][which][wave but the owner]
-        u32x4 df[CT][2][JT][3][64];         // d and the scaled d: [tile][which][step][term]
-    };
-    f32x4 sc[2][C + 1];  // a chunk's sc and, last, dn
+    u32x4 k[KP][NT][C][UR];
+    Area area[KP];
+    u32x4 df[2][JT][3][64];  // d and the scaled d, B operands: [which][step][term]
 };
 
-template <class T, int DK, int KP, int NW>
-__global__ __launch_bounds__(64 * NW) void k_delta_seq(GDNDelta p, const ChunkOps<kChunk<T>> *__restrict__ ops_all,
-                                                        const Planes<T, DK> *__restrict__ planes, int pairs) {
-    using Lds = SeqLds<T, DK, KP, NW>;
-    constexpr int kSeqT = 64 * NW;
-    constexpr int C = Lds::C, NT = Lds::NT, CT = Lds::CT, MT = Lds::MT, JT = Lds::JT, kBuf = Lds::kBuf;
+template <class T, int DK, int KP>
+__global__ __launch_bounds__(64 * KP, sizeof(SeqLds<T, DK, KP>) <= (80 << 10) ? 2 : 1) void k_delta_seq(
+    GDNDelta p, const int *__restrict__ order, const ChunkOps<kChunk<T>> *__restrict__ ops_all,
+    const Planes<T, DK> *__restrict__ planes, int pairs) {
+    using Lds = SeqLds<T, DK, KP>;
+    constexpr int C = Lds::C, NT = Lds::NT, MT = Lds::MT, JT = Lds::JT;
     constexpr int KS = DK / 32 / KP;              // 32-key steps of a wave
-    constexpr int OT = MT >= KP ? MT / KP : 1;    // token tiles a wave owns
-    constexpr int kUnits = NT * C * DK / 8, PU = (kUnits + kSeqT - 1) / kSeqT;
-    constexpr int kSc = C + 1;
-    static_assert(KS >= 1 && MT >= KP, "whole steps and tiles");
+    constexpr int OT = MT >= KP ? MT / KP : 1;    // token tiles a wave owns (with KP > MT, the first MT waves)
+    constexpr int UR = Lds::UR;                   // 16-byte units of a row's keys
+    constexpr int kStage = NT * C * UR / 64;      // a lane's units of a chunk's K
+    static_assert(KS >= 1 && (UR == 4 || UR == 8) && (KP == 2 || KP == 4), "the layouts below");
     __shared__ Lds lds;
     const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
-    const int t = threadIdx.x, w = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63, li = lane & 15, kk = lane >> 4;
-    const int ks = w % KP, ct = w / KP;
+    const int t = threadIdx.x, ks = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63, li = lane & 15, kk = lane >> 4;
     // the column groups of a (sequence, head) share its operands: one XCD's
     // (workgroups go to the eight in turn)
-    const int groups = (int)p.value_dim / (16 * CT), x = blockIdx.x >> 3;
+    const int groups = (int)p.value_dim / 16, x = blockIdx.x >> 3;
     const int pair = (x / groups) * 8 + (blockIdx.x & 7), cg = x % groups;
     if (pair >= pairs) return;
-    const int seq = pair / (int)p.n_v_heads, hv = pair % (int)p.n_v_heads;
+    const int seq = order[pair / (int)p.n_v_heads], hv = pair % (int)p.n_v_heads;
     const int hk = hv / (int)(p.n_v_heads / p.n_qk_heads);
     const int slot = __builtin_amdgcn_readfirstlane(slot_of(p, seq));
     if (slot < 0) return;
     Span sp = span_of(p, seq);
     sp.first = __builtin_amdgcn_readfirstlane(sp.first);
     sp.n = __builtin_amdgcn_readfirstlane(sp.n);
-    const int chunks = (sp.n + C - 1) / C, col = 16 * (CT * cg + ct) + li;
+    const int chunks = (sp.n + C - 1) / C, col = 16 * cg + li;
     const size_t place = (size_t)place_of<C>(sp.first, seq);
     const ChunkOps<C> *ops = ops_all + place * p.n_v_heads + hv;
     // the state's key of tile a, register r of step s: key0 + 32 s + 4 a + r
@@ -444,9 +562,11 @@ __global__ __launch_bounds__(64 * NW) void k_delta_seq(GDNDelta p, const ChunkOp
             for (int r = 0; r < 4; ++r)
                 S[s][a][r] = p.state_in ? p.state_in[state_at + (size_t)(32 * s + 4 * a + r) * p.value_dim] : 0.0f;
 
-    // the tiles this wave owns; tile i has column steps 0 .. i / 2
-    auto tile_of = [&](int o) { return o == 0 ? ks : MT - 1 - ks; };
-    constexpr int kTri = KP == 4 ? 2 : OT == 2 ? 3 : 1;  // their matrix tiles
+    // the token tiles this wave owns; tile i's matrix rows have steps 0 .. i / 2
+    const bool owns = KP <= MT || ks < MT;
+    auto owner = [&](int i) { return i < KP ? i : MT - 1 - i; };
+    auto tile_of = [&](int o) { return o == 0 ? (owns ? ks : 0) : MT - 1 - ks; };
+    constexpr int kTri = C == 32 ? 1 : KP == 4 ? 2 : 3;  // their matrix tiles
     // rows at a chunk's uniform address, their offsets in 32 bits
     constexpr uint32_t kSize = T::kWords / 2;
     const uint32_t k_row = (uint32_t)p.k_stride * kSize, q_row = (uint32_t)p.q_stride * kSize,
@@ -454,69 +574,66 @@ __global__ __launch_bounds__(64 * NW) void k_delta_seq(GDNDelta p, const ChunkOp
     auto rows_at = [&](const void *x, int64_t stride, int row, int head) __attribute__((always_inline)) {
         return static_cast<const char *>(x) + ((size_t)row * stride + head) * kSize;
     };
-    u32x4 kreg[PU], qreg[PU], tri[kTri][3];
-    f32x4 sreg;
+    u32x4 kreg[kStage], qreg[kStage], tri[kTri][3];
+    f32x4 sc[OT][4];
+    float vv[OT][4], dn;
+    // rows past the sequence's end: its last one, whose products meet zero
+    // factors (the planes hold zeros there)
     auto fetch_rows = [&](int c) __attribute__((always_inline)) {
+        const int n = sp.n - C * c;
         if constexpr (NT == 1) {
-            // rows past the sequence's end: its last one, whose products meet
-            // zero factors
-            const int n = sp.n - C * c;
             const char *kp = rows_at(p.k, p.k_stride, sp.first + C * c, hk * DK),
                        *qp = rows_at(p.q, p.q_stride, sp.first + C * c, hk * DK);
 #pragma unroll
-            for (int i = 0; i < PU; ++i) {
-                static_assert(kUnits % kSeqT == 0, "whole units a thread");
-                const int u = t + i * kSeqT, row = min(u / (DK / 8), n - 1), at = 16 * (u % (DK / 8));
+            for (int i = 0; i < kStage; ++i) {
+                const int row = min((64 * i + lane) / UR, n - 1), at = 2 * ks * (DK / KP) + 16 * (lane % UR);
                 kreg[i] = *reinterpret_cast<const u32x4 *>(kp + (__umul24(row, k_row) + at));
                 qreg[i] = *reinterpret_cast<const u32x4 *>(qp + (__umul24(row, q_row) + at));
             }
         } else {
             const Planes<T, DK> &pl = planes[(place + c) * p.n_qk_heads + hk];
+            const int row = lane / UR, at = ks * (DK / KP) + 8 * (lane % UR);
 #pragma unroll
-            for (int i = 0; i < PU; ++i) {
-                const int u = min(t + i * kSeqT, kUnits - 1);
-                kreg[i] = reinterpret_cast<const u32x4 *>(pl.k)[u];
-                qreg[i] = reinterpret_cast<const u32x4 *>(pl.q)[u];
+            for (int i = 0; i < kStage; ++i) {
+                constexpr int kRows = 64 / UR;
+                const int j = i * kRows / C, r = i * kRows % C;
+                kreg[i] = *reinterpret_cast<const u32x4 *>(&pl.k[j][r + row][at]);
+                qreg[i] = *reinterpret_cast<const u32x4 *>(&pl.q[j][r + row][at]);
             }
         }
+    };
+    auto fetch_own = [&](int c) __attribute__((always_inline)) {
         const ChunkOps<C> &o = ops[(size_t)c * p.n_v_heads];
-        sreg = t < C ? o.sc[min(t, C - 1)] : o.dn;
+        const char *vp = rows_at(p.v, p.v_stride, sp.first + C * c, hv * (int)p.value_dim);
+        const int n = sp.n - C * c;
+#pragma unroll
+        for (int i = 0; i < OT; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int m = 16 * tile_of(i) + 4 * kk + r;
+                sc[i][r] = o.sc[m];
+                vv[i][r] = T::get(vp + (__umul24(min(m, n - 1), v_row) + col * kSize), 0);
+            }
     };
     auto fetch_tri = [&](const u32x4(&m)[kTriTiles<C>][3][64]) __attribute__((always_inline)) {
-        auto &f = tri;
 #pragma unroll
         for (int q = 0; q < 3; ++q) {
-            if constexpr (KP == 4) {
-                // tile ks: one step or two (a second load of the first, unused)
-                f[0][q] = m[tri_tile(ks, 0)][q][lane];
-                f[1][q] = m[tri_tile(ks, ks / 2)][q][lane];
+            if constexpr (C == 32) {
+                tri[0][q] = m[tile_of(0)][q][lane];
+            } else if constexpr (KP == 4) {
+                // tile ks: one step or two (else the first's again, unused)
+                tri[0][q] = m[tri_tile(ks, 0)][q][lane];
+                tri[1][q] = m[tri_tile(ks, ks / 2)][q][lane];
             } else {
-                f[0][q] = m[ks][q][lane];
-                if constexpr (OT == 2) {
-                    f[1][q] = m[tri_tile(3 - ks, 0)][q][lane];
-                    f[2][q] = m[tri_tile(3 - ks, 1)][q][lane];
-                }
+                tri[0][q] = m[ks][q][lane];
+                tri[1][q] = m[tri_tile(3 - ks, 0)][q][lane];
+                tri[2][q] = m[tri_tile(3 - ks, 1)][q][lane];
             }
         }
-    };
-    auto put_units = [&](u32x4 *dst, const u32x4(&src)[PU]) __attribute__((always_inline)) {
-#pragma unroll
-        for (int i = 0; i < PU; ++i) {
-            const int u = t + i * kSeqT;
-            if (kUnits % kSeqT == 0 || u < kUnits) dst[u ^ ((u / (DK / 8)) & 7)] = src[i];
-        }
-    };
-    auto put_sc = [&](int c) __attribute__((always_inline)) {
-        if (t < kSc) lds.sc[c & 1][t] = sreg;
     };
     // this wave's rows of the matrix in `tri` times the terms in LDS, in a
     // chain for each order of the terms' products
-    auto tri_product = [&](const u32x4(&b)[JT][3][64], f32x4(&y)[OT]) __attribute__((always_inline)) {
-        u32x4 bo[JT][3];
-#pragma unroll
-        for (int j = 0; j < JT; ++j)
-#pragma unroll
-            for (int q = 0; q < 3; ++q) bo[j][q] = b[j][q][lane];
+    auto tri_product = [&](const u32x4(&bo)[JT][3], f32x4(&y)[OT]) __attribute__((always_inline)) {
         f32x4 acc[kTri][3];
 #pragma unroll
         for (int i = 0; i < kTri; ++i)
@@ -525,93 +642,111 @@ __global__ __launch_bounds__(64 * NW) void k_delta_seq(GDNDelta p, const ChunkOp
         for_terms<3, 3>([&](int m, int q) __attribute__((always_inline)) {
 #pragma unroll
             for (int i = 0; i < kTri; ++i) {
-                const int j = KP == 4 ? i : i == 2;
+                const int j = kTri == 2 ? i : i == 2;
                 acc[i][m + q] = mfma_bf16(tri[i][m], bo[j][q], acc[i][m + q]);
             }
         });
         f32x4 sum[kTri];
 #pragma unroll
         for (int i = 0; i < kTri; ++i) sum[i] = (acc[i][2] + acc[i][1]) + acc[i][0];
-        if constexpr (KP == 4) {
-            y[0] = ks < 2 ? sum[0] : sum[0] + sum[1];
-        } else {
-            y[0] = sum[0];
-            if constexpr (OT == 2) y[1] = sum[1] + sum[2];
+        y[0] = sum[0];
+        if constexpr (kTri == 2) {
+            if (ks >= 2) y[0] += sum[1];
         }
+        if constexpr (kTri == 3) y[1] = sum[1] + sum[2];
     };
     // the terms of a tile's values, as half a B operand
-    auto put_terms = [&](u32x4(&dst)[JT][3][64], int tile, const f32x4 v) __attribute__((always_inline)) {
+    auto put_terms = [&](auto &&block, int tile, const f32x4 v) __attribute__((always_inline)) {
         u32x2 e[3];
         split3(v, e);
 #pragma unroll
-        for (int q = 0; q < 3; ++q) reinterpret_cast<u32x2 *>(&dst[tile >> 1][q][lane])[tile & 1] = e[q];
+        for (int q = 0; q < 3; ++q) reinterpret_cast<u32x2 *>(&block(3 * (tile >> 1) + q)[lane])[tile & 1] = e[q];
     };
+    auto b_block = [&](int i) -> u32x4(&)[64] { return lds.area[i / Lds::kB].b[i % Lds::kB]; };
+    auto d_block = [&](int i) -> u32x4(&)[64] { return lds.df[0][i / 3][i % 3]; };
+    auto f_block = [&](int i) -> u32x4(&)[64] { return lds.df[1][i / 3][i % 3]; };
+    auto get_operand = [&](auto &&block, u32x4(&b)[JT][3]) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < JT; ++j)
+#pragma unroll
+            for (int q = 0; q < 3; ++q) b[j][q] = block(3 * j + q)[lane];
+    };
+    // the place in wave a's area of its share of a tile
+    auto slot_in = [&](int a, int tile) {
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < MT; ++i) n += i < tile && owner(i) != a;
+        return n;
+    };
+    u32x4(&kl)[NT][C][UR] = lds.k[ks], (&ql)[NT][C][UR] = lds.area[ks].q;
+    auto put_rows = [&]() __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < kStage; ++i) {
+            constexpr int kRows = 64 / UR;
+            const int j = i * kRows / C, r = i * kRows % C + lane / UR;
+            const int u = (lane % UR) ^ (UR == 8 ? r & 7 : (r >> 1) & 3);
+            kl[j][r][u] = kreg[i];
+            ql[j][r][u] = qreg[i];
+        }
+    };
+    auto unit = [&](int row, int u) { return u ^ (UR == 8 ? row & 7 : (row >> 1) & 3); };
 
     if (chunks > 0) {
         fetch_rows(0);
-        fetch_tri(ops[0].tf);
-        put_units(&lds.k[0][0][0][0], kreg);
-        put_units(&lds.q[0][0][0], qreg);
-        put_sc(0);
+        if (owns) {
+            fetch_own(0);
+            fetch_tri(ops[0].tf);
+        }
+        dn = ops[0].dn.x;
+        put_rows();
     }
     for (int c = 0; c < chunks; ++c) {
-        const int n = min(C, sp.n - C * c), cn = min(c + 1, chunks - 1);
-        const char *vp = rows_at(p.v, p.v_stride, sp.first + C * c, hv * (int)p.value_dim);
-        const auto &kc = lds.k[kBuf == 2 ? c & 1 : 0];
-        const f32x4 *sc = lds.sc[c & 1];
-        __syncthreads();  // this chunk's K, Q and scalars
-        float v[OT][4];
+        const int n = min(C, sp.n - C * c), cn = min(c + 1, chunks - 1);  // (the last chunk is fetched again, unused)
+        const ChunkOps<C> &next_ops = ops[(size_t)cn * p.n_v_heads];
+        fetch_rows(cn);
+        // this wave's share of K S and Q S
+        f32x4 y[MT][2];
 #pragma unroll
-        for (int o = 0; o < OT; ++o)
+        for (int i = 0; i < MT; ++i) y[i][0] = y[i][1] = zero;
 #pragma unroll
-            for (int r = 0; r < 4; ++r) {
-                const int m = min(16 * tile_of(o) + 4 * kk + r, n - 1);
-                v[o][r] = T::get(vp + (__umul24(m, v_row) + col * kSize), 0);
-            }
-        fetch_rows(cn);  // (the last chunk's again, unused)
-        {
-            // this wave's share of K S and Q S
-            f32x4 y[MT][2];
+        for (int s = 0; s < KS; ++s) {
+            u32x2 lo[3], hi[3];
+            split3(S[s][0], lo);
+            split3(S[s][1], hi);
+            u32x4 sb[3];
 #pragma unroll
-            for (int i = 0; i < MT; ++i) y[i][0] = y[i][1] = zero;
-#pragma unroll
-            for (int s = 0; s < KS; ++s) {
-                u32x2 lo[3], hi[3];
-                split3(S[s][0], lo);
-                split3(S[s][1], hi);
-                u32x4 sb[3];
-#pragma unroll
-                for (int q = 0; q < 3; ++q) sb[q] = (u32x4){lo[q].x, lo[q].y, hi[q].x, hi[q].y};
-                u32x4 ka[MT][NT], qa[MT][NT];
-                const int u = (key0 / 8 + 4 * s) ^ (li & 7);
-#pragma unroll
-                for (int i = 0; i < MT; ++i)
-#pragma unroll
-                    for (int j = 0; j < NT; ++j) {
-                        ka[i][j] = kc[j][16 * i + li][u];
-                        qa[i][j] = lds.q[j][16 * i + li][u];
-                    }
-                // eight chains in turn: a product that waits for the one
-                // before it takes twice its time
-                for_terms<NT, 3>([&](int a, int b) __attribute__((always_inline)) {
-#pragma unroll
-                    for (int i = 0; i < MT; ++i) {
-                        y[i][0] = mfma_bf16(ka[i][a], sb[b], y[i][0]);
-                        y[i][1] = mfma_bf16(qa[i][a], sb[b], y[i][1]);
-                    }
-                });
-            }
-            auto owner = [&](int i) { return i < KP ? i : MT - 1 - i; };
+            for (int q = 0; q < 3; ++q) sb[q] = (u32x4){lo[q].x, lo[q].y, hi[q].x, hi[q].y};
+            u32x4 ka[MT][NT], qa[MT][NT];
 #pragma unroll
             for (int i = 0; i < MT; ++i)
-                if (owner(i) != ks) {
-                    const int at = ks < owner(i) ? ks : ks - 1;
-                    lds.part[ct][i][0][at][lane] = y[i][0];
-                    lds.part[ct][i][1][at][lane] = y[i][1];
+#pragma unroll
+                for (int j = 0; j < NT; ++j) {
+                    const int m = 16 * i + li;
+                    ka[i][j] = kl[j][m][unit(m, 4 * s + kk)];
+                    qa[i][j] = ql[j][m][unit(m, 4 * s + kk)];
                 }
-            __syncthreads();
-            // b, and what stands of o, of the owned tiles
-            f32x4 qs[OT], sw[OT];
+            // chains in turn: a product that waits for the one before it takes
+            // twice its time
+            for_terms<NT, 3>([&](int a, int b) __attribute__((always_inline)) {
+#pragma unroll
+                for (int i = 0; i < MT; ++i) {
+                    y[i][0] = mfma_bf16(ka[i][a], sb[b], y[i][0]);
+                    y[i][1] = mfma_bf16(qa[i][a], sb[b], y[i][1]);
+                }
+            });
+            __builtin_amdgcn_sched_barrier(0);  // a step's fragments at a time: registers
+        }
+#pragma unroll
+        for (int i = 0; i < MT; ++i)
+            if (owner(i) != ks) {
+                f32x4(&part)[2][64] = lds.area[ks].part[slot_in(ks, i)];
+                part[0][lane] = y[i][0];
+                part[1][lane] = y[i][1];
+            }
+        __syncthreads();
+        f32x4 qs[OT], sw[OT];
+        if (owns) {
+            // b, and what stands of o
 #pragma unroll
             for (int o = 0; o < OT; ++o) {
                 const int tile = tile_of(o);
@@ -623,70 +758,76 @@ __global__ __launch_bounds__(64 * NW) void k_delta_seq(GDNDelta p, const ChunkOp
                         qv = y[i][1];
                     }
 #pragma unroll
-                for (int a = 0; a < KP - 1; ++a) {
-                    kv += lds.part[ct][tile][0][a][lane];
-                    qv += lds.part[ct][tile][1][a][lane];
+                for (int a = 1; a < KP; ++a) {
+                    const int from = (ks + a) % KP;
+                    const f32x4(&part)[2][64] = lds.area[from].part[slot_in(from, tile)];
+                    kv += part[0][lane];
+                    qv += part[1][lane];
                 }
                 f32x4 b;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const f32x4 e = sc[16 * tile + 4 * kk + r];
-                    b[r] = e.y * (v[o][r] - e.x * kv[r]);
+                    const f32x4 e = sc[o][r];
+                    b[r] = e.y * (vv[o][r] - e.x * kv[r]);
                     qs[o][r] = e.z * qv[r];
                     sw[o][r] = e.w;
                 }
-                put_terms(lds.b[ct], tile, b);
+                put_terms(b_block, tile, b);
             }
-            __syncthreads();
+            fetch_own(cn);
+        }
+        __syncthreads();
+        if (owns) {
             f32x4 d[OT];
-            tri_product(lds.b[ct], d);
+            u32x4 bo[JT][3];
+            get_operand(b_block, bo);
+            tri_product(bo, d);
             fetch_tri(ops[(size_t)c * p.n_v_heads].mf);
 #pragma unroll
             for (int o = 0; o < OT; ++o) {
-                put_terms(lds.df[ct][1], tile_of(o), d[o] * sw[o]);
-                put_terms(lds.df[ct][0], tile_of(o), d[o]);
+                put_terms(f_block, tile_of(o), d[o] * sw[o]);
+                put_terms(d_block, tile_of(o), d[o]);
             }
-            __syncthreads();
-            // the update, and the rows of o
-            u32x4 fo[JT][3];
+        }
+        __syncthreads();
+        // the update, and the rows of o
+        u32x4 fo[JT][3];
+        get_operand(f_block, fo);
 #pragma unroll
-            for (int j = 0; j < JT; ++j)
+        for (int s = 0; s < KS; ++s) {
+            u32x4 a[2][JT][NT];
 #pragma unroll
-                for (int q = 0; q < 3; ++q) fo[j][q] = lds.df[ct][1][j][q][lane];
-            // the next chunk's rows (q's place, b's until here, is free)
-            if (kBuf == 2) put_units(&lds.k[(c + 1) & 1][0][0][0], kreg);
-            put_units(&lds.q[0][0][0], qreg);
-            put_sc(c + 1);
-            const float dn = sc[C].x;
+            for (int h = 0; h < 2; ++h)
 #pragma unroll
-            for (int s = 0; s < KS; ++s) {
-                u32x4 a[2][JT][NT];
+                for (int j = 0; j < JT; ++j)
 #pragma unroll
-                for (int h = 0; h < 2; ++h)
+                    for (int q = 0; q < NT; ++q) {
+                        // this lane's address: token + l % 16 / 4 of each group
+                        // of four, keys of group l % 4
+                        const int m = 32 * j + 4 * kk + (li >> 2), u = unit(m, 4 * s + (li & 3));
+                        const u32x2 lo = read_transposed(reinterpret_cast<const u32x2 *>(&kl[q][m][u]) + h);
+                        const u32x2 hi = read_transposed(
+                            reinterpret_cast<const u32x2 *>(&kl[q][m + 16][unit(m + 16, 4 * s + (li & 3))]) + h);
+                        a[h][j][q] = (u32x4){lo.x, lo.y, hi.x, hi.y};
+                    }
+            S[s][0] *= dn;
+            S[s][1] *= dn;
+            for_terms<NT, 3>([&](int e, int f) __attribute__((always_inline)) {
 #pragma unroll
-                    for (int j = 0; j < JT; ++j)
+                for (int j = 0; j < JT; ++j)
 #pragma unroll
-                        for (int q = 0; q < NT; ++q) {
-                            // this lane's address: token + l % 16 / 4 of each
-                            // group of four, keys of group l % 4
-                            const int m = 32 * j + 4 * kk + (li >> 2);
-                            const int u = (ks * (DK / KP) / 8 + 4 * s + (li & 3)) ^ (m & 7);
-                            const u32x2 lo = read_transposed(reinterpret_cast<const u32x2 *>(&kc[q][m][u]) + h);
-                            const u32x2 hi = read_transposed(reinterpret_cast<const u32x2 *>(&kc[q][m + 16][u]) + h);
-                            a[h][j][q] = (u32x4){lo.x, lo.y, hi.x, hi.y};
-                        }
-                S[s][0] *= dn;
-                S[s][1] *= dn;
-                for_terms<NT, 3>([&](int e, int f) __attribute__((always_inline)) {
-#pragma unroll
-                    for (int j = 0; j < JT; ++j)
-#pragma unroll
-                        for (int h = 0; h < 2; ++h) S[s][h] = mfma_bf16(a[h][j][e], fo[j][f], S[s][h]);
-                });
-            }
+                    for (int h = 0; h < 2; ++h) S[s][h] = mfma_bf16(a[h][j][e], fo[j][f], S[s][h]);
+            });
+        }
+        dn = next_ops.dn.x;
+        // (q's area, the shares' and b's until here, is free)
+        put_rows();
+        if (owns) {
             f32x4 om[OT];
-            tri_product(lds.df[ct][0], om);
-            fetch_tri(ops[(size_t)cn * p.n_v_heads].tf);
+            u32x4 bo[JT][3];
+            get_operand(d_block, bo);
+            tri_product(bo, om);
+            fetch_tri(next_ops.tf);
             char *op = const_cast<char *>(rows_at(p.o, p.o_stride, sp.first + C * c, hv * (int)p.value_dim));
             auto put_o = [&](int o, int r) __attribute__((always_inline)) {
                 const int m = 16 * tile_of(o) + 4 * kk + r;
@@ -704,10 +845,6 @@ __global__ __launch_bounds__(64 * NW) void k_delta_seq(GDNDelta p, const ChunkOp
                     for (int r = 0; r < 4; ++r)
                         if (16 * tile_of(o) + 4 * kk + r < n) put_o(o, r);
             }
-        }
-        if (kBuf == 1) {
-            __syncthreads();
-            put_units(&lds.k[0][0][0][0], kreg);
         }
     }
     if (p.state_out) {
@@ -818,13 +955,10 @@ __global__ __launch_bounds__(kT) void k_delta_step(GDNDelta p) {
 
 // ------------------------------------------------------------ host
 
-#ifndef SEQ_ONE
-#define SEQ_ONE 256
-#define SEQ_TWO 1000000
-#endif
 int chunk_of(const GDNDelta *a) { return a->dtype == GDN_DTYPE_BF16 ? kChunk<Bf16> : kChunk<Fp32>; }
 size_t places(const GDNDelta *a) { return (size_t)a->n_tokens / chunk_of(a) + a->n_seqs; }
-// The chunks' matrices, then k and q in terms.
+// The workspace: the sequences' order, the chunks' matrices, k and q in terms.
+size_t order_bytes(const GDNDelta *a) { return ((size_t)a->n_seqs * sizeof(int) + 255) / 256 * 256; }
 size_t ops_bytes(const GDNDelta *a) {
     return places(a) * a->n_v_heads *
            (a->dtype == GDN_DTYPE_BF16 ? sizeof(ChunkOps<kChunk<Bf16>>) : sizeof(ChunkOps<kChunk<Fp32>>));
@@ -881,29 +1015,22 @@ int launched(const char *who) {
     return 0;
 }
 
-template <class T, int DK, int KP, int NW>
-void launch_seq(const GDNDelta &a, const ChunkOps<kChunk<T>> *ops, const Planes<T, DK> *planes, hipStream_t s) {
-    const int pairs = (int)(a.n_seqs * a.n_v_heads), groups = (int)a.value_dim / (16 * (NW / KP));
-    hipLaunchKernelGGL((k_delta_seq<T, DK, KP, NW>), dim3((unsigned)((pairs + 7) / 8 * 8 * groups)), dim3(64 * NW), 0, s,
-                       a, ops, planes, pairs);
+template <class T, int DK, int KP>
+void launch_seq(const GDNDelta &a, const int *order, const ChunkOps<kChunk<T>> *ops, const Planes<T, DK> *planes, hipStream_t s) {
+    const int pairs = (int)(a.n_seqs * a.n_v_heads), groups = (int)a.value_dim / 16;
+    hipLaunchKernelGGL((k_delta_seq<T, DK, KP>), dim3((unsigned)((pairs + 7) / 8 * 8 * groups)),
+                       dim3(64 * KP), 0, s, a, order, ops, planes, pairs);
 }
 template <class T, int DK>
 void launch_prefill(const GDNDelta &a, void *ws, hipStream_t s) {
-    constexpr int C = kChunk<T>;
-    auto *ops = static_cast<ChunkOps<C> *>(ws);
-    auto *planes = reinterpret_cast<Planes<T, DK> *>(static_cast<char *>(ws) + ops_bytes(&a));
-    if (a.n_tokens != 0)
-        hipLaunchKernelGGL((k_delta_prep<T, DK>), dim3((unsigned)places(&a), a.n_v_heads), dim3(4 * C), 0, s, a, ops,
-                           planes);
-    const size_t tiles = (size_t)a.n_seqs * a.n_v_heads * (a.value_dim / 16);
-    if constexpr (C == 64 && DK >= 128) {
-        if (tiles <= SEQ_ONE) launch_seq<T, DK, 4, 4>(a, ops, planes, s);
-        else if (tiles <= SEQ_TWO) launch_seq<T, DK, 4, 8>(a, ops, planes, s);
-        else launch_seq<T, DK, 2, 8>(a, ops, planes, s);
-    } else {
-        if (tiles <= SEQ_ONE) launch_seq<T, DK, 2, 4>(a, ops, planes, s);
-        else launch_seq<T, DK, 2, 8>(a, ops, planes, s);
-    }
+    constexpr int C = kChunk<T>, KP = DK == 64 ? 2 : 4;
+    char *mem = static_cast<char *>(ws);
+    int *order = reinterpret_cast<int *>(mem);
+    auto *ops = reinterpret_cast<ChunkOps<C> *>(mem + order_bytes(&a));
+    auto *planes = reinterpret_cast<Planes<T, DK> *>(mem + order_bytes(&a) + ops_bytes(&a));
+    hipLaunchKernelGGL((k_delta_prep<T, DK>), dim3((unsigned)places(&a) + 1, a.n_v_heads), dim3(4 * C), 0, s, a, order,
+                       ops, planes);
+    launch_seq<T, DK, KP>(a, order, ops, planes, s);
 }
 template <class T>
 void launch_prefill_dk(const GDNDelta &a, void *ws, hipStream_t s) {
@@ -935,7 +1062,7 @@ void launch_step_dk(const GDNDelta &a, hipStream_t s) {
 extern "C" size_t gdn_delta_prefill_workspace(const GDNDelta *args) {
     using namespace gdn::delta;
     if (args == nullptr || args->dtype < GDN_DTYPE_BF16 || args->dtype > GDN_DTYPE_FP32) return 0;
-    return ops_bytes(args) + plane_bytes(args);
+    return order_bytes(args) + ops_bytes(args) + plane_bytes(args);
 }
 
 extern "C" int gdn_delta_prefill(const GDNDelta *args, void *workspace, size_t workspace_bytes, void *stream) {

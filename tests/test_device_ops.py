@@ -74,13 +74,16 @@ def test_delta_places_hold_every_chunk(dtype, chunk):
 
     rng = random.Random(3)
     lib = _lib.load()
-    one = lib.gdn_delta_prefill_workspace(ctypes.byref(delta(dtype=dtype, n_tokens=0, n_seqs=1)))
+
+    def bytes_for(n_tokens, n_seqs):
+        return lib.gdn_delta_prefill_workspace(ctypes.byref(delta(dtype=dtype, n_tokens=n_tokens, n_seqs=n_seqs)))
+
+    one = bytes_for(chunk, 1) - bytes_for(0, 1)
     for _ in range(200):
         lens = [rng.choice([0, 1, chunk - 1, chunk, chunk + 1, rng.randint(0, 5 * chunk)]) for _ in range(rng.randint(1, 9))]
         start = rng.randint(0, chunk)
         total = start + sum(lens) + rng.randint(0, 70)
-        places = lib.gdn_delta_prefill_workspace(
-            ctypes.byref(delta(dtype=dtype, n_tokens=total, n_seqs=len(lens)))) // one
+        places = bytes_for(total, len(lens)) // one  # (the sequences' order is less than a place)
         used, first = [], start
         for i, n in enumerate(lens):
             used += [first // chunk + i + c for c in range(-(-n // chunk))]
