@@ -169,24 +169,6 @@ __device__ __forceinline__ float exp2_of(double y) {
     return __builtin_ldexpf(__builtin_amdgcn_exp2f((float)(y - n)), (int)n);
 }
 
-// The sums of a wave's values up to each lane, by data-parallel moves.
-template <int CTRL, int ROWS>
-__device__ __forceinline__ double moved(double v) {
-    const uint64_t u = __builtin_bit_cast(uint64_t, v);
-    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)u, CTRL, ROWS, 0xf, false),
-                   hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(u >> 32), CTRL, ROWS, 0xf, false);
-    return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
-}
-__device__ __forceinline__ double wave_scan(double v) {
-    v += moved<0x111, 0xf>(v);  // row_shr 1, 2, 4, 8
-    v += moved<0x112, 0xf>(v);
-    v += moved<0x114, 0xf>(v);
-    v += moved<0x118, 0xf>(v);
-    v += moved<0x142, 0xa>(v);  // row_bcast 15 into rows 1 and 3, 31 into 2 and 3
-    v += moved<0x143, 0xc>(v);
-    return v;
-}
-
 // Column `col` of the inverse of a unit lower triangular 16 x 16 block whose
 // row r is lane r's `row`: forward substitution, row M's values broadcast
 // over its 16 lanes (row_newbcast).
@@ -290,7 +272,7 @@ __global__ __launch_bounds__(4 * kChunk<T>) void k_delta_prep(GDNDelta p, int *_
         // a decay of zero is one too small for FP32, so that differences of G
         // stay numbers; G in powers of two
         gv = gv < -1e5f ? -1e5f : gv;
-        const double sum = wave_scan(t < n ? (double)gv * 1.44269504088896340736 : 0.0);
+        const double sum = wave_scan64(t < n ? (double)gv * 1.44269504088896340736 : 0.0);
         if (t < C) {
             glog[t] = sum;
             bet[t] = t < n ? bv : 0.0f;
@@ -734,7 +716,13 @@ __global__ __launch_bounds__(64 * KP, sizeof(SeqLds<T, DK, KP>) <= (80 << 10) ? 
                     y[i][1] = mfma_bf16(qa[i][a], sb[b], y[i][1]);
                 }
             });
-            __builtin_amdgcn_sched_barrier(0);  // a step's fragments at a time: registers
+        }
+        // a load between two products each: issued in a row they hold the wave
+        // for 900 cycles
+#pragma unroll
+        for (int i = 0; i < 2 * kStage; ++i) {
+            __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
         }
 #pragma unroll
         for (int i = 0; i < MT; ++i)

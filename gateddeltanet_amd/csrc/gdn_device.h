@@ -178,6 +178,28 @@ __device__ __forceinline__ uint32_t wave_reduce64(uint32_t v, Op op) {
     return v;
 }
 
+// The sums of a wave's values up to and with each lane's, by data-parallel
+// moves (row_shr 1, 2, 4, 8, row_bcast 15 into rows 1 and 3, 31 into 2 and 3);
+// lane 63 has the whole.
+template <int CTRL, int ROWS, class V>
+__device__ __forceinline__ V wave_moved(V v) {
+    static_assert(sizeof(V) == 8, "two registers");
+    const uint64_t u = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)u, CTRL, ROWS, 0xf, false),
+                   hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(u >> 32), CTRL, ROWS, 0xf, false);
+    return __builtin_bit_cast(V, ((uint64_t)hi << 32) | lo);
+}
+template <class V>  // double or uint64_t
+__device__ __forceinline__ V wave_scan64(V v) {
+    v += wave_moved<0x111, 0xf>(v);
+    v += wave_moved<0x112, 0xf>(v);
+    v += wave_moved<0x114, 0xf>(v);
+    v += wave_moved<0x118, 0xf>(v);
+    v += wave_moved<0x142, 0xa>(v);
+    v += wave_moved<0x143, 0xc>(v);
+    return v;
+}
+
 // Balanced pairwise sum of the 64 values (the lower six levels of
 // gdn_tree_reduce_256); FP32 addition is commutative, so the sums equal an
 // XOR butterfly's.

@@ -144,109 +144,106 @@ __global__ __launch_bounds__(kPT) void k_process(GDNLogits p) {
 
 // A workgroup a row.  Weights are whole numbers of 2^-shift, so counts and
 // sums over the row are the same in any order.  The kept tokens are the first
-// ones of the ranking up to a border (key, index): one histogram over kBins
+// ones of the ranking up to a border (logit, index): one histogram over kBins
 // steps of 1 / 32 in (max - x) / temperature -- what lies past them has no
 // weight -- gives the step the border is in, and the step's tokens, usually
 // some tens, are ranked against each other in LDS.  More than fit there go
-// through histograms of 11, 11 and 10 bits of their keys.
+// through histograms of 10 bits of their keys at a time.  A row that fits stays
+// in LDS from its one reading on (HELD); what each pass then costs is its
+// instructions, so the FP64 weights are formed only for the tokens that need
+// them: a token's bounds are compared in FP32 first.
 constexpr int kST = 1024, kBins = kST, kWaves = kST / 64;
-constexpr int kList = 1024;           // tokens of a step that are ranked directly
-constexpr int kRadix = 2048;          // bins of a key histogram
-constexpr int kCells = (1 << 20) / 256;  // pieces of the longest row
+constexpr int kList = 512;             // tokens of a step that are ranked directly
+constexpr int kHeldBytes = 128 << 10;  // of a row in LDS
+constexpr int kMostVocab = 1 << 20;
 
 // The 32-bit key of x that grows as x falls (x not NaN; the zeros are equal).
 __device__ __forceinline__ uint32_t fall_key(float x) {
     const uint32_t u = f2u(x + 0.0f);
     return u & 0x80000000u ? u : ~u & 0x7fffffffu;
 }
-
-// exp(-x), x >= 0, to 2 units of 2^-24 (0 for infinity and NaN): the base-2
-// exponential with the rounding error of its argument made good.
-__device__ __forceinline__ float exp_neg(float x) {
-    constexpr float kL = 1.44269502f, kLo = 1.92596299e-8f;  // log2(e)
-    const float y = x * kL, e = __builtin_fmaf(x, kLo, __builtin_fmaf(x, kL, -y));
-    const float p = __builtin_amdgcn_exp2f(-y);
-    return y < 126.0f ? __builtin_fmaf(p, -0.693147181f * e, p) : 0.0f;
-}
-
-__device__ __forceinline__ uint64_t shfl_up64(uint64_t v, int d) {
-    return ((uint64_t)(uint32_t)__shfl_up((int)(v >> 32), d) << 32) | (uint32_t)__shfl_up((int)v, d);
-}
-__device__ __forceinline__ uint64_t wave_scan(uint64_t v, int lane) {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) {
-        const uint64_t o = shfl_up64(v, d);
-        if (lane >= d) v += o;
-    }
-    return v;
-}
+__device__ __forceinline__ float of_key(uint32_t k) { return u2f(k & 0x80000000u ? k : ~k & 0x7fffffffu); }
 
 struct Ranked {
-    uint32_t key;
+    float x;
     int at;
     uint64_t w;
 };
+template <class T, bool HELD>
 struct SampleLds {
+    static constexpr int kHeld = HELD ? kHeldBytes / (int)sizeof(typename T::E) : T::kVec;
+    // pieces of 64 vectors
+    static constexpr int kCells = (HELD ? kHeld : kMostVocab) / (64 * T::kVec);
+    typename T::E held[kHeld] __attribute__((aligned(16)));
     double power[kBins];  // exp(-b / 32) 2^shift
     union {
         struct {
-            unsigned long long mass[kRadix];
-            uint32_t count[kRadix];
+            unsigned long long mass[kBins];
+            uint32_t count[kBins];
         };
         Ranked list[kList];
         uint64_t cell[kCells];
     };
-    uint64_t wsum[kWaves];
+    uint64_t wsum[2][kWaves];
     float wmax[kWaves];
     int warg[kWaves];
     double wexp[kWaves];
     uint64_t base;    // weight ranked before a bin found
     double left;      // of the goal, in it
-    uint32_t key;     // a border
+    float x;          // a border
     int at;
     uint32_t bin, n;
 };
 
-// The sum over the workgroup before each thread, and the whole sum.
-__device__ __forceinline__ uint64_t block_scan(uint64_t v, uint64_t *wsum, uint64_t &total) {
+// The sum over the workgroup before each thread, and the whole sum; `turn`
+// alternates between calls.
+__device__ __forceinline__ uint64_t block_scan(uint64_t v, uint64_t (&wsum)[kWaves], uint64_t &total) {
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
-    const uint64_t s = wave_scan(v, lane);
-    __syncthreads();
+    const uint64_t s = wave_scan64(v);
     if (lane == 63) wsum[w] = s;
     __syncthreads();
     uint64_t at = 0, all = 0;
 #pragma unroll
     for (int i = 0; i < kWaves; ++i) {
-        at += i < w ? wsum[i] : 0;
-        all += wsum[i];
+        const uint64_t o = wsum[i];
+        at += i < w ? o : 0;
+        all += o;
     }
     total = all;
     return at + s - v;
 }
 
 // A row and how its tokens fall and weigh.
-template <class T>
+template <class T, bool HELD>
 struct Row {
     static constexpr int V = T::kVec;
+    typedef SampleLds<T, HELD> Lds;
     const typename T::E *row;
-    const double *power;
+    Lds *lds;
     int n;
     float top;
     double top_d, inv_temp, step;  // step: 32 / temperature
 
-    // f(value, index), a wave's 64 V tokens consecutive
-    template <class F>
-    __device__ __forceinline__ void each(F &&f) const {
-#pragma unroll 2
-        for (int at = (int)threadIdx.x * V; at < n; at += kST * V) {
-            float x[V];
-            load_vec<T>(row, at, n, __builtin_nanf(""), x);
+    __device__ __forceinline__ void load(int at, float (&x)[V]) const {
+        if constexpr (HELD) {
+            const Vec<T> v = *reinterpret_cast<const Vec<T> *>(__builtin_assume_aligned(&lds->held[at], 16));
 #pragma unroll
-            for (int j = 0; j < V; ++j) f(x[j], at + j);
+            for (int j = 0; j < V; ++j) x[j] = T::get(v.e[j]);
+        } else {
+            load_vec<T>(row, at, n, __builtin_nanf(""), x);
         }
     }
-    // how far below the highest; NaN for NaN, whose bin and exponential are
-    // those of infinity
+    // f(values, index of the first), a wave's 64 V tokens consecutive
+    template <class F>
+    __device__ __forceinline__ void each(F &&f) const {
+#pragma unroll 4
+        for (int at = (int)threadIdx.x * V; at < n; at += kST * V) {
+            float x[V];
+            load(at, x);
+            f(x, at);
+        }
+    }
+    // how far below the highest; NaN for NaN, whose bin is that of infinity
     __device__ __forceinline__ double fall(float v) const { return v == top ? 0.0 : top_d - (double)v; }
     // kBins where the weight is 0: exp(-32) is half a unit of 2^-45
     __device__ __forceinline__ int bin(double d) const { return (int)__builtin_fmin(d * step, (double)kBins); }
@@ -264,25 +261,41 @@ struct Row {
         y = __builtin_fma(y, t, 1.0);
         y = __builtin_fma(y, t, 1.0);
         // the sum's low bits are the rounded number
-        return __builtin_bit_cast(uint64_t, __builtin_fma(power[b], y, 0x1p52)) & 0xfffffffffffffull;
+        return __builtin_bit_cast(uint64_t, __builtin_fma(lds->power[b], y, 0x1p52)) & 0xfffffffffffffull;
     }
-    __device__ __forceinline__ uint64_t weight(double d) const { return weight(d, bin(d)); }
+    // FP32 bounds that hold every token of the steps b .. e - 1 (and a few
+    // others: rounding)
+    __device__ __forceinline__ void bounds(int b, int e, float &lo, float &hi) const {
+        const double slack = __builtin_fabs(top_d) * 0x1p-22 + 0x1p-126;
+        hi = (float)(top_d - (double)b / step + slack);
+        lo = (float)(top_d - (double)e / step - slack);
+        if (!(hi < top)) hi = top;
+        if (!(lo > -kInf)) lo = -kInf;  // (-infinity - infinity too)
+    }
 };
 
 // The border of the tokens of step `b` whose ranked counts (by_mass: weights)
-// first reach `left`, into lds.key and lds.at; their weight is the result.
-template <class T>
-__device__ uint64_t border_in(const Row<T> &r, SampleLds &lds, int b, bool by_mass, double left) {
+// first reach `left`, into lds.x and lds.at; their weight is the result.
+template <class T, bool HELD>
+__device__ __forceinline__ uint64_t border_in(const Row<T, HELD> &r, SampleLds<T, HELD> &lds, int b, bool by_mass,
+                                              double left) {
+    constexpr int V = T::kVec;
     const int t = threadIdx.x;
+    float lo, hi;
+    r.bounds(b, b + 1, lo, hi);
     __syncthreads();
     if (t == 0) lds.n = 0;
     __syncthreads();
-    r.each([&](float v, int at) __attribute__((always_inline)) {
-        const double d = r.fall(v);
-        if (r.bin(d) == b) {
-            const uint32_t i = atomicAdd(&lds.n, 1u);
-            if (i < (uint32_t)kList) lds.list[i] = Ranked{fall_key(v), at, r.weight(d, b)};
-        }
+    r.each([&](const float(&x)[V], int at) __attribute__((always_inline)) {
+#pragma unroll
+        for (int j = 0; j < V; ++j)
+            if (x[j] >= lo && x[j] <= hi) {
+                const double d = r.fall(x[j]);
+                if (r.bin(d) == b) {
+                    const uint32_t i = atomicAdd(&lds.n, 1u);
+                    if (i < (uint32_t)kList) lds.list[i] = Ranked{x[j], at + j, r.weight(d, b)};
+                }
+            }
     });
     __syncthreads();
     const int n = (int)lds.n;
@@ -294,7 +307,7 @@ __device__ uint64_t border_in(const Row<T> &r, SampleLds &lds, int b, bool by_ma
             uint64_t before = 0;
             for (int i = 0; i < n; ++i) {
                 const Ranked o = lds.list[i];
-                if (o.key < me.key || (o.key == me.key && o.at < me.at)) {
+                if (o.x > me.x || (o.x == me.x && o.at < me.at)) {
                     ++rank;
                     before += o.w;
                 }
@@ -303,7 +316,7 @@ __device__ uint64_t border_in(const Row<T> &r, SampleLds &lds, int b, bool by_ma
                          to = by_mass ? (double)(before + me.w) : (double)(rank + 1);
             // rounding in `left` past the step's end: its last token
             if ((from < left && to >= left) || (rank == n - 1 && to < left)) {
-                lds.key = me.key;
+                lds.x = me.x;
                 lds.at = me.at;
                 lds.base = before + me.w;
             }
@@ -311,44 +324,41 @@ __device__ uint64_t border_in(const Row<T> &r, SampleLds &lds, int b, bool by_ma
         __syncthreads();
         return lds.base;
     }
-    uint64_t base = 0;
-    uint32_t prefix = 0, have = 0;
-    uint64_t each_w = 0;
-    for (int level = 0; level < 3; ++level) {
-        const int sh = level == 0 ? 21 : level == 1 ? 10 : 0;
-        const uint32_t bits = level == 2 ? 0x3ffu : 0x7ffu;
-        const uint32_t above = level == 0 ? 0u : ~0u << (level == 1 ? 21 : 10);
+    uint64_t base = 0, each_w = 0;
+    uint32_t prefix = 0, above = 0, have = 0;
+    for (int sh = 22; sh >= 0; sh -= sh > 2 ? 10 : sh == 2 ? 2 : 1) {
+        const uint32_t bits = sh == 0 ? 3u : 0x3ffu;
         __syncthreads();
+        lds.count[t] = 0;
+        lds.mass[t] = 0;
+        __syncthreads();
+        r.each([&](const float(&x)[V], int) __attribute__((always_inline)) {
 #pragma unroll
-        for (int i = 0; i < kRadix / kST; ++i) {
-            lds.count[t + i * kST] = 0;
-            lds.mass[t + i * kST] = 0;
-        }
-        __syncthreads();
-        r.each([&](float v, int) __attribute__((always_inline)) {
-            const double d = r.fall(v);
-            const uint32_t key = fall_key(v);
-            if (r.bin(d) == b && (key & above) == prefix) {
-                atomicAdd(&lds.count[(key >> sh) & bits], 1u);
-                atomicAdd(&lds.mass[(key >> sh) & bits], (unsigned long long)r.weight(d, b));
-            }
+            for (int j = 0; j < V; ++j)
+                if (x[j] >= lo && x[j] <= hi) {
+                    const double d = r.fall(x[j]);
+                    const uint32_t key = fall_key(x[j]);
+                    if (r.bin(d) == b && (key & above) == prefix) {
+                        atomicAdd(&lds.count[(key >> sh) & bits], 1u);
+                        atomicAdd(&lds.mass[(key >> sh) & bits], (unsigned long long)r.weight(d, b));
+                    }
+                }
         });
         __syncthreads();
-        const int at = 2 * t;
-        const uint64_t m0 = lds.mass[at], m1 = lds.mass[at + 1], c0 = lds.count[at], c1 = lds.count[at + 1];
+        const uint64_t m = lds.mass[t], c = lds.count[t];
         uint64_t all_m, all_c;
-        const uint64_t mb = block_scan(m0 + m1, lds.wsum, all_m), cb = block_scan(c0 + c1, lds.wsum, all_c);
-        const uint64_t v0 = by_mass ? m0 : c0, v1 = by_mass ? m1 : c1, vb = by_mass ? mb : cb;
+        const uint64_t mb = block_scan(m, lds.wsum[0], all_m), cb = block_scan(c, lds.wsum[1], all_c);
+        const uint64_t v = by_mass ? m : c, vb = by_mass ? mb : cb;
         // what the bin above holds is all here: rounding past it ends there
         const double goal = __builtin_fmin(left, (double)(by_mass ? all_m : all_c));
-        if (v0 + v1 != 0 && (double)vb < goal && (double)(vb + v0 + v1) >= goal) {
-            const bool second = !((double)(vb + v0) >= goal);
-            lds.bin = at + second;
-            lds.left = goal - (double)(vb + (second ? v0 : 0));
-            lds.base = mb + (second ? m0 : 0);
+        if (v != 0 && (double)vb < goal && (double)(vb + v) >= goal) {
+            lds.bin = (uint32_t)t;
+            lds.left = goal - (double)vb;
+            lds.base = mb;
         }
         __syncthreads();
         prefix |= lds.bin << sh;
+        above |= bits << sh;
         left = lds.left;
         base += lds.base;
         have = lds.count[lds.bin];
@@ -357,67 +367,88 @@ __device__ uint64_t border_in(const Row<T> &r, SampleLds &lds, int b, bool by_ma
     // of the border key's tokens (one weight all), the first `need` are kept
     uint64_t need = by_mass ? (uint64_t)__builtin_ceil(left / (double)each_w) : (uint64_t)left;
     need = need < 1 ? 1 : (need < have ? need : have);
+    const float edge = of_key(prefix);
     // the place of the last of these: the pieces' counts, then the piece's own
-    constexpr int V = T::kVec;
     const int n_cells = (r.n + 64 * V - 1) / (64 * V), lane = t & 63, w = t >> 6;
     __syncthreads();
     for (int c = w; c < n_cells; c += kWaves) {
-        float x[V];
-        load_vec<T>(r.row, (c * 64 + lane) * V, r.n, __builtin_nanf(""), x);
-        uint64_t k = 0;
+        const int at = (c * 64 + lane) * V;
+        float x[V] = {};
+        uint32_t k = 0;
+        if (at < r.n) {
+            r.load(at, x);
 #pragma unroll
-        for (int j = 0; j < V; ++j) k += x[j] == x[j] && fall_key(x[j]) == prefix;
-        k = wave_scan(k, lane);
-        if (lane == 63) lds.cell[c] = k;
+            for (int j = 0; j < V; ++j) k += x[j] == edge;
+        }
+        const uint64_t sum = wave_scan64((uint64_t)k);
+        if (lane == 63) lds.cell[c] = sum;
     }
     __syncthreads();
     const int per = (n_cells + kST - 1) / kST;
     uint64_t mine = 0, all;
     for (int i = 0; i < per; ++i) mine += t * per + i < n_cells ? lds.cell[t * per + i] : 0;
-    uint64_t at = block_scan(mine, lds.wsum, all);
+    uint64_t at = block_scan(mine, lds.wsum[0], all);
     if (at < need && at + mine >= need) {
         int c = t * per;
         while (at + lds.cell[c] < need) at += lds.cell[c++];
-        for (int i = c * 64 * V; i < r.n; ++i) {
-            const float v = T::get(r.row[i]);
-            if (v == v && fall_key(v) == prefix && ++at == need) {
-                lds.key = prefix;
+        for (int i = c * 64 * V; i < r.n; ++i)
+            if (T::get(r.row[i]) == edge && ++at == need) {
+                lds.x = edge;
                 lds.at = i;
                 break;
             }
-        }
     }
     __syncthreads();
     return base + need * each_w;
 }
 
-template <class T>
+template <class T, bool HELD>
 __global__ __launch_bounds__(kST) void k_sample(GDNSample p, int shift) {
     constexpr int V = T::kVec;
-    __shared__ SampleLds lds;
+    __shared__ SampleLds<T, HELD> lds;
     const int ri = blockIdx.x, t = threadIdx.x, lane = t & 63, w = t >> 6;
-    Row<T> r;
+    Row<T, HELD> r;
     r.row = static_cast<const typename T::E *>(p.logits) + (size_t)ri * p.logits_stride;
     r.n = (int)p.vocab;
-    r.power = lds.power;
+    r.lds = &lds;
 
     // the highest logit, and its first place
     float top = -kInf;
     int arg = 0x7fffffff;
-    r.each([&](float v, int at) __attribute__((always_inline)) {
-        if (v > top) {
-            top = v;
-            arg = at;
-        }
-    });
+    auto higher = [&](const float(&x)[V], int at) __attribute__((always_inline)) {
 #pragma unroll
-    for (int s = 1; s < 64; s <<= 1) {
-        const float ov = __shfl_xor(top, s);
-        const int oi = __shfl_xor(arg, s);
-        if (ov > top || (ov == top && oi < arg)) {
-            top = ov;
-            arg = oi;
+        for (int j = 0; j < V; ++j)
+            if (x[j] > top) {
+                top = x[j];
+                arg = at + j;
+            }
+    };
+    if constexpr (HELD) {
+        // eight vectors of every thread on their way at a time
+        constexpr int kAhead = 8;
+        for (int first = t * V; first < r.n; first += kAhead * kST * V) {
+            float x[kAhead][V];
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i)
+                if (first + i * kST * V < r.n) load_vec<T>(r.row, first + i * kST * V, r.n, __builtin_nanf(""), x[i]);
+#pragma unroll
+            for (int i = 0; i < kAhead; ++i)
+                if (first + i * kST * V < r.n) {
+                    higher(x[i], first + i * kST * V);
+                    Vec<T> v;
+#pragma unroll
+                    for (int j = 0; j < V; ++j) v.e[j] = T::put(x[i][j]);
+                    *reinterpret_cast<Vec<T> *>(__builtin_assume_aligned(&lds.held[first + i * kST * V], 16)) = v;
+                }
         }
+    } else {
+        r.each(higher);
+    }
+    {
+        const float most = u2f(wave_reduce64(f2u(top), [](uint32_t a, uint32_t b) { return f2u(__builtin_fmaxf(u2f(a), u2f(b))); }));
+        arg = top == most ? arg : 0x7fffffff;
+        top = most;
+        arg = (int)wave_reduce64((uint32_t)arg, [](uint32_t a, uint32_t b) { return a < b ? a : b; });
     }
     if (lane == 0) {
         lds.wmax[w] = top;
@@ -429,16 +460,19 @@ __global__ __launch_bounds__(kST) void k_sample(GDNSample p, int shift) {
     const float tp = p.top_p ? p.top_p[ri] : 1.0f;
     const bool first_only = tp <= 0.0f;
     const bool by_k = !greedy && !first_only && k > 0 && k < r.n, by_p = !greedy && !first_only && tp < 1.0f;
-    lds.power[t] = __builtin_ldexp(exp(-(double)t / 32.0), shift);
+    if (!greedy) lds.power[t] = __builtin_ldexp(exp(-(double)t / 32.0), shift);
     lds.count[t] = 0;
     lds.mass[t] = 0;
     __syncthreads();
 #pragma unroll
-    for (int i = 0; i < kWaves; ++i)
-        if (lds.wmax[i] > top || (lds.wmax[i] == top && lds.warg[i] < arg)) {
-            top = lds.wmax[i];
-            arg = lds.warg[i];
+    for (int i = 0; i < kWaves; ++i) {
+        const float m = lds.wmax[i];
+        const int a = lds.warg[i];
+        if (m > top || (m == top && a < arg)) {
+            top = m;
+            arg = a;
         }
+    }
     if (arg == 0x7fffffff) {  // nothing above -infinity
         if (t == 0) {
             p.tokens[ri] = -1;
@@ -450,95 +484,105 @@ __global__ __launch_bounds__(kST) void k_sample(GDNSample p, int shift) {
     r.top_d = (double)top;
     r.inv_temp = 1.0 / (double)temp;
     r.step = 32.0 * r.inv_temp;
+    float lowest, unused;
+    r.bounds(0, kBins, lowest, unused);
 
     // the sum of exponentials, and the steps' counts and weights
     double sum = 0.0;
     auto pass = [&](auto sum_on, auto count_on, auto mass_on) __attribute__((always_inline)) {
-        r.each([&](float v, int) __attribute__((always_inline)) {
-            const double d = r.fall(v);
-            if (sum_on) sum += (double)exp_neg((float)d);
-            if (count_on || mass_on) {
-                const int b = r.bin(d);
-                if (b < kBins) {
-                    if (count_on) atomicAdd(&lds.count[b], 1u);
-                    if (mass_on) atomicAdd(&lds.mass[b], (unsigned long long)r.weight(d, b));
+        r.each([&](const float(&x)[V], int) __attribute__((always_inline)) {
+            if constexpr (sum_on) {
+                float s = 0.0f;
+#pragma unroll
+                for (int j = 0; j < V; ++j) {
+                    // exp(-d), the rounding of its base-2 argument made good; 0
+                    // for NaN and what is too small
+                    constexpr float kL = 1.44269502f, kLo = 1.92596299e-8f;  // log2(e)
+                    const float d = x[j] == top ? 0.0f : top - x[j], y = d * kL,
+                                e = __builtin_fmaf(d, kLo, __builtin_fmaf(d, kL, -y)),
+                                q = __builtin_amdgcn_exp2f(-y);
+                    s += y < 126.0f ? __builtin_fmaf(q, -0.693147181f * e, q) : 0.0f;
                 }
+                sum += (double)s;
+            }
+            if constexpr (count_on || mass_on) {
+#pragma unroll
+                for (int j = 0; j < V; ++j)
+                    if (x[j] >= lowest) {
+                        const double d = r.fall(x[j]);
+                        const int b = r.bin(d);
+                        if (b < kBins) {
+                            if constexpr (count_on) atomicAdd(&lds.count[b], 1u);
+                            if constexpr (mass_on) atomicAdd(&lds.mass[b], (unsigned long long)r.weight(d, b));
+                        }
+                    }
             }
         });
     };
     constexpr std::true_type on;
     constexpr std::false_type off;
-    if (by_k && by_p) pass(on, on, on);
-    else if (by_k) pass(on, on, off);
-    else if (by_p) pass(on, off, on);
-    else if (p.logprobs) pass(on, off, off);
-    double log_sum = 0.0;
-    if (p.logprobs) {
+    if (p.logprobs) pass(on, off, off);
+    if (by_k && by_p) pass(off, on, on);
+    else if (by_k) pass(off, on, off);
+    else if (by_p) pass(off, off, on);
+    sum = wave_scan64(sum);
+    if (lane == 63) lds.wexp[w] = sum;
+    __syncthreads();
+    // (the thread that writes a result finishes it)
+    auto log_sum = [&]() __attribute__((always_inline)) {
+        double s = 0.0;
 #pragma unroll
-        for (int d = 1; d < 64; d <<= 1) sum += __shfl_xor(sum, d);
-        if (lane == 0) lds.wexp[w] = sum;
-        __syncthreads();
-        sum = 0.0;
-#pragma unroll
-        for (int i = 0; i < kWaves; ++i) sum += lds.wexp[i];
-        log_sum = log(sum);
-    }
+        for (int i = 0; i < kWaves; ++i) s += lds.wexp[i];
+        return log(s);
+    };
     if (greedy) {
         if (t == 0) {
             p.tokens[ri] = arg;
-            if (p.logprobs) p.logprobs[ri] = (float)-log_sum;
+            if (p.logprobs) p.logprobs[ri] = (float)-log_sum();
         }
         return;
     }
 
-    // the border: tokens of a key below it are kept, of its key those up to
-    // place edge_at
-    uint32_t edge = 0xffffffffu;
+    // the border: higher tokens are kept, of its logit those up to edge_at
+    float edge = -kInf;
     int edge_at = 0x7fffffff;
     if (by_k || by_p) {
-        __syncthreads();
         const uint64_t count = lds.count[t], mass = lds.mass[t];
         uint64_t n_all = 0, kept = 0, n_before = 0, m_before = 0;
-        if (by_k) n_before = block_scan(count, lds.wsum, n_all);
-        if (by_p) m_before = block_scan(mass, lds.wsum, kept);
-        if (by_k && (uint64_t)k <= n_all) {
-            if (n_before < (uint64_t)k && n_before + count >= (uint64_t)k) {
+        if (by_k) n_before = block_scan(count, lds.wsum[0], n_all);
+        if (by_p) m_before = block_scan(mass, lds.wsum[1], kept);
+        // by counts, then by weights: tokens past the first border rank behind
+        // all that reach the second goal, which is less than the whole weight
+        for (int turn = 0; turn < 2; ++turn) {
+            const bool by_mass = turn == 1;
+            if (by_mass ? !by_p : !by_k || (uint64_t)k > n_all) continue;
+            const double goal = by_mass ? (double)tp * (double)kept : (double)k;
+            const uint64_t before = by_mass ? m_before : n_before, own = by_mass ? mass : count;
+            __syncthreads();
+            if (own != 0 && (double)before < goal && (double)(before + own) >= goal) {
                 lds.bin = t;
-                lds.left = (double)((uint64_t)k - n_before);
+                lds.left = goal - (double)before;
                 lds.base = m_before;
             }
             __syncthreads();
             const uint64_t base = lds.base;
-            kept = base + border_in(r, lds, (int)lds.bin, false, lds.left);
-            edge = lds.key;
-            edge_at = lds.at;
-        }
-        if (by_p) {
-            const double goal = (double)tp * (double)kept;
-            __syncthreads();
-            // a goal that rounds past the last step's end ends there
-            if (mass != 0 && (double)m_before < goal && (double)(m_before + mass) >= goal) {
-                lds.bin = t;
-                lds.left = goal - (double)m_before;
-            }
-            __syncthreads();
-            // tokens past the first border rank behind all that reach the goal
-            border_in(r, lds, (int)lds.bin, true, lds.left);
-            if (lds.key < edge || (lds.key == edge && lds.at < edge_at)) {
-                edge = lds.key;
+            kept = base + border_in(r, lds, (int)lds.bin, by_mass, lds.left);
+            if (lds.x > edge || (lds.x == edge && lds.at < edge_at)) {
+                edge = lds.x;
                 edge_at = lds.at;
             }
         }
     } else if (first_only) {
-        edge = fall_key(top);
+        edge = top;
         edge_at = arg;
     }
     const float mp = p.min_p ? p.min_p[ri] : 0.0f;
     const double least = mp > 0.0f ? __builtin_ldexp((double)__builtin_fminf(mp, 1.0f), shift) : 0.0;
+    const float from = edge > lowest ? edge : lowest;
     auto weight = [&](float v, int at) __attribute__((always_inline)) -> uint64_t {
-        const uint32_t key = fall_key(v);
-        if (!(key < edge || (key == edge && at <= edge_at))) return 0;
-        const uint64_t s = r.weight(r.fall(v));
+        if (!(v >= from) || (v == edge && at > edge_at)) return 0;
+        const double d = r.fall(v);
+        const uint64_t s = r.weight(d, r.bin(d));
         return (double)s >= least ? s : 0;
     };
 
@@ -548,19 +592,21 @@ __global__ __launch_bounds__(kST) void k_sample(GDNSample p, int shift) {
     __syncthreads();
     for (int c = w; c < cells; c += kWaves) {
         const int at = (c * 64 + lane) * V;
-        float x[V];
-        load_vec<T>(r.row, at, r.n, __builtin_nanf(""), x);
         uint64_t s = 0;
+        if (at < r.n) {
+            float x[V];
+            r.load(at, x);
 #pragma unroll
-        for (int j = 0; j < V; ++j) s += weight(x[j], at + j);
-        if (__ballot(s != 0) != 0) s = wave_scan(s, lane);
+            for (int j = 0; j < V; ++j) s += weight(x[j], at + j);
+        }
+        if (__ballot(s != 0) != 0) s = wave_scan64(s);
         if (lane == 63) lds.cell[c] = s;
     }
     __syncthreads();
     uint64_t mine = 0, all;
     const int per = (cells + kST - 1) / kST;
     for (int i = 0; i < per; ++i) mine += t * per + i < cells ? lds.cell[t * per + i] : 0;
-    uint64_t at = block_scan(mine, lds.wsum, all);
+    uint64_t at = block_scan(mine, lds.wsum[0], all);
     const double u = (double)p.uniform[ri];
     uint64_t goal = u > 0.0 ? (uint64_t)__builtin_fmin(u * (double)all, 9.2e18) : 0;
     goal = goal < all ? goal : all - 1;
@@ -574,14 +620,14 @@ __global__ __launch_bounds__(kST) void k_sample(GDNSample p, int shift) {
     if (w == 0) {
         const int c0 = (int)lds.bin * 64 * V + lane * V;
         float y[V];
-        load_vec<T>(r.row, c0, r.n, __builtin_nanf(""), y);
         uint64_t s[V], own = 0;
+        if (c0 < r.n) r.load(c0, y);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
-            s[j] = weight(y[j], c0 + j);
+            s[j] = c0 < r.n ? weight(y[j], c0 + j) : 0;
             own += s[j];
         }
-        uint64_t run = lds.base + wave_scan(own, lane) - own;
+        uint64_t run = lds.base + wave_scan64(own) - own;
         if (run <= goal && run + own > goal) {
             int j = 0;
 #pragma unroll
@@ -594,7 +640,7 @@ __global__ __launch_bounds__(kST) void k_sample(GDNSample p, int shift) {
                 }
             }
             p.tokens[ri] = c0 + j;
-            if (p.logprobs) p.logprobs[ri] = (float)(-r.fall(T::get(r.row[c0 + j])) - log_sum);
+            if (p.logprobs) p.logprobs[ri] = (float)(-r.fall(T::get(r.row[c0 + j])) - log_sum());
         }
     }
 }
@@ -652,7 +698,7 @@ extern "C" int gdn_sample_tokens(const GDNSample *args, void *stream) {
     if (args == nullptr) return refuse(who, "args is NULL");
     const GDNSample &a = *args;
     if (a.dtype < GDN_DTYPE_BF16 || a.dtype > GDN_DTYPE_FP32) return refuse(who, "unknown dtype");
-    if (a.vocab > (1u << 20)) return refuse(who, "the vocabulary is larger than 2^20");
+    if (a.vocab > (uint32_t)kMostVocab) return refuse(who, "the vocabulary is larger than 2^20");
     if (a.rows > 0x7fffffffu) return refuse(who, "at most 2^31 - 1 rows");
     if (a.rows == 0) return 0;
     if (a.vocab == 0) return refuse(who, "the vocabulary is empty");
@@ -663,8 +709,15 @@ extern "C" int gdn_sample_tokens(const GDNSample *args, void *stream) {
     const int shift = a.vocab <= (1u << 18) ? 45 : 43;
     const dim3 grid(a.rows), block(kST);
     hipStream_t s = static_cast<hipStream_t>(stream);
-    if (a.dtype == GDN_DTYPE_BF16) hipLaunchKernelGGL(k_sample<Bf16>, grid, block, 0, s, a, shift);
-    else if (a.dtype == GDN_DTYPE_FP16) hipLaunchKernelGGL(k_sample<Fp16>, grid, block, 0, s, a, shift);
-    else hipLaunchKernelGGL(k_sample<Fp32>, grid, block, 0, s, a, shift);
+    auto launch = [&](auto type) {
+        using T = decltype(type);
+        if (a.vocab <= (uint32_t)SampleLds<T, true>::kHeld)
+            hipLaunchKernelGGL((k_sample<T, true>), grid, block, 0, s, a, shift);
+        else
+            hipLaunchKernelGGL((k_sample<T, false>), grid, block, 0, s, a, shift);
+    };
+    if (a.dtype == GDN_DTYPE_BF16) launch(Bf16());
+    else if (a.dtype == GDN_DTYPE_FP16) launch(Fp16());
+    else launch(Fp32());
     return launched(who);
 }
