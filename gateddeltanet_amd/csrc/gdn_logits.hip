@@ -236,7 +236,8 @@ struct Row {
     // f(values, index of the first), a wave's 64 V tokens consecutive
     template <class F>
     __device__ __forceinline__ void each(F &&f) const {
-#pragma unroll 4
+        constexpr int kUnroll = 16 / V;
+#pragma unroll kUnroll
         for (int at = (int)threadIdx.x * V; at < n; at += kST * V) {
             float x[V];
             load(at, x);
@@ -412,6 +413,13 @@ __global__ __launch_bounds__(kST) void k_sample(GDNSample p, int shift) {
     r.n = (int)p.vocab;
     r.lds = &lds;
 
+    const float temp = p.temperature ? p.temperature[ri] : 0.0f;
+    const int k = p.top_k ? p.top_k[ri] : 0;
+    const float tp = p.top_p ? p.top_p[ri] : 1.0f, mp = p.min_p ? p.min_p[ri] : 0.0f;
+    const double u = p.temperature ? (double)p.uniform[ri] : 0.0;
+    const bool greedy = !(temp > 0.0f), first_only = tp <= 0.0f;
+    const bool by_k = !greedy && !first_only && k > 0 && k < r.n, by_p = !greedy && !first_only && tp < 1.0f;
+
     // the highest logit, and its first place
     float top = -kInf;
     int arg = 0x7fffffff;
@@ -424,26 +432,35 @@ __global__ __launch_bounds__(kST) void k_sample(GDNSample p, int shift) {
             }
     };
     if constexpr (HELD) {
-        // eight vectors of every thread on their way at a time
-        constexpr int kAhead = 8;
-        for (int first = t * V; first < r.n; first += kAhead * kST * V) {
-            float x[kAhead][V];
+        // every vector of a thread on its way at a time
+        constexpr int kAhead = SampleLds<T, HELD>::kHeld / (kST * V);
+        const int whole = r.n / V, rest = r.n % V;
+        if (whole > 0) {
+            Vec<T> v[kAhead];
 #pragma unroll
             for (int i = 0; i < kAhead; ++i)
-                if (first + i * kST * V < r.n) load_vec<T>(r.row, first + i * kST * V, r.n, __builtin_nanf(""), x[i]);
+                __builtin_memcpy(&v[i], r.row + (size_t)min(i * kST + t, whole - 1) * V, sizeof(v[i]));
 #pragma unroll
             for (int i = 0; i < kAhead; ++i)
-                if (first + i * kST * V < r.n) {
-                    higher(x[i], first + i * kST * V);
-                    Vec<T> v;
+                if (i * kST + t < whole) {
+                    float x[V];
 #pragma unroll
-                    for (int j = 0; j < V; ++j) v.e[j] = T::put(x[i][j]);
-                    *reinterpret_cast<Vec<T> *>(__builtin_assume_aligned(&lds.held[first + i * kST * V], 16)) = v;
+                    for (int j = 0; j < V; ++j) x[j] = T::get(v[i].e[j]);
+                    higher(x, (i * kST + t) * V);
+                    *reinterpret_cast<Vec<T> *>(__builtin_assume_aligned(&lds.held[(i * kST + t) * V], 16)) = v[i];
                 }
+        }
+        if (rest > 0 && t == kST - 1) {
+            float x[V];
+            load_vec<T>(r.row, whole * V, r.n, __builtin_nanf(""), x);
+            higher(x, whole * V);
+#pragma unroll
+            for (int j = 0; j < V; ++j) lds.held[whole * V + j] = T::put(x[j]);
         }
     } else {
         r.each(higher);
     }
+    const float own_top = top;
     {
         const float most = u2f(wave_reduce64(f2u(top), [](uint32_t a, uint32_t b) { return f2u(__builtin_fmaxf(u2f(a), u2f(b))); }));
         arg = top == most ? arg : 0x7fffffff;
@@ -454,12 +471,6 @@ __global__ __launch_bounds__(kST) void k_sample(GDNSample p, int shift) {
         lds.wmax[w] = top;
         lds.warg[w] = arg;
     }
-    const float temp = p.temperature ? p.temperature[ri] : 0.0f;
-    const bool greedy = !(temp > 0.0f);
-    const int k = p.top_k ? p.top_k[ri] : 0;
-    const float tp = p.top_p ? p.top_p[ri] : 1.0f;
-    const bool first_only = tp <= 0.0f;
-    const bool by_k = !greedy && !first_only && k > 0 && k < r.n, by_p = !greedy && !first_only && tp < 1.0f;
     if (!greedy) lds.power[t] = __builtin_ldexp(exp(-(double)t / 32.0), shift);
     lds.count[t] = 0;
     lds.mass[t] = 0;
@@ -487,47 +498,71 @@ __global__ __launch_bounds__(kST) void k_sample(GDNSample p, int shift) {
     float lowest, unused;
     r.bounds(0, kBins, lowest, unused);
 
-    // the sum of exponentials, and the steps' counts and weights
+    // as many tokens as are asked for are no lower than `bound`: every thread's
+    // highest, counted by steps, tells (for top-p a guess, made good below)
+    float bound = lowest;
+    if (by_k || by_p) {
+        const int b = r.bin(r.fall(own_top));
+        if (b < kBins) atomicAdd(&lds.count[b], 1u);
+        if (t == 0) lds.bin = kBins;
+        __syncthreads();
+        const uint64_t n = lds.count[t], enough = by_k ? (uint64_t)k : 64;
+        lds.count[t] = 0;
+        uint64_t all;
+        const uint64_t before = block_scan(n, lds.wsum[0], all);
+        if (before < enough && before + n >= enough) lds.bin = (uint32_t)t;
+        __syncthreads();
+        if (lds.bin < (uint32_t)kBins) r.bounds((int)lds.bin, (int)lds.bin + 1, bound, unused);
+    }
+
+    // the sum of exponentials, the whole weight where only top-p needs it, and
+    // the steps' counts and weights
     double sum = 0.0;
-    auto pass = [&](auto sum_on, auto count_on, auto mass_on) __attribute__((always_inline)) {
+    uint64_t whole = 0;
+    const bool total = by_p && !by_k;
+    auto sums = [&](auto total_on) __attribute__((always_inline)) {
         r.each([&](const float(&x)[V], int) __attribute__((always_inline)) {
-            if constexpr (sum_on) {
-                float s = 0.0f;
+            float s = 0.0f;
 #pragma unroll
-                for (int j = 0; j < V; ++j) {
-                    // exp(-d), the rounding of its base-2 argument made good; 0
-                    // for NaN and what is too small
-                    constexpr float kL = 1.44269502f, kLo = 1.92596299e-8f;  // log2(e)
-                    const float d = x[j] == top ? 0.0f : top - x[j], y = d * kL,
-                                e = __builtin_fmaf(d, kLo, __builtin_fmaf(d, kL, -y)),
-                                q = __builtin_amdgcn_exp2f(-y);
-                    s += y < 126.0f ? __builtin_fmaf(q, -0.693147181f * e, q) : 0.0f;
+            for (int j = 0; j < V; ++j) {
+                // exp(-d), the rounding of its base-2 argument made good; 0 for
+                // NaN and what is too small
+                constexpr float kL = 1.44269502f, kLo = 1.92596299e-8f;  // log2(e)
+                const float d = x[j] == top ? 0.0f : top - x[j], y = d * kL,
+                            e = __builtin_fmaf(d, kLo, __builtin_fmaf(d, kL, -y)), q = __builtin_amdgcn_exp2f(-y);
+                s += y < 126.0f ? __builtin_fmaf(q, -0.693147181f * e, q) : 0.0f;
+                if constexpr (total_on) {
+                    const double f = r.fall(x[j]);
+                    whole += r.weight(f, r.bin(f));
                 }
-                sum += (double)s;
             }
-            if constexpr (count_on || mass_on) {
-#pragma unroll
-                for (int j = 0; j < V; ++j)
-                    if (x[j] >= lowest) {
-                        const double d = r.fall(x[j]);
-                        const int b = r.bin(d);
-                        if (b < kBins) {
-                            if constexpr (count_on) atomicAdd(&lds.count[b], 1u);
-                            if constexpr (mass_on) atomicAdd(&lds.mass[b], (unsigned long long)r.weight(d, b));
-                        }
-                    }
-            }
+            sum += (double)s;
         });
     };
-    constexpr std::true_type on;
-    constexpr std::false_type off;
-    if (p.logprobs) pass(on, off, off);
-    if (by_k && by_p) pass(off, on, on);
-    else if (by_k) pass(off, on, off);
-    else if (by_p) pass(off, off, on);
+    auto steps = [&](float from, float below) __attribute__((always_inline)) {
+        r.each([&](const float(&x)[V], int) __attribute__((always_inline)) {
+#pragma unroll
+            for (int j = 0; j < V; ++j)
+                if (x[j] >= from && !(x[j] >= below)) {  // (below NaN: all)
+                    const double d = r.fall(x[j]);
+                    const int b = r.bin(d);
+                    if (b < kBins) {
+                        if (by_k) atomicAdd(&lds.count[b], 1u);
+                        if (by_p) atomicAdd(&lds.mass[b], (unsigned long long)r.weight(d, b));
+                    }
+                }
+        });
+    };
+    if (total) sums(std::true_type());
+    else if (p.logprobs) sums(std::false_type());
     sum = wave_scan64(sum);
     if (lane == 63) lds.wexp[w] = sum;
-    __syncthreads();
+    uint64_t kept = 0;
+    if (total) {
+        block_scan(whole, lds.wsum[1], kept);
+    } else {
+        __syncthreads();
+    }
     // (the thread that writes a result finishes it)
     auto log_sum = [&]() __attribute__((always_inline)) {
         double s = 0.0;
@@ -547,10 +582,18 @@ __global__ __launch_bounds__(kST) void k_sample(GDNSample p, int shift) {
     float edge = -kInf;
     int edge_at = 0x7fffffff;
     if (by_k || by_p) {
-        const uint64_t count = lds.count[t], mass = lds.mass[t];
-        uint64_t n_all = 0, kept = 0, n_before = 0, m_before = 0;
-        if (by_k) n_before = block_scan(count, lds.wsum[0], n_all);
-        if (by_p) m_before = block_scan(mass, lds.wsum[1], kept);
+        steps(bound, __builtin_nanf(""));
+        __syncthreads();
+        uint64_t count = lds.count[t], mass = lds.mass[t], n_all = 0, m_all = 0, n_before = 0, m_before = 0;
+        if (by_p) m_before = block_scan(mass, lds.wsum[0], m_all);
+        if (by_k) n_before = block_scan(count, lds.wsum[1], n_all);
+        if (total && (double)m_all < (double)tp * (double)kept) {
+            steps(lowest, bound);
+            __syncthreads();
+            mass = lds.mass[t];
+            m_before = block_scan(mass, lds.wsum[1], m_all);
+        }
+        if (!total) kept = m_all;
         // by counts, then by weights: tokens past the first border rank behind
         // all that reach the second goal, which is less than the whole weight
         for (int turn = 0; turn < 2; ++turn) {
@@ -576,7 +619,6 @@ __global__ __launch_bounds__(kST) void k_sample(GDNSample p, int shift) {
         edge = top;
         edge_at = arg;
     }
-    const float mp = p.min_p ? p.min_p[ri] : 0.0f;
     const double least = mp > 0.0f ? __builtin_ldexp((double)__builtin_fminf(mp, 1.0f), shift) : 0.0;
     const float from = edge > lowest ? edge : lowest;
     auto weight = [&](float v, int at) __attribute__((always_inline)) -> uint64_t {
@@ -607,7 +649,6 @@ __global__ __launch_bounds__(kST) void k_sample(GDNSample p, int shift) {
     const int per = (cells + kST - 1) / kST;
     for (int i = 0; i < per; ++i) mine += t * per + i < cells ? lds.cell[t * per + i] : 0;
     uint64_t at = block_scan(mine, lds.wsum[0], all);
-    const double u = (double)p.uniform[ri];
     uint64_t goal = u > 0.0 ? (uint64_t)__builtin_fmin(u * (double)all, 9.2e18) : 0;
     goal = goal < all ? goal : all - 1;
     if (at <= goal && at + mine > goal) {
