@@ -184,6 +184,7 @@ struct SampleLds {
         Ranked list[kList];
         uint64_t cell[kCells];
     };
+    Ranked high[kList];  // the tokens above the bound
     uint64_t wsum[2][kWaves];
     float wmax[kWaves];
     int warg[kWaves];
@@ -192,7 +193,7 @@ struct SampleLds {
     double left;      // of the goal, in it
     float x;          // a border
     int at;
-    uint32_t bin, n;
+    uint32_t bin, n, n_high;
 };
 
 // The sum over the workgroup before each thread, and the whole sum; `turn`
@@ -277,9 +278,10 @@ struct Row {
 
 // The border of the tokens of step `b` whose ranked counts (by_mass: weights)
 // first reach `left`, into lds.x and lds.at; their weight is the result.
+// listed: the step's tokens are all in lds.high.
 template <class T, bool HELD>
 __device__ __forceinline__ uint64_t border_in(const Row<T, HELD> &r, SampleLds<T, HELD> &lds, int b, bool by_mass,
-                                              double left) {
+                                              double left, bool listed) {
     constexpr int V = T::kVec;
     const int t = threadIdx.x;
     float lo, hi;
@@ -287,17 +289,21 @@ __device__ __forceinline__ uint64_t border_in(const Row<T, HELD> &r, SampleLds<T
     __syncthreads();
     if (t == 0) lds.n = 0;
     __syncthreads();
-    r.each([&](const float(&x)[V], int at) __attribute__((always_inline)) {
+    if (listed) {
+        if (t < (int)lds.n_high && r.bin(r.fall(lds.high[t].x)) == b) lds.list[atomicAdd(&lds.n, 1u)] = lds.high[t];
+    } else {
+        r.each([&](const float(&x)[V], int at) __attribute__((always_inline)) {
 #pragma unroll
-        for (int j = 0; j < V; ++j)
-            if (x[j] >= lo && x[j] <= hi) {
-                const double d = r.fall(x[j]);
-                if (r.bin(d) == b) {
-                    const uint32_t i = atomicAdd(&lds.n, 1u);
-                    if (i < (uint32_t)kList) lds.list[i] = Ranked{x[j], at + j, r.weight(d, b)};
+            for (int j = 0; j < V; ++j)
+                if (x[j] >= lo && x[j] <= hi) {
+                    const double d = r.fall(x[j]);
+                    if (r.bin(d) == b) {
+                        const uint32_t i = atomicAdd(&lds.n, 1u);
+                        if (i < (uint32_t)kList) lds.list[i] = Ranked{x[j], at + j, r.weight(d, b)};
+                    }
                 }
-            }
-    });
+        });
+    }
     __syncthreads();
     const int n = (int)lds.n;
     if (n <= kList) {
@@ -407,6 +413,7 @@ template <class T, bool HELD>
 __global__ __launch_bounds__(kST) void k_sample(GDNSample p, int shift) {
     constexpr int V = T::kVec;
     __shared__ SampleLds<T, HELD> lds;
+    static_assert(sizeof(lds) <= 160 << 10, "the LDS of a CU");
     const int ri = blockIdx.x, t = threadIdx.x, lane = t & 63, w = t >> 6;
     Row<T, HELD> r;
     r.row = static_cast<const typename T::E *>(p.logits) + (size_t)ri * p.logits_stride;
@@ -504,7 +511,10 @@ __global__ __launch_bounds__(kST) void k_sample(GDNSample p, int shift) {
     if (by_k || by_p) {
         const int b = r.bin(r.fall(own_top));
         if (b < kBins) atomicAdd(&lds.count[b], 1u);
-        if (t == 0) lds.bin = kBins;
+        if (t == 0) {
+            lds.bin = kBins;
+            lds.n_high = 0;
+        }
         __syncthreads();
         const uint64_t n = lds.count[t], enough = by_k ? (uint64_t)k : 64;
         lds.count[t] = 0;
@@ -539,16 +549,21 @@ __global__ __launch_bounds__(kST) void k_sample(GDNSample p, int shift) {
             sum += (double)s;
         });
     };
-    auto steps = [&](float from, float below) __attribute__((always_inline)) {
-        r.each([&](const float(&x)[V], int) __attribute__((always_inline)) {
+    auto steps = [&](float from, float below, bool first) __attribute__((always_inline)) {
+        r.each([&](const float(&x)[V], int at) __attribute__((always_inline)) {
 #pragma unroll
             for (int j = 0; j < V; ++j)
                 if (x[j] >= from && !(x[j] >= below)) {  // (below NaN: all)
                     const double d = r.fall(x[j]);
                     const int b = r.bin(d);
                     if (b < kBins) {
+                        const uint64_t s = r.weight(d, b);
                         if (by_k) atomicAdd(&lds.count[b], 1u);
-                        if (by_p) atomicAdd(&lds.mass[b], (unsigned long long)r.weight(d, b));
+                        if (by_p) atomicAdd(&lds.mass[b], (unsigned long long)s);
+                        if (first) {
+                            const uint32_t i = atomicAdd(&lds.n_high, 1u);
+                            if (i < (uint32_t)kList) lds.high[i] = Ranked{x[j], at + j, s};
+                        }
                     }
                 }
         });
@@ -581,14 +596,17 @@ __global__ __launch_bounds__(kST) void k_sample(GDNSample p, int shift) {
     // the border: higher tokens are kept, of its logit those up to edge_at
     float edge = -kInf;
     int edge_at = 0x7fffffff;
+    bool listed = false;  // what is kept is in lds.high
     if (by_k || by_p) {
-        steps(bound, __builtin_nanf(""));
+        steps(bound, __builtin_nanf(""), bound > lowest);
         __syncthreads();
+        listed = bound > lowest && lds.n_high <= (uint32_t)kList;
         uint64_t count = lds.count[t], mass = lds.mass[t], n_all = 0, m_all = 0, n_before = 0, m_before = 0;
         if (by_p) m_before = block_scan(mass, lds.wsum[0], m_all);
         if (by_k) n_before = block_scan(count, lds.wsum[1], n_all);
         if (total && (double)m_all < (double)tp * (double)kept) {
-            steps(lowest, bound);
+            listed = false;
+            steps(lowest, bound, false);
             __syncthreads();
             mass = lds.mass[t];
             m_before = block_scan(mass, lds.wsum[1], m_all);
@@ -609,7 +627,7 @@ __global__ __launch_bounds__(kST) void k_sample(GDNSample p, int shift) {
             }
             __syncthreads();
             const uint64_t base = lds.base;
-            kept = base + border_in(r, lds, (int)lds.bin, by_mass, lds.left);
+            kept = base + border_in(r, lds, (int)lds.bin, by_mass, lds.left, listed);
             if (lds.x > edge || (lds.x == edge && lds.at < edge_at)) {
                 edge = lds.x;
                 edge_at = lds.at;
@@ -632,7 +650,16 @@ __global__ __launch_bounds__(kST) void k_sample(GDNSample p, int shift) {
     // the token in it
     const int cells = (r.n + 64 * V - 1) / (64 * V);
     __syncthreads();
-    for (int c = w; c < cells; c += kWaves) {
+    if (listed) {
+        for (int c = t; c < cells; c += kST) lds.cell[c] = 0;
+        __syncthreads();
+        if (t < (int)lds.n_high) {
+            const Ranked h = lds.high[t];
+            if ((h.x > edge || (h.x == edge && h.at <= edge_at)) && (double)h.w >= least)
+                atomicAdd(reinterpret_cast<unsigned long long *>(&lds.cell[h.at / (64 * V)]), (unsigned long long)h.w);
+        }
+    }
+    for (int c = listed ? cells : w; c < cells; c += kWaves) {
         const int at = (c * 64 + lane) * V;
         uint64_t s = 0;
         if (at < r.n) {
