@@ -71,34 +71,59 @@ __device__ __forceinline__ void store_vec(typename T::E *row, int at, int n, con
 // kTile tokens of a row: grid (tiles, rows).  The tile's share of the row's
 // history is counted in LDS (whole-number atomics, so no order shows): the
 // output's occurrences, and a bit for any occurrence.  A bias' entry number
-// goes in by maximum, so the last of equal ids holds.
-constexpr int kTile = 8192, kPT = 512;
+// goes in by maximum, so the last of equal ids holds.  The tile's logits are on
+// their way meanwhile.
+constexpr int kTile = 8192, kPT = 1024;
 constexpr uint32_t kSeen = 0x80000000u;
 
 template <class T>
 __global__ __launch_bounds__(kPT) void k_process(GDNLogits p) {
+    constexpr int V = T::kVec, NV = kTile / (V * kPT), kAhead = 4;
     extern __shared__ __attribute__((aligned(16))) uint32_t mem[];
     uint32_t *count = mem, *entry = mem + (p.history ? kTile : 0);
     const int r = blockIdx.y, t0 = blockIdx.x * kTile, t = threadIdx.x;
     const int n = min((int)p.vocab - t0, kTile);
+    const typename T::E *in = static_cast<const typename T::E *>(p.logits) + (size_t)r * p.logits_stride + t0;
+    typename T::E *out = static_cast<typename T::E *>(p.out) + (size_t)r * p.out_stride + t0;
+    float x[NV][V];
+#pragma unroll
+    for (int i = 0; i < NV; ++i)
+        if ((i * kPT + t) * V < n) load_vec<T>(in, (i * kPT + t) * V, n, 0.0f, x[i]);
     int len = 0, prompt = 0, b0 = 0, b1 = 0;
+    const u32x4 none = {0u, 0u, 0u, 0u};
     if (p.history) {
         len = min(max(p.history_len[r], 0), (int)p.history_width);
         prompt = p.prompt_len ? p.prompt_len[r] : 0;
-        for (int i = t; i < kTile / 4; i += kPT) reinterpret_cast<u32x4 *>(count)[i] = (u32x4){0u, 0u, 0u, 0u};
+        for (int i = t; i < kTile / 4; i += kPT) reinterpret_cast<u32x4 *>(count)[i] = none;
     }
     if (p.bias_offsets) {
         b0 = min(max(p.bias_offsets[r], 0), (int)p.n_bias);
         b1 = min(max(p.bias_offsets[r + 1], b0), (int)p.n_bias);
-        for (int i = t; i < kTile / 4; i += kPT) reinterpret_cast<u32x4 *>(entry)[i] = (u32x4){0u, 0u, 0u, 0u};
+        for (int i = t; i < kTile / 4; i += kPT) reinterpret_cast<u32x4 *>(entry)[i] = none;
+    }
+    const float rep = p.repetition ? p.repetition[r] : 1.0f, pres = p.presence ? p.presence[r] : 0.0f,
+                freq = p.frequency ? p.frequency[r] : 0.0f;
+    const int mi = p.mask ? (p.mask_index ? p.mask_index[r] : r) : -1;
+    const uint32_t *mask = mi >= 0 && mi < (int)p.n_masks ? p.mask + (size_t)mi * p.mask_stride + t0 / 32 : nullptr;
+    uint32_t allowed[NV];
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int at = (i * kPT + t) * V;
+        allowed[i] = mask && at < n ? mask[at / 32] >> (at & 31) : ~0u;
     }
     __syncthreads();
     const int32_t *hist = p.history + (size_t)r * p.history_stride;
-    for (int i = t; i < len; i += kPT) {
-        const uint32_t id = (uint32_t)hist[i] - (uint32_t)t0;
-        if (id < (uint32_t)n) {
-            if (i >= prompt) atomicAdd(&count[id], 1u);
-            atomicOr(&count[id], kSeen);
+    for (int i0 = t; i0 < len; i0 += kAhead * kPT) {
+        uint32_t id[kAhead];
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) id[a] = (uint32_t)hist[min(i0 + a * kPT, len - 1)] - (uint32_t)t0;
+#pragma unroll
+        for (int a = 0; a < kAhead; ++a) {
+            const int i = i0 + a * kPT;
+            if (i < len && id[a] < (uint32_t)n) {
+                if (i >= prompt) atomicAdd(&count[id[a]], 1u);
+                atomicOr(&count[id[a]], kSeen);
+            }
         }
     }
     for (int i = b0 + t; i < b1; i += kPT) {
@@ -106,37 +131,30 @@ __global__ __launch_bounds__(kPT) void k_process(GDNLogits p) {
         if (id < (uint32_t)n) atomicMax(&entry[id], (uint32_t)(i - b0) + 1u);
     }
     __syncthreads();
-    const float rep = p.repetition ? p.repetition[r] : 1.0f, pres = p.presence ? p.presence[r] : 0.0f,
-                freq = p.frequency ? p.frequency[r] : 0.0f;
-    const int mi = p.mask ? (p.mask_index ? p.mask_index[r] : r) : -1;
-    const uint32_t *mask = mi >= 0 && mi < (int)p.n_masks ? p.mask + (size_t)mi * p.mask_stride + t0 / 32 : nullptr;
-    const typename T::E *in = static_cast<const typename T::E *>(p.logits) + (size_t)r * p.logits_stride + t0;
-    typename T::E *out = static_cast<typename T::E *>(p.out) + (size_t)r * p.out_stride + t0;
-    constexpr int V = T::kVec;
-    for (int at = t * V; at < n; at += kPT * V) {
-        float x[V];
-        load_vec<T>(in, at, n, 0.0f, x);
-        const uint32_t allowed = mask ? mask[at / 32] >> (at & 31) : ~0u;
+#pragma unroll
+    for (int i = 0; i < NV; ++i) {
+        const int at = (i * kPT + t) * V;
+        if (at >= n) break;
         uint32_t c[V] = {}, b[V] = {};
         if (p.history) {
 #pragma unroll
-            for (int i = 0; i < V; ++i) c[i] = count[at + i];
+            for (int j = 0; j < V; ++j) c[j] = count[at + j];
         }
         if (p.bias_offsets) {
 #pragma unroll
-            for (int i = 0; i < V; ++i) b[i] = entry[at + i];
+            for (int j = 0; j < V; ++j) b[j] = entry[at + j];
         }
 #pragma unroll
-        for (int i = 0; i < V; ++i) {
-            if (c[i]) {
-                x[i] = x[i] > 0.0f ? x[i] / rep : x[i] * rep;
-                const uint32_t said = c[i] & ~kSeen;
-                if (said) x[i] = (x[i] - freq * (float)said) - pres;
+        for (int j = 0; j < V; ++j) {
+            if (c[j]) {
+                x[i][j] = x[i][j] > 0.0f ? x[i][j] / rep : x[i][j] * rep;
+                const uint32_t said = c[j] & ~kSeen;
+                if (said) x[i][j] = (x[i][j] - freq * (float)said) - pres;
             }
-            if (b[i]) x[i] = x[i] + p.bias_values[b0 + (int)b[i] - 1];
-            if (!((allowed >> i) & 1u)) x[i] = -kInf;
+            if (b[j]) x[i][j] = x[i][j] + p.bias_values[b0 + (int)b[j] - 1];
+            if (!((allowed[i] >> j) & 1u)) x[i][j] = -kInf;
         }
-        store_vec<T>(out, at, n, x);
+        store_vec<T>(out, at, n, x[i]);
     }
 }
 
@@ -223,7 +241,7 @@ struct Row {
     Lds *lds;
     int n;
     float top;
-    double top_d, inv_temp, step;  // step: 32 / temperature
+    double top_d, inv_temp, step, width;  // 32 / temperature, temperature / 32
 
     __device__ __forceinline__ void load(int at, float (&x)[V]) const {
         if constexpr (HELD) {
@@ -269,8 +287,8 @@ struct Row {
     // others: rounding)
     __device__ __forceinline__ void bounds(int b, int e, float &lo, float &hi) const {
         const double slack = __builtin_fabs(top_d) * 0x1p-22 + 0x1p-126;
-        hi = (float)(top_d - (double)b / step + slack);
-        lo = (float)(top_d - (double)e / step - slack);
+        hi = (float)(top_d - (double)b * width + slack);
+        lo = (float)(top_d - (double)e * width - slack);
         if (!(hi < top)) hi = top;
         if (!(lo > -kInf)) lo = -kInf;  // (-infinity - infinity too)
     }
@@ -502,6 +520,7 @@ __global__ __launch_bounds__(kST) void k_sample(GDNSample p, int shift) {
     r.top_d = (double)top;
     r.inv_temp = 1.0 / (double)temp;
     r.step = 32.0 * r.inv_temp;
+    r.width = (double)temp * (1.0 / 32.0);
     float lowest, unused;
     r.bounds(0, kBins, lowest, unused);
 
@@ -529,18 +548,18 @@ __global__ __launch_bounds__(kST) void k_sample(GDNSample p, int shift) {
     // the steps' counts and weights
     double sum = 0.0;
     uint64_t whole = 0;
-    const bool total = by_p && !by_k;
+    const bool total = by_p && !by_k, endless = top == kInf;
     auto sums = [&](auto total_on) __attribute__((always_inline)) {
         r.each([&](const float(&x)[V], int) __attribute__((always_inline)) {
             float s = 0.0f;
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                // exp(-d), the rounding of its base-2 argument made good; 0 for
-                // NaN and what is too small
+                // exp(-d) to (2 + d) 2^-24 of it; 0 for NaN and what is too
+                // small (of two infinities: with the highest's 1 below)
                 constexpr float kL = 1.44269502f, kLo = 1.92596299e-8f;  // log2(e)
-                const float d = x[j] == top ? 0.0f : top - x[j], y = d * kL,
-                            e = __builtin_fmaf(d, kLo, __builtin_fmaf(d, kL, -y)), q = __builtin_amdgcn_exp2f(-y);
-                s += y < 126.0f ? __builtin_fmaf(q, -0.693147181f * e, q) : 0.0f;
+                const float d = top - x[j];
+                s += __builtin_fmaxf(__builtin_amdgcn_exp2f(-__builtin_fmaf(d, kL, d * kLo)), 0.0f);
+                if (endless) s += x[j] == top ? 1.0f : 0.0f;
                 if constexpr (total_on) {
                     const double f = r.fall(x[j]);
                     whole += r.weight(f, r.bin(f));
@@ -551,6 +570,10 @@ __global__ __launch_bounds__(kST) void k_sample(GDNSample p, int shift) {
     };
     auto steps = [&](float from, float below, bool first) __attribute__((always_inline)) {
         r.each([&](const float(&x)[V], int at) __attribute__((always_inline)) {
+            float most = x[0];
+#pragma unroll
+            for (int j = 1; j < V; ++j) most = __builtin_fmaxf(most, x[j]);
+            if (!(most >= from)) return;
 #pragma unroll
             for (int j = 0; j < V; ++j)
                 if (x[j] >= from && !(x[j] >= below)) {  // (below NaN: all)
