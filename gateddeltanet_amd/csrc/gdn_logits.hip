@@ -214,22 +214,21 @@ struct SampleLds {
     uint32_t bin, n, n_high;
 };
 
-// The sum over the workgroup before each thread, and the whole sum; `turn`
-// alternates between calls.
+__device__ __forceinline__ uint64_t lane_of(uint64_t v, int lane) {
+    return ((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)(v >> 32), lane) << 32) |
+           (uint32_t)__builtin_amdgcn_readlane((int)v, lane);
+}
+// The sum over the workgroup before each thread, and the whole sum.  Between
+// two uses of one `wsum` stands a barrier.
 __device__ __forceinline__ uint64_t block_scan(uint64_t v, uint64_t (&wsum)[kWaves], uint64_t &total) {
-    const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    static_assert(kWaves <= 64, "a lane a wave");
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint64_t s = wave_scan64(v);
     if (lane == 63) wsum[w] = s;
     __syncthreads();
-    uint64_t at = 0, all = 0;
-#pragma unroll
-    for (int i = 0; i < kWaves; ++i) {
-        const uint64_t o = wsum[i];
-        at += i < w ? o : 0;
-        all += o;
-    }
-    total = all;
-    return at + s - v;
+    const uint64_t waves = wave_scan64(lane < kWaves ? wsum[lane] : 0);
+    total = lane_of(waves, kWaves - 1);
+    return (w ? lane_of(waves, w - 1) : 0) + s - v;
 }
 
 // A row and how its tokens fall and weigh.
@@ -486,12 +485,12 @@ __global__ __launch_bounds__(kST) void k_sample(GDNSample p, int shift) {
         r.each(higher);
     }
     const float own_top = top;
-    {
-        const float most = u2f(wave_reduce64(f2u(top), [](uint32_t a, uint32_t b) { return f2u(__builtin_fmaxf(u2f(a), u2f(b))); }));
-        arg = top == most ? arg : 0x7fffffff;
-        top = most;
-        arg = (int)wave_reduce64((uint32_t)arg, [](uint32_t a, uint32_t b) { return a < b ? a : b; });
-    }
+    // the highest of a wave's values and its first place, in every lane
+    auto first_of_highest = [&](float v, int at) __attribute__((always_inline)) {
+        top = u2f(wave_reduce64(f2u(v), [](uint32_t a, uint32_t b) { return f2u(__builtin_fmaxf(u2f(a), u2f(b))); }));
+        arg = (int)wave_reduce64((uint32_t)(v == top ? at : 0x7fffffff), [](uint32_t a, uint32_t b) { return a < b ? a : b; });
+    };
+    first_of_highest(top, arg);
     if (lane == 0) {
         lds.wmax[w] = top;
         lds.warg[w] = arg;
@@ -500,15 +499,7 @@ __global__ __launch_bounds__(kST) void k_sample(GDNSample p, int shift) {
     lds.count[t] = 0;
     lds.mass[t] = 0;
     __syncthreads();
-#pragma unroll
-    for (int i = 0; i < kWaves; ++i) {
-        const float m = lds.wmax[i];
-        const int a = lds.warg[i];
-        if (m > top || (m == top && a < arg)) {
-            top = m;
-            arg = a;
-        }
-    }
+    first_of_highest(lane < kWaves ? lds.wmax[lane] : -kInf, lane < kWaves ? lds.warg[lane] : 0x7fffffff);
     if (arg == 0x7fffffff) {  // nothing above -infinity
         if (t == 0) {
             p.tokens[ri] = -1;
