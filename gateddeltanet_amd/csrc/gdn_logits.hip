@@ -202,7 +202,8 @@ struct SampleLds {
         Ranked list[kList];
         uint64_t cell[kCells];
     };
-    Ranked high[kList];  // the tokens above the bound
+    float high[kWaves][64];  // the tokens above the bound that a wave met, and their places
+    int high_at[kWaves][64];
     uint64_t wsum[2][kWaves];
     float wmax[kWaves];
     int warg[kWaves];
@@ -211,7 +212,7 @@ struct SampleLds {
     double left;      // of the goal, in it
     float x;          // a border
     int at;
-    uint32_t bin, n, n_high;
+    uint32_t bin, n, crowded;
 };
 
 __device__ __forceinline__ uint64_t lane_of(uint64_t v, int lane) {
@@ -295,10 +296,10 @@ struct Row {
 
 // The border of the tokens of step `b` whose ranked counts (by_mass: weights)
 // first reach `left`, into lds.x and lds.at; their weight is the result.
-// listed: the step's tokens are all in lds.high.
+// listed: the step's tokens are among the threads' `own` (none: at < 0).
 template <class T, bool HELD>
 __device__ __forceinline__ uint64_t border_in(const Row<T, HELD> &r, SampleLds<T, HELD> &lds, int b, bool by_mass,
-                                              double left, bool listed) {
+                                              double left, bool listed, const Ranked &own) {
     constexpr int V = T::kVec;
     const int t = threadIdx.x;
     float lo, hi;
@@ -307,7 +308,10 @@ __device__ __forceinline__ uint64_t border_in(const Row<T, HELD> &r, SampleLds<T
     if (t == 0) lds.n = 0;
     __syncthreads();
     if (listed) {
-        if (t < (int)lds.n_high && r.bin(r.fall(lds.high[t].x)) == b) lds.list[atomicAdd(&lds.n, 1u)] = lds.high[t];
+        if (own.at >= 0 && r.bin(r.fall(own.x)) == b) {
+            const uint32_t i = atomicAdd(&lds.n, 1u);
+            if (i < (uint32_t)kList) lds.list[i] = own;
+        }
     } else {
         r.each([&](const float(&x)[V], int at) __attribute__((always_inline)) {
 #pragma unroll
@@ -523,7 +527,7 @@ __global__ __launch_bounds__(kST) void k_sample(GDNSample p, int shift) {
         if (b < kBins) atomicAdd(&lds.count[b], 1u);
         if (t == 0) {
             lds.bin = kBins;
-            lds.n_high = 0;
+            lds.crowded = 0;
         }
         __syncthreads();
         const uint64_t n = lds.count[t], enough = by_k ? (uint64_t)k : 64;
@@ -559,28 +563,52 @@ __global__ __launch_bounds__(kST) void k_sample(GDNSample p, int shift) {
             sum += (double)s;
         });
     };
-    auto steps = [&](float from, float below, bool first) __attribute__((always_inline)) {
-        r.each([&](const float(&x)[V], int at) __attribute__((always_inline)) {
-            float most = x[0];
-#pragma unroll
-            for (int j = 1; j < V; ++j) most = __builtin_fmaxf(most, x[j]);
-            if (!(most >= from)) return;
+    auto count_in = [&](float v) __attribute__((always_inline)) -> uint64_t {
+        const double d = r.fall(v);
+        const int b = r.bin(d);
+        const uint64_t s = r.weight(d, b);
+        if (b < kBins) {
+            if (by_k) atomicAdd(&lds.count[b], 1u);
+            if (by_p) atomicAdd(&lds.mass[b], (unsigned long long)s);
+        }
+        return s;
+    };
+    auto steps = [&](float from, float below) __attribute__((always_inline)) {
+        r.each([&](const float(&x)[V], int) __attribute__((always_inline)) {
 #pragma unroll
             for (int j = 0; j < V; ++j)
-                if (x[j] >= from && !(x[j] >= below)) {  // (below NaN: all)
-                    const double d = r.fall(x[j]);
-                    const int b = r.bin(d);
-                    if (b < kBins) {
-                        const uint64_t s = r.weight(d, b);
-                        if (by_k) atomicAdd(&lds.count[b], 1u);
-                        if (by_p) atomicAdd(&lds.mass[b], (unsigned long long)s);
-                        if (first) {
-                            const uint32_t i = atomicAdd(&lds.n_high, 1u);
-                            if (i < (uint32_t)kList) lds.high[i] = Ranked{x[j], at + j, s};
-                        }
-                    }
-                }
+                if (x[j] >= from && !(x[j] >= below)) count_in(x[j]);  // (below NaN: all)
         });
+    };
+    // the tokens above the bound, a thread each: few lie among many, so the
+    // waves gather theirs before anything is formed from them.  False if one
+    // met more than it has lanes
+    Ranked own = {0.0f, -1, 0};
+    auto gather = [&]() __attribute__((always_inline)) {
+        int n = 0;  // the wave's
+        r.each([&](const float(&x)[V], int at) __attribute__((always_inline)) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const uint64_t who = __ballot(x[j] >= bound);
+                if (who == 0) continue;
+                const int i = n + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0u));
+                if (x[j] >= bound && i < 64) {
+                    lds.high[w][i] = x[j];
+                    lds.high_at[w][i] = at + j;
+                }
+                n += __builtin_popcountll(who);
+            }
+        });
+        n = __builtin_amdgcn_readfirstlane(n);
+        if (n > 64 && lane == 0) lds.crowded = 1;
+        __syncthreads();
+        if (lds.crowded) return false;
+        if (lane < n) {
+            own.x = lds.high[w][lane];
+            own.at = lds.high_at[w][lane];
+            own.w = count_in(own.x);
+        }
+        return true;
     };
     if (total) sums(std::true_type());
     else if (p.logprobs) sums(std::false_type());
@@ -610,17 +638,20 @@ __global__ __launch_bounds__(kST) void k_sample(GDNSample p, int shift) {
     // the border: higher tokens are kept, of its logit those up to edge_at
     float edge = -kInf;
     int edge_at = 0x7fffffff;
-    bool listed = false;  // what is kept is in lds.high
+    bool listed = false;  // what is kept is among the threads' own
     if (by_k || by_p) {
-        steps(bound, __builtin_nanf(""), bound > lowest);
+        listed = bound > lowest && gather();
+        if (!listed) {
+            own.at = -1;
+            steps(bound, __builtin_nanf(""));
+        }
         __syncthreads();
-        listed = bound > lowest && lds.n_high <= (uint32_t)kList;
         uint64_t count = lds.count[t], mass = lds.mass[t], n_all = 0, m_all = 0, n_before = 0, m_before = 0;
         if (by_p) m_before = block_scan(mass, lds.wsum[0], m_all);
         if (by_k) n_before = block_scan(count, lds.wsum[1], n_all);
         if (total && (double)m_all < (double)tp * (double)kept) {
             listed = false;
-            steps(lowest, bound, false);
+            steps(lowest, bound);
             __syncthreads();
             mass = lds.mass[t];
             m_before = block_scan(mass, lds.wsum[1], m_all);
@@ -632,16 +663,16 @@ __global__ __launch_bounds__(kST) void k_sample(GDNSample p, int shift) {
             const bool by_mass = turn == 1;
             if (by_mass ? !by_p : !by_k || (uint64_t)k > n_all) continue;
             const double goal = by_mass ? (double)tp * (double)kept : (double)k;
-            const uint64_t before = by_mass ? m_before : n_before, own = by_mass ? mass : count;
+            const uint64_t before = by_mass ? m_before : n_before, here = by_mass ? mass : count;
             __syncthreads();
-            if (own != 0 && (double)before < goal && (double)(before + own) >= goal) {
+            if (here != 0 && (double)before < goal && (double)(before + here) >= goal) {
                 lds.bin = t;
                 lds.left = goal - (double)before;
                 lds.base = m_before;
             }
             __syncthreads();
             const uint64_t base = lds.base;
-            kept = base + border_in(r, lds, (int)lds.bin, by_mass, lds.left, listed);
+            kept = base + border_in(r, lds, (int)lds.bin, by_mass, lds.left, listed, own);
             if (lds.x > edge || (lds.x == edge && lds.at < edge_at)) {
                 edge = lds.x;
                 edge_at = lds.at;
@@ -667,11 +698,8 @@ __global__ __launch_bounds__(kST) void k_sample(GDNSample p, int shift) {
     if (listed) {
         for (int c = t; c < cells; c += kST) lds.cell[c] = 0;
         __syncthreads();
-        if (t < (int)lds.n_high) {
-            const Ranked h = lds.high[t];
-            if ((h.x > edge || (h.x == edge && h.at <= edge_at)) && (double)h.w >= least)
-                atomicAdd(reinterpret_cast<unsigned long long *>(&lds.cell[h.at / (64 * V)]), (unsigned long long)h.w);
-        }
+        if (own.at >= 0 && (own.x > edge || (own.x == edge && own.at <= edge_at)) && (double)own.w >= least)
+            atomicAdd(reinterpret_cast<unsigned long long *>(&lds.cell[own.at / (64 * V)]), (unsigned long long)own.w);
     }
     for (int c = listed ? cells : w; c < cells; c += kWaves) {
         const int at = (c * 64 + lane) * V;
@@ -702,15 +730,15 @@ __global__ __launch_bounds__(kST) void k_sample(GDNSample p, int shift) {
     if (w == 0) {
         const int c0 = (int)lds.bin * 64 * V + lane * V;
         float y[V];
-        uint64_t s[V], own = 0;
+        uint64_t s[V], mine_w = 0;
         if (c0 < r.n) r.load(c0, y);
 #pragma unroll
         for (int j = 0; j < V; ++j) {
             s[j] = c0 < r.n ? weight(y[j], c0 + j) : 0;
-            own += s[j];
+            mine_w += s[j];
         }
-        uint64_t run = lds.base + wave_scan64(own) - own;
-        if (run <= goal && run + own > goal) {
+        uint64_t run = lds.base + wave_scan64(mine_w) - mine_w;
+        if (run <= goal && run + mine_w > goal) {
             int j = 0;
 #pragma unroll
             for (int i = 0; i < V; ++i) {
