@@ -205,7 +205,8 @@ SIGNATURES = {
     "gdn_delta_prefill": (c_int, [POINTER(GDNDelta), c_void_p, c_size_t, c_void_p]),
     "gdn_delta_step": (c_int, [POINTER(GDNDelta), c_void_p]),
     "gdn_logits_process": (c_int, [POINTER(GDNLogits), c_void_p]),
-    "gdn_sample_tokens": (c_int, [POINTER(GDNSample), c_void_p]),
+    "gdn_sample_workspace": (c_size_t, [POINTER(GDNSample)]),
+    "gdn_sample_tokens": (c_int, [POINTER(GDNSample), c_void_p, c_size_t, c_void_p]),
     "gdn_model_load": (c_int, [POINTER(GDNModel), ctypes.c_char_p]),
     "gdn_model_load_fp32": (c_int, [POINTER(GDNModel), ctypes.c_char_p]),
     "gdn_model_free": (None, [POINTER(GDNModel)]),

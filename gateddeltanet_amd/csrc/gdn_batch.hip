@@ -2933,7 +2933,12 @@ int b_sample(GDNBatchEngine *e, const GDNBatchSampling &h, int32_t *tokens, floa
                  boff = add(n_bias ? h.bias_offsets : nullptr, n + 1), bid = add(n_bias ? h.bias_ids : nullptr, n_bias),
                  bval = add(n_bias ? h.bias_values : nullptr, n_bias), mask = add(h.mask, (size_t)n * words),
                  uni = add(h.uniform, n), temp = add(h.temperature, n), tk = add(h.top_k, n), tp = add(h.top_p, n),
-                 mp = add(h.min_p, n), out = (blk.bytes.size() + 15) / 16 * 16, need = out + (size_t)n * 8;
+                 mp = add(h.min_p, n), out = (blk.bytes.size() + 15) / 16 * 16, work = out + (size_t)(n + 1) / 2 * 16;
+    GDNSample s = {};
+    s.dtype = GDN_DTYPE_FP32;
+    s.rows = n;
+    s.vocab = e->vocab;
+    const size_t work_bytes = gdn_sample_workspace(&s), need = work + work_bytes;
     if (need > e->c_args_cap) {
         (void)hipFree(e->c_args);
         e->c_args = nullptr;
@@ -2976,10 +2981,6 @@ int b_sample(GDNBatchEngine *e, const GDNBatchSampling &h, int32_t *tokens, floa
         a.mask = static_cast<const uint32_t *>(at(mask));
         if (gdn_logits_process(&a, e->stream) != 0) return -1;
     }
-    GDNSample s = {};
-    s.dtype = GDN_DTYPE_FP32;
-    s.rows = n;
-    s.vocab = e->vocab;
     s.logits_stride = e->vocab;
     s.logits = any ? e->c_logits : e->logits;
     s.uniform = static_cast<const float *>(at(uni));
@@ -2989,7 +2990,7 @@ int b_sample(GDNBatchEngine *e, const GDNBatchSampling &h, int32_t *tokens, floa
     s.min_p = static_cast<const float *>(at(mp));
     s.tokens = reinterpret_cast<int32_t *>(e->c_args + out);
     s.logprobs = reinterpret_cast<float *>(e->c_args + out + (size_t)n * 4);
-    if (gdn_sample_tokens(&s, e->stream) != 0) return -1;
+    if (gdn_sample_tokens(&s, e->c_args + work, work_bytes, e->stream) != 0) return -1;
     GDN_HIP(hipMemcpyAsync(tokens, s.tokens, (size_t)n * 4, hipMemcpyDeviceToHost, e->stream));
     if (logprobs) GDN_HIP(hipMemcpyAsync(logprobs, s.logprobs, (size_t)n * 4, hipMemcpyDeviceToHost, e->stream));
     GDN_HIP(hipStreamSynchronize(e->stream));

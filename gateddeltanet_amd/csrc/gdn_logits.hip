@@ -174,6 +174,7 @@ constexpr int kST = 1024, kBins = kST, kWaves = kST / 64;
 constexpr int kList = 512;             // tokens of a step that are ranked directly
 constexpr int kHeldBytes = 128 << 10;  // of a row in LDS
 constexpr int kMostVocab = 1 << 20;
+constexpr int kNowhere = 0x7fffffff;
 
 // The 32-bit key of x that grows as x falls (x not NaN; the zeros are equal).
 __device__ __forceinline__ uint32_t fall_key(float x) {
@@ -193,7 +194,6 @@ struct SampleLds {
     // pieces of 64 vectors
     static constexpr int kCells = (HELD ? kHeld : kMostVocab) / (64 * T::kVec);
     typename T::E held[kHeld] __attribute__((aligned(16)));
-    double power[kBins];  // exp(-b / 32) 2^shift
     union {
         struct {
             unsigned long long mass[kBins];
@@ -241,8 +241,19 @@ struct Row {
     Lds *lds;
     int n;
     float top;
-    double top_d, inv_temp, step, width;  // 32 / temperature, temperature / 32
+    bool endless;  // the highest is infinity
+    int shift;
+    double top_d, rate, step, width;  // log2(e) / temperature, 32 / temperature, temperature / 32
 
+    __device__ __forceinline__ void set(float highest, float temp, int to) {
+        top = highest;
+        top_d = (double)highest;
+        endless = highest == kInf;
+        shift = to;
+        rate = 1.44269504088896340736 / (double)temp;
+        step = 32.0 / (double)temp;
+        width = (double)temp * (1.0 / 32.0);
+    }
     __device__ __forceinline__ void load(int at, float (&x)[V]) const {
         if constexpr (HELD) {
             const Vec<T> v = *reinterpret_cast<const Vec<T> *>(__builtin_assume_aligned(&lds->held[at], 16));
@@ -263,17 +274,25 @@ struct Row {
             f(x, at);
         }
     }
-    // how far below the highest; NaN for NaN, whose bin is that of infinity
-    __device__ __forceinline__ double fall(float v) const { return v == top ? 0.0 : top_d - (double)v; }
+    // how far below the highest; NaN for NaN, whose bin and weight are those of
+    // infinity
+    __device__ __forceinline__ double fall(float v) const {
+        if (endless) return v == top ? 0.0 : (double)kInf;
+        return top_d - (double)v;
+    }
     // kBins where the weight is 0: exp(-32) is half a unit of 2^-45
     __device__ __forceinline__ int bin(double d) const { return (int)__builtin_fmin(d * step, (double)kBins); }
-    // exp(-d / temperature) 2^shift, rounded to a whole number: from the
-    // step's power and the Taylor series of what is left (1 / 32 at most: the
-    // first term left out is 6e-15)
-    __device__ __forceinline__ uint64_t weight(double d, int b) const {
-        if (b >= kBins) return 0;
-        const double t = __builtin_fma(-d, inv_temp, (double)b * (1.0 / 32.0));
-        double y = 1.0 / 720.0;
+    // exp(-d / temperature) 2^shift, rounded to a whole number: the Taylor
+    // series of the exponential about the nearest power of two (|t| <= ln 2 / 2:
+    // the first term left out is 6e-15)
+    __device__ __forceinline__ uint64_t weight(double d) const {
+        const double z = __builtin_fmin(d * rate, 1000.0), n = __builtin_rint(z), t = (n - z) * 0.69314718055994530942;
+        double y = 1.0 / 39916800.0;
+        y = __builtin_fma(y, t, 1.0 / 3628800.0);
+        y = __builtin_fma(y, t, 1.0 / 362880.0);
+        y = __builtin_fma(y, t, 1.0 / 40320.0);
+        y = __builtin_fma(y, t, 1.0 / 5040.0);
+        y = __builtin_fma(y, t, 1.0 / 720.0);
         y = __builtin_fma(y, t, 1.0 / 120.0);
         y = __builtin_fma(y, t, 1.0 / 24.0);
         y = __builtin_fma(y, t, 1.0 / 6.0);
@@ -281,7 +300,7 @@ struct Row {
         y = __builtin_fma(y, t, 1.0);
         y = __builtin_fma(y, t, 1.0);
         // the sum's low bits are the rounded number
-        return __builtin_bit_cast(uint64_t, __builtin_fma(lds->power[b], y, 0x1p52)) & 0xfffffffffffffull;
+        return __builtin_bit_cast(uint64_t, __builtin_ldexp(y, shift - (int)n) + 0x1p52) & 0xfffffffffffffull;
     }
     // FP32 bounds that hold every token of the steps b .. e - 1 (and a few
     // others: rounding)
@@ -320,7 +339,7 @@ __device__ __forceinline__ uint64_t border_in(const Row<T, HELD> &r, SampleLds<T
                     const double d = r.fall(x[j]);
                     if (r.bin(d) == b) {
                         const uint32_t i = atomicAdd(&lds.n, 1u);
-                        if (i < (uint32_t)kList) lds.list[i] = Ranked{x[j], at + j, r.weight(d, b)};
+                        if (i < (uint32_t)kList) lds.list[i] = Ranked{x[j], at + j, r.weight(d)};
                     }
                 }
         });
@@ -368,7 +387,7 @@ __device__ __forceinline__ uint64_t border_in(const Row<T, HELD> &r, SampleLds<T
                     const uint32_t key = fall_key(x[j]);
                     if (r.bin(d) == b && (key & above) == prefix) {
                         atomicAdd(&lds.count[(key >> sh) & bits], 1u);
-                        atomicAdd(&lds.mass[(key >> sh) & bits], (unsigned long long)r.weight(d, b));
+                        atomicAdd(&lds.mass[(key >> sh) & bits], (unsigned long long)r.weight(d));
                     }
                 }
         });
@@ -430,38 +449,181 @@ __device__ __forceinline__ uint64_t border_in(const Row<T, HELD> &r, SampleLds<T
     return base + need * each_w;
 }
 
+// What a row is asked for.
+struct Ask {
+    float temp, top_p, min_p;
+    int k;
+    double u;
+    bool greedy, first_only, by_k, by_p;
+    __device__ __forceinline__ Ask(const GDNSample &p, int r) {
+        temp = p.temperature ? p.temperature[r] : 0.0f;
+        k = p.top_k ? p.top_k[r] : 0;
+        top_p = p.top_p ? p.top_p[r] : 1.0f;
+        min_p = p.min_p ? p.min_p[r] : 0.0f;
+        u = p.temperature ? (double)p.uniform[r] : 0.0;
+        greedy = !(temp > 0.0f);
+        first_only = top_p <= 0.0f;
+        by_k = !greedy && !first_only && k > 0 && k < (int)p.vocab;
+        by_p = !greedy && !first_only && top_p < 1.0f;
+    }
+};
+
+// The highest of a wave's values and its first place, in every lane.
+__device__ __forceinline__ void first_of_highest(float &v, int &at) {
+    const float most = u2f(wave_reduce64(f2u(v), [](uint32_t a, uint32_t b) { return f2u(__builtin_fmaxf(u2f(a), u2f(b))); }));
+    at = (int)wave_reduce64((uint32_t)(v == most ? at : kNowhere), [](uint32_t a, uint32_t b) { return a < b ? a : b; });
+    v = most;
+}
+template <class T>
+__device__ __forceinline__ void higher(const float (&x)[T::kVec], int at, float &top, int &arg) {
+#pragma unroll
+    for (int j = 0; j < T::kVec; ++j)
+        if (x[j] > top) {
+            top = x[j];
+            arg = at + j;
+        }
+}
+
+// The sum of exp(x - top), each to (2 + d) 2^-24 of it; 0 for NaN and what is
+// too small (of two infinities: with the highest's 1).
+template <class R, int V>
+__device__ __forceinline__ float exponentials(const R &r, const float (&x)[V]) {
+    constexpr float kL = 1.44269502f, kLo = 1.92596299e-8f;  // log2(e)
+    float s = 0.0f;
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        const float d = r.top - x[j];
+        s += __builtin_fmaxf(__builtin_amdgcn_exp2f(-__builtin_fmaf(d, kL, d * kLo)), 0.0f);
+        if (r.endless) s += x[j] == r.top ? 1.0f : 0.0f;
+    }
+    return s;
+}
+
+// What is kept: tokens above `edge`, of its logit those up to place edge_at, of
+// weight `least` and more.
+struct Keep {
+    float edge = -kInf, from = -kInf;
+    int edge_at = kNowhere;
+    double least = 0.0;
+    template <class R>
+    __device__ __forceinline__ void finish(const R &r, const Ask &ask, float lowest) {
+        from = edge > lowest ? edge : lowest;
+        least = ask.min_p > 0.0f ? __builtin_ldexp((double)__builtin_fminf(ask.min_p, 1.0f), r.shift) : 0.0;
+    }
+    __device__ __forceinline__ bool has(float x, int at) const { return x > edge || (x == edge && at <= edge_at); }
+    template <class R>
+    __device__ __forceinline__ uint64_t weight(const R &r, float x, int at) const {
+        if (!(x >= from) || (x == edge && at > edge_at)) return 0;
+        const uint64_t s = r.weight(r.fall(x));
+        return (double)s >= least ? s : 0;
+    }
+    // of the 64 V tokens from `c`, in lane 63
+    template <class R>
+    __device__ __forceinline__ uint64_t piece(const R &r, int c, int lane) const {
+        const int at = (c * 64 + lane) * R::V;
+        uint64_t s = 0;
+        if (at < r.n) {
+            float x[R::V];
+            r.load(at, x);
+#pragma unroll
+            for (int j = 0; j < R::V; ++j) s += weight(r, x[j], at + j);
+        }
+        return __ballot(s != 0) != 0 ? wave_scan64(s) : 0;
+    }
+};
+
+// The borders asked for, from the steps' counts and weights (a thread a step);
+// `kept`: the weight that top-p is a share of, unless top-k gives another.
 template <class T, bool HELD>
+__device__ __forceinline__ void borders(const Row<T, HELD> &r, SampleLds<T, HELD> &lds, const Ask &ask, uint64_t count,
+                                        uint64_t mass, uint64_t n_before, uint64_t m_before, uint64_t n_all, uint64_t kept,
+                                        bool listed, const Ranked &own, Keep &keep) {
+    // by counts, then by weights: tokens past the first border rank behind all
+    // that reach the second goal, which is less than the whole weight
+    for (int turn = 0; turn < 2; ++turn) {
+        const bool by_mass = turn == 1;
+        if (by_mass ? !ask.by_p : !ask.by_k || (uint64_t)ask.k > n_all) continue;
+        const double goal = by_mass ? (double)ask.top_p * (double)kept : (double)ask.k;
+        const uint64_t before = by_mass ? m_before : n_before, here = by_mass ? mass : count;
+        __syncthreads();
+        if (here != 0 && (double)before < goal && (double)(before + here) >= goal) {
+            lds.bin = threadIdx.x;
+            lds.left = goal - (double)before;
+            lds.base = m_before;
+        }
+        __syncthreads();
+        const uint64_t base = lds.base;
+        kept = base + border_in(r, lds, (int)lds.bin, by_mass, lds.left, listed, own);
+        if (lds.x > keep.edge || (lds.x == keep.edge && lds.at < keep.edge_at)) {
+            keep.edge = lds.x;
+            keep.edge_at = lds.at;
+        }
+    }
+}
+
+// The token up to which the pieces' kept weights (lds.cell) reach the draw, in
+// one lane of wave 0; -1 elsewhere.
+template <class T, bool HELD>
+__device__ __forceinline__ int drawn(const Row<T, HELD> &r, SampleLds<T, HELD> &lds, const Keep &keep, double u) {
+    constexpr int V = T::kVec;
+    const int t = threadIdx.x, lane = t & 63, w = t >> 6;
+    const int cells = (r.n + 64 * V - 1) / (64 * V), per = (cells + kST - 1) / kST;
+    uint64_t mine = 0, all;
+    for (int i = 0; i < per; ++i) mine += t * per + i < cells ? lds.cell[t * per + i] : 0;
+    uint64_t at = block_scan(mine, lds.wsum[0], all);
+    uint64_t goal = u > 0.0 ? (uint64_t)__builtin_fmin(u * (double)all, 9.2e18) : 0;
+    goal = goal < all ? goal : all - 1;
+    if (at <= goal && at + mine > goal) {
+        int c = t * per;
+        while (at + lds.cell[c] <= goal) at += lds.cell[c++];
+        lds.bin = (uint32_t)c;
+        lds.base = at;
+    }
+    __syncthreads();
+    if (w != 0) return -1;
+    const int c0 = (int)lds.bin * 64 * V + lane * V;
+    float y[V];
+    uint64_t s[V], here = 0;
+    if (c0 < r.n) r.load(c0, y);
+#pragma unroll
+    for (int j = 0; j < V; ++j) {
+        s[j] = c0 < r.n ? keep.weight(r, y[j], c0 + j) : 0;
+        here += s[j];
+    }
+    uint64_t run = lds.base + wave_scan64(here) - here;
+    if (!(run <= goal && run + here > goal)) return -1;
+    int j = 0;
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        if (run + s[i] <= goal) {
+            run += s[i];
+            j = i + 1;
+        } else {
+            break;
+        }
+    }
+    return c0 + j;
+}
+
+// Rows that LDS holds.
+template <class T>
 __global__ __launch_bounds__(kST) void k_sample(GDNSample p, int shift) {
     constexpr int V = T::kVec;
-    __shared__ SampleLds<T, HELD> lds;
+    __shared__ SampleLds<T, true> lds;
     static_assert(sizeof(lds) <= 160 << 10, "the LDS of a CU");
     const int ri = blockIdx.x, t = threadIdx.x, lane = t & 63, w = t >> 6;
-    Row<T, HELD> r;
+    Row<T, true> r;
     r.row = static_cast<const typename T::E *>(p.logits) + (size_t)ri * p.logits_stride;
     r.n = (int)p.vocab;
     r.lds = &lds;
+    const Ask ask(p, ri);
 
-    const float temp = p.temperature ? p.temperature[ri] : 0.0f;
-    const int k = p.top_k ? p.top_k[ri] : 0;
-    const float tp = p.top_p ? p.top_p[ri] : 1.0f, mp = p.min_p ? p.min_p[ri] : 0.0f;
-    const double u = p.temperature ? (double)p.uniform[ri] : 0.0;
-    const bool greedy = !(temp > 0.0f), first_only = tp <= 0.0f;
-    const bool by_k = !greedy && !first_only && k > 0 && k < r.n, by_p = !greedy && !first_only && tp < 1.0f;
-
-    // the highest logit, and its first place
+    // the highest logit, and its first place; every vector of a thread on its
+    // way at a time
     float top = -kInf;
-    int arg = 0x7fffffff;
-    auto higher = [&](const float(&x)[V], int at) __attribute__((always_inline)) {
-#pragma unroll
-        for (int j = 0; j < V; ++j)
-            if (x[j] > top) {
-                top = x[j];
-                arg = at + j;
-            }
-    };
-    if constexpr (HELD) {
-        // every vector of a thread on its way at a time
-        constexpr int kAhead = SampleLds<T, HELD>::kHeld / (kST * V);
+    int arg = kNowhere;
+    {
+        constexpr int kAhead = SampleLds<T, true>::kHeld / (kST * V);
         const int whole = r.n / V, rest = r.n % V;
         if (whole > 0) {
             Vec<T> v[kAhead];
@@ -474,55 +636,45 @@ __global__ __launch_bounds__(kST) void k_sample(GDNSample p, int shift) {
                     float x[V];
 #pragma unroll
                     for (int j = 0; j < V; ++j) x[j] = T::get(v[i].e[j]);
-                    higher(x, (i * kST + t) * V);
+                    higher<T>(x, (i * kST + t) * V, top, arg);
                     *reinterpret_cast<Vec<T> *>(__builtin_assume_aligned(&lds.held[(i * kST + t) * V], 16)) = v[i];
                 }
         }
         if (rest > 0 && t == kST - 1) {
             float x[V];
             load_vec<T>(r.row, whole * V, r.n, __builtin_nanf(""), x);
-            higher(x, whole * V);
+            higher<T>(x, whole * V, top, arg);
 #pragma unroll
             for (int j = 0; j < V; ++j) lds.held[whole * V + j] = T::put(x[j]);
         }
-    } else {
-        r.each(higher);
     }
     const float own_top = top;
-    // the highest of a wave's values and its first place, in every lane
-    auto first_of_highest = [&](float v, int at) __attribute__((always_inline)) {
-        top = u2f(wave_reduce64(f2u(v), [](uint32_t a, uint32_t b) { return f2u(__builtin_fmaxf(u2f(a), u2f(b))); }));
-        arg = (int)wave_reduce64((uint32_t)(v == top ? at : 0x7fffffff), [](uint32_t a, uint32_t b) { return a < b ? a : b; });
-    };
     first_of_highest(top, arg);
     if (lane == 0) {
         lds.wmax[w] = top;
         lds.warg[w] = arg;
     }
-    if (!greedy) lds.power[t] = __builtin_ldexp(exp(-(double)t / 32.0), shift);
     lds.count[t] = 0;
     lds.mass[t] = 0;
     __syncthreads();
-    first_of_highest(lane < kWaves ? lds.wmax[lane] : -kInf, lane < kWaves ? lds.warg[lane] : 0x7fffffff);
-    if (arg == 0x7fffffff) {  // nothing above -infinity
+    top = lane < kWaves ? lds.wmax[lane] : -kInf;
+    arg = lane < kWaves ? lds.warg[lane] : kNowhere;
+    first_of_highest(top, arg);
+    if (arg == kNowhere) {  // nothing above -infinity
         if (t == 0) {
             p.tokens[ri] = -1;
             if (p.logprobs) p.logprobs[ri] = -kInf;
         }
         return;
     }
-    r.top = top;
-    r.top_d = (double)top;
-    r.inv_temp = 1.0 / (double)temp;
-    r.step = 32.0 * r.inv_temp;
-    r.width = (double)temp * (1.0 / 32.0);
+    r.set(top, ask.temp, shift);
     float lowest, unused;
     r.bounds(0, kBins, lowest, unused);
 
     // as many tokens as are asked for are no lower than `bound`: every thread's
     // highest, counted by steps, tells (for top-p a guess, made good below)
     float bound = lowest;
-    if (by_k || by_p) {
+    if (ask.by_k || ask.by_p) {
         const int b = r.bin(r.fall(own_top));
         if (b < kBins) atomicAdd(&lds.count[b], 1u);
         if (t == 0) {
@@ -530,7 +682,7 @@ __global__ __launch_bounds__(kST) void k_sample(GDNSample p, int shift) {
             lds.crowded = 0;
         }
         __syncthreads();
-        const uint64_t n = lds.count[t], enough = by_k ? (uint64_t)k : 64;
+        const uint64_t n = lds.count[t], enough = ask.by_k ? (uint64_t)ask.k : 64;
         lds.count[t] = 0;
         uint64_t all;
         const uint64_t before = block_scan(n, lds.wsum[0], all);
@@ -543,33 +695,22 @@ __global__ __launch_bounds__(kST) void k_sample(GDNSample p, int shift) {
     // the steps' counts and weights
     double sum = 0.0;
     uint64_t whole = 0;
-    const bool total = by_p && !by_k, endless = top == kInf;
-    auto sums = [&](auto total_on) __attribute__((always_inline)) {
+    const bool total = ask.by_p && !ask.by_k;
+    if (total)
         r.each([&](const float(&x)[V], int) __attribute__((always_inline)) {
-            float s = 0.0f;
+            sum += (double)exponentials(r, x);
 #pragma unroll
-            for (int j = 0; j < V; ++j) {
-                // exp(-d) to (2 + d) 2^-24 of it; 0 for NaN and what is too
-                // small (of two infinities: with the highest's 1 below)
-                constexpr float kL = 1.44269502f, kLo = 1.92596299e-8f;  // log2(e)
-                const float d = top - x[j];
-                s += __builtin_fmaxf(__builtin_amdgcn_exp2f(-__builtin_fmaf(d, kL, d * kLo)), 0.0f);
-                if (endless) s += x[j] == top ? 1.0f : 0.0f;
-                if constexpr (total_on) {
-                    const double f = r.fall(x[j]);
-                    whole += r.weight(f, r.bin(f));
-                }
-            }
-            sum += (double)s;
+            for (int j = 0; j < V; ++j) whole += r.weight(r.fall(x[j]));
         });
-    };
+    else if (p.logprobs)
+        r.each([&](const float(&x)[V], int) __attribute__((always_inline)) { sum += (double)exponentials(r, x); });
     auto count_in = [&](float v) __attribute__((always_inline)) -> uint64_t {
         const double d = r.fall(v);
         const int b = r.bin(d);
-        const uint64_t s = r.weight(d, b);
+        const uint64_t s = r.weight(d);
         if (b < kBins) {
-            if (by_k) atomicAdd(&lds.count[b], 1u);
-            if (by_p) atomicAdd(&lds.mass[b], (unsigned long long)s);
+            if (ask.by_k) atomicAdd(&lds.count[b], 1u);
+            if (ask.by_p) atomicAdd(&lds.mass[b], (unsigned long long)s);
         }
         return s;
     };
@@ -610,8 +751,6 @@ __global__ __launch_bounds__(kST) void k_sample(GDNSample p, int shift) {
         }
         return true;
     };
-    if (total) sums(std::true_type());
-    else if (p.logprobs) sums(std::false_type());
     sum = wave_scan64(sum);
     if (lane == 63) lds.wexp[w] = sum;
     uint64_t kept = 0;
@@ -627,7 +766,7 @@ __global__ __launch_bounds__(kST) void k_sample(GDNSample p, int shift) {
         for (int i = 0; i < kWaves; ++i) s += lds.wexp[i];
         return log(s);
     };
-    if (greedy) {
+    if (ask.greedy) {
         if (t == 0) {
             p.tokens[ri] = arg;
             if (p.logprobs) p.logprobs[ri] = (float)-log_sum();
@@ -635,21 +774,20 @@ __global__ __launch_bounds__(kST) void k_sample(GDNSample p, int shift) {
         return;
     }
 
-    // the border: higher tokens are kept, of its logit those up to edge_at
-    float edge = -kInf;
-    int edge_at = 0x7fffffff;
+    Keep keep;
     bool listed = false;  // what is kept is among the threads' own
-    if (by_k || by_p) {
+    if (ask.by_k || ask.by_p) {
         listed = bound > lowest && gather();
         if (!listed) {
             own.at = -1;
             steps(bound, __builtin_nanf(""));
         }
         __syncthreads();
-        uint64_t count = lds.count[t], mass = lds.mass[t], n_all = 0, m_all = 0, n_before = 0, m_before = 0;
-        if (by_p) m_before = block_scan(mass, lds.wsum[0], m_all);
-        if (by_k) n_before = block_scan(count, lds.wsum[1], n_all);
-        if (total && (double)m_all < (double)tp * (double)kept) {
+        uint64_t mass = lds.mass[t], n_all = 0, m_all = 0, n_before = 0, m_before = 0;
+        const uint64_t count = lds.count[t];
+        if (ask.by_p) m_before = block_scan(mass, lds.wsum[0], m_all);
+        if (ask.by_k) n_before = block_scan(count, lds.wsum[1], n_all);
+        if (total && (double)m_all < (double)ask.top_p * (double)kept) {
             listed = false;
             steps(lowest, bound);
             __syncthreads();
@@ -657,101 +795,243 @@ __global__ __launch_bounds__(kST) void k_sample(GDNSample p, int shift) {
             m_before = block_scan(mass, lds.wsum[1], m_all);
         }
         if (!total) kept = m_all;
-        // by counts, then by weights: tokens past the first border rank behind
-        // all that reach the second goal, which is less than the whole weight
-        for (int turn = 0; turn < 2; ++turn) {
-            const bool by_mass = turn == 1;
-            if (by_mass ? !by_p : !by_k || (uint64_t)k > n_all) continue;
-            const double goal = by_mass ? (double)tp * (double)kept : (double)k;
-            const uint64_t before = by_mass ? m_before : n_before, here = by_mass ? mass : count;
-            __syncthreads();
-            if (here != 0 && (double)before < goal && (double)(before + here) >= goal) {
-                lds.bin = t;
-                lds.left = goal - (double)before;
-                lds.base = m_before;
-            }
-            __syncthreads();
-            const uint64_t base = lds.base;
-            kept = base + border_in(r, lds, (int)lds.bin, by_mass, lds.left, listed, own);
-            if (lds.x > edge || (lds.x == edge && lds.at < edge_at)) {
-                edge = lds.x;
-                edge_at = lds.at;
-            }
-        }
-    } else if (first_only) {
-        edge = top;
-        edge_at = arg;
+        borders(r, lds, ask, count, mass, n_before, m_before, n_all, kept, listed, own, keep);
+    } else if (ask.first_only) {
+        keep.edge = top;
+        keep.edge_at = arg;
     }
-    const double least = mp > 0.0f ? __builtin_ldexp((double)__builtin_fminf(mp, 1.0f), shift) : 0.0;
-    const float from = edge > lowest ? edge : lowest;
-    auto weight = [&](float v, int at) __attribute__((always_inline)) -> uint64_t {
-        if (!(v >= from) || (v == edge && at > edge_at)) return 0;
-        const double d = r.fall(v);
-        const uint64_t s = r.weight(d, r.bin(d));
-        return (double)s >= least ? s : 0;
-    };
+    keep.finish(r, ask, lowest);
 
-    // the kept weights by pieces of 64 V tokens, the piece the draw falls in,
-    // the token in it
+    // the kept weights by pieces of 64 V tokens
     const int cells = (r.n + 64 * V - 1) / (64 * V);
     __syncthreads();
     if (listed) {
         for (int c = t; c < cells; c += kST) lds.cell[c] = 0;
         __syncthreads();
-        if (own.at >= 0 && (own.x > edge || (own.x == edge && own.at <= edge_at)) && (double)own.w >= least)
+        if (own.at >= 0 && keep.has(own.x, own.at) && (double)own.w >= keep.least)
             atomicAdd(reinterpret_cast<unsigned long long *>(&lds.cell[own.at / (64 * V)]), (unsigned long long)own.w);
-    }
-    for (int c = listed ? cells : w; c < cells; c += kWaves) {
-        const int at = (c * 64 + lane) * V;
-        uint64_t s = 0;
-        if (at < r.n) {
-            float x[V];
-            r.load(at, x);
-#pragma unroll
-            for (int j = 0; j < V; ++j) s += weight(x[j], at + j);
+    } else {
+        for (int c = w; c < cells; c += kWaves) {
+            const uint64_t s = keep.piece(r, c, lane);
+            if (lane == 63) lds.cell[c] = s;
         }
-        if (__ballot(s != 0) != 0) s = wave_scan64(s);
-        if (lane == 63) lds.cell[c] = s;
     }
     __syncthreads();
-    uint64_t mine = 0, all;
-    const int per = (cells + kST - 1) / kST;
-    for (int i = 0; i < per; ++i) mine += t * per + i < cells ? lds.cell[t * per + i] : 0;
-    uint64_t at = block_scan(mine, lds.wsum[0], all);
-    uint64_t goal = u > 0.0 ? (uint64_t)__builtin_fmin(u * (double)all, 9.2e18) : 0;
-    goal = goal < all ? goal : all - 1;
-    if (at <= goal && at + mine > goal) {
-        int c = t * per;
-        while (at + lds.cell[c] <= goal) at += lds.cell[c++];
-        lds.bin = (uint32_t)c;
-        lds.base = at;
+    const int token = drawn(r, lds, keep, ask.u);
+    if (token >= 0) {
+        p.tokens[ri] = token;
+        if (p.logprobs) p.logprobs[ri] = (float)(-r.fall(T::get(r.row[token])) - log_sum());
+    }
+}
+
+// Longer rows, a row's slices by workgroups of their own: the highest logit;
+// sums and the steps' counts and weights; the borders (a workgroup a row, which
+// reads the row once for each); the kept weights of the pieces; the token.  One
+// workgroup for all of it takes 300 us for 131072 tokens.
+constexpr int kSlices = 32;
+struct WideRow {
+    float top[kSlices];
+    int arg[kSlices];
+    double sum[kSlices];
+    unsigned long long mass[kBins];
+    uint32_t count[kBins];
+    Keep keep;
+    double log_sum;
+    int done, pad;
+    uint64_t cell[];
+};
+template <class T>
+__host__ __device__ constexpr size_t wide_bytes(uint32_t vocab) {
+    return (sizeof(WideRow) + (vocab + 64 * T::kVec - 1) / (64 * T::kVec) * sizeof(uint64_t) + 15) / 16 * 16;
+}
+template <class T>
+__device__ __forceinline__ WideRow &wide_row(void *ws, const GDNSample &p, int r) {
+    return *reinterpret_cast<WideRow *>(static_cast<char *>(ws) + (size_t)r * wide_bytes<T>(p.vocab));
+}
+// The tokens of slice i of n: whole pieces.
+template <class T>
+__device__ __forceinline__ void slice_of(const GDNSample &p, int i, int n, int &c0, int &c1) {
+    const int cells = ((int)p.vocab + 64 * T::kVec - 1) / (64 * T::kVec);
+    c0 = (int)((int64_t)cells * i / n);
+    c1 = (int)((int64_t)cells * (i + 1) / n);
+}
+template <class T>
+__device__ __forceinline__ void wide_set(Row<T, false> &r, const GDNSample &p, int ri, int shift, const WideRow &row,
+                                         int slices, float temp, int &arg) {
+    const int lane = threadIdx.x & 63;
+    float top = lane < slices ? row.top[lane] : -kInf;
+    arg = lane < slices ? row.arg[lane] : kNowhere;
+    first_of_highest(top, arg);
+    r.row = static_cast<const typename T::E *>(p.logits) + (size_t)ri * p.logits_stride;
+    r.n = (int)p.vocab;
+    r.set(top, temp, shift);
+}
+
+// f(values, index of the first) over the tokens of pieces c0 .. c1 - 1
+template <class R, class F>
+__device__ __forceinline__ void each_in(const R &r, int c0, int c1, F &&f) {
+    const int end = min(c1 * 64 * R::V, r.n);
+    for (int at = (c0 * 64 + (int)threadIdx.x) * R::V; at < end; at += kST * R::V) {
+        float x[R::V];
+        r.load(at, x);
+        f(x, at);
+    }
+}
+
+template <class T>
+__global__ __launch_bounds__(kST) void k_wide_top(GDNSample p, void *ws) {
+    __shared__ float wmax[kWaves];
+    __shared__ int warg[kWaves];
+    const int ri = blockIdx.y, t = threadIdx.x, lane = t & 63, w = t >> 6;
+    WideRow &row = wide_row<T>(ws, p, ri);
+    Row<T, false> r;
+    r.row = static_cast<const typename T::E *>(p.logits) + (size_t)ri * p.logits_stride;
+    r.n = (int)p.vocab;
+    int c0, c1;
+    slice_of<T>(p, blockIdx.x, gridDim.x, c0, c1);
+    float top = -kInf;
+    int arg = kNowhere;
+    each_in(r, c0, c1, [&](const float(&x)[T::kVec], int at) __attribute__((always_inline)) { higher<T>(x, at, top, arg); });
+    for (int i = blockIdx.x * kST + t; i < kBins; i += gridDim.x * kST) {
+        row.mass[i] = 0;
+        row.count[i] = 0;
+    }
+    first_of_highest(top, arg);
+    if (lane == 0) {
+        wmax[w] = top;
+        warg[w] = arg;
     }
     __syncthreads();
-    if (w == 0) {
-        const int c0 = (int)lds.bin * 64 * V + lane * V;
-        float y[V];
-        uint64_t s[V], mine_w = 0;
-        if (c0 < r.n) r.load(c0, y);
+    top = lane < kWaves ? wmax[lane] : -kInf;
+    arg = lane < kWaves ? warg[lane] : kNowhere;
+    first_of_highest(top, arg);
+    if (t == 0) {
+        row.top[blockIdx.x] = top;
+        row.arg[blockIdx.x] = arg;
+    }
+}
+
+template <class T>
+__global__ __launch_bounds__(kST) void k_wide_steps(GDNSample p, int shift, void *ws) {
+    constexpr int V = T::kVec;
+    __shared__ unsigned long long mass[kBins];
+    __shared__ uint32_t count[kBins];
+    __shared__ double wexp[kWaves];
+    const int ri = blockIdx.y, t = threadIdx.x, lane = t & 63, w = t >> 6;
+    WideRow &row = wide_row<T>(ws, p, ri);
+    const Ask ask(p, ri);
+    Row<T, false> r;
+    int arg;
+    wide_set(r, p, ri, shift, row, gridDim.x, ask.temp, arg);
+    if (arg == kNowhere) return;
+    count[t] = 0;
+    mass[t] = 0;
+    __syncthreads();
+    int c0, c1;
+    slice_of<T>(p, blockIdx.x, gridDim.x, c0, c1);
+    double sum = 0.0;
+    each_in(r, c0, c1, [&](const float(&x)[V], int) __attribute__((always_inline)) {
+        sum += (double)exponentials(r, x);
+        if (ask.by_k || ask.by_p) {
 #pragma unroll
-        for (int j = 0; j < V; ++j) {
-            s[j] = c0 < r.n ? weight(y[j], c0 + j) : 0;
-            mine_w += s[j];
-        }
-        uint64_t run = lds.base + wave_scan64(mine_w) - mine_w;
-        if (run <= goal && run + mine_w > goal) {
-            int j = 0;
-#pragma unroll
-            for (int i = 0; i < V; ++i) {
-                if (run + s[i] <= goal) {
-                    run += s[i];
-                    j = i + 1;
-                } else {
-                    break;
+            for (int j = 0; j < V; ++j) {
+                const double d = r.fall(x[j]);
+                const int b = r.bin(d);
+                if (b < kBins) {
+                    if (ask.by_k) atomicAdd(&count[b], 1u);
+                    if (ask.by_p) atomicAdd(&mass[b], (unsigned long long)r.weight(d));
                 }
             }
-            p.tokens[ri] = c0 + j;
-            if (p.logprobs) p.logprobs[ri] = (float)(-r.fall(T::get(r.row[c0 + j])) - log_sum());
         }
+    });
+    sum = wave_scan64(sum);
+    if (lane == 63) wexp[w] = sum;
+    __syncthreads();
+    if (count[t]) atomicAdd(&row.count[t], count[t]);
+    if (mass[t]) atomicAdd(&row.mass[t], mass[t]);
+    if (t == 0) {
+        double s = 0.0;
+#pragma unroll
+        for (int i = 0; i < kWaves; ++i) s += wexp[i];
+        row.sum[blockIdx.x] = s;
+    }
+}
+
+template <class T>
+__global__ __launch_bounds__(kST) void k_wide_border(GDNSample p, int shift, void *ws, int slices) {
+    __shared__ SampleLds<T, false> lds;
+    const int ri = blockIdx.x, t = threadIdx.x;
+    WideRow &row = wide_row<T>(ws, p, ri);
+    const Ask ask(p, ri);
+    Row<T, false> r;
+    int arg;
+    wide_set(r, p, ri, shift, row, slices, ask.temp, arg);
+    const bool none = arg == kNowhere;
+    double log_sum = 0.0;
+    if (t == 0) {
+        for (int i = 0; i < slices; ++i) log_sum += none ? 1.0 : row.sum[i];
+        log_sum = log(log_sum);
+        row.log_sum = log_sum;
+        row.done = none || ask.greedy;
+    }
+    if (none || ask.greedy) {  // nothing above -infinity, or the highest
+        if (t == 0) {
+            p.tokens[ri] = none ? -1 : arg;
+            if (p.logprobs) p.logprobs[ri] = none ? -kInf : (float)-log_sum;
+        }
+        return;
+    }
+    float lowest, unused;
+    r.bounds(0, kBins, lowest, unused);
+    Keep keep;
+    if (ask.by_k || ask.by_p) {
+        const uint64_t count = row.count[t], mass = row.mass[t];
+        uint64_t n_all, m_all;
+        const uint64_t n_before = block_scan(count, lds.wsum[0], n_all), m_before = block_scan(mass, lds.wsum[1], m_all);
+        borders(r, lds, ask, count, mass, n_before, m_before, n_all, m_all, false, Ranked{0.0f, -1, 0}, keep);
+    } else if (ask.first_only) {
+        keep.edge = r.top;
+        keep.edge_at = arg;
+    }
+    keep.finish(r, ask, lowest);
+    if (t == 0) row.keep = keep;
+}
+
+template <class T>
+__global__ __launch_bounds__(kST) void k_wide_pieces(GDNSample p, int shift, void *ws) {
+    const int ri = blockIdx.y, lane = threadIdx.x & 63, w = threadIdx.x >> 6;
+    WideRow &row = wide_row<T>(ws, p, ri);
+    if (row.done) return;
+    const Ask ask(p, ri);
+    Row<T, false> r;
+    int arg, c0, c1;
+    wide_set(r, p, ri, shift, row, gridDim.x, ask.temp, arg);
+    const Keep keep = row.keep;
+    slice_of<T>(p, blockIdx.x, gridDim.x, c0, c1);
+    for (int c = c0 + w; c < c1; c += kWaves) {
+        const uint64_t s = keep.piece(r, c, lane);
+        if (lane == 63) row.cell[c] = s;
+    }
+}
+
+template <class T>
+__global__ __launch_bounds__(kST) void k_wide_draw(GDNSample p, int shift, void *ws, int slices) {
+    __shared__ SampleLds<T, false> lds;
+    const int ri = blockIdx.x, t = threadIdx.x;
+    WideRow &row = wide_row<T>(ws, p, ri);
+    if (row.done) return;
+    const Ask ask(p, ri);
+    Row<T, false> r;
+    int arg;
+    wide_set(r, p, ri, shift, row, slices, ask.temp, arg);
+    const Keep keep = row.keep;
+    const int cells = (r.n + 64 * T::kVec - 1) / (64 * T::kVec);
+    for (int c = t; c < cells; c += kST) lds.cell[c] = row.cell[c];
+    __syncthreads();
+    const int token = drawn(r, lds, keep, ask.u);
+    if (token >= 0) {
+        p.tokens[ri] = token;
+        if (p.logprobs) p.logprobs[ri] = (float)(-r.fall(T::get(r.row[token])) - row.log_sum);
     }
 }
 
@@ -802,32 +1082,62 @@ extern "C" int gdn_logits_process(const GDNLogits *args, void *stream) {
     return launched(who);
 }
 
-extern "C" int gdn_sample_tokens(const GDNSample *args, void *stream) {
+namespace gdn {
+namespace lg {
+template <class T>
+bool held(const GDNSample &a) {
+    return a.vocab <= (uint32_t)SampleLds<T, true>::kHeld;
+}
+template <class T>
+void launch_sample(const GDNSample &a, void *ws, hipStream_t s) {
+    // 2^shift times the vocabulary stays below 2^63
+    const int shift = a.vocab <= (1u << 18) ? 45 : 43;
+    const dim3 rows(a.rows), block(kST);
+    if (held<T>(a)) {
+        hipLaunchKernelGGL(k_sample<T>, rows, block, 0, s, a, shift);
+        return;
+    }
+    // slices for two workgroups a CU
+    const int slices = a.rows >= 512 ? 1 : a.rows * kSlices <= 512 ? kSlices : 512 / (int)a.rows;
+    const dim3 parts(slices, a.rows);
+    hipLaunchKernelGGL(k_wide_top<T>, parts, block, 0, s, a, ws);
+    hipLaunchKernelGGL(k_wide_steps<T>, parts, block, 0, s, a, shift, ws);
+    hipLaunchKernelGGL(k_wide_border<T>, rows, block, 0, s, a, shift, ws, slices);
+    hipLaunchKernelGGL(k_wide_pieces<T>, parts, block, 0, s, a, shift, ws);
+    hipLaunchKernelGGL(k_wide_draw<T>, rows, block, 0, s, a, shift, ws, slices);
+}
+}  // namespace lg
+}  // namespace gdn
+
+extern "C" size_t gdn_sample_workspace(const GDNSample *args) {
+    using namespace gdn::lg;
+    if (args == nullptr || args->vocab > (uint32_t)kMostVocab) return 0;
+    const GDNSample &a = *args;
+    if (a.dtype == GDN_DTYPE_BF16) return held<Bf16>(a) ? 0 : a.rows * wide_bytes<Bf16>(a.vocab);
+    if (a.dtype == GDN_DTYPE_FP16) return held<Fp16>(a) ? 0 : a.rows * wide_bytes<Fp16>(a.vocab);
+    if (a.dtype == GDN_DTYPE_FP32) return held<Fp32>(a) ? 0 : a.rows * wide_bytes<Fp32>(a.vocab);
+    return 0;
+}
+
+extern "C" int gdn_sample_tokens(const GDNSample *args, void *workspace, size_t workspace_bytes, void *stream) {
     using namespace gdn::lg;
     constexpr const char *who = "gdn_sample_tokens";
     if (args == nullptr) return refuse(who, "args is NULL");
     const GDNSample &a = *args;
     if (a.dtype < GDN_DTYPE_BF16 || a.dtype > GDN_DTYPE_FP32) return refuse(who, "unknown dtype");
     if (a.vocab > (uint32_t)kMostVocab) return refuse(who, "the vocabulary is larger than 2^20");
-    if (a.rows > 0x7fffffffu) return refuse(who, "at most 2^31 - 1 rows");
+    if (a.rows > 65535) return refuse(who, "at most 65535 rows");
     if (a.rows == 0) return 0;
     if (a.vocab == 0) return refuse(who, "the vocabulary is empty");
     if (!a.logits || !a.tokens || (a.temperature && !a.uniform)) return refuse(who, "a buffer pointer is NULL");
     if (misaligned(a.logits, a.dtype)) return refuse(who, "logits is misaligned");
     if (a.rows > 1 && a.logits_stride < (int64_t)a.vocab) return refuse(who, "the row stride is smaller than the row");
-    // 2^shift times the vocabulary stays below 2^63
-    const int shift = a.vocab <= (1u << 18) ? 45 : 43;
-    const dim3 grid(a.rows), block(kST);
+    const size_t need = gdn_sample_workspace(args);
+    if (need != 0 && (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0 || workspace_bytes < need))
+        return refuse(who, "the workspace is missing, misaligned or too small");
     hipStream_t s = static_cast<hipStream_t>(stream);
-    auto launch = [&](auto type) {
-        using T = decltype(type);
-        if (a.vocab <= (uint32_t)SampleLds<T, true>::kHeld)
-            hipLaunchKernelGGL((k_sample<T, true>), grid, block, 0, s, a, shift);
-        else
-            hipLaunchKernelGGL((k_sample<T, false>), grid, block, 0, s, a, shift);
-    };
-    if (a.dtype == GDN_DTYPE_BF16) launch(Bf16());
-    else if (a.dtype == GDN_DTYPE_FP16) launch(Fp16());
-    else launch(Fp32());
+    if (a.dtype == GDN_DTYPE_BF16) launch_sample<Bf16>(a, workspace, s);
+    else if (a.dtype == GDN_DTYPE_FP16) launch_sample<Fp16>(a, workspace, s);
+    else launch_sample<Fp32>(a, workspace, s);
     return launched(who);
 }

@@ -230,5 +230,8 @@ def sample_tokens(logits: torch.Tensor, uniform: Optional[torch.Tensor] = None, 
                     _on(dev, "temperature", temperature, _F32, one), _on(dev, "top_k", top_k, _I32, one),
                     _on(dev, "top_p", top_p, _F32, one), _on(dev, "min_p", min_p, _F32, one),
                     _on(dev, "tokens", tokens, _I32, one), _on(dev, "logprobs", logprobs, _F32, one))
-    _launch(dev, "gdn_sample_tokens", L.load().gdn_sample_tokens, ctypes.byref(a))
+    lib, ref = L.load(), ctypes.byref(a)
+    size = lib.gdn_sample_workspace(ref)
+    ws = torch.empty(size, dtype=torch.uint8, device=logits.device) if size else None
+    _launch(dev, "gdn_sample_tokens", lib.gdn_sample_tokens, ref, ws.data_ptr() if size else 0, size)
     return tokens, logprobs

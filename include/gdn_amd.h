@@ -731,7 +731,9 @@ int gdn_logits_process(const GDNLogits *args, void *stream);
  * NaN logits are never chosen and carry no weight; a row without a logit above
  * -infinity gives token -1 and log-probability -infinity.  Weights are held in
  * 64-bit fixed point, 45 bits behind the point (fewer from 2^18 tokens on), so
- * their sums do not depend on an order.  vocab is at most 2^20. */
+ * their sums do not depend on an order.  vocab is at most 2^20, rows 65535.
+ * `workspace`: gdn_sample_workspace(args) bytes at a multiple of 16 bytes (0 for
+ * rows of up to 128 KiB), needed until the work is done. */
 typedef struct {
     int32_t dtype;              /* GDN_DTYPE_* of logits */
     uint32_t rows, vocab, reserved;
@@ -743,7 +745,8 @@ typedef struct {
     int32_t *tokens;
     float *logprobs;
 } GDNSample;
-int gdn_sample_tokens(const GDNSample *args, void *stream);
+size_t gdn_sample_workspace(const GDNSample *args);
+int gdn_sample_tokens(const GDNSample *args, void *workspace, size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

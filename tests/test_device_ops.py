@@ -118,20 +118,32 @@ def sample(**change):
 
 
 @pytest.mark.parametrize("change", [
-    dict(dtype=-2), dict(vocab=(1 << 20) + 1), dict(vocab=0), dict(rows=1 << 31), dict(logits=0), dict(tokens=0),
+    dict(dtype=-2), dict(vocab=(1 << 20) + 1), dict(vocab=0), dict(rows=65536), dict(logits=0), dict(tokens=0),
     dict(uniform=0), dict(logits=AT + 2), dict(logits_stride=999),
 ], ids=lambda c: "-".join(f"{k}={v}" for k, v in c.items()))
 def test_sample_refuses(change, capfd):
-    assert _lib.load().gdn_sample_tokens(ctypes.byref(sample(**change)), None) == -1
+    assert _lib.load().gdn_sample_tokens(ctypes.byref(sample(**change)), None, 0, None) == -1
     assert "gdn_sample_tokens: " in capfd.readouterr().err
+
+
+def test_sample_workspace():
+    lib = _lib.load()
+    for dtype, most in ((_lib.DTYPE_BF16, 65536), (_lib.DTYPE_FP16, 65536), (_lib.DTYPE_FP32, 32768)):
+        assert lib.gdn_sample_workspace(ctypes.byref(sample(dtype=dtype, vocab=most))) == 0
+        a = sample(dtype=dtype, vocab=most + 1, logits_stride=most + 1)
+        need = lib.gdn_sample_workspace(ctypes.byref(a))
+        assert need > 0
+        for at, size in ((None, need), (AT + 8, need), (AT, need - 1)):
+            assert lib.gdn_sample_tokens(ctypes.byref(a), at, size, None) == -1
+    assert lib.gdn_sample_workspace(None) == 0
 
 
 def test_nothing_to_do_and_null():
     lib = _lib.load()
-    assert lib.gdn_logits_process(None, None) == -1 and lib.gdn_sample_tokens(None, None) == -1
+    assert lib.gdn_logits_process(None, None) == -1 and lib.gdn_sample_tokens(None, None, 0, None) == -1
     assert lib.gdn_logits_process(ctypes.byref(logits(rows=0)), None) == 0
     assert lib.gdn_logits_process(ctypes.byref(logits(vocab=0)), None) == 0
-    assert lib.gdn_sample_tokens(ctypes.byref(sample(rows=0)), None) == 0
+    assert lib.gdn_sample_tokens(ctypes.byref(sample(rows=0)), None, 0, None) == 0
 
 
 def test_tensors_must_be_on_a_gpu():
