@@ -263,15 +263,40 @@ struct Row {
             load_vec<T>(row, at, n, __builtin_nanf(""), x);
         }
     }
-    // f(values, index of the first), a wave's 64 V tokens consecutive
+    // f(values, index of the first), a wave's 64 V tokens consecutive; from
+    // memory eight vectors of a thread on their way at a time
     template <class F>
     __device__ __forceinline__ void each(F &&f) const {
-        constexpr int kUnroll = 16 / V;
+        if constexpr (HELD) {
+            constexpr int kUnroll = 16 / V;
 #pragma unroll kUnroll
-        for (int at = (int)threadIdx.x * V; at < n; at += kST * V) {
-            float x[V];
-            load(at, x);
-            f(x, at);
+            for (int at = (int)threadIdx.x * V; at < n; at += kST * V) {
+                float x[V];
+                load(at, x);
+                f(x, at);
+            }
+        } else {
+            constexpr int kAhead = 8;
+            const int whole = n / V;
+            for (int first = (int)threadIdx.x; first < whole; first += kAhead * kST) {
+                Vec<T> v[kAhead];
+#pragma unroll
+                for (int a = 0; a < kAhead; ++a)
+                    __builtin_memcpy(&v[a], row + (size_t)min(first + a * kST, whole - 1) * V, sizeof(v[a]));
+#pragma unroll
+                for (int a = 0; a < kAhead; ++a)
+                    if (first + a * kST < whole) {
+                        float x[V];
+#pragma unroll
+                        for (int j = 0; j < V; ++j) x[j] = T::get(v[a].e[j]);
+                        f(x, (first + a * kST) * V);
+                    }
+            }
+            if (n % V != 0 && threadIdx.x == kST - 1) {
+                float x[V];
+                load(whole * V, x);
+                f(x, whole * V);
+            }
         }
     }
     // how far below the highest; NaN for NaN, whose bin and weight are those of
@@ -313,41 +338,94 @@ struct Row {
     }
 };
 
-// The border of the tokens of step `b` whose ranked counts (by_mass: weights)
-// first reach `left`, into lds.x and lds.at; their weight is the result.
-// listed: the step's tokens are among the threads' `own` (none: at < 0).
+// The border of the tokens of step `b` (there are `inside`) whose ranked counts
+// (by_mass: weights) first reach `left`, into lds.x and lds.at; their weight is
+// the result.  listed: they are among the threads' `own` (none: at < 0).
 template <class T, bool HELD>
-__device__ __forceinline__ uint64_t border_in(const Row<T, HELD> &r, SampleLds<T, HELD> &lds, int b, bool by_mass,
-                                              double left, bool listed, const Ranked &own) {
+__device__ __forceinline__ uint64_t border_in(const Row<T, HELD> &r, SampleLds<T, HELD> &lds, int b, uint32_t inside,
+                                              bool by_mass, double left, bool listed, const Ranked &own) {
     constexpr int V = T::kVec;
     const int t = threadIdx.x;
     float lo, hi;
     r.bounds(b, b + 1, lo, hi);
-    __syncthreads();
-    if (t == 0) lds.n = 0;
-    __syncthreads();
-    if (listed) {
-        if (own.at >= 0 && r.bin(r.fall(own.x)) == b) {
-            const uint32_t i = atomicAdd(&lds.n, 1u);
-            if (i < (uint32_t)kList) lds.list[i] = own;
-        }
-    } else {
+    // f(token, index, fall) over the step's
+    auto each_of = [&](auto &&f) __attribute__((always_inline)) {
         r.each([&](const float(&x)[V], int at) __attribute__((always_inline)) {
+            float most = x[0];
+#pragma unroll
+            for (int j = 1; j < V; ++j) most = __builtin_fmaxf(most, x[j]);
+            if (!(most >= lo)) return;
 #pragma unroll
             for (int j = 0; j < V; ++j)
                 if (x[j] >= lo && x[j] <= hi) {
                     const double d = r.fall(x[j]);
-                    if (r.bin(d) == b) {
-                        const uint32_t i = atomicAdd(&lds.n, 1u);
-                        if (i < (uint32_t)kList) lds.list[i] = Ranked{x[j], at + j, r.weight(d)};
-                    }
+                    if (r.bin(d) == b) f(x[j], at + j, d);
                 }
         });
+    };
+    // the bin of a histogram in lds that the goal is in, into lds.bin; moves
+    // base and left to it and gives its count
+    uint64_t base = 0;
+    auto find = [&]() __attribute__((always_inline)) -> uint32_t {
+        __syncthreads();
+        const uint64_t m = lds.mass[t], c = lds.count[t];
+        uint64_t all_m, all_c;
+        const uint64_t mb = block_scan(m, lds.wsum[0], all_m), cb = block_scan(c, lds.wsum[1], all_c);
+        const uint64_t v = by_mass ? m : c, vb = by_mass ? mb : cb;
+        // what the bin above holds is all here: rounding past it ends there
+        const double goal = __builtin_fmin(left, (double)(by_mass ? all_m : all_c));
+        if (v != 0 && (double)vb < goal && (double)(vb + v) >= goal) {
+            lds.bin = (uint32_t)t;
+            lds.left = goal - (double)vb;
+            lds.base = mb;
+        }
+        __syncthreads();
+        left = lds.left;
+        base += lds.base;
+        return lds.count[lds.bin];
+    };
+    auto clear = [&]() __attribute__((always_inline)) {
+        __syncthreads();
+        lds.count[t] = 0;
+        lds.mass[t] = 0;
+        __syncthreads();
+    };
+    auto put = [&](int i, double d) __attribute__((always_inline)) {
+        atomicAdd(&lds.count[i], 1u);
+        atomicAdd(&lds.mass[i], (unsigned long long)r.weight(d));
+    };
+    // a crowded step in kBins parts
+    auto part_of = [&](double d) __attribute__((always_inline)) {
+        return min(max((int)((d * r.step - (double)b) * (double)kBins), 0), kBins - 1);
+    };
+    int part = -1;
+    if (!listed && inside > (uint32_t)kList) {
+        clear();
+        each_of([&](float, int, double d) __attribute__((always_inline)) { put(part_of(d), d); });
+        inside = find();
+        part = (int)lds.bin;
     }
-    __syncthreads();
-    const int n = (int)lds.n;
-    if (n <= kList) {
+    if (listed || inside <= (uint32_t)kList) {
+        __syncthreads();
+        if (t == 0) lds.n = 0;
+        __syncthreads();
+        auto add = [&](float x, int at, uint64_t w) __attribute__((always_inline)) {
+            const uint32_t i = atomicAdd(&lds.n, 1u);
+            if (i < (uint32_t)kList) lds.list[i] = Ranked{x, at, w};
+        };
+        if (listed) {
+            if (own.at >= 0 && r.bin(r.fall(own.x)) == b) add(own.x, own.at, own.w);
+        } else {
+            each_of([&](float x, int at, double d) __attribute__((always_inline)) {
+                if (part < 0 || part_of(d) == part) add(x, at, r.weight(d));
+            });
+        }
+        __syncthreads();
+        inside = lds.n;
+    }
+    if (inside <= (uint32_t)kList) {
         // the tokens' own ranks
+        const int n = (int)inside;
         if (t < n) {
             const Ranked me = lds.list[t];
             int rank = 0;
@@ -369,46 +447,21 @@ __device__ __forceinline__ uint64_t border_in(const Row<T, HELD> &r, SampleLds<T
             }
         }
         __syncthreads();
-        return lds.base;
+        return base + lds.base;
     }
-    uint64_t base = 0, each_w = 0;
+    // by their keys' bits (listed tokens that crowd a step too)
+    uint64_t each_w = 0;
     uint32_t prefix = 0, above = 0, have = 0;
     for (int sh = 22; sh >= 0; sh -= sh > 2 ? 10 : sh == 2 ? 2 : 1) {
         const uint32_t bits = sh == 0 ? 3u : 0x3ffu;
-        __syncthreads();
-        lds.count[t] = 0;
-        lds.mass[t] = 0;
-        __syncthreads();
-        r.each([&](const float(&x)[V], int) __attribute__((always_inline)) {
-#pragma unroll
-            for (int j = 0; j < V; ++j)
-                if (x[j] >= lo && x[j] <= hi) {
-                    const double d = r.fall(x[j]);
-                    const uint32_t key = fall_key(x[j]);
-                    if (r.bin(d) == b && (key & above) == prefix) {
-                        atomicAdd(&lds.count[(key >> sh) & bits], 1u);
-                        atomicAdd(&lds.mass[(key >> sh) & bits], (unsigned long long)r.weight(d));
-                    }
-                }
+        clear();
+        each_of([&](float x, int, double d) __attribute__((always_inline)) {
+            const uint32_t key = fall_key(x);
+            if ((key & above) == prefix && (part < 0 || part_of(d) == part)) put((int)((key >> sh) & bits), d);
         });
-        __syncthreads();
-        const uint64_t m = lds.mass[t], c = lds.count[t];
-        uint64_t all_m, all_c;
-        const uint64_t mb = block_scan(m, lds.wsum[0], all_m), cb = block_scan(c, lds.wsum[1], all_c);
-        const uint64_t v = by_mass ? m : c, vb = by_mass ? mb : cb;
-        // what the bin above holds is all here: rounding past it ends there
-        const double goal = __builtin_fmin(left, (double)(by_mass ? all_m : all_c));
-        if (v != 0 && (double)vb < goal && (double)(vb + v) >= goal) {
-            lds.bin = (uint32_t)t;
-            lds.left = goal - (double)vb;
-            lds.base = mb;
-        }
-        __syncthreads();
+        have = find();
         prefix |= lds.bin << sh;
         above |= bits << sh;
-        left = lds.left;
-        base += lds.base;
-        have = lds.count[lds.bin];
         each_w = lds.mass[lds.bin] / have;
     }
     // of the border key's tokens (one weight all), the first `need` are kept
@@ -550,10 +603,11 @@ __device__ __forceinline__ void borders(const Row<T, HELD> &r, SampleLds<T, HELD
             lds.bin = threadIdx.x;
             lds.left = goal - (double)before;
             lds.base = m_before;
+            lds.n = (uint32_t)count;
         }
         __syncthreads();
         const uint64_t base = lds.base;
-        kept = base + border_in(r, lds, (int)lds.bin, by_mass, lds.left, listed, own);
+        kept = base + border_in(r, lds, (int)lds.bin, lds.n, by_mass, lds.left, listed, own);
         if (lds.x > keep.edge || (lds.x == keep.edge && lds.at < keep.edge_at)) {
             keep.edge = lds.x;
             keep.edge_at = lds.at;
@@ -709,7 +763,7 @@ __global__ __launch_bounds__(kST) void k_sample(GDNSample p, int shift) {
         const int b = r.bin(d);
         const uint64_t s = r.weight(d);
         if (b < kBins) {
-            if (ask.by_k) atomicAdd(&lds.count[b], 1u);
+            atomicAdd(&lds.count[b], 1u);
             if (ask.by_p) atomicAdd(&lds.mass[b], (unsigned long long)s);
         }
         return s;
@@ -783,14 +837,14 @@ __global__ __launch_bounds__(kST) void k_sample(GDNSample p, int shift) {
             steps(bound, __builtin_nanf(""));
         }
         __syncthreads();
-        uint64_t mass = lds.mass[t], n_all = 0, m_all = 0, n_before = 0, m_before = 0;
-        const uint64_t count = lds.count[t];
+        uint64_t count = lds.count[t], mass = lds.mass[t], n_all = 0, m_all = 0, n_before = 0, m_before = 0;
         if (ask.by_p) m_before = block_scan(mass, lds.wsum[0], m_all);
         if (ask.by_k) n_before = block_scan(count, lds.wsum[1], n_all);
         if (total && (double)m_all < (double)ask.top_p * (double)kept) {
             listed = false;
             steps(lowest, bound);
             __syncthreads();
+            count = lds.count[t];
             mass = lds.mass[t];
             m_before = block_scan(mass, lds.wsum[1], m_all);
         }
@@ -938,7 +992,7 @@ __global__ __launch_bounds__(kST) void k_wide_steps(GDNSample p, int shift, void
                 const double d = r.fall(x[j]);
                 const int b = r.bin(d);
                 if (b < kBins) {
-                    if (ask.by_k) atomicAdd(&count[b], 1u);
+                    atomicAdd(&count[b], 1u);
                     if (ask.by_p) atomicAdd(&mass[b], (unsigned long long)r.weight(d));
                 }
             }
