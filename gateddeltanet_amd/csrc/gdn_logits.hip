@@ -202,8 +202,10 @@ struct SampleLds {
         Ranked list[kList];
         uint64_t cell[kCells];
     };
-    float high[kWaves][64];  // the tokens above the bound that a wave met, and their places
-    int high_at[kWaves][64];
+    // tokens gathered from the row, and their places
+    static constexpr int kSome = HELD ? kST : 8 * kST;
+    float some[kSome];
+    int some_at[kSome];
     uint64_t wsum[2][kWaves];
     float wmax[kWaves];
     int warg[kWaves];
@@ -212,7 +214,7 @@ struct SampleLds {
     double left;      // of the goal, in it
     float x;          // a border
     int at;
-    uint32_t bin, n, crowded;
+    uint32_t bin, n, n_some, crowded;
 };
 
 __device__ __forceinline__ uint64_t lane_of(uint64_t v, int lane) {
@@ -348,20 +350,51 @@ __device__ __forceinline__ uint64_t border_in(const Row<T, HELD> &r, SampleLds<T
     const int t = threadIdx.x;
     float lo, hi;
     r.bounds(b, b + 1, lo, hi);
+    // The step's tokens lie among many others, so that nearly every wave would
+    // form their weights for a few lanes: they are gathered first where they
+    // fit (131072 tokens: 30 us a pass otherwise)
+    constexpr int kSome = SampleLds<T, HELD>::kSome;
+    uint32_t n_some = kSome + 1;
+    if (!listed) {
+        __syncthreads();
+        if (t == 0) lds.n_some = 0;
+        __syncthreads();
+        r.each([&](const float(&x)[V], int at) __attribute__((always_inline)) {
+#pragma unroll
+            for (int j = 0; j < V; ++j) {
+                const bool in = x[j] >= lo && x[j] <= hi;
+                const uint64_t who = __ballot(in);
+                if (who == 0) continue;
+                const int before = (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0u));
+                uint32_t i = 0;
+                if (in && before == 0) i = atomicAdd(&lds.n_some, (uint32_t)__builtin_popcountll(who));
+                i = (uint32_t)__builtin_amdgcn_readlane((int)i, __builtin_ctzll(who)) + before;
+                if (in && i < (uint32_t)kSome) {
+                    lds.some[i] = x[j];
+                    lds.some_at[i] = at + j;
+                }
+            }
+        });
+        __syncthreads();
+        n_some = lds.n_some;
+    }
     // f(token, index, fall) over the step's
     auto each_of = [&](auto &&f) __attribute__((always_inline)) {
-        r.each([&](const float(&x)[V], int at) __attribute__((always_inline)) {
-            float most = x[0];
+        auto one = [&](float x, int at) __attribute__((always_inline)) {
+            const double d = r.fall(x);
+            if (r.bin(d) == b) f(x, at, d);
+        };
+        if (listed) {
+            if (own.at >= 0) one(own.x, own.at);
+        } else if (n_some <= (uint32_t)kSome) {
+            for (uint32_t i = t; i < n_some; i += kST) one(lds.some[i], lds.some_at[i]);
+        } else {
+            r.each([&](const float(&x)[V], int at) __attribute__((always_inline)) {
 #pragma unroll
-            for (int j = 1; j < V; ++j) most = __builtin_fmaxf(most, x[j]);
-            if (!(most >= lo)) return;
-#pragma unroll
-            for (int j = 0; j < V; ++j)
-                if (x[j] >= lo && x[j] <= hi) {
-                    const double d = r.fall(x[j]);
-                    if (r.bin(d) == b) f(x[j], at + j, d);
-                }
-        });
+                for (int j = 0; j < V; ++j)
+                    if (x[j] >= lo && x[j] <= hi) one(x[j], at + j);
+            });
+        }
     };
     // the bin of a histogram in lds that the goal is in, into lds.bin; moves
     // base and left to it and gives its count
@@ -399,27 +432,21 @@ __device__ __forceinline__ uint64_t border_in(const Row<T, HELD> &r, SampleLds<T
         return min(max((int)((d * r.step - (double)b) * (double)kBins), 0), kBins - 1);
     };
     int part = -1;
-    if (!listed && inside > (uint32_t)kList) {
+    if (inside > (uint32_t)kList) {
         clear();
         each_of([&](float, int, double d) __attribute__((always_inline)) { put(part_of(d), d); });
         inside = find();
         part = (int)lds.bin;
     }
-    if (listed || inside <= (uint32_t)kList) {
+    if (inside <= (uint32_t)kList) {
         __syncthreads();
         if (t == 0) lds.n = 0;
         __syncthreads();
-        auto add = [&](float x, int at, uint64_t w) __attribute__((always_inline)) {
+        each_of([&](float x, int at, double d) __attribute__((always_inline)) {
+            if (part >= 0 && part_of(d) != part) return;
             const uint32_t i = atomicAdd(&lds.n, 1u);
-            if (i < (uint32_t)kList) lds.list[i] = Ranked{x, at, w};
-        };
-        if (listed) {
-            if (own.at >= 0 && r.bin(r.fall(own.x)) == b) add(own.x, own.at, own.w);
-        } else {
-            each_of([&](float x, int at, double d) __attribute__((always_inline)) {
-                if (part < 0 || part_of(d) == part) add(x, at, r.weight(d));
-            });
-        }
+            if (i < (uint32_t)kList) lds.list[i] = Ranked{x, at, r.weight(d)};
+        });
         __syncthreads();
         inside = lds.n;
     }
@@ -449,7 +476,7 @@ __device__ __forceinline__ uint64_t border_in(const Row<T, HELD> &r, SampleLds<T
         __syncthreads();
         return base + lds.base;
     }
-    // by their keys' bits (listed tokens that crowd a step too)
+    // by their keys' bits
     uint64_t each_w = 0;
     uint32_t prefix = 0, above = 0, have = 0;
     for (int sh = 22; sh >= 0; sh -= sh > 2 ? 10 : sh == 2 ? 2 : 1) {
@@ -788,8 +815,8 @@ __global__ __launch_bounds__(kST) void k_sample(GDNSample p, int shift) {
                 if (who == 0) continue;
                 const int i = n + (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0u));
                 if (x[j] >= bound && i < 64) {
-                    lds.high[w][i] = x[j];
-                    lds.high_at[w][i] = at + j;
+                    lds.some[64 * w + i] = x[j];
+                    lds.some_at[64 * w + i] = at + j;
                 }
                 n += __builtin_popcountll(who);
             }
@@ -799,8 +826,8 @@ __global__ __launch_bounds__(kST) void k_sample(GDNSample p, int shift) {
         __syncthreads();
         if (lds.crowded) return false;
         if (lane < n) {
-            own.x = lds.high[w][lane];
-            own.at = lds.high_at[w][lane];
+            own.x = lds.some[t];
+            own.at = lds.some_at[t];
             own.w = count_in(own.x);
         }
         return true;
@@ -1021,10 +1048,10 @@ __global__ __launch_bounds__(kST) void k_wide_border(GDNSample p, int shift, voi
     int arg;
     wide_set(r, p, ri, shift, row, slices, ask.temp, arg);
     const bool none = arg == kNowhere;
-    double log_sum = 0.0;
+    const int lane = t & 63;
+    const uint64_t sums = __builtin_bit_cast(uint64_t, wave_scan64(lane < slices && !none ? row.sum[lane] : 0.0));
+    const double log_sum = log(__builtin_bit_cast(double, lane_of(sums, 63)));
     if (t == 0) {
-        for (int i = 0; i < slices; ++i) log_sum += none ? 1.0 : row.sum[i];
-        log_sum = log(log_sum);
         row.log_sum = log_sum;
         row.done = none || ask.greedy;
     }
