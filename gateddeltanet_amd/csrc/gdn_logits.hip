@@ -204,7 +204,7 @@ struct SampleLds {
     };
     // tokens gathered from the row, and their places
     static constexpr int kSome = HELD ? kST : 8 * kST;
-    float some[kSome];
+    float some[kSome] __attribute__((aligned(8)));
     int some_at[kSome];
     uint64_t wsum[2][kWaves];
     float wmax[kWaves];
@@ -451,19 +451,40 @@ __device__ __forceinline__ uint64_t border_in(const Row<T, HELD> &r, SampleLds<T
         inside = lds.n;
     }
     if (inside <= (uint32_t)kList) {
-        // the tokens' own ranks
+        // the tokens' own ranks, several threads a token: i % each of them
+        // compares with every each-th
         const int n = (int)inside;
+        int lanes = kST / kList;
+        while (lanes < 64 && 2 * lanes * n <= kST) lanes *= 2;
+        unsigned long long *befores = reinterpret_cast<unsigned long long *>(lds.some);
+        static_assert(sizeof(lds.some) >= kList * sizeof(uint64_t) && kList <= kBins, "room for ranks and weights before");
+        if (t < kList) {
+            lds.count[t] = 0;
+            befores[t] = 0;
+        }
+        __syncthreads();
+        const int who = t / lanes;
+        if (who < n) {
+            const Ranked me = lds.list[who];
+            uint32_t rank = 0;
+            uint64_t before = 0;
+#pragma unroll 4
+            for (int i = t % lanes; i < n; i += lanes) {
+                const Ranked o = lds.list[i];
+                const bool first = o.x > me.x || (o.x == me.x && o.at < me.at);
+                rank += first;
+                before += first ? o.w : 0;
+            }
+            if (rank != 0) {
+                atomicAdd(&lds.count[who], rank);
+                atomicAdd(&befores[who], (unsigned long long)before);
+            }
+        }
+        __syncthreads();
         if (t < n) {
             const Ranked me = lds.list[t];
-            int rank = 0;
-            uint64_t before = 0;
-            for (int i = 0; i < n; ++i) {
-                const Ranked o = lds.list[i];
-                if (o.x > me.x || (o.x == me.x && o.at < me.at)) {
-                    ++rank;
-                    before += o.w;
-                }
-            }
+            const int rank = (int)lds.count[t];
+            const uint64_t before = befores[t];
             const double from = by_mass ? (double)before : (double)rank,
                          to = by_mass ? (double)(before + me.w) : (double)(rank + 1);
             // rounding in `left` past the step's end: its last token
