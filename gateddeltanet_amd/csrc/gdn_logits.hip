@@ -209,7 +209,7 @@ struct SampleLds {
     uint64_t wsum[2][kWaves];
     float wmax[kWaves];
     int warg[kWaves];
-    double wexp[kWaves];
+    double wexp[kWaves], guess[2][kWaves];
     uint64_t base;    // weight ranked before a bin found
     double left;      // of the goal, in it
     float x;          // a border
@@ -635,10 +635,11 @@ struct Keep {
 
 // The borders asked for, from the steps' counts and weights (a thread a step);
 // `kept`: the weight that top-p is a share of, unless top-k gives another.
+// Returns the weight up to the last.
 template <class T, bool HELD>
-__device__ __forceinline__ void borders(const Row<T, HELD> &r, SampleLds<T, HELD> &lds, const Ask &ask, uint64_t count,
-                                        uint64_t mass, uint64_t n_before, uint64_t m_before, uint64_t n_all, uint64_t kept,
-                                        bool listed, const Ranked &own, Keep &keep) {
+__device__ __forceinline__ uint64_t borders(const Row<T, HELD> &r, SampleLds<T, HELD> &lds, const Ask &ask, uint64_t count,
+                                            uint64_t mass, uint64_t n_before, uint64_t m_before, uint64_t n_all,
+                                            uint64_t kept, bool listed, const Ranked &own, Keep &keep) {
     // by counts, then by weights: tokens past the first border rank behind all
     // that reach the second goal, which is less than the whole weight
     for (int turn = 0; turn < 2; ++turn) {
@@ -661,6 +662,7 @@ __device__ __forceinline__ void borders(const Row<T, HELD> &r, SampleLds<T, HELD
             keep.edge_at = lds.at;
         }
     }
+    return kept;
 }
 
 // The token up to which the pieces' kept weights (lds.cell) reach the draw, in
@@ -793,19 +795,32 @@ __global__ __launch_bounds__(kST) void k_sample(GDNSample p, int shift) {
         if (lds.bin < (uint32_t)kBins) r.bounds((int)lds.bin, (int)lds.bin + 1, bound, unused);
     }
 
-    // the sum of exponentials, the whole weight where only top-p needs it, and
-    // the steps' counts and weights
+    // the sum of exponentials; where top-p stands alone also an estimate of the
+    // weights above the bound and of all, in FP32: each to 2e-6 (46 2^-24 for the
+    // argument, 2^-23 for the exponential), a thread's sum of 64 at most to 4e-6
+    constexpr double kOff = 1e-5;
     double sum = 0.0;
-    uint64_t whole = 0;
-    const bool total = ask.by_p && !ask.by_k;
-    if (total)
+    const bool alone = ask.by_p && !ask.by_k;
+    if (alone) {
+        const float rate = (float)r.rate;
+        float all = 0.0f, high = 0.0f;
         r.each([&](const float(&x)[V], int) __attribute__((always_inline)) {
             sum += (double)exponentials(r, x);
 #pragma unroll
-            for (int j = 0; j < V; ++j) whole += r.weight(r.fall(x[j]));
+            for (int j = 0; j < V; ++j) {
+                const float q = __builtin_fmaxf(__builtin_amdgcn_exp2f((x[j] - top) * rate), 0.0f);
+                all += q;
+                high += x[j] >= bound ? q : 0.0f;
+            }
         });
-    else if (p.logprobs)
+        const double d = wave_scan64((double)all), h = wave_scan64((double)high);
+        if (lane == 63) {
+            lds.guess[0][w] = d;
+            lds.guess[1][w] = h;
+        }
+    } else if (p.logprobs) {
         r.each([&](const float(&x)[V], int) __attribute__((always_inline)) { sum += (double)exponentials(r, x); });
+    }
     auto count_in = [&](float v) __attribute__((always_inline)) -> uint64_t {
         const double d = r.fall(v);
         const int b = r.bin(d);
@@ -816,11 +831,11 @@ __global__ __launch_bounds__(kST) void k_sample(GDNSample p, int shift) {
         }
         return s;
     };
-    auto steps = [&](float from, float below) __attribute__((always_inline)) {
+    auto steps = [&](float from) __attribute__((always_inline)) {
         r.each([&](const float(&x)[V], int) __attribute__((always_inline)) {
 #pragma unroll
             for (int j = 0; j < V; ++j)
-                if (x[j] >= from && !(x[j] >= below)) count_in(x[j]);  // (below NaN: all)
+                if (x[j] >= from) count_in(x[j]);
         });
     };
     // the tokens above the bound, a thread each: few lie among many, so the
@@ -855,12 +870,7 @@ __global__ __launch_bounds__(kST) void k_sample(GDNSample p, int shift) {
     };
     sum = wave_scan64(sum);
     if (lane == 63) lds.wexp[w] = sum;
-    uint64_t kept = 0;
-    if (total) {
-        block_scan(whole, lds.wsum[1], kept);
-    } else {
-        __syncthreads();
-    }
+    __syncthreads();
     // (the thread that writes a result finishes it)
     auto log_sum = [&]() __attribute__((always_inline)) {
         double s = 0.0;
@@ -879,25 +889,41 @@ __global__ __launch_bounds__(kST) void k_sample(GDNSample p, int shift) {
     Keep keep;
     bool listed = false;  // what is kept is among the threads' own
     if (ask.by_k || ask.by_p) {
-        listed = bound > lowest && gather();
-        if (!listed) {
-            own.at = -1;
-            steps(bound, __builtin_nanf(""));
-        }
-        __syncthreads();
-        uint64_t count = lds.count[t], mass = lds.mass[t], n_all = 0, m_all = 0, n_before = 0, m_before = 0;
-        if (ask.by_p) m_before = block_scan(mass, lds.wsum[0], m_all);
-        if (ask.by_k) n_before = block_scan(count, lds.wsum[1], n_all);
-        if (total && (double)m_all < (double)ask.top_p * (double)kept) {
-            listed = false;
-            steps(lowest, bound);
+        double all = 0.0, high = 0.0;
+        if (alone)
+#pragma unroll
+            for (int i = 0; i < kWaves; ++i) {
+                all += lds.guess[0][i];
+                high += lds.guess[1][i];
+            }
+        // Top-p alone: if the estimates place its border above the bound, from
+        // the tokens there, and it holds if the goal's whole uncertainty lies
+        // inside the border's token.  Else from all tokens
+        for (int turn = 0; turn < 2; ++turn) {
+            const bool guess = alone && turn == 0;
+            listed = bound > lowest && (alone ? guess && !r.endless && high > (double)ask.top_p * all * (1.0 + 4.0 * kOff) : true) &&
+                     gather();
+            if (!listed) {
+                if (guess) continue;
+                own.at = -1;
+                if (alone) {
+                    __syncthreads();
+                    lds.count[t] = 0;
+                    lds.mass[t] = 0;
+                    __syncthreads();
+                }
+                steps(alone ? lowest : bound);
+            }
             __syncthreads();
-            count = lds.count[t];
-            mass = lds.mass[t];
-            m_before = block_scan(mass, lds.wsum[1], m_all);
+            const uint64_t count = lds.count[t], mass = lds.mass[t];
+            uint64_t n_all, m_all;
+            const uint64_t m_before = block_scan(mass, lds.wsum[0], m_all), n_before = block_scan(count, lds.wsum[1], n_all);
+            const double whole = __builtin_ldexp(all, shift);
+            const uint64_t kept = borders(r, lds, ask, count, mass, n_before, m_before, n_all,
+                                          guess ? (uint64_t)(whole * (1.0 - kOff)) : m_all, listed, own, keep);
+            if (!guess || (double)ask.top_p * whole * (1.0 + kOff) <= (double)kept) break;
+            keep = Keep();
         }
-        if (!total) kept = m_all;
-        borders(r, lds, ask, count, mass, n_before, m_before, n_all, kept, listed, own, keep);
     } else if (ask.first_only) {
         keep.edge = top;
         keep.edge_at = arg;
