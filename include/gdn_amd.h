@@ -639,7 +639,8 @@ int gdn_test_prefill_gemm(int kind, const float *W, const float *X, uint32_t N, 
  *              not read.
  *   *_dim      64, 128 or 256, heads contiguous in a row
  *   *_stride   elements between rows (g and beta: one stride).  q, k, v and o
- *              rows start at multiples of 16 bytes
+ *              rows start at multiples of 16 bytes and lie less than 16 MB
+ *              apart; o overlaps no input
  *   g, beta    FP32; g is the log of the decay (<= 0 in a stable model;
  *              -inf clears the state)
  *   state_in, state_out   [n_slots][n_v_heads][key_dim][value_dim] FP32, at
@@ -649,8 +650,9 @@ int gdn_test_prefill_gemm(int kind, const float *W, const float *X, uint32_t N, 
  *   slots      [n_seqs] the sequences' slots (NULL: slot i).  A sequence with
  *              a slot outside 0 .. n_slots - 1 is left out (a padded row):
  *              its o is left as it was.  No slot may occur twice.
- * A value that is not finite reaches its own sequence and head only, there
- * also the tokens up to 63 before it. */
+ * Sums are FP32.  A squared norm or a state beyond FP32's range is not finite
+ * afterwards.  A value that is not finite reaches its own sequence and head
+ * only, in gdn_delta_prefill there also the tokens up to 63 before it. */
 typedef struct {
     int32_t dtype;              /* GDN_DTYPE_* of q, k, v and o */
     uint32_t n_tokens, n_seqs;

@@ -262,6 +262,45 @@ def test_prefill_of_single_tokens_is_the_step():
     close(S, T.double(), 2 * tol(256), "state")
 
 
+def test_nothing_to_do():
+    """No sequences: nothing is touched.  No tokens: the states go through."""
+    q, k, v, gate, beta = inputs(5, 1, 2, 64, 64, BF16, 1)
+    out = torch.full_like(v, 7.0)
+    S = torch.ones((3, 2, 64, 64), device="cuda")
+    g.delta_prefill(q, k, v, gate, beta, torch.zeros(1, dtype=torch.int32).cuda(), state_in=S, state_out=S, out=out)
+    assert (out == 7).all() and (S == 1).all()
+    none = [x[:0] for x in (q, k, v, gate, beta)]
+    T = torch.zeros_like(S)
+    o = g.delta_prefill(*none, torch.zeros(4, dtype=torch.int32).cuda(), state_in=S, state_out=T)
+    assert o.shape == (0, 2, 64) and torch.equal(S, T)
+    assert g.delta_step(*none, S).shape == (0, 2, 64) and (S == 1).all()
+
+
+def test_many_sequences_of_all_lengths():
+    """More sequences than the order's steps tell apart, some longer than its
+    last step."""
+    lens = [(7 * i) % 90 for i in range(400)]
+    q, k, v, gate, beta = inputs(sum(lens), 1, 1, 64, 64, BF16, 22)
+    cu = torch.tensor([0] + lens).cumsum(0).to(torch.int32).cuda()
+    S = torch.zeros((400, 1, 64, 64), device="cuda")
+    out = g.delta_prefill(q, k, v, gate, beta, cu, state_out=S)
+    for i in range(0, 400, 29):
+        s = slice(int(cu[i]), int(cu[i + 1]))
+        o, want = reference(q[s], k[s], v[s], gate[s], beta[s], torch.zeros_like(S[i]))
+        close(out[s], o, tol(64), f"o {i}")
+        close(S[i], want, tol(64), f"state {i}")
+    q, k, v, gate, beta = inputs(17000, 1, 1, 64, 64, BF16, 23)
+    cu = torch.tensor([0, 100, 17000], dtype=torch.int32).cuda()  # 265 chunks
+    S = torch.zeros((2, 1, 64, 64), device="cuda")
+    g.delta_prefill(q, k, v, gate, beta, cu, state_out=S)
+    T = torch.zeros_like(S[:1])
+    for a in range(100, 17000, 4225):
+        s = slice(a, a + 4225)
+        g.delta_prefill(q[s], k[s], v[s], gate[s], beta[s], torch.tensor([0, 4225], dtype=torch.int32).cuda(),
+                        state_in=T, state_out=T)
+    close(S[1], T[0].double(), 2 * tol(64), "state of 16900 tokens")
+
+
 def test_decays_at_their_ends():
     """g = -inf and a decay below FP32 clear the state, also in the middle of
     a chunk; g = 0 and beta = 0 leave it."""

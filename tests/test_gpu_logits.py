@@ -325,6 +325,112 @@ def test_sample_strided_rows_at_any_address():
     check_sample(x, u, temp, k, p, mp)
 
 
+def test_sample_without_logprobs_and_into_the_callers_tensors():
+    import ctypes
+
+    from gateddeltanet_amd import _lib
+
+    for vocab, dtype in ((5000, torch.float32), (70000, torch.bfloat16)):
+        x = row_logits(4, vocab, dtype, 21)
+        u = torch.tensor([0.1, 0.4, 0.7, 0.95]).cuda()
+        temp = torch.tensor([0.0, 0.7, 1.0, 1.5]).cuda()
+        p = torch.tensor([0.9, 0.5, 0.99, 1.0]).cuda()
+        want, lp = g.sample_tokens(x, u, temperature=temp, top_p=p)
+        tokens, logprobs = torch.zeros(4, dtype=torch.int32).cuda(), torch.zeros(4).cuda()
+        got = g.sample_tokens(x, u, temperature=temp, top_p=p, tokens=tokens, logprobs=logprobs)
+        assert got[0] is tokens and got[1] is logprobs and torch.equal(tokens, want) and torch.equal(logprobs, lp)
+        tokens.zero_()
+        a = _lib.GDNSample({torch.float32: 2, torch.bfloat16: 0}[dtype], 4, vocab, 0, vocab, x.data_ptr(), u.data_ptr(),
+                           temp.data_ptr(), 0, p.data_ptr(), 0, tokens.data_ptr(), 0)
+        lib = _lib.load()
+        ws = torch.empty(lib.gdn_sample_workspace(ctypes.byref(a)) + 16, dtype=torch.uint8).cuda()
+        assert lib.gdn_sample_tokens(ctypes.byref(a), ws.data_ptr(), ws.numel(), torch.cuda.current_stream().cuda_stream) == 0
+        assert torch.equal(tokens, want)
+
+
+@pytest.mark.parametrize("rows", [1, 20, 300, 600])
+def test_sample_wide_batches(rows):
+    """Long rows in 32 slices, fewer, and one."""
+    x = row_logits(rows, 33000, torch.float32, rows)
+    u, temp, k, p, mp = settings(rows, rows)
+    check_sample(x, u, temp, k, p, mp)
+
+
+def test_sample_top_p_alone_on_both_sides_of_its_estimate():
+    """Borders among the few highest tokens, in the bulk, and on a border
+    between tokens that FP32 cannot tell apart: equal weights of which the
+    share is a whole number."""
+    x = row_logits(12, 30000, torch.float32, 31, spread=2.0)
+    x[:, 100] += 14.0
+    u = [i / 12 for i in range(12)]
+    for temp in (0.5, 1.0, 2.0):
+        check_sample(x, u, [temp] * 12, p=[0.01, 0.1, 0.3, 0.5, 0.6, 0.7, 0.8, 0.9, 0.95, 0.99, 0.999, 0.9999])
+    y = torch.full((6, 20000), -30.0).cuda()
+    y[:, 7:8 + 63] = 5.0  # 64 equal tokens, the others at e^-35
+    check_sample(y, u[:6], [1.0] * 6, p=[0.125, 0.25, 0.5, 0.75, 0.015625, 0.984375])
+
+
+def test_two_streams_at_once():
+    """Calls of all operators on two streams do not share anything."""
+    from test_gpu_delta import inputs
+
+    def work(seed):
+        data = inputs(300, 1, 2, 128, 128, torch.float16, seed)
+        cu = torch.tensor([0, 100, 300], dtype=torch.int32).cuda()
+        S = torch.zeros((2, 2, 128, 128), device="cuda")
+        x = row_logits(6, 70000, torch.bfloat16, seed)
+        u, t, p = (torch.full((6,), v).cuda() for v in (0.3, 0.9, 0.95))
+        h = torch.arange(600, dtype=torch.int32).cuda().view(6, 100)
+        n = torch.full((6,), 100, dtype=torch.int32).cuda()
+        torch.cuda.synchronize()
+
+        def go():
+            o = g.delta_prefill(*data, cu, state_out=S)
+            o2 = g.delta_step(*(z[:2] for z in data), S)
+            y = g.logits_process(x, history=h, history_len=n, presence=t)
+            return [o, o2, S.clone(), y, *g.sample_tokens(y, u, temperature=t, top_p=p)]
+        return go
+
+    a, b = work(1), work(2)
+    want = [[z.clone() for z in f()] for f in (a, b)]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in range(2)]
+    for _ in range(5):
+        got = []
+        for f, s in zip((a, b), streams):
+            with torch.cuda.stream(s):
+                got.append(f())
+        torch.cuda.synchronize()
+        for w, z in zip(want, got):
+            assert all(torch.equal(i, j) for i, j in zip(w, z))
+
+
+def test_wide_rows_captured():
+    x = row_logits(3, 100001, torch.bfloat16, 41)
+    u, t, p = (torch.full((3,), v).cuda() for v in (0.3, 1.1, 0.9))
+    k = torch.tensor([0, 50, 3], dtype=torch.int32).cuda()
+
+    def work():
+        return g.sample_tokens(x, u, temperature=t, top_p=p, top_k=k)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        work()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = work()
+    for seed in range(4):
+        x.copy_(row_logits(3, 100001, torch.bfloat16, 50 + seed))
+        u.fill_(0.2 * (seed + 1))
+        want = [z.clone() for z in work()]
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(captured[0], want[0]) and torch.equal(captured[1], want[1])
+
+
 def test_sample_follows_the_distribution():
     """Evenly spread draws meet each token as often as its probability."""
     x = torch.tensor([[0.0, 1.0, 2.0, -1.0]]).cuda().expand(4096, 4).contiguous()
