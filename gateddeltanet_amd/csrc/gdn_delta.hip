@@ -848,14 +848,15 @@ __global__ __launch_bounds__(64 * KP, sizeof(SeqLds<T, DK, KP>) <= (80 << 10) ? 
 
 // ------------------------------------------------------------ a single token
 
-// A (sequence, value head)'s token for NC value columns: grid (value_dim / NC,
+// A (sequence, value head)'s token for 64 value columns: grid (value_dim / 64,
 // value heads, sequences).  The state tile goes through registers once: with
 // a = exp(g), the sums S^T k and S^T q are formed from the state as it is read,
 //   d = beta (v - a S^T k);  o = scale (a S^T q + (k . q) d);  S' = a S + k d^T
 // so its bytes, in and out, are what bounds the kernel.
-template <class T, int DK, int NC>
+constexpr int kStepCols = 64;
+template <class T, int DK>
 __global__ __launch_bounds__(kT) void k_delta_step(GDNDelta p) {
-    constexpr int L = NC / 4, RP = kT / L, NR = (DK + RP - 1) / RP;  // lanes a row, rows a pass, passes
+    constexpr int NC = kStepCols, L = NC / 4, RP = kT / L, NR = (DK + RP - 1) / RP;  // lanes a row, rows a pass, passes
     static_assert(DK % RP == 0, "whole passes");
     __shared__ __attribute__((aligned(16))) float kq[2][DK];
     __shared__ float part[3][4];
@@ -982,11 +983,11 @@ int check(const char *who, const GDNDelta *a, bool packed) {
     const uintptr_t at = reinterpret_cast<uintptr_t>(a->q) | reinterpret_cast<uintptr_t>(a->k) |
                          reinterpret_cast<uintptr_t>(a->v) | reinterpret_cast<uintptr_t>(a->o) |
                          reinterpret_cast<uintptr_t>(a->state_in) | reinterpret_cast<uintptr_t>(a->state_out);
-    if ((at & 15) != 0 || ((a->q_stride | a->k_stride | a->v_stride | a->o_stride) % per16) != 0)
+    const int64_t strides = a->n_tokens > 1 ? a->q_stride | a->k_stride | a->v_stride | a->o_stride : 0;
+    if ((at & 15) != 0 || strides % per16 != 0)
         return refuse(who, "rows of q, k, v and o and the states start at multiples of 16 bytes");
     // rows' offsets inside a chunk are formed in 24 x 24 bits
-    if (((a->q_stride | a->k_stride | a->v_stride | a->o_stride) * size) >> 24 != 0)
-        return refuse(who, "a row stride is negative or larger than 16 MB");
+    if (strides < 0 || strides >= (1 << 24) / size) return refuse(who, "a row stride is negative, or 16 MB or more");
     const int64_t dq = (int64_t)a->n_qk_heads * a->key_dim, dv = (int64_t)a->n_v_heads * a->value_dim;
     if (a->n_tokens > 1 && (a->q_stride < dq || a->k_stride < dq || a->v_stride < dv || a->o_stride < dv ||
                             a->g_stride < (int64_t)a->n_v_heads))
@@ -1029,13 +1030,7 @@ void launch_prefill_dk(const GDNDelta &a, void *ws, hipStream_t s) {
 
 template <class T, int DK>
 void launch_step(const GDNDelta &a, hipStream_t s) {
-    // columns a workgroup: whole 256-byte row pieces, or 64-byte ones where
-    // the former would leave CUs idle
-    const size_t wide = (size_t)a.n_seqs * a.n_v_heads * (a.value_dim / 64);
-    if (wide >= 256)
-        hipLaunchKernelGGL((k_delta_step<T, DK, 64>), dim3(a.value_dim / 64, a.n_v_heads, a.n_seqs), dim3(kT), 0, s, a);
-    else
-        hipLaunchKernelGGL((k_delta_step<T, DK, 16>), dim3(a.value_dim / 16, a.n_v_heads, a.n_seqs), dim3(kT), 0, s, a);
+    hipLaunchKernelGGL((k_delta_step<T, DK>), dim3(a.value_dim / kStepCols, a.n_v_heads, a.n_seqs), dim3(kT), 0, s, a);
 }
 template <class T>
 void launch_step_dk(const GDNDelta &a, hipStream_t s) {
@@ -1058,7 +1053,9 @@ extern "C" int gdn_delta_prefill(const GDNDelta *args, void *workspace, size_t w
     constexpr const char *who = "gdn_delta_prefill";
     const int rc = check(who, args, true);
     if (rc != 0) return rc < 0 ? -1 : 0;
-    if (places(args) > 0x7fffffffu / 4 || (uint64_t)args->n_seqs * args->n_v_heads > (1u << 24))
+    // a grid has fewer than 2^32 threads along an axis
+    constexpr uint64_t most = (1ull << 32) / (64 * 4) - 8;
+    if (places(args) >= most || (uint64_t)args->n_seqs * args->n_v_heads > most / (args->value_dim / 16) - 8)
         return refuse(who, "too many chunks or heads for one launch");
     if (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0 ||
         workspace_bytes < gdn_delta_prefill_workspace(args))

@@ -1197,8 +1197,9 @@ extern "C" int gdn_logits_process(const GDNLogits *args, void *stream) {
     if (a.rows > 1 && (a.logits_stride < (int64_t)a.vocab || a.out_stride < (int64_t)a.vocab ||
                        (a.history && a.history_stride < (int64_t)a.history_width)))
         return refuse(who, "a row stride is smaller than the row");
-    if (a.history_width > 0x7fffffffu || a.n_bias > 0x7fffffffu || a.n_masks > 0x7fffffffu)
-        return refuse(who, "a size passes 2^31 - 1");
+    // (the kernel's steps past an end stay in 32 bits)
+    if (a.history_width > (1u << 30) || a.n_bias > (1u << 30) || a.n_masks > (1u << 30))
+        return refuse(who, "a width or count is larger than 2^30");
     if (a.mask && a.mask_stride < (int64_t)((a.vocab + 31) / 32)) return refuse(who, "mask rows are shorter than the vocabulary");
     if (a.mask && !a.mask_index && a.n_masks < a.rows) return refuse(who, "fewer masks than rows, and no mask_index");
     const dim3 grid((a.vocab + kTile - 1) / kTile, a.rows);

@@ -5,7 +5,8 @@ sequences, and the way from a batch's logits to its tokens.
 Arguments are torch tensors on one GPU; work goes to that GPU's current stream
 and is not waited for, and every call can be captured into a graph.  Where a
 function makes its output or workspace, it takes them from torch's allocator on
-that stream.  Errors raise ``GDNError``, before anything is enqueued.
+that stream.  Errors raise ``GDNError``, before anything is enqueued.  Nothing
+here is recorded for gradients.
 """
 from __future__ import annotations
 
@@ -200,6 +201,8 @@ def logits_process(logits: torch.Tensor, *, history: Optional[torch.Tensor] = No
         if words * 32 < vocab:
             _fail(f"mask: {words} words are fewer than {vocab} tokens")
         n_masks, m_index = mask.shape[0], _on(dev, "mask_index", mask_index, _I32, one)
+        if mask_index is None and n_masks < rows:
+            _fail(f"mask: {n_masks} masks for {rows} rows, and no mask_index")
     elif mask_index is not None:
         _fail("mask_index needs a mask")
     a = L.GDNLogits(dtype, rows, vocab, width, n_bias, n_masks, stride, into, h_stride, m_stride, logits.data_ptr(),

@@ -355,7 +355,10 @@ class BatchState:
 
         def put(name, value, dtype, shape=(n,)):
             if value is not None:
-                keep.append(np.ascontiguousarray(np.broadcast_to(np.asarray(value, dtype), shape)))
+                try:
+                    keep.append(np.ascontiguousarray(np.broadcast_to(np.asarray(value, dtype), shape)))
+                except (ValueError, OverflowError) as e:
+                    raise GDNError(f"{name}: expected {np.dtype(dtype).name} {shape}: {e}") from None
                 setattr(a, name, keep[-1].ctypes.data)
 
         def ragged(lists):
@@ -371,15 +374,17 @@ class BatchState:
         if histories is not None:
             at = ragged(histories)
             put("history_offsets", at, np.int32, (n + 1,))
-            put("history", np.concatenate([np.asarray(x, np.int32) for x in histories]), np.int32, (at[-1],))
+            put("history", [t for x in histories for t in x], np.int32, (at[-1],))
         if biases is not None:
             at = ragged(biases)
             put("bias_offsets", at, np.int32, (n + 1,))
             put("bias_ids", [t for b in biases for t in b], np.int32, (at[-1],))
             put("bias_values", [v for b in biases for v in b.values()], np.float32, (at[-1],))
         if mask is not None:
-            bits = np.zeros((n, (vocab + 31) // 32 * 32), bool)
-            bits[:, :vocab] = np.broadcast_to(np.asarray(mask, bool), (n, vocab))
+            mask, bits = np.asarray(mask, bool), np.zeros((n, (vocab + 31) // 32 * 32), bool)
+            if mask.shape not in ((vocab,), (1, vocab), (n, vocab)):
+                raise GDNError(f"mask: expected bool {(n, vocab)}, got {mask.shape}")
+            bits[:, :vocab] = mask
             put("mask", np.packbits(bits, axis=1, bitorder="little").view(np.uint32), np.uint32, (n, bits.shape[1] // 32))
         tokens, logprobs = np.empty(n, np.int32), np.empty(n, np.float32)
         _check(L.load().gdn_batch_sample(self.ptr, ctypes.byref(a), iptr(tokens), fptr(logprobs)), "gdn_batch_sample")

@@ -638,9 +638,9 @@ int gdn_test_prefill_gemm(int kind, const float *W, const float *X, uint32_t N, 
  *              n_tokens = n_seqs, row i is sequence i's token, cu_seqlens is
  *              not read.
  *   *_dim      64, 128 or 256, heads contiguous in a row
- *   *_stride   elements between rows (g and beta: one stride).  q, k, v and o
- *              rows start at multiples of 16 bytes and lie less than 16 MB
- *              apart; o overlaps no input
+ *   *_stride   elements between rows (g and beta: one stride; with one row not
+ *              looked at).  q, k, v and o rows start at multiples of 16 bytes
+ *              and lie less than 16 MB apart; o overlaps no input
  *   g, beta    FP32; g is the log of the decay (<= 0 in a stable model;
  *              -inf clears the state)
  *   state_in, state_out   [n_slots][n_v_heads][key_dim][value_dim] FP32, at
@@ -700,7 +700,7 @@ int gdn_delta_step(const GDNDelta *args, void *stream);
  *   mask        [n_masks][mask_stride] words, bit t % 32 of word t / 32 set for
  *               an allowed token; row r uses mask mask_index[r] (NULL: r; an
  *               index outside 0 .. n_masks - 1: none).  mask NULL: none
- * vocab is at most 2^24. */
+ * vocab is at most 2^24, history_width, n_bias and n_masks 2^30. */
 typedef struct {
     int32_t dtype;              /* GDN_DTYPE_* of logits and out */
     uint32_t rows, vocab;

@@ -162,3 +162,32 @@ def test_tensors_must_be_on_a_gpu():
 def test_batch_sample_refuses_without_an_engine():
     state, tokens = _lib.GDNBatchState(), (ctypes.c_int32 * 4)()
     assert _lib.load().gdn_batch_sample(ctypes.byref(state), None, tokens, None) == -1
+
+
+@pytest.mark.parametrize("change", [dict(history_width=(1 << 30) + 1, history_stride=1 << 31),
+                                    dict(n_bias=(1 << 30) + 1), dict(n_masks=(1 << 30) + 1)],
+                         ids=lambda c: next(iter(c)))
+def test_logits_process_refuses_what_32_bits_cannot_step_over(change, capfd):
+    assert _lib.load().gdn_logits_process(ctypes.byref(logits(**change)), None) == -1
+    assert "2^30" in capfd.readouterr().err
+
+
+@pytest.mark.parametrize("change", [
+    dict(n_tokens=0x7fffffff),                                         # 2^25 chunks of 64
+    dict(n_seqs=65535, n_slots=65535, n_v_heads=256, v_stride=32768, o_stride=32768, g_stride=256),
+    dict(n_seqs=65535, n_slots=65535, n_v_heads=20, v_stride=5120, o_stride=5120, g_stride=20, value_dim=256),
+], ids=["chunks", "heads", "tiles"])
+def test_prefill_refuses_what_no_grid_holds(change, capfd):
+    a = delta(**change)
+    assert _lib.load().gdn_delta_prefill(ctypes.byref(a), AT, 1 << 62, None) == -1
+    assert "too many chunks or heads" in capfd.readouterr().err
+
+
+@pytest.mark.parametrize("change", [dict(q_stride=1 << 23), dict(k_stride=-1024), dict(o_stride=1 << 40)],
+                         ids=["16MB", "negative", "large"])
+def test_delta_refuses_strides(change, capfd):
+    lib = _lib.load()
+    assert lib.gdn_delta_prefill(ctypes.byref(delta(**change)), AT, 1 << 62, None) == -1
+    assert "row stride" in capfd.readouterr().err
+    assert lib.gdn_delta_step(ctypes.byref(delta(step=True, **change)), None) == -1
+    assert "row stride" in capfd.readouterr().err

@@ -419,3 +419,15 @@ def test_tensor_refusals():
         g.delta_step(odd, k, v, gate, beta, P)
     with pytest.raises(g.GDNError):
         g.delta_step(q, k, v, gate, beta, S)
+
+
+def test_one_row_of_any_stride():
+    """A single token's rows have no stride to keep to."""
+    q, k, v, gate, beta = inputs(1, 1, 2, 64, 128, BF16, 51)
+    odd = [torch.as_strided(x, x.shape, (s, *x.stride()[1:])) for x, s in ((q, 3), (k, 1 << 40), (v, 0), (gate, 7))]
+    S = torch.ones((1, 2, 64, 128), device="cuda")
+    T = S.clone()
+    cu = torch.tensor([0, 1], dtype=torch.int32).cuda()
+    assert torch.equal(g.delta_step(*odd, beta, S), g.delta_step(q, k, v, gate, beta, T)) and torch.equal(S, T)
+    assert torch.equal(g.delta_prefill(*odd, beta, cu, state_out=S), g.delta_prefill(q, k, v, gate, beta, cu, state_out=T))
+    assert torch.equal(S, T)

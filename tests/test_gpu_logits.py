@@ -581,3 +581,35 @@ def test_batch_sample():
     finally:
         bs.free()
         m.free()
+
+
+def test_batch_sample_after_a_prefill_and_its_refusals():
+    m = g.Model.synth(num_layers=1, seed=3)
+    bs = g.BatchState(m, 3)
+    try:
+        bs.step([1, 2, 3])
+        seed = bs.prefill(1, [5, 6, 7, 8])
+        tok, lp = bs.sample()
+        assert tok[1] == seed
+        for s in range(3):
+            x = bs.logits(s).astype(np.float64)
+            assert tok[s] == x.argmax() and abs(lp[s] + np.log(np.exp(x - x.max()).sum())) < 1e-5
+        one = np.ones(32000, bool)
+        one[tok[0]] = False
+        again, _ = bs.sample(mask=one)  # one mask for all
+        assert again[0] != tok[0] and (bs.sample(mask=one[None])[0] == again).all()
+        for kw in (dict(mask=True), dict(mask=np.ones((2, 32000), bool)), dict(mask=one[:-1]), dict(top_k=[1, 2]),
+                   dict(temperature=[0.0] * 4, uniform=0.0), dict(histories=[[1 << 40], [], []]),
+                   dict(biases=[{}, {}]), dict(histories=[[], []])):
+            with pytest.raises(g.GDNError):
+                bs.sample(**kw)
+    finally:
+        bs.free()
+        m.free()
+
+
+def test_process_refuses_fewer_masks_than_rows():
+    x = torch.zeros((2, 64)).cuda()
+    for n in (0, 1):
+        with pytest.raises(g.GDNError, match="masks for 2 rows"):
+            g.logits_process(x, mask=torch.zeros((n, 2), dtype=torch.int32).cuda())
