@@ -203,9 +203,10 @@ struct SampleLds {
         uint64_t cell[kCells];
     };
     // tokens gathered from the row, and their places
-    static constexpr int kSome = HELD ? kST : 8 * kST;
-    float some[kSome] __attribute__((aligned(8)));
+    static constexpr int kSome = HELD ? 3 * kST / 2 : 8 * kST;
+    float some[kSome];
     int some_at[kSome];
+    uint64_t before[kList];
     uint64_t wsum[2][kWaves];
     float wmax[kWaves];
     int warg[kWaves];
@@ -214,7 +215,7 @@ struct SampleLds {
     double left;      // of the goal, in it
     float x;          // a border
     int at;
-    uint32_t bin, n, n_some, crowded;
+    uint32_t bin, n, ahead, n_some, all_above, crowded;
 };
 
 __device__ __forceinline__ uint64_t lane_of(uint64_t v, int lane) {
@@ -340,29 +341,34 @@ struct Row {
     }
 };
 
-// The border of the tokens of step `b` (there are `inside`) whose ranked counts
+// The border of the tokens of step `b` (there are `inside`, and `ahead` above) whose ranked counts
 // (by_mass: weights) first reach `left`, into lds.x and lds.at; their weight is
 // the result.  listed: they are among the threads' `own` (none: at < 0).
 template <class T, bool HELD>
-__device__ __forceinline__ uint64_t border_in(const Row<T, HELD> &r, SampleLds<T, HELD> &lds, int b, uint32_t inside,
-                                              bool by_mass, double left, bool listed, const Ranked &own) {
+__device__ __forceinline__ uint64_t border_in(const Row<T, HELD> &r, SampleLds<T, HELD> &lds, int b, uint32_t ahead,
+                                              uint32_t inside, bool by_mass, double left, bool listed, const Ranked &own) {
     constexpr int V = T::kVec;
     const int t = threadIdx.x;
     float lo, hi;
     r.bounds(b, b + 1, lo, hi);
     // The step's tokens lie among many others, so that nearly every wave would
     // form their weights for a few lanes: they are gathered first where they
-    // fit (131072 tokens: 30 us a pass otherwise)
+    // fit (131072 tokens: 30 us a pass otherwise); with those above them, for
+    // the draw, if the row is held and these fit too
     constexpr int kSome = SampleLds<T, HELD>::kSome;
     uint32_t n_some = kSome + 1;
-    if (!listed) {
+    for (int turn = HELD && ahead + inside <= (uint32_t)kSome ? 0 : 1; turn < 2 && !listed && n_some > (uint32_t)kSome; ++turn) {
+        const float most = turn == 0 ? kInf : hi;
         __syncthreads();
-        if (t == 0) lds.n_some = 0;
+        if (t == 0) {
+            lds.n_some = 0;
+            lds.all_above = turn == 0;
+        }
         __syncthreads();
         r.each([&](const float(&x)[V], int at) __attribute__((always_inline)) {
 #pragma unroll
             for (int j = 0; j < V; ++j) {
-                const bool in = x[j] >= lo && x[j] <= hi;
+                const bool in = x[j] >= lo && x[j] <= most;
                 const uint64_t who = __ballot(in);
                 if (who == 0) continue;
                 const int before = (int)__builtin_amdgcn_mbcnt_hi((uint32_t)(who >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)who, 0u));
@@ -456,11 +462,10 @@ __device__ __forceinline__ uint64_t border_in(const Row<T, HELD> &r, SampleLds<T
         const int n = (int)inside;
         int lanes = kST / kList;
         while (lanes < 64 && 2 * lanes * n <= kST) lanes *= 2;
-        unsigned long long *befores = reinterpret_cast<unsigned long long *>(lds.some);
-        static_assert(sizeof(lds.some) >= kList * sizeof(uint64_t) && kList <= kBins, "room for ranks and weights before");
+        static_assert(kList <= kBins, "room for ranks");
         if (t < kList) {
             lds.count[t] = 0;
-            befores[t] = 0;
+            lds.before[t] = 0;
         }
         __syncthreads();
         const int who = t / lanes;
@@ -477,14 +482,14 @@ __device__ __forceinline__ uint64_t border_in(const Row<T, HELD> &r, SampleLds<T
             }
             if (rank != 0) {
                 atomicAdd(&lds.count[who], rank);
-                atomicAdd(&befores[who], (unsigned long long)before);
+                atomicAdd(reinterpret_cast<unsigned long long *>(&lds.before[who]), (unsigned long long)before);
             }
         }
         __syncthreads();
         if (t < n) {
             const Ranked me = lds.list[t];
             const int rank = (int)lds.count[t];
-            const uint64_t before = befores[t];
+            const uint64_t before = lds.before[t];
             const double from = by_mass ? (double)before : (double)rank,
                          to = by_mass ? (double)(before + me.w) : (double)(rank + 1);
             // rounding in `left` past the step's end: its last token
@@ -653,10 +658,11 @@ __device__ __forceinline__ uint64_t borders(const Row<T, HELD> &r, SampleLds<T, 
             lds.left = goal - (double)before;
             lds.base = m_before;
             lds.n = (uint32_t)count;
+            lds.ahead = (uint32_t)n_before;
         }
         __syncthreads();
         const uint64_t base = lds.base;
-        kept = base + border_in(r, lds, (int)lds.bin, lds.n, by_mass, lds.left, listed, own);
+        kept = base + border_in(r, lds, (int)lds.bin, lds.ahead, lds.n, by_mass, lds.left, listed, own);
         if (lds.x > keep.edge || (lds.x == keep.edge && lds.at < keep.edge_at)) {
             keep.edge = lds.x;
             keep.edge_at = lds.at;
@@ -784,6 +790,7 @@ __global__ __launch_bounds__(kST) void k_sample(GDNSample p, int shift) {
         if (t == 0) {
             lds.bin = kBins;
             lds.crowded = 0;
+            lds.all_above = 0;
         }
         __syncthreads();
         const uint64_t n = lds.count[t], enough = ask.by_k ? (uint64_t)ask.k : 64;
@@ -887,7 +894,8 @@ __global__ __launch_bounds__(kST) void k_sample(GDNSample p, int shift) {
     }
 
     Keep keep;
-    bool listed = false;  // what is kept is among the threads' own
+    bool listed = false;    // what is kept is among the threads' own
+    bool gathered = false;  // or among lds.some
     if (ask.by_k || ask.by_p) {
         double all = 0.0, high = 0.0;
         if (alone)
@@ -921,6 +929,7 @@ __global__ __launch_bounds__(kST) void k_sample(GDNSample p, int shift) {
             const double whole = __builtin_ldexp(all, shift);
             const uint64_t kept = borders(r, lds, ask, count, mass, n_before, m_before, n_all,
                                           guess ? (uint64_t)(whole * (1.0 - kOff)) : m_all, listed, own, keep);
+            gathered = !listed && lds.all_above && lds.n_some <= (uint32_t)SampleLds<T, true>::kSome;
             if (!guess || (double)ask.top_p * whole * (1.0 + kOff) <= (double)kept) break;
             keep = Keep();
         }
@@ -933,11 +942,19 @@ __global__ __launch_bounds__(kST) void k_sample(GDNSample p, int shift) {
     // the kept weights by pieces of 64 V tokens
     const int cells = (r.n + 64 * V - 1) / (64 * V);
     __syncthreads();
-    if (listed) {
+    if (listed || gathered) {
         for (int c = t; c < cells; c += kST) lds.cell[c] = 0;
         __syncthreads();
-        if (own.at >= 0 && keep.has(own.x, own.at) && (double)own.w >= keep.least)
-            atomicAdd(reinterpret_cast<unsigned long long *>(&lds.cell[own.at / (64 * V)]), (unsigned long long)own.w);
+        auto add = [&](int at, uint64_t s) __attribute__((always_inline)) {
+            if ((double)s >= keep.least)
+                atomicAdd(reinterpret_cast<unsigned long long *>(&lds.cell[at / (64 * V)]), (unsigned long long)s);
+        };
+        if (listed) {
+            if (own.at >= 0 && keep.has(own.x, own.at)) add(own.at, own.w);
+        } else {
+            for (uint32_t i = t; i < lds.n_some; i += kST)
+                if (keep.has(lds.some[i], lds.some_at[i])) add(lds.some_at[i], r.weight(r.fall(lds.some[i])));
+        }
     } else {
         for (int c = w; c < cells; c += kWaves) {
             const uint64_t s = keep.piece(r, c, lane);

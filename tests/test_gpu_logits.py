@@ -370,6 +370,21 @@ def test_sample_top_p_alone_on_both_sides_of_its_estimate():
     check_sample(y, u[:6], [1.0] * 6, p=[0.125, 0.25, 0.5, 0.75, 0.015625, 0.984375])
 
 
+@pytest.mark.parametrize("kind", TYPES)
+def test_sample_keeps_more_and_less_than_it_gathers(kind):
+    """Kept tokens by the thousand, on both sides of what LDS lists hold."""
+    x = row_logits(10, 20000, TYPES[kind], 61, spread=0.7)
+    def f(*a):
+        return np.array(a, np.float32).tolist()
+
+    u = f(*(0.05 + i / 11 for i in range(10)))
+    k = [1000, 1400, 1500, 1530, 1536, 1540, 1600, 2000, 5000, 0]
+    check_sample(x, u, [1.0] * 10, k=k)
+    check_sample(x, u, f(*[1.3] * 10), k=k, p=f(0.5, 0.99, 0.9, 1.0, 0.999, 0.7, 0.95, 0.8, 0.3, 0.2))
+    check_sample(x, u, [1.0] * 10, p=f(0.1, 0.12, 0.14, 0.16, 0.18, 0.2, 0.22, 0.24, 0.26, 0.3),
+                 mp=f(0.0, 0.3) * 5)
+
+
 def test_two_streams_at_once():
     """Calls of all operators on two streams do not share anything."""
     from test_gpu_delta import inputs
