@@ -200,6 +200,10 @@ __device__ __forceinline__ void subst(const float (&row)[16], int li, float (&co
 // and for the whole's halves on FP32 MFMAs.
 // The last place's workgroup orders the sequences for k_delta_seq, longest
 // first, by counting their chunks in 256 steps.
+// Bound by latency: loads, the products, 16 steps of substitution, four stages
+// of the inverse.  BF16, 8 heads of 256: 10.1 us for 70 tokens, 18.9 for 4096 (36
+// MB, 1.9 TB/s), 32.6 for 8111 in 24 sequences; FP32, 2005 tokens, 8 heads of 128:
+// 15.7 us.
 template <class T, int DK>
 __global__ __launch_bounds__(4 * kChunk<T>) void k_delta_prep(GDNDelta p, int *__restrict__ order,
                                                               ChunkOps<kChunk<T>> *__restrict__ ops_all,
@@ -484,6 +488,15 @@ __global__ __launch_bounds__(4 * kChunk<T>) void k_delta_prep(GDNDelta p, int *_
 // of b, d and the scaled d in LDS as the B operands that the tile's waves read.
 // Three barriers a chunk; every operand of the next chunk is on its way into
 // registers meanwhile, in the order of its use.
+// Bound, with few sequences, by a chunk's chain of dependent products: 64 chunks
+// of 8 heads of 256 x 256 in 193 us, 3.0 us each, the matrix unit busy for 1536
+// of 7200 cycles; with many, by the operands that a head's 16 column tiles read
+// through L2 (8111 tokens in 24 sequences: 199 us, 9 TB/s).  FP32, 2005 tokens in
+// 5 sequences, 8 heads of 128 x 128: 60 us.  Measured against it at 4096 tokens:
+// all keys in one wave 656 us (the products of a tile in a row); two waves and
+// 64 columns 432 (registers spill); 32 columns with K and Q shared by eight waves
+// 259; fragments read from memory 269; two workgroups a CU by force 415 (spills).
+// A wave takes 32 keys or more, so KP is 2 for 64 keys, else 4.
 template <class T, int DK, int KP>
 struct SeqLds {
     static constexpr int C = kChunk<T>, NT = T::kTerms, MT = C / 16, JT = C / 32, UR = DK / KP / 8;
@@ -852,7 +865,12 @@ __global__ __launch_bounds__(64 * KP, sizeof(SeqLds<T, DK, KP>) <= (80 << 10) ? 
 // value heads, sequences).  The state tile goes through registers once: with
 // a = exp(g), the sums S^T k and S^T q are formed from the state as it is read,
 //   d = beta (v - a S^T k);  o = scale (a S^T q + (k . q) d);  S' = a S + k d^T
-// so its bytes, in and out, are what bounds the kernel.
+// so its bytes, in and out, are what bounds the kernel: 64 sequences of 8 heads of
+// 256 x 256, 268 MB, in 57 us (4.7 TB/s; 41 us where the last-level cache still
+// holds part of them), one in 5.7 us, two memory latencies and two reductions.
+// 64 columns: whole 256-byte pieces of a row.  16 columns fill more CUs in small
+// batches and lose there too (4 heads: 9.5 against 6.3 us at 8 sequences, 14.0
+// against 7.7 at 15; 4.9 against 5.1 at one).
 constexpr int kStepCols = 64;
 template <class T, int DK>
 __global__ __launch_bounds__(kT) void k_delta_step(GDNDelta p) {
