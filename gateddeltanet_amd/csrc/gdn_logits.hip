@@ -188,7 +188,10 @@ __global__ __launch_bounds__(kPT) void k_process(GDNLogits p) {
 // against slices (below), 64 x 32000: 18 against 30 us for top-k, 37 against 36 for
 // the flat top-p; 1024 x 32000: 76 against 137, 146 against 182.
 constexpr int kST = 1024, kBins = kST, kWaves = kST / 64;
-constexpr int kList = 512;             // tokens of a step that are ranked directly
+constexpr int kList = 512;             // tokens that are ranked against each other
+// A step of more tokens is cut in parts first, 2.4 us; ranking 65 takes 1.9 us, 111
+// 2.8, 196 6.7, 276 16.  512 here: 8 x 131072 54 to 58 us for 46 to 50; 64: equal.
+constexpr int kFew = 128;
 constexpr int kHeldBytes = 128 << 10;  // of a row in LDS
 constexpr int kMostVocab = 1 << 20;
 constexpr int kNowhere = 0x7fffffff;
@@ -455,7 +458,7 @@ __device__ __forceinline__ uint64_t border_in(const Row<T, HELD> &r, SampleLds<T
         return min(max((int)((d * r.step - (double)b) * (double)kBins), 0), kBins - 1);
     };
     int part = -1;
-    if (inside > (uint32_t)kList) {
+    if (inside > (uint32_t)kFew) {
         clear();
         each_of([&](float, int, double d) __attribute__((always_inline)) { put(part_of(d), d); });
         inside = find();
@@ -988,8 +991,10 @@ __global__ __launch_bounds__(kST) void k_sample(GDNSample p, int shift) {
 
 // Longer rows, a row's slices by workgroups of their own: the highest logit;
 // sums and the steps' counts and weights; the borders (a workgroup a row, which
-// reads the row once for each); the kept weights of the pieces; the token.  One
-// workgroup for all of it takes 300 us for 131072 tokens.
+// reads the row once for each); the kept weights of the pieces; the token.  8 rows
+// of 131072 BF16 logits, top-p 0.9: 37 us (top-k 50: 32, neither: 21); one
+// workgroup a row for all of it took twice the slices' time when both were built
+// alike (305 against 163 us).
 constexpr int kSlices = 32;
 struct WideRow {
     float top[kSlices];
@@ -1260,7 +1265,8 @@ void launch_sample(const GDNSample &a, void *ws, hipStream_t s) {
         hipLaunchKernelGGL(k_sample<T>, rows, block, 0, s, a, shift);
         return;
     }
-    // slices for two workgroups a CU
+    // slices for two workgroups a CU (131072 tokens, against one and four: 32 rows
+    // 47.6, 47.4 and 54.9 us, 128 rows 87.6, 90.6 and 90.0)
     const int slices = a.rows >= 512 ? 1 : a.rows * kSlices <= 512 ? kSlices : 512 / (int)a.rows;
     const dim3 parts(slices, a.rows);
     hipLaunchKernelGGL(k_wide_top<T>, parts, block, 0, s, a, ws);
