@@ -476,7 +476,7 @@ __global__ __launch_bounds__(4 * kChunk<T>) void k_delta_prep(GDNDelta p, int *_
 // One (sequence, value head)'s chunks in order:
 //   d = T (beta (v - exp(G) K S));  o = exp(G) Q S + M d;
 //   S' = exp(G_{n-1}) S + K^T (exp(G_{n-1} - G) d)
-// A workgroup has a tile of 16 value columns, its KP waves a KP-th of the keys
+// A workgroup has CT tiles of 16 value columns, its KP waves a KP-th of the keys
 // each.  A wave's state is the accumulator tiles of its updates, and lies
 // so that it is also the B operand of its K S and Q S: of a 32-key step, lane l
 // holds keys 8 (l / 16) .. + 7 of column l % 16, the first four in one tile, the
@@ -497,29 +497,34 @@ __global__ __launch_bounds__(4 * kChunk<T>) void k_delta_prep(GDNDelta p, int *_
 // 64 columns 432 (registers spill); 32 columns with K and Q shared by eight waves
 // 259; fragments read from memory 269; two workgroups a CU by force 415 (spills).
 // A wave takes 32 keys or more, so KP is 2 for 64 keys, else 4.
-template <class T, int DK, int KP>
+template <class T, int DK, int KP, int CT>
 struct SeqLds {
     static constexpr int C = kChunk<T>, NT = T::kTerms, MT = C / 16, JT = C / 32, UR = DK / KP / 8;
     // tiles a wave does not own, blocks of b that its area holds
-    static constexpr int kFor = KP <= MT ? MT - MT / KP : MT, kB = (3 * JT + KP - 1) / KP;
+    static constexpr int kFor = KP <= MT ? MT - MT / KP : MT, kB = (3 * CT * JT + KP - 1) / KP;
     // q's area takes the shares for other waves and b once Q S is formed
     union Area {
         u32x4 q[NT][C][UR];
         struct {
-            f32x4 part[kFor][2][64];  // [tile][K S, Q S]
-            u32x4 b[kB][64];          // block 3 step + term is the KP-th part's
+            f32x4 part[kFor][CT][2][64];  // [tile][column tile][K S, Q S]
+            u32x4 b[kB][64];              // the column tiles' blocks 3 step + term, a KP-th of them
         };
     };
     u32x4 k[KP][NT][C][UR];
     Area area[KP];
-    u32x4 df[2][JT][3][64];  // d and the scaled d, B operands: [which][step][term]
+    u32x4 df[2][CT][JT][3][64];  // d and the scaled d, B operands: [which][column tile][step][term]
 };
 
-template <class T, int DK, int KP>
-__global__ __launch_bounds__(64 * KP, sizeof(SeqLds<T, DK, KP>) <= (80 << 10) ? 2 : 1) void k_delta_seq(
+// Workgroups that a CU's LDS holds (its registers hold one where two tiles of
+// columns meet two of tokens).
+template <class T, int DK, int KP, int CT>
+constexpr int kSeqPerCu = sizeof(SeqLds<T, DK, KP, CT>) <= (80 << 10) ? 2 : 1;
+
+template <class T, int DK, int KP, int CT>
+__global__ __launch_bounds__(64 * KP, (kSeqPerCu<T, DK, KP, CT> == 2 && (CT == 1 || KP == 4 || kChunk<T> == 32)) ? 2 : 1) void k_delta_seq(
     GDNDelta p, const int *__restrict__ order, const ChunkOps<kChunk<T>> *__restrict__ ops_all,
     const Planes<T, DK> *__restrict__ planes, int pairs) {
-    using Lds = SeqLds<T, DK, KP>;
+    using Lds = SeqLds<T, DK, KP, CT>;
     constexpr int C = Lds::C, NT = Lds::NT, MT = Lds::MT, JT = Lds::JT;
     constexpr int KS = DK / 32 / KP;              // 32-key steps of a wave
     constexpr int OT = MT >= KP ? MT / KP : 1;    // token tiles a wave owns (with KP > MT, the first MT waves)
@@ -531,7 +536,7 @@ __global__ __launch_bounds__(64 * KP, sizeof(SeqLds<T, DK, KP>) <= (80 << 10) ? 
     const int t = threadIdx.x, ks = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63, li = lane & 15, kk = lane >> 4;
     // the column groups of a (sequence, head) share its operands: one XCD's
     // (workgroups go to the eight in turn)
-    const int groups = (int)p.value_dim / 16, x = blockIdx.x >> 3;
+    const int groups = (int)p.value_dim / (16 * CT), x = blockIdx.x >> 3;
     const int pair = (x / groups) * 8 + (blockIdx.x & 7), cg = x % groups;
     if (pair >= pairs) return;
     const int seq = order[pair / (int)p.n_v_heads], hv = pair % (int)p.n_v_heads;
@@ -541,21 +546,24 @@ __global__ __launch_bounds__(64 * KP, sizeof(SeqLds<T, DK, KP>) <= (80 << 10) ? 
     Span sp = span_of(p, seq);
     sp.first = __builtin_amdgcn_readfirstlane(sp.first);
     sp.n = __builtin_amdgcn_readfirstlane(sp.n);
-    const int chunks = (sp.n + C - 1) / C, col = 16 * cg + li;
+    const int chunks = (sp.n + C - 1) / C, col = 16 * CT * cg + li;
     const size_t place = (size_t)place_of<C>(sp.first, seq);
     const ChunkOps<C> *ops = ops_all + place * p.n_v_heads + hv;
     // the state's key of tile a, register r of step s: key0 + 32 s + 4 a + r
     const int key0 = ks * (DK / KP) + 8 * kk;
     const size_t state_at = (((size_t)slot * p.n_v_heads + hv) * DK + key0) * p.value_dim + col;
 
-    f32x4 S[KS][2];
+    f32x4 S[CT][KS][2];
 #pragma unroll
     for (int s = 0; s < KS; ++s)
 #pragma unroll
         for (int a = 0; a < 2; ++a)
 #pragma unroll
             for (int r = 0; r < 4; ++r)
-                S[s][a][r] = p.state_in ? p.state_in[state_at + (size_t)(32 * s + 4 * a + r) * p.value_dim] : 0.0f;
+#pragma unroll
+                for (int ct = 0; ct < CT; ++ct)
+                    S[ct][s][a][r] =
+                        p.state_in ? p.state_in[state_at + (size_t)(32 * s + 4 * a + r) * p.value_dim + 16 * ct] : 0.0f;
 
     // the token tiles this wave owns; tile i's matrix rows have steps 0 .. i / 2
     const bool owns = KP <= MT || ks < MT;
@@ -571,7 +579,7 @@ __global__ __launch_bounds__(64 * KP, sizeof(SeqLds<T, DK, KP>) <= (80 << 10) ? 
     };
     u32x4 kreg[kStage], qreg[kStage], tri[kTri][3];
     f32x4 sc[OT][4];
-    float vv[OT][4], dn;
+    float vv[OT][CT][4], dn;
     // rows past the sequence's end: its last one, whose products meet zero
     // factors (the planes hold zeros there)
     auto fetch_rows = [&](int c) __attribute__((always_inline)) {
@@ -607,7 +615,9 @@ __global__ __launch_bounds__(64 * KP, sizeof(SeqLds<T, DK, KP>) <= (80 << 10) ? 
             for (int r = 0; r < 4; ++r) {
                 const int m = 16 * tile_of(i) + 4 * kk + r;
                 sc[i][r] = o.sc[m];
-                vv[i][r] = T::get(vp + (__umul24(min(m, n - 1), v_row) + col * kSize), 0);
+#pragma unroll
+                for (int ct = 0; ct < CT; ++ct)
+                    vv[i][ct][r] = T::get(vp + (__umul24(min(m, n - 1), v_row) + (col + 16 * ct) * kSize), 0);
             }
     };
     auto fetch_tri = [&](const u32x4(&m)[kTriTiles<C>][3][64]) __attribute__((always_inline)) {
@@ -651,20 +661,23 @@ __global__ __launch_bounds__(64 * KP, sizeof(SeqLds<T, DK, KP>) <= (80 << 10) ? 
         if constexpr (kTri == 3) y[1] = sum[1] + sum[2];
     };
     // the terms of a tile's values, as half a B operand
-    auto put_terms = [&](auto &&block, int tile, const f32x4 v) __attribute__((always_inline)) {
+    auto put_terms = [&](auto &&block, int ct, int tile, const f32x4 v) __attribute__((always_inline)) {
         u32x2 e[3];
         split3(v, e);
 #pragma unroll
-        for (int q = 0; q < 3; ++q) reinterpret_cast<u32x2 *>(&block(3 * (tile >> 1) + q)[lane])[tile & 1] = e[q];
+        for (int q = 0; q < 3; ++q) reinterpret_cast<u32x2 *>(&block(ct, 3 * (tile >> 1) + q)[lane])[tile & 1] = e[q];
     };
-    auto b_block = [&](int i) -> u32x4(&)[64] { return lds.area[i / Lds::kB].b[i % Lds::kB]; };
-    auto d_block = [&](int i) -> u32x4(&)[64] { return lds.df[0][i / 3][i % 3]; };
-    auto f_block = [&](int i) -> u32x4(&)[64] { return lds.df[1][i / 3][i % 3]; };
-    auto get_operand = [&](auto &&block, u32x4(&b)[JT][3]) __attribute__((always_inline)) {
+    auto b_block = [&](int ct, int i) -> u32x4(&)[64] {
+        i += 3 * JT * ct;
+        return lds.area[i / Lds::kB].b[i % Lds::kB];
+    };
+    auto d_block = [&](int ct, int i) -> u32x4(&)[64] { return lds.df[0][ct][i / 3][i % 3]; };
+    auto f_block = [&](int ct, int i) -> u32x4(&)[64] { return lds.df[1][ct][i / 3][i % 3]; };
+    auto get_operand = [&](auto &&block, int ct, u32x4(&b)[JT][3]) __attribute__((always_inline)) {
 #pragma unroll
         for (int j = 0; j < JT; ++j)
 #pragma unroll
-            for (int q = 0; q < 3; ++q) b[j][q] = block(3 * j + q)[lane];
+            for (int q = 0; q < 3; ++q) b[j][q] = block(ct, 3 * j + q)[lane];
     };
     // the place in wave a's area of its share of a tile
     auto slot_in = [&](int a, int tile) {
@@ -700,17 +713,22 @@ __global__ __launch_bounds__(64 * KP, sizeof(SeqLds<T, DK, KP>) <= (80 << 10) ? 
         const ChunkOps<C> &next_ops = ops[(size_t)cn * p.n_v_heads];
         fetch_rows(cn);
         // this wave's share of K S and Q S
-        f32x4 y[MT][2];
+        f32x4 y[MT][CT][2];
 #pragma unroll
-        for (int i = 0; i < MT; ++i) y[i][0] = y[i][1] = zero;
+        for (int i = 0; i < MT; ++i)
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) y[i][ct][0] = y[i][ct][1] = zero;
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
-            u32x2 lo[3], hi[3];
-            split3(S[s][0], lo);
-            split3(S[s][1], hi);
-            u32x4 sb[3];
+            u32x4 sb[CT][3];
 #pragma unroll
-            for (int q = 0; q < 3; ++q) sb[q] = (u32x4){lo[q].x, lo[q].y, hi[q].x, hi[q].y};
+            for (int ct = 0; ct < CT; ++ct) {
+                u32x2 lo[3], hi[3];
+                split3(S[ct][s][0], lo);
+                split3(S[ct][s][1], hi);
+#pragma unroll
+                for (int q = 0; q < 3; ++q) sb[ct][q] = (u32x4){lo[q].x, lo[q].y, hi[q].x, hi[q].y};
+            }
             u32x4 ka[MT][NT], qa[MT][NT];
 #pragma unroll
             for (int i = 0; i < MT; ++i)
@@ -724,10 +742,12 @@ __global__ __launch_bounds__(64 * KP, sizeof(SeqLds<T, DK, KP>) <= (80 << 10) ? 
             // twice its time
             for_terms<NT, 3>([&](int a, int b) __attribute__((always_inline)) {
 #pragma unroll
-                for (int i = 0; i < MT; ++i) {
-                    y[i][0] = mfma_bf16(ka[i][a], sb[b], y[i][0]);
-                    y[i][1] = mfma_bf16(qa[i][a], sb[b], y[i][1]);
-                }
+                for (int i = 0; i < MT; ++i)
+#pragma unroll
+                    for (int ct = 0; ct < CT; ++ct) {
+                        y[i][ct][0] = mfma_bf16(ka[i][a], sb[ct][b], y[i][ct][0]);
+                        y[i][ct][1] = mfma_bf16(qa[i][a], sb[ct][b], y[i][ct][1]);
+                    }
             });
         }
         // a load between two products each: issued in a row they hold the wave
@@ -735,65 +755,77 @@ __global__ __launch_bounds__(64 * KP, sizeof(SeqLds<T, DK, KP>) <= (80 << 10) ? 
 #pragma unroll
         for (int i = 0; i < 2 * kStage; ++i) {
             __builtin_amdgcn_sched_group_barrier(0x020, 1, 0);
-            __builtin_amdgcn_sched_group_barrier(0x008, 2, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, 2 * CT, 0);
         }
 #pragma unroll
         for (int i = 0; i < MT; ++i)
             if (owner(i) != ks) {
-                f32x4(&part)[2][64] = lds.area[ks].part[slot_in(ks, i)];
-                part[0][lane] = y[i][0];
-                part[1][lane] = y[i][1];
+                f32x4(&part)[CT][2][64] = lds.area[ks].part[slot_in(ks, i)];
+#pragma unroll
+                for (int ct = 0; ct < CT; ++ct) {
+                    part[ct][0][lane] = y[i][ct][0];
+                    part[ct][1][lane] = y[i][ct][1];
+                }
             }
         __syncthreads();
-        f32x4 qs[OT], sw[OT];
+        f32x4 qs[OT][CT], sw[OT];
         if (owns) {
             // b, and what stands of o
 #pragma unroll
             for (int o = 0; o < OT; ++o) {
                 const int tile = tile_of(o);
-                f32x4 kv = zero, qv = zero;
 #pragma unroll
-                for (int i = 0; i < MT; ++i)
-                    if (i == tile) {
-                        kv = y[i][0];
-                        qv = y[i][1];
+                for (int ct = 0; ct < CT; ++ct) {
+                    f32x4 kv = zero, qv = zero;
+#pragma unroll
+                    for (int i = 0; i < MT; ++i)
+                        if (i == tile) {
+                            kv = y[i][ct][0];
+                            qv = y[i][ct][1];
+                        }
+#pragma unroll
+                    for (int a = 1; a < KP; ++a) {
+                        const int from = (ks + a) % KP;
+                        const f32x4(&part)[CT][2][64] = lds.area[from].part[slot_in(from, tile)];
+                        kv += part[ct][0][lane];
+                        qv += part[ct][1][lane];
                     }
+                    f32x4 b;
 #pragma unroll
-                for (int a = 1; a < KP; ++a) {
-                    const int from = (ks + a) % KP;
-                    const f32x4(&part)[2][64] = lds.area[from].part[slot_in(from, tile)];
-                    kv += part[0][lane];
-                    qv += part[1][lane];
+                    for (int r = 0; r < 4; ++r) {
+                        const f32x4 e = sc[o][r];
+                        b[r] = e.y * (vv[o][ct][r] - e.x * kv[r]);
+                        qs[o][ct][r] = e.z * qv[r];
+                        sw[o][r] = e.w;
+                    }
+                    put_terms(b_block, ct, tile, b);
                 }
-                f32x4 b;
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const f32x4 e = sc[o][r];
-                    b[r] = e.y * (vv[o][r] - e.x * kv[r]);
-                    qs[o][r] = e.z * qv[r];
-                    sw[o][r] = e.w;
-                }
-                put_terms(b_block, tile, b);
             }
             fetch_own(cn);
         }
         __syncthreads();
         if (owns) {
-            f32x4 d[OT];
-            u32x4 bo[JT][3];
-            get_operand(b_block, bo);
-            tri_product(bo, d);
+            f32x4 d[CT][OT];
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) {
+                u32x4 bo[JT][3];
+                get_operand(b_block, ct, bo);
+                tri_product(bo, d[ct]);
+            }
             fetch_tri(ops[(size_t)c * p.n_v_heads].mf);
 #pragma unroll
-            for (int o = 0; o < OT; ++o) {
-                put_terms(f_block, tile_of(o), d[o] * sw[o]);
-                put_terms(d_block, tile_of(o), d[o]);
-            }
+            for (int ct = 0; ct < CT; ++ct)
+#pragma unroll
+                for (int o = 0; o < OT; ++o) {
+                    put_terms(f_block, ct, tile_of(o), d[ct][o] * sw[o]);
+                    put_terms(d_block, ct, tile_of(o), d[ct][o]);
+                }
         }
         __syncthreads();
         // the update, and the rows of o
-        u32x4 fo[JT][3];
-        get_operand(f_block, fo);
+        u32x4 fo[CT][JT][3];
+#pragma unroll
+        for (int ct = 0; ct < CT; ++ct) get_operand(f_block, ct, fo[ct]);
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
             u32x4 a[2][JT][NT];
@@ -811,28 +843,38 @@ __global__ __launch_bounds__(64 * KP, sizeof(SeqLds<T, DK, KP>) <= (80 << 10) ? 
                             reinterpret_cast<const u32x2 *>(&kl[q][m + 16][unit(m + 16, 4 * s + (li & 3))]) + h);
                         a[h][j][q] = (u32x4){lo.x, lo.y, hi.x, hi.y};
                     }
-            S[s][0] *= dn;
-            S[s][1] *= dn;
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) {
+                S[ct][s][0] *= dn;
+                S[ct][s][1] *= dn;
+            }
             for_terms<NT, 3>([&](int e, int f) __attribute__((always_inline)) {
 #pragma unroll
                 for (int j = 0; j < JT; ++j)
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) S[s][h] = mfma_bf16(a[h][j][e], fo[j][f], S[s][h]);
+                    for (int h = 0; h < 2; ++h)
+#pragma unroll
+                        for (int ct = 0; ct < CT; ++ct) S[ct][s][h] = mfma_bf16(a[h][j][e], fo[ct][j][f], S[ct][s][h]);
             });
         }
         dn = next_ops.dn.x;
         // (q's area, the shares' and b's until here, is free)
         put_rows();
         if (owns) {
-            f32x4 om[OT];
-            u32x4 bo[JT][3];
-            get_operand(d_block, bo);
-            tri_product(bo, om);
+            f32x4 om[CT][OT];
+#pragma unroll
+            for (int ct = 0; ct < CT; ++ct) {
+                u32x4 bo[JT][3];
+                get_operand(d_block, ct, bo);
+                tri_product(bo, om[ct]);
+            }
             fetch_tri(next_ops.tf);
             char *op = const_cast<char *>(rows_at(p.o, p.o_stride, sp.first + C * c, hv * (int)p.value_dim));
             auto put_o = [&](int o, int r) __attribute__((always_inline)) {
                 const int m = 16 * tile_of(o) + 4 * kk + r;
-                T::put(op + (__umul24(m, o_row) + col * kSize), 0, qs[o][r] + om[o][r]);
+#pragma unroll
+                for (int ct = 0; ct < CT; ++ct)
+                    T::put(op + (__umul24(m, o_row) + (col + 16 * ct) * kSize), 0, qs[o][ct][r] + om[ct][o][r]);
             };
             if (n == C) {
 #pragma unroll
@@ -855,7 +897,9 @@ __global__ __launch_bounds__(64 * KP, sizeof(SeqLds<T, DK, KP>) <= (80 << 10) ? 
             for (int a = 0; a < 2; ++a)
 #pragma unroll
                 for (int r = 0; r < 4; ++r)
-                    p.state_out[state_at + (size_t)(32 * s + 4 * a + r) * p.value_dim] = S[s][a][r];
+#pragma unroll
+                    for (int ct = 0; ct < CT; ++ct)
+                        p.state_out[state_at + (size_t)(32 * s + 4 * a + r) * p.value_dim + 16 * ct] = S[ct][s][a][r];
     }
 }
 
@@ -1022,10 +1066,10 @@ int launched(const char *who) {
     return 0;
 }
 
-template <class T, int DK, int KP>
+template <class T, int DK, int KP, int CT>
 void launch_seq(const GDNDelta &a, const int *order, const ChunkOps<kChunk<T>> *ops, const Planes<T, DK> *planes, hipStream_t s) {
-    const int pairs = (int)(a.n_seqs * a.n_v_heads), groups = (int)a.value_dim / 16;
-    hipLaunchKernelGGL((k_delta_seq<T, DK, KP>), dim3((unsigned)((pairs + 7) / 8 * 8 * groups)),
+    const int pairs = (int)(a.n_seqs * a.n_v_heads), groups = (int)a.value_dim / (16 * CT);
+    hipLaunchKernelGGL((k_delta_seq<T, DK, KP, CT>), dim3((unsigned)((pairs + 7) / 8 * 8 * groups)),
                        dim3(64 * KP), 0, s, a, order, ops, planes, pairs);
 }
 template <class T, int DK>
@@ -1037,7 +1081,18 @@ void launch_prefill(const GDNDelta &a, void *ws, hipStream_t s) {
     auto *planes = reinterpret_cast<Planes<T, DK> *>(mem + order_bytes(&a) + ops_bytes(&a));
     hipLaunchKernelGGL((k_delta_prep<T, DK>), dim3((unsigned)places(&a) + 1, a.n_v_heads), dim3(4 * C), 0, s, a, order,
                        ops, planes);
-    launch_seq<T, DK, KP>(a, order, ops, planes, s);
+    // 32 columns a workgroup where as many workgroups of them fit a CU and fill
+    // all.  1024 tokens a sequence, 8 heads, 16 against 32 columns: FP32, 128 x 128,
+    // 16 sequences 293 and 235 us, 8 (half the CUs' places) 125 and 131; FP32, 256 x
+    // 256, 4 sequences 218 and 178; FP16, 128 x 128, 16 sequences 208 and 181; BF16,
+    // 64 x 64, 64 sequences 332 and 278, 32 equal.  Where a CU holds one of them for
+    // two of the others: BF16, 256 x 256, 8 sequences 182 and 194.
+    constexpr int kPerCu = kSeqPerCu<T, DK, KP, 1>;
+    if constexpr (kSeqPerCu<T, DK, KP, 2> == kPerCu) {
+        if ((size_t)a.n_seqs * a.n_v_heads * (a.value_dim / 32) >= 256 * kPerCu)
+            return launch_seq<T, DK, KP, 2>(a, order, ops, planes, s);
+    }
+    launch_seq<T, DK, KP, 1>(a, order, ops, planes, s);
 }
 template <class T>
 void launch_prefill_dk(const GDNDelta &a, void *ws, hipStream_t s) {

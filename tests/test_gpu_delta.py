@@ -105,6 +105,25 @@ def test_prefill(dtype, dk, dv, hq, hv):
     check_packed([0, 1, 31, 32, 33, 63, 64, 65, 0, 130, 16, 17], hq, hv, dk, dv, dtype, True, shuffle=True, seed=dk + dv)
 
 
+@pytest.mark.parametrize("dtype,dk,dv,hq,hv,n", [(FP32, 128, 128, 8, 16, 8), (FP32, 256, 256, 4, 8, 6), (FP16, 128, 128, 16, 16, 9),
+                                                 (FP16, 64, 256, 4, 16, 5), (BF16, 64, 64, 4, 16, 17), (FP32, 64, 64, 2, 16, 16),
+                                                 (BF16, 256, 256, 2, 8, 9)])
+def test_prefill_of_batches_that_fill_the_gpu(dtype, dk, dv, hq, hv, n):
+    """A sequence's results are its own alone, bit for bit."""
+    lens = [0, 1, 33, 100, 64, 7, 32, 65][: n] + [5 + i for i in range(n - 8)]
+    q, k, v, gate, beta = inputs(sum(lens), hq, hv, dk, dv, dtype, n + dk)
+    cu = torch.tensor([0] + lens).cumsum(0).to(torch.int32).cuda()
+    out, pool = check_packed(lens, hq, hv, dk, dv, dtype, True, seed=n + dk)
+    gen = torch.Generator(device="cuda").manual_seed(n + dk + 1)
+    S0 = 0.3 * torch.randn((n, hv, dk, dv), generator=gen, device="cuda")
+    for i in range(0, n, 3):
+        s = slice(int(cu[i]), int(cu[i + 1]))
+        S = S0[i:i + 1].clone()
+        o = g.delta_prefill(q[s], k[s], v[s], gate[s], beta[s], torch.tensor([0, lens[i]], dtype=torch.int32).cuda(),
+                            state_in=S, state_out=S)
+        assert torch.equal(o, out[s]) and torch.equal(S[0], pool[i]), i
+
+
 @pytest.mark.parametrize("lens", [[1], [2], [15], [64], [128], [129], [1, 1, 1, 1, 1, 1, 1, 1, 1], [0], [0, 0, 7, 0]])
 def test_prefill_lengths_from_zero_state(lens):
     check_packed(lens, 1, 2, 256, 256, BF16, False, seed=len(lens) + sum(lens))
