@@ -374,7 +374,13 @@ class BatchState:
         if histories is not None:
             at = ragged(histories)
             put("history_offsets", at, np.int32, (n + 1,))
-            put("history", [t for x in histories for t in x], np.int32, (at[-1],))
+            try:
+                ids = np.concatenate([np.asarray(x, np.int64).reshape(-1) for x in histories])
+            except (ValueError, OverflowError, TypeError) as e:
+                raise GDNError(f"histories: expected token ids: {e}") from None
+            if ids.size and (ids.min() < -(1 << 31) or ids.max() >= 1 << 31):
+                raise GDNError("histories: a token id passes 32 bits")
+            put("history", ids, np.int32, (at[-1],))
         if biases is not None:
             at = ragged(biases)
             put("bias_offsets", at, np.int32, (n + 1,))

@@ -628,3 +628,33 @@ def test_process_refuses_fewer_masks_than_rows():
     for n in (0, 1):
         with pytest.raises(g.GDNError, match="masks for 2 rows"):
             g.logits_process(x, mask=torch.zeros((n, 2), dtype=torch.int32).cuda())
+
+
+def test_batch_sample_of_a_large_vocabulary():
+    """Rows of logits longer than LDS: a workspace behind the call's arrays."""
+    from gateddeltanet_amd.engine import default_config
+
+    cfg = default_config(1)
+    cfg.vocab_size = 40000
+    m = g.Model.synth(config=cfg, seed=4)
+    n = 3
+    bs = g.BatchState(m, n)
+    try:
+        greedy = bs.step([1, 2, 39999])
+        logits = np.stack([bs.logits(s) for s in range(n)])
+        for _ in range(2):
+            tok, lp = bs.sample()
+            np.testing.assert_array_equal(tok, greedy)
+            u, temp, k, p, mp = settings(n, 7)
+            mask = np.random.default_rng(5).random((n, 40000)) < 0.7
+            tok, lp = bs.sample(u, temperature=temp, top_k=k, top_p=p, min_p=mp, histories=[[39999] * 5, [], [7]],
+                                frequency=0.5, mask=mask)
+            for s in range(n):
+                hist = [[39999] * 5, [], [7]][s]
+                y, _ = process_ref(logits[s], np.array(hist, np.int64), len(hist), 0, np.float32(1), np.float32(0),
+                                   np.float32(0.5), {}, mask[s])
+                t, want = sample_ref(y.astype(np.float32), u[s], temp[s], k[s], p[s], mp[s])
+                assert tok[s] == t and abs(lp[s] - want) < 1e-5, (s, tok[s], t, lp[s], want)
+    finally:
+        bs.free()
+        m.free()
