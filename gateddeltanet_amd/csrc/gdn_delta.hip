@@ -1039,6 +1039,7 @@ int check(const char *who, const GDNDelta *a, bool packed) {
     if (a->n_slots > 0x7fffffffu) return refuse(who, "at most 2^31 - 1 slots");
     if (a->n_seqs == 0 || (!packed && a->n_tokens == 0)) return 1;
     if (!packed && a->n_tokens != a->n_seqs) return refuse(who, "a step has one token a sequence");
+    if (!a->slots && a->n_slots < a->n_seqs) return refuse(who, "n_slots is smaller than n_seqs, and there are no slots");
     if ((packed && !a->cu_seqlens) || (a->n_tokens != 0 && (!a->q || !a->k || !a->v || !a->o || !a->g || !a->beta)))
         return refuse(who, "a buffer pointer is NULL");
     const int64_t size = a->dtype == GDN_DTYPE_FP32 ? 4 : 2, per16 = 16 / size;

@@ -647,7 +647,8 @@ int gdn_test_prefill_gemm(int kind, const float *W, const float *X, uint32_t N, 
  *              multiples of 16 bytes; the same buffer, or two that do not
  *              overlap.  state_in NULL: every sequence starts from zero;
  *              state_out NULL: the states are not kept.
- *   slots      [n_seqs] the sequences' slots (NULL: slot i).  A sequence with
+ *   slots      [n_seqs] the sequences' slots (NULL: slot i, and n_slots is at
+ *              least n_seqs, without states too).  A sequence with
  *              a slot outside 0 .. n_slots - 1 is left out (a padded row):
  *              its o is left as it was.  No slot may occur twice.
  * Sums are FP32.  A squared norm or a state beyond FP32's range is not finite

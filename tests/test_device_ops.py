@@ -191,3 +191,15 @@ def test_delta_refuses_strides(change, capfd):
     assert "row stride" in capfd.readouterr().err
     assert lib.gdn_delta_step(ctypes.byref(delta(step=True, **change)), None) == -1
     assert "row stride" in capfd.readouterr().err
+
+
+def test_delta_refuses_too_few_slots(capfd):
+    """Without slots every sequence has the one of its number: none is left out
+    silently, with states or without."""
+    lib = _lib.load()
+    for change in (dict(n_slots=1), dict(n_slots=0, state_in=0, state_out=0)):
+        a = delta(slots=0, **change)
+        assert lib.gdn_delta_prefill(ctypes.byref(a), AT, 1 << 62, None) == -1
+        assert "n_slots" in capfd.readouterr().err
+        assert lib.gdn_delta_step(ctypes.byref(delta(step=True, slots=0, **change)), None) == -1
+        assert "n_slots" in capfd.readouterr().err
