@@ -11,6 +11,8 @@ here is recorded for gradients.
 from __future__ import annotations
 
 import ctypes
+import functools
+import struct
 from typing import Optional, Tuple
 
 import torch
@@ -39,8 +41,40 @@ def _on(dev: int, name: str, x, dtype, shape) -> int:
           f"{tuple(x.shape)} strides {x.stride()} on {x.device}")
 
 
-def _launch(dev: int, what: str, fn, *args) -> None:
-    """fn(*args, stream) with GPU dev as the current one."""
+# A call's struct as bytes: 0.7 us less than filling a ctypes object, and a value
+# that passes its field is an error.
+_CODES = {ctypes.c_int32: "i", ctypes.c_uint32: "I", ctypes.c_int64: "q", ctypes.c_float: "f", ctypes.c_void_p: "P"}
+
+
+def _packer(cls):
+    code = struct.Struct("@" + "".join(_CODES[t] for _, t in cls._fields_))
+    if code.size != ctypes.sizeof(cls):
+        raise TypeError(f"{cls.__name__}: {code.size} bytes packed, {ctypes.sizeof(cls)} wanted")
+
+    def pack(*values) -> bytes:
+        try:
+            return code.pack(*values)
+        except (struct.error, OverflowError) as e:
+            raise GDNError(f"{cls.__name__}: {e}") from None
+
+    return pack
+
+
+_pack_delta, _pack_logits, _pack_sample = _packer(L.GDNDelta), _packer(L.GDNLogits), _packer(L.GDNSample)
+
+
+@functools.lru_cache(maxsize=None)
+def _entry(name: str):
+    """The library's entry point, its struct taken as bytes."""
+    fn = L.load()[name]  # (an object apart from the attribute's)
+    fn.restype, args = L.SIGNATURES[name]
+    fn.argtypes = [ctypes.c_char_p, *args[1:]]
+    return fn
+
+
+def _launch(dev: int, what: str, *args) -> None:
+    """The entry point `what` (*args, stream) with GPU dev as the current one."""
+    fn = _entry(what)
     if torch.cuda.current_device() == dev:
         rc = fn(*args, _raw_stream(dev))
     else:
@@ -79,7 +113,7 @@ def _delta(q, k, v, g, beta, out, state_in, state_out, slots, n_seqs, cu, scale,
     at_out = at_in if state_out is state_in else _on(dev, "state_out", state_out, _F32, states)
     if slots is None and n_slots < n_seqs:
         _fail(f"{n_seqs} sequences without slots need as many states, got {n_slots}")
-    return dev, L.GDNDelta(
+    return dev, _pack_delta(
         dtype, n, n_seqs, hq, hv, dk, dv, 1 if l2norm else 0, dk**-0.5 if scale is None else scale, n_slots, sq[0],
         sk[0], sv[0], so[0], sg[0], q.data_ptr(), k.data_ptr(), v.data_ptr(), out.data_ptr(), g.data_ptr(),
         beta.data_ptr(), _on(dev, "cu_seqlens", cu, _I32, (n_seqs + 1,)), _on(dev, "slots", slots, _I32, (n_seqs,)),
@@ -110,11 +144,10 @@ def delta_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Te
     if n_seqs < 0:
         _fail("cu_seqlens: expected int32 [sequences + 1]")
     dev, args = _delta(q, k, v, g, beta, out, state_in, state_out, slots, n_seqs, cu_seqlens, scale, l2norm)
-    lib, ref = L.load(), ctypes.byref(args)
     if workspace is None:
-        workspace = torch.empty(lib.gdn_delta_prefill_workspace(ref), dtype=torch.uint8, device=q.device)
+        workspace = torch.empty(_entry("gdn_delta_prefill_workspace")(args), dtype=torch.uint8, device=q.device)
     size = workspace.numel()
-    _launch(dev, "gdn_delta_prefill", lib.gdn_delta_prefill, ref,
+    _launch(dev, "gdn_delta_prefill", args,
             _on(dev, "workspace", workspace, torch.uint8, (size,)), size)
     return out
 
@@ -130,7 +163,7 @@ def delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tenso
         out = torch.empty_like(v, memory_format=torch.contiguous_format)
     dev, args = _delta(q, k, v, g, beta, out, state, state if state_out is None else state_out, slots, q.shape[0], None,
                        scale, l2norm)
-    _launch(dev, "gdn_delta_step", L.load().gdn_delta_step, ctypes.byref(args))
+    _launch(dev, "gdn_delta_step", args)
     return out
 
 
@@ -205,9 +238,9 @@ def logits_process(logits: torch.Tensor, *, history: Optional[torch.Tensor] = No
             _fail(f"mask: {n_masks} masks for {rows} rows, and no mask_index")
     elif mask_index is not None:
         _fail("mask_index needs a mask")
-    a = L.GDNLogits(dtype, rows, vocab, width, n_bias, n_masks, stride, into, h_stride, m_stride, logits.data_ptr(),
-                    out.data_ptr(), hist, length, prompt, rep, pres, freq, b_at, b_ids, b_values, m_at, m_index)
-    _launch(dev, "gdn_logits_process", L.load().gdn_logits_process, ctypes.byref(a))
+    a = _pack_logits(dtype, rows, vocab, width, n_bias, n_masks, stride, into, h_stride, m_stride, logits.data_ptr(),
+                     out.data_ptr(), hist, length, prompt, rep, pres, freq, b_at, b_ids, b_values, m_at, m_index)
+    _launch(dev, "gdn_logits_process", a)
     return out
 
 
@@ -229,12 +262,11 @@ def sample_tokens(logits: torch.Tensor, uniform: Optional[torch.Tensor] = None, 
         tokens = torch.empty(one, dtype=_I32, device=logits.device)
     if logprobs is None:
         logprobs = torch.empty(one, dtype=_F32, device=logits.device)
-    a = L.GDNSample(dtype, rows, vocab, 0, stride, logits.data_ptr(), _on(dev, "uniform", uniform, _F32, one),
-                    _on(dev, "temperature", temperature, _F32, one), _on(dev, "top_k", top_k, _I32, one),
-                    _on(dev, "top_p", top_p, _F32, one), _on(dev, "min_p", min_p, _F32, one),
-                    _on(dev, "tokens", tokens, _I32, one), _on(dev, "logprobs", logprobs, _F32, one))
-    lib, ref = L.load(), ctypes.byref(a)
-    size = lib.gdn_sample_workspace(ref)
+    a = _pack_sample(dtype, rows, vocab, 0, stride, logits.data_ptr(), _on(dev, "uniform", uniform, _F32, one),
+                     _on(dev, "temperature", temperature, _F32, one), _on(dev, "top_k", top_k, _I32, one),
+                     _on(dev, "top_p", top_p, _F32, one), _on(dev, "min_p", min_p, _F32, one),
+                     _on(dev, "tokens", tokens, _I32, one), _on(dev, "logprobs", logprobs, _F32, one))
+    size = _entry("gdn_sample_workspace")(a)
     ws = torch.empty(size, dtype=torch.uint8, device=logits.device) if size else None
-    _launch(dev, "gdn_sample_tokens", lib.gdn_sample_tokens, ref, ws.data_ptr() if size else 0, size)
+    _launch(dev, "gdn_sample_tokens", a, ws.data_ptr() if size else 0, size)
     return tokens, logprobs
