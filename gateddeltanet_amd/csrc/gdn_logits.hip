@@ -701,7 +701,8 @@ __device__ __forceinline__ int drawn(const Row<T, HELD> &r, SampleLds<T, HELD> &
     uint64_t mine = 0, all;
     for (int i = 0; i < per; ++i) mine += t * per + i < cells ? lds.cell[t * per + i] : 0;
     uint64_t at = block_scan(mine, lds.wsum[0], all);
-    uint64_t goal = u > 0.0 ? (uint64_t)__builtin_fmin(u * (double)all, 9.2e18) : 0;
+    // (u is bounded, not the product: `all` may be 2^63)
+    uint64_t goal = u > 0.0 ? (uint64_t)(__builtin_fmin(u, 1.0) * (double)all) : 0;
     goal = goal < all ? goal : all - 1;
     if (at <= goal && at + mine > goal) {
         int c = t * per;
@@ -1258,7 +1259,7 @@ bool held(const GDNSample &a) {
 }
 template <class T>
 void launch_sample(const GDNSample &a, void *ws, hipStream_t s) {
-    // 2^shift times the vocabulary stays below 2^63
+    // 2^shift times the vocabulary is at most 2^63
     const int shift = a.vocab <= (1u << 18) ? 45 : 43;
     const dim3 rows(a.rows), block(kST);
     if (held<T>(a)) {

@@ -733,7 +733,7 @@ int gdn_logits_process(const GDNLogits *args, void *stream);
  * is, at temperature 1 with no token left out.
  * NaN logits are never chosen and carry no weight; a row without a logit above
  * -infinity gives token -1 and log-probability -infinity.  Weights are held in
- * 64-bit fixed point, 45 bits behind the point (fewer from 2^18 tokens on), so
+ * 64-bit fixed point, 45 bits behind the point (43 above 2^18 tokens), so
  * their sums do not depend on an order.  vocab is at most 2^20, rows 65535.
  * `workspace`: gdn_sample_workspace(args) bytes at a multiple of 16 bytes (0 for
  * rows of up to 128 KiB), needed until the work is done. */

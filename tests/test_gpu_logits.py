@@ -658,3 +658,22 @@ def test_batch_sample_of_a_large_vocabulary():
     finally:
         bs.free()
         m.free()
+
+
+@pytest.mark.parametrize("kind", list(TYPES))
+@pytest.mark.parametrize("vocab", [32768, 261999, 2**18, 2**18 + 1, 2**20 - 1, 2**20])
+def test_sample_of_a_flat_row_reaches_every_token(kind, vocab):
+    """Equal weights, of equal logits or of an infinite temperature: their sum
+    is the largest there is, 2^63 at 2^18 and at 2^20 tokens."""
+    us = [0.0, 0.5, 0.998, 0.999, float(np.float32(1 - 2.0**-24))]
+    n = len(us)
+    flat = torch.full((n, vocab), 0.75, dtype=TYPES[kind], device="cuda")
+    spread = row_logits(n, vocab, TYPES[kind], vocab)
+    want = [int(np.float64(np.float32(u)) * vocab) for u in us]
+    assert want[-1] == vocab - 1
+    assert check_sample(flat, us, [1.0] * n).tolist() == want
+    assert check_sample(spread, us, [math.inf] * n).tolist() == want
+    # a border among equals: the tokens before ceil(p vocab)
+    kept = math.ceil(np.float64(np.float32(0.999)) * vocab)
+    want = [int(np.float64(np.float32(u)) * kept) for u in us]
+    assert check_sample(flat, us, [1.0] * n, p=[0.999] * n).tolist() == want
