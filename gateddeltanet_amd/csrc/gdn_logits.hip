@@ -824,9 +824,14 @@ __global__ __launch_bounds__(kST) void k_sample(GDNSample p, int shift) {
     }
 
     // the sum of exponentials; where top-p stands alone also an estimate of the
-    // weights above the bound and of all, in FP32: each to 2e-6 (46 2^-24 for the
-    // argument, 2^-23 for the exponential), a thread's sum of 64 at most to 4e-6
-    constexpr double kOff = 1e-5;
+    // weights above the bound and of all, in FP32.  A weight's argument, at most
+    // 46.2 powers of two, is rounded three times (difference, rate, product), the
+    // exponential to 2^-23 of it, then each of a thread's additions; smaller
+    // weights are below 2^-30 of the whole together.  kOff is twice the sum of
+    // these (9.7e-6 for 64 tokens a thread)
+    constexpr int kTokens = SampleLds<T, true>::kHeld / kST;  // a thread's
+    constexpr double kRoundings = 3 * 46.2 * 0.69315 * 0x1p-24 + 0x1p-23 + kTokens * 0x1p-24, kOff = 2e-5;
+    static_assert(kOff >= 1.5 * kRoundings, "the border's uncertainty");
     double sum = 0.0;
     const bool alone = ask.by_p && !ask.by_k;
     if (alone) {

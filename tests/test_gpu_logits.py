@@ -677,3 +677,35 @@ def test_sample_of_a_flat_row_reaches_every_token(kind, vocab):
     kept = math.ceil(np.float64(np.float32(0.999)) * vocab)
     want = [int(np.float64(np.float32(u)) * kept) for u in us]
     assert check_sample(flat, us, [1.0] * n, p=[0.999] * n).tolist() == want
+
+
+@pytest.mark.parametrize("kind,vocab", [("fp32", 1000), ("fp32", 32768), ("bf16", 65536), ("fp16", 65536), ("fp32", 40000)])
+@pytest.mark.parametrize("temperature", [0.4, 1.0])
+def test_sample_top_p_next_to_a_border(kind, vocab, temperature):
+    """The FP32 numbers just below and above the share of the tokens before
+    one, and others up to 3e-5 away: with the last token of the ranking at the
+    end of the row, a number near 1 draws it exactly if it is kept."""
+    ranks = [1, 2, 5, 13, 40, 100]
+    off = [0.0, 3e-7, 1e-6, 3e-6, 8e-6, 1.2e-5, 3e-5]
+    base = row_logits(len(ranks), vocab, TYPES[kind], vocab + 1, spread=2.0)
+    xs, ps, keeps = [], [], []
+    for x, j in zip(base, ranks):
+        d = x.double().cpu().numpy()
+        order = np.argsort(-d, kind="stable")
+        # the border's token has no equal
+        j = next((i for i in range(j, 0, -1) if d[order[i - 1]] > d[order[i]] > d[order[i + 1]]), None)
+        if j is None:
+            continue
+        w = np.exp((d - d.max()) / np.float64(np.float32(temperature)))
+        share = w[order[:j]].sum() / w.sum()
+        x[[int(order[j]), vocab - 1]] = x[[vocab - 1, int(order[j])]]
+        for e in off:
+            below = np.nextafter(np.float32(share * (1 - e)), np.float32(0))
+            above = np.nextafter(np.float32(share * (1 + e)), np.float32(1))
+            for p, kept in ((below, False), (above, True)):
+                assert abs(float(p) - share) > 1e-9 * share and (float(p) > share) == kept
+                xs.append(x), ps.append(float(p)), keeps.append(kept)
+    n = len(xs)
+    assert n >= 2 * 3 * len(off)
+    tok = check_sample(torch.stack(xs), [1 - 2.0**-24] * n, [temperature] * n, p=ps)
+    assert [t == vocab - 1 for t in tok.tolist()] == keeps
