@@ -99,7 +99,10 @@ def _delta(q, k, v, g, beta, out, state_in, state_out, slots, n_seqs, cu, scale,
         _fail(f"shapes do not agree: q {tuple(qs)}, k {tuple(k.shape)}, v {tuple(vs)}, out {tuple(out.shape)}")
     sq, sk, sv, so = q.stride(), k.stride(), v.stride(), out.stride()
     heads, values = (dk, 1), (dv, 1)
-    if n and (sq[1:] != heads or sk[1:] != heads or sv[1:] != values or so[1:] != values):
+    if n and (sq[1:] != heads or sk[1:] != heads or sv[1:] != values or so[1:] != values) and not (
+            # (a single head's stride is not used)
+            sq[2] == sk[2] == sv[2] == so[2] == 1 and (hq == 1 or sq[1] == sk[1] == dk) and (
+                hv == 1 or sv[1] == so[1] == dv)):
         _fail(f"heads must be contiguous in a row: strides q {sq}, k {sk}, v {sv}, out {so}")
     gates, sg, sb = (n, hv), g.stride(), beta.stride()
     if g.shape != gates or beta.shape != gates or g.dtype is not _F32 or beta.dtype is not _F32 or (

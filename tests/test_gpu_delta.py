@@ -450,3 +450,35 @@ def test_one_row_of_any_stride():
     assert torch.equal(g.delta_step(*odd, beta, S), g.delta_step(q, k, v, gate, beta, T)) and torch.equal(S, T)
     assert torch.equal(g.delta_prefill(*odd, beta, cu, state_out=S), g.delta_prefill(q, k, v, gate, beta, cu, state_out=T))
     assert torch.equal(S, T)
+
+
+@pytest.mark.parametrize("hv", [1, 3])
+def test_single_heads_of_transposed_views(hv):
+    """Heads in front, as [heads][tokens][dim] holds them: a single head's rows
+    are rows all the same, several heads' are not."""
+    n, dk, dv = 40, 64, 128
+    q, k, v, gate, beta = inputs(n, 1, hv, dk, dv, BF16, 61)
+    cu = torch.tensor([0, 7, n], dtype=torch.int32).cuda()
+
+    def heads_first(x):
+        return torch.empty((x.shape[1], n, x.shape[2]), dtype=BF16, device="cuda").copy_(x.transpose(0, 1)).transpose(0, 1)
+
+    fq, fk, fv = heads_first(q), heads_first(k), heads_first(v)
+    assert fq.stride(1) == n * dk
+    out = torch.empty_like(v)
+    S, T = (torch.ones((n, hv, dk, dv), device="cuda") for _ in range(2))
+    for f, a, b in ((g.delta_prefill, (cu,), (cu,)), (g.delta_step, (S,), (T,))):
+        want = f(q, k, v, gate, beta, *a)
+        assert torch.equal(f(fq, fk, v, gate, beta, *b), want)
+        if hv == 1:
+            into = torch.empty((1, n, dv), dtype=BF16, device="cuda").transpose(0, 1)
+            if f is g.delta_step:
+                T.fill_(1.0)
+            assert f(fq, fk, fv, gate, beta, *b, out=into) is into and torch.equal(into, want)
+            values = fv.repeat_interleave(2, 2)[..., ::2]  # values apart from each other
+        else:
+            values = fv
+        for kw in (dict(v=values), dict(out=values)):
+            with pytest.raises(g.GDNError, match="contiguous in a row"):
+                f(q, k, kw.get("v", v), gate, beta, *b, out=kw.get("out", out))
+    assert torch.equal(S, T)
