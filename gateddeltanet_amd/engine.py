@@ -356,8 +356,13 @@ class BatchState:
         def put(name, value, dtype, shape=(n,)):
             if value is not None:
                 try:
-                    keep.append(np.ascontiguousarray(np.broadcast_to(np.asarray(value, dtype), shape)))
-                except (ValueError, OverflowError) as e:
+                    given = np.asarray(value)
+                    with np.errstate(invalid="ignore"):
+                        x = given.astype(dtype)
+                    if dtype is np.int32 and (x != given).any():
+                        raise ValueError("not a whole number, or one past 32 bits")
+                    keep.append(np.ascontiguousarray(np.broadcast_to(x, shape)))
+                except (ValueError, OverflowError, TypeError) as e:
                     raise GDNError(f"{name}: expected {np.dtype(dtype).name} {shape}: {e}") from None
                 setattr(a, name, keep[-1].ctypes.data)
 
@@ -374,12 +379,7 @@ class BatchState:
         if histories is not None:
             at = ragged(histories)
             put("history_offsets", at, np.int32, (n + 1,))
-            try:
-                ids = np.concatenate([np.asarray(x, np.int64).reshape(-1) for x in histories])
-            except (ValueError, OverflowError, TypeError) as e:
-                raise GDNError(f"histories: expected token ids: {e}") from None
-            if ids.size and (ids.min() < -(1 << 31) or ids.max() >= 1 << 31):
-                raise GDNError("histories: a token id passes 32 bits")
+            ids = np.concatenate([np.asarray(x).reshape(-1) for x in histories])
             put("history", ids, np.int32, (at[-1],))
         if biases is not None:
             at = ragged(biases)

@@ -203,3 +203,33 @@ def test_delta_refuses_too_few_slots(capfd):
         assert "n_slots" in capfd.readouterr().err
         assert lib.gdn_delta_step(ctypes.byref(delta(step=True, slots=0, **change)), None) == -1
         assert "n_slots" in capfd.readouterr().err
+
+
+def test_batch_sample_refuses_integers_that_do_not_fit():
+    """A setting is taken as it is given or not at all: none wraps past 32 bits
+    or loses its fraction on the way to the engine."""
+    import types
+
+    import numpy as np
+
+    state = object.__new__(g.BatchState)
+    state.n_streams, state._live, state._s = 2, False, _lib.GDNBatchState()
+    state.model = types.SimpleNamespace(config=types.SimpleNamespace(vocab_size=100))
+    none = [{}, {}]
+    for name, kw in [("top_k", dict(top_k=np.array([2**32 + 1, 1]))), ("top_k", dict(top_k=[50.7, 1])),
+                     ("top_k", dict(top_k=1e10)), ("top_k", dict(top_k=float("nan"))), ("top_k", dict(top_k=2**70)),
+                     ("top_k", dict(top_k=["many", 1])), ("top_k", dict(top_k=[None, 1])),
+                     ("top_k", dict(top_k=np.array([2**63, 1], np.uint64))),
+                     ("prompt_len", dict(histories=[[1], [2]], prompt_len=np.array([1, 2**40]))),
+                     ("prompt_len", dict(histories=[[1], [2]], prompt_len=0.5)),
+                     ("history", dict(histories=[[5.5], [1]])), ("history", dict(histories=[[1], np.array([2**31])])),
+                     ("history", dict(histories=[[-2**31 - 1], []])), ("history", dict(histories=[[None], []])),
+                     ("bias_ids", dict(biases=[{np.int64(2**32 + 5): 1.0}, {}])),
+                     ("bias_ids", dict(biases=[{5.5: 1.0}, {}])), ("bias_values", dict(biases=[{5: "much"}, {}]))]:
+        with pytest.raises(g.GDNError, match=f"^{name}: expected"):
+            state.sample(**kw)
+    # what fits comes as far as the engine, which is missing here
+    for kw in (dict(top_k=[50.0, np.int64(2)]), dict(top_k=-1), dict(histories=[[], []], prompt_len=[0, 1]), dict(biases=none),
+               dict(histories=[np.array([2**31 - 1]), [-2**31]], biases=[{np.int64(5): 1}, {}])):
+        with pytest.raises(g.GDNError, match="^gdn_batch_sample failed"):
+            state.sample(**kw)
