@@ -1058,30 +1058,23 @@ int check(const char *who, const GDNDelta *a, bool packed) {
     return 0;
 }
 
-int launched(const char *who) {
-    const hipError_t rc = hipGetLastError();
-    if (rc != hipSuccess) {
-        std::fprintf(stderr, "%s: launch failed: %s\n", who, hipGetErrorString(rc));
-        return -1;
-    }
-    return 0;
-}
-
 template <class T, int DK, int KP, int CT>
-void launch_seq(const GDNDelta &a, const int *order, const ChunkOps<kChunk<T>> *ops, const Planes<T, DK> *planes, hipStream_t s) {
+hipError_t launch_seq(const GDNDelta &a, const int *order, const ChunkOps<kChunk<T>> *ops, const Planes<T, DK> *planes,
+                      hipStream_t s) {
     const int pairs = (int)(a.n_seqs * a.n_v_heads), groups = (int)a.value_dim / (16 * CT);
-    hipLaunchKernelGGL((k_delta_seq<T, DK, KP, CT>), dim3((unsigned)((pairs + 7) / 8 * 8 * groups)),
-                       dim3(64 * KP), 0, s, a, order, ops, planes, pairs);
+    return launch(k_delta_seq<T, DK, KP, CT>, dim3((unsigned)((pairs + 7) / 8 * 8 * groups)), dim3(64 * KP), 0, s, a, order,
+                  ops, planes, pairs);
 }
 template <class T, int DK>
-void launch_prefill(const GDNDelta &a, void *ws, hipStream_t s) {
+hipError_t launch_prefill(const GDNDelta &a, void *ws, hipStream_t s) {
     constexpr int C = kChunk<T>, KP = DK == 64 ? 2 : 4;
     char *mem = static_cast<char *>(ws);
     int *order = reinterpret_cast<int *>(mem);
     auto *ops = reinterpret_cast<ChunkOps<C> *>(mem + order_bytes(&a));
     auto *planes = reinterpret_cast<Planes<T, DK> *>(mem + order_bytes(&a) + ops_bytes(&a));
-    hipLaunchKernelGGL((k_delta_prep<T, DK>), dim3((unsigned)places(&a) + 1, a.n_v_heads), dim3(4 * C), 0, s, a, order,
-                       ops, planes);
+    const hipError_t rc = launch(k_delta_prep<T, DK>, dim3((unsigned)places(&a) + 1, a.n_v_heads), dim3(4 * C), 0, s, a,
+                                 order, ops, planes);
+    if (rc != hipSuccess) return rc;
     // 32 columns a workgroup where as many workgroups of them fit a CU and fill
     // all.  1024 tokens a sequence, 8 heads, 16 against 32 columns: FP32, 128 x 128,
     // 16 sequences 293 and 235 us, 8 (half the CUs' places) 125 and 131; FP32, 256 x
@@ -1093,24 +1086,22 @@ void launch_prefill(const GDNDelta &a, void *ws, hipStream_t s) {
         if ((size_t)a.n_seqs * a.n_v_heads * (a.value_dim / 32) >= 256 * kPerCu)
             return launch_seq<T, DK, KP, 2>(a, order, ops, planes, s);
     }
-    launch_seq<T, DK, KP, 1>(a, order, ops, planes, s);
+    return launch_seq<T, DK, KP, 1>(a, order, ops, planes, s);
 }
 template <class T>
-void launch_prefill_dk(const GDNDelta &a, void *ws, hipStream_t s) {
-    if (a.key_dim == 256) launch_prefill<T, 256>(a, ws, s);
-    else if (a.key_dim == 128) launch_prefill<T, 128>(a, ws, s);
-    else launch_prefill<T, 64>(a, ws, s);
+hipError_t launch_prefill_dk(const GDNDelta &a, void *ws, hipStream_t s) {
+    return a.key_dim == 256   ? launch_prefill<T, 256>(a, ws, s)
+           : a.key_dim == 128 ? launch_prefill<T, 128>(a, ws, s)
+                              : launch_prefill<T, 64>(a, ws, s);
 }
 
 template <class T, int DK>
-void launch_step(const GDNDelta &a, hipStream_t s) {
-    hipLaunchKernelGGL((k_delta_step<T, DK>), dim3(a.value_dim / kStepCols, a.n_v_heads, a.n_seqs), dim3(kT), 0, s, a);
+hipError_t launch_step(const GDNDelta &a, hipStream_t s) {
+    return launch(k_delta_step<T, DK>, dim3(a.value_dim / kStepCols, a.n_v_heads, a.n_seqs), dim3(kT), 0, s, a);
 }
 template <class T>
-void launch_step_dk(const GDNDelta &a, hipStream_t s) {
-    if (a.key_dim == 256) launch_step<T, 256>(a, s);
-    else if (a.key_dim == 128) launch_step<T, 128>(a, s);
-    else launch_step<T, 64>(a, s);
+hipError_t launch_step_dk(const GDNDelta &a, hipStream_t s) {
+    return a.key_dim == 256 ? launch_step<T, 256>(a, s) : a.key_dim == 128 ? launch_step<T, 128>(a, s) : launch_step<T, 64>(a, s);
 }
 
 }  // namespace delta
@@ -1135,10 +1126,9 @@ extern "C" int gdn_delta_prefill(const GDNDelta *args, void *workspace, size_t w
         workspace_bytes < gdn_delta_prefill_workspace(args))
         return refuse(who, "the workspace is missing, misaligned or too small");
     hipStream_t s = static_cast<hipStream_t>(stream);
-    if (args->dtype == GDN_DTYPE_BF16) launch_prefill_dk<Bf16>(*args, workspace, s);
-    else if (args->dtype == GDN_DTYPE_FP16) launch_prefill_dk<Fp16>(*args, workspace, s);
-    else launch_prefill_dk<Fp32>(*args, workspace, s);
-    return launched(who);
+    return gdn::launched(who, args->dtype == GDN_DTYPE_BF16   ? launch_prefill_dk<Bf16>(*args, workspace, s)
+                              : args->dtype == GDN_DTYPE_FP16 ? launch_prefill_dk<Fp16>(*args, workspace, s)
+                                                              : launch_prefill_dk<Fp32>(*args, workspace, s));
 }
 
 extern "C" int gdn_delta_step(const GDNDelta *args, void *stream) {
@@ -1147,8 +1137,7 @@ extern "C" int gdn_delta_step(const GDNDelta *args, void *stream) {
     const int rc = check(who, args, false);
     if (rc != 0) return rc < 0 ? -1 : 0;
     hipStream_t s = static_cast<hipStream_t>(stream);
-    if (args->dtype == GDN_DTYPE_BF16) launch_step_dk<Bf16>(*args, s);
-    else if (args->dtype == GDN_DTYPE_FP16) launch_step_dk<Fp16>(*args, s);
-    else launch_step_dk<Fp32>(*args, s);
-    return launched(who);
+    return gdn::launched(who, args->dtype == GDN_DTYPE_BF16   ? launch_step_dk<Bf16>(*args, s)
+                              : args->dtype == GDN_DTYPE_FP16 ? launch_step_dk<Fp16>(*args, s)
+                                                              : launch_step_dk<Fp32>(*args, s));
 }

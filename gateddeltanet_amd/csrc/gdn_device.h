@@ -8,6 +8,7 @@
 
 #include <cstdint>
 #include <cstdio>
+#include <type_traits>
 
 #include "gdn_amd.h"
 #include "gdn_libm.h"
@@ -24,6 +25,22 @@
     } while (0)
 
 namespace gdn {
+
+// Host side: the kernel on a stream, and its own error.  (hipGetLastError would
+// report an earlier call's as well, after the launch.)  None is left behind.
+template <class... P, class... A>
+hipError_t launch(void (*kernel)(P...), dim3 grid, dim3 block, size_t lds, hipStream_t stream, const A &...args) {
+    static_assert((std::is_same_v<P, A> && ...), "arguments of the kernel's own types");
+    void *at[] = {const_cast<void *>(static_cast<const void *>(&args))...};
+    const hipError_t rc = hipLaunchKernel(reinterpret_cast<const void *>(kernel), grid, block, at, lds, stream);
+    if (rc != hipSuccess) (void)hipGetLastError();
+    return rc;
+}
+inline int launched(const char *who, hipError_t rc) {
+    if (rc == hipSuccess) return 0;
+    std::fprintf(stderr, "%s: launch failed: %s\n", who, hipGetErrorString(rc));
+    return -1;
+}
 
 constexpr int kH = 2048;   // hidden
 constexpr int kNH = 8;     // heads

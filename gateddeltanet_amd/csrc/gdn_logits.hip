@@ -1212,14 +1212,6 @@ int refuse(const char *who, const char *why) {
     std::fprintf(stderr, "%s: %s\n", who, why);
     return -1;
 }
-int launched(const char *who) {
-    const hipError_t rc = hipGetLastError();
-    if (rc != hipSuccess) {
-        std::fprintf(stderr, "%s: launch failed: %s\n", who, hipGetErrorString(rc));
-        return -1;
-    }
-    return 0;
-}
 bool misaligned(const void *p, int32_t dtype) {
     return (reinterpret_cast<uintptr_t>(p) & (dtype == GDN_DTYPE_FP32 ? 3 : 1)) != 0;
 }
@@ -1250,10 +1242,8 @@ extern "C" int gdn_logits_process(const GDNLogits *args, void *stream) {
     const dim3 grid((a.vocab + kTile - 1) / kTile, a.rows);
     const size_t lds = sizeof(uint32_t) * kTile * ((a.history != nullptr) + (a.bias_offsets != nullptr));
     hipStream_t s = static_cast<hipStream_t>(stream);
-    if (a.dtype == GDN_DTYPE_BF16) hipLaunchKernelGGL(k_process<Bf16>, grid, dim3(kPT), lds, s, a);
-    else if (a.dtype == GDN_DTYPE_FP16) hipLaunchKernelGGL(k_process<Fp16>, grid, dim3(kPT), lds, s, a);
-    else hipLaunchKernelGGL(k_process<Fp32>, grid, dim3(kPT), lds, s, a);
-    return launched(who);
+    const auto kernel = a.dtype == GDN_DTYPE_BF16 ? k_process<Bf16> : a.dtype == GDN_DTYPE_FP16 ? k_process<Fp16> : k_process<Fp32>;
+    return gdn::launched(who, gdn::launch(kernel, grid, dim3(kPT), lds, s, a));
 }
 
 namespace gdn {
@@ -1263,23 +1253,21 @@ bool held(const GDNSample &a) {
     return a.vocab <= (uint32_t)SampleLds<T, true>::kHeld;
 }
 template <class T>
-void launch_sample(const GDNSample &a, void *ws, hipStream_t s) {
+hipError_t launch_sample(const GDNSample &a, void *ws, hipStream_t s) {
     // 2^shift times the vocabulary is at most 2^63
     const int shift = a.vocab <= (1u << 18) ? 45 : 43;
     const dim3 rows(a.rows), block(kST);
-    if (held<T>(a)) {
-        hipLaunchKernelGGL(k_sample<T>, rows, block, 0, s, a, shift);
-        return;
-    }
+    if (held<T>(a)) return launch(k_sample<T>, rows, block, 0, s, a, shift);
     // slices for two workgroups a CU (131072 tokens, against one and four: 32 rows
     // 47.6, 47.4 and 54.9 us, 128 rows 87.6, 90.6 and 90.0)
     const int slices = a.rows >= 512 ? 1 : a.rows * kSlices <= 512 ? kSlices : 512 / (int)a.rows;
     const dim3 parts(slices, a.rows);
-    hipLaunchKernelGGL(k_wide_top<T>, parts, block, 0, s, a, ws);
-    hipLaunchKernelGGL(k_wide_steps<T>, parts, block, 0, s, a, shift, ws);
-    hipLaunchKernelGGL(k_wide_border<T>, rows, block, 0, s, a, shift, ws, slices);
-    hipLaunchKernelGGL(k_wide_pieces<T>, parts, block, 0, s, a, shift, ws);
-    hipLaunchKernelGGL(k_wide_draw<T>, rows, block, 0, s, a, shift, ws, slices);
+    hipError_t rc = launch(k_wide_top<T>, parts, block, 0, s, a, ws);
+    if (rc == hipSuccess) rc = launch(k_wide_steps<T>, parts, block, 0, s, a, shift, ws);
+    if (rc == hipSuccess) rc = launch(k_wide_border<T>, rows, block, 0, s, a, shift, ws, slices);
+    if (rc == hipSuccess) rc = launch(k_wide_pieces<T>, parts, block, 0, s, a, shift, ws);
+    if (rc == hipSuccess) rc = launch(k_wide_draw<T>, rows, block, 0, s, a, shift, ws, slices);
+    return rc;
 }
 }  // namespace lg
 }  // namespace gdn
@@ -1311,8 +1299,7 @@ extern "C" int gdn_sample_tokens(const GDNSample *args, void *workspace, size_t 
     if (need != 0 && (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0 || workspace_bytes < need))
         return refuse(who, "the workspace is missing, misaligned or too small");
     hipStream_t s = static_cast<hipStream_t>(stream);
-    if (a.dtype == GDN_DTYPE_BF16) launch_sample<Bf16>(a, workspace, s);
-    else if (a.dtype == GDN_DTYPE_FP16) launch_sample<Fp16>(a, workspace, s);
-    else launch_sample<Fp32>(a, workspace, s);
-    return launched(who);
+    return gdn::launched(who, a.dtype == GDN_DTYPE_BF16   ? launch_sample<Bf16>(a, workspace, s)
+                              : a.dtype == GDN_DTYPE_FP16 ? launch_sample<Fp16>(a, workspace, s)
+                                                          : launch_sample<Fp32>(a, workspace, s));
 }

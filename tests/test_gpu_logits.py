@@ -709,3 +709,34 @@ def test_sample_top_p_next_to_a_border(kind, vocab, temperature):
     assert n >= 2 * 3 * len(off)
     tok = check_sample(torch.stack(xs), [1 - 2.0**-24] * n, [temperature] * n, p=ps)
     assert [t == vocab - 1 for t in tok.tolist()] == keeps
+
+
+@pytest.mark.parametrize("op", ["delta_prefill", "delta_step", "logits_process", "sample_tokens"])
+def test_an_error_of_an_earlier_call_is_not_reported_as_a_launchs(op):
+    """A HIP call of the program's own that failed (no device of that number)
+    and was not asked about: the operators run, and leave its error to it."""
+    from test_gpu_delta import inputs
+
+    from gateddeltanet_amd import _lib
+
+    hip = _lib.load()  # (resolves the runtime's symbols too)
+    q = inputs(4, 1, 1, 64, 64, torch.float32, 3)
+    S, out = torch.zeros((4, 1, 64, 64), device="cuda"), torch.empty((4, 1, 64), device="cuda")
+    x = row_logits(4, 1000, torch.float32, 3)
+    cu = torch.tensor([0, 4], dtype=torch.int32).cuda()
+    ws = torch.empty(1 << 20, dtype=torch.uint8, device="cuda")
+    y, tok, lp = torch.empty_like(x), torch.empty(4, dtype=torch.int32, device="cuda"), torch.empty(4, device="cuda")
+    call = {"delta_prefill": lambda: g.delta_prefill(*q, cu, out=out, workspace=ws),
+            "delta_step": lambda: g.delta_step(*q, S, out=out), "logits_process": lambda: g.logits_process(x, out=y),
+            "sample_tokens": lambda: g.sample_tokens(x, tokens=tok, logprobs=lp)}[op]
+    call()
+    torch.cuda.synchronize()
+    hip.hipGetLastError()
+    try:
+        wrong = hip.hipSetDevice(1 << 20)
+        assert wrong != 0
+        call()
+        assert hip.hipGetLastError() == wrong
+    finally:
+        hip.hipGetLastError()
+    torch.cuda.synchronize()
