@@ -1058,6 +1058,19 @@ int check(const char *who, const GDNDelta *a, bool packed) {
     return 0;
 }
 
+// Whether o shares memory with q, k or v, or one of two pools of states with the other.
+bool overlaps(const GDNDelta &a) {
+    const int size = a.dtype == GDN_DTYPE_FP32 ? 4 : 2;
+    const uint64_t q = (uint64_t)a.n_qk_heads * a.key_dim * size, v = (uint64_t)a.n_v_heads * a.value_dim * size;
+    if (gdn::rows_overlap(a.o, v, a.o_stride * size, a.q, q, a.q_stride * size, a.n_tokens) ||
+        gdn::rows_overlap(a.o, v, a.o_stride * size, a.k, q, a.k_stride * size, a.n_tokens) ||
+        gdn::rows_overlap(a.o, v, a.o_stride * size, a.v, v, a.v_stride * size, a.n_tokens))
+        return true;
+    if (!a.state_in || !a.state_out || a.state_in == a.state_out) return false;
+    const uint64_t in = reinterpret_cast<uintptr_t>(a.state_in), out = reinterpret_cast<uintptr_t>(a.state_out);
+    return (in < out ? out - in : in - out) / (4ull * a.n_v_heads * a.key_dim * a.value_dim) < a.n_slots;
+}
+
 template <class T, int DK, int KP, int CT>
 hipError_t launch_seq(const GDNDelta &a, const int *order, const ChunkOps<kChunk<T>> *ops, const Planes<T, DK> *planes,
                       hipStream_t s) {
@@ -1125,6 +1138,7 @@ extern "C" int gdn_delta_prefill(const GDNDelta *args, void *workspace, size_t w
     if (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0 ||
         workspace_bytes < gdn_delta_prefill_workspace(args))
         return refuse(who, "the workspace is missing, misaligned or too small");
+    if (overlaps(*args)) return refuse(who, "o overlaps q, k or v, or state_out a part of state_in");
     hipStream_t s = static_cast<hipStream_t>(stream);
     return gdn::launched(who, args->dtype == GDN_DTYPE_BF16   ? launch_prefill_dk<Bf16>(*args, workspace, s)
                               : args->dtype == GDN_DTYPE_FP16 ? launch_prefill_dk<Fp16>(*args, workspace, s)
@@ -1136,6 +1150,7 @@ extern "C" int gdn_delta_step(const GDNDelta *args, void *stream) {
     constexpr const char *who = "gdn_delta_step";
     const int rc = check(who, args, false);
     if (rc != 0) return rc < 0 ? -1 : 0;
+    if (overlaps(*args)) return refuse(who, "o overlaps q, k or v, or state_out a part of state_in");
     hipStream_t s = static_cast<hipStream_t>(stream);
     return gdn::launched(who, args->dtype == GDN_DTYPE_BF16   ? launch_step_dk<Bf16>(*args, s)
                               : args->dtype == GDN_DTYPE_FP16 ? launch_step_dk<Fp16>(*args, s)

@@ -42,6 +42,20 @@ inline int launched(const char *who, hipError_t rc) {
     return -1;
 }
 
+// Whether two matrices of as many rows, widths and strides in bytes, share a
+// byte; of different strides only whether the first rows do.  (Columns of one
+// buffer lie in each other's range and share none.)
+inline bool rows_overlap(const void *a, uint64_t a_width, int64_t a_stride, const void *b, uint64_t b_width, int64_t b_stride,
+                         uint64_t rows) {
+    const uint64_t x = reinterpret_cast<uintptr_t>(a), y = reinterpret_cast<uintptr_t>(b);
+    const uint64_t x_end = x + (rows - 1) * (uint64_t)a_stride + a_width, y_end = y + (rows - 1) * (uint64_t)b_stride + b_width;
+    if (rows == 0 || x_end <= y || y_end <= x) return false;
+    if (y - x < a_width || x - y < b_width) return true;  // the first rows
+    if (a_stride != b_stride) return false;
+    const uint64_t s = (uint64_t)a_stride, at = x <= y ? (y - x) % s : (s - (x - y) % s) % s;  // of b's rows in a's
+    return at < a_width || at + b_width > s;
+}
+
 constexpr int kH = 2048;   // hidden
 constexpr int kNH = 8;     // heads
 constexpr int kHD = 256;   // head dim (dk = dv)

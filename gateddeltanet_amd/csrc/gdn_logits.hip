@@ -1239,6 +1239,10 @@ extern "C" int gdn_logits_process(const GDNLogits *args, void *stream) {
         return refuse(who, "a width or count is larger than 2^30");
     if (a.mask && a.mask_stride < (int64_t)((a.vocab + 31) / 32)) return refuse(who, "mask rows are shorter than the vocabulary");
     if (a.mask && !a.mask_index && a.n_masks < a.rows) return refuse(who, "fewer masks than rows, and no mask_index");
+    const int64_t size = a.dtype == GDN_DTYPE_FP32 ? 4 : 2;
+    if (!(a.logits == a.out && (a.rows == 1 || a.logits_stride == a.out_stride)) &&
+        gdn::rows_overlap(a.logits, a.vocab * size, a.logits_stride * size, a.out, a.vocab * size, a.out_stride * size, a.rows))
+        return refuse(who, "out overlaps logits, and is not the same rows");
     const dim3 grid((a.vocab + kTile - 1) / kTile, a.rows);
     const size_t lds = sizeof(uint32_t) * kTile * ((a.history != nullptr) + (a.bias_offsets != nullptr));
     hipStream_t s = static_cast<hipStream_t>(stream);

@@ -138,7 +138,8 @@ def delta_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Te
     dim][value dim], may be one tensor; sequence i's is slot slots[i] (int32;
     None: i), and a sequence with a slot outside the tensor is left out.
     scale: None for key dim^-1/2.  Returns out, [tokens][value heads][value
-    dim]; where it is made here, rows of no sequence hold nothing defined.
+    dim], apart from every input; where it is made here, rows of no sequence
+    hold nothing defined.
     workspace: uint8, gdn_delta_prefill_workspace bytes (None: allocated).
     """
     if out is None:

@@ -233,3 +233,44 @@ def test_batch_sample_refuses_integers_that_do_not_fit():
                dict(histories=[np.array([2**31 - 1]), [-2**31]], biases=[{np.int64(5): 1}, {}])):
         with pytest.raises(g.GDNError, match="^gdn_batch_sample failed"):
             state.sample(**kw)
+
+
+def apart(**change):
+    """A delta call whose buffers are megabytes apart."""
+    a = delta(**change)
+    for i, name in enumerate(("q", "k", "v", "o", "state_in", "state_out")):
+        if name not in change:
+            setattr(a, name, AT + (i << 24))
+    return a
+
+
+PART = 4 * 8 * 128 * 128  # bytes of a state
+O_AT, STATE_AT = AT + (3 << 24), AT + (4 << 24)
+
+
+@pytest.mark.parametrize("change", [
+    dict(o=AT), dict(o=AT + (1 << 24)), dict(o=AT + (2 << 24)), dict(q=O_AT + 16), dict(k=O_AT - 16),
+    dict(v=O_AT + 2048 * 3 + 16, v_stride=1024), dict(v=O_AT + 1024, v_stride=2048, o_stride=2048),
+    dict(q=O_AT + 2 * 2048 - 16, q_stride=2048, o_stride=2048),
+    dict(q=O_AT - 2 * 4096 + 2048 - 16, q_stride=2048, o_stride=2048),
+    dict(state_out=STATE_AT + 16), dict(state_out=STATE_AT + 4 * PART - 16), dict(state_out=STATE_AT - 4 * PART + 16),
+], ids=lambda c: "-".join(c))
+def test_delta_refuses_an_output_over_an_input(change, capfd):
+    lib = _lib.load()
+    assert lib.gdn_delta_prefill(ctypes.byref(apart(**change)), AT, 1 << 40, None) == -1
+    assert "overlap" in capfd.readouterr().err
+    a = apart(step=True, **change)
+    a.n_tokens = a.n_seqs = 10
+    a.n_slots = 4
+    assert lib.gdn_delta_step(ctypes.byref(a), None) == -1
+    assert "overlap" in capfd.readouterr().err
+
+
+@pytest.mark.parametrize("change", [
+    dict(out_stride=1024), dict(out=AT + 4), dict(out=AT - 4), dict(out=AT + 4000, rows=3), dict(out=AT - 3 * 4000),
+    dict(logits_stride=2500, out_stride=2500, out=AT + 4 * 999), dict(logits_stride=1999, out_stride=1999, out=AT + 4000),
+    dict(rows=1, out=AT + 4 * 999),
+], ids=lambda c: "-".join(f"{k}={v}" for k, v in c.items()))
+def test_logits_process_refuses_other_rows_of_its_input(change, capfd):
+    assert _lib.load().gdn_logits_process(ctypes.byref(logits(**change)), None) == -1
+    assert "overlaps logits" in capfd.readouterr().err

@@ -740,3 +740,25 @@ def test_an_error_of_an_earlier_call_is_not_reported_as_a_launchs(op):
     finally:
         hip.hipGetLastError()
     torch.cuda.synchronize()
+
+
+def test_process_into_columns_beside_the_logits():
+    """One buffer's columns, logits and output in turn: nothing is shared, so
+    it is taken; shifted by a column or a row it would be, and is not."""
+    both = row_logits(5, 2000, torch.float32, 8)
+    x, out = both[:, :1000], both[:, 1000:]
+    p = torch.ones(5).cuda()
+    hist, n = torch.arange(5, dtype=torch.int32).view(5, 1).cuda(), torch.ones(5, dtype=torch.int32).cuda()
+    want = x.clone()
+    want[range(5), range(5)] -= 1.0
+    g.logits_process(x, history=hist, history_len=n, presence=p, out=out)
+    assert torch.equal(out, want)
+    g.logits_process(x[1:], history=hist[1:], history_len=n[1:], presence=p[1:], out=out[:4])
+    assert torch.equal(out[:4], want[1:])
+    before = both.clone()
+    for bad in (both[:, 1:1001], both[:, 999:1999]):
+        with pytest.raises(g.GDNError):
+            g.logits_process(x, out=bad)
+    with pytest.raises(g.GDNError):
+        g.logits_process(x[:4], out=x[1:])
+    assert torch.equal(both, before)
