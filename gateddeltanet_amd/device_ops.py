@@ -6,7 +6,9 @@ Arguments are torch tensors on one GPU; work goes to that GPU's current stream
 and is not waited for, and every call can be captured into a graph.  Where a
 function makes its output or workspace, it takes them from torch's allocator on
 that stream.  Errors raise ``GDNError``, before anything is enqueued.  Nothing
-here is recorded for gradients.
+here is recorded for gradients, so where torch records them a floating-point
+argument that requires one is an error; a tensor written in place counts as
+modified, as after torch's own in-place operations.
 """
 from __future__ import annotations
 
@@ -16,6 +18,7 @@ import struct
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd.graph import increment_version
 
 from . import _lib as L
 from .engine import GDNError
@@ -29,6 +32,14 @@ _F32, _I32 = torch.float32, torch.int32
 
 def _fail(what: str) -> None:
     raise GDNError(what)
+
+
+def _apart_from_gradients(*tensors) -> None:
+    if torch.is_grad_enabled():
+        for x in tensors:
+            if x is not None and x.requires_grad:
+                _fail("an argument requires gradients, which these operators do not form: detach it, or call under "
+                      "torch.no_grad()")
 
 
 def _on(dev: int, name: str, x, dtype, shape) -> int:
@@ -86,6 +97,7 @@ def _launch(dev: int, what: str, *args) -> None:
 
 def _delta(q, k, v, g, beta, out, state_in, state_out, slots, n_seqs, cu, scale, l2norm):
     """(GPU, GDNDelta) of a call, checked."""
+    _apart_from_gradients(q, k, v, g, beta, out, state_in, state_out)
     qt, dev = q.dtype, q.get_device()
     dtype = _DTYPES.get(qt)
     if dtype is None or dev < 0:
@@ -142,7 +154,8 @@ def delta_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Te
     hold nothing defined.
     workspace: uint8, gdn_delta_prefill_workspace bytes (None: allocated).
     """
-    if out is None:
+    made = out is None
+    if made:
         out = torch.empty_like(v, memory_format=torch.contiguous_format)
     n_seqs = cu_seqlens.shape[0] - 1 if cu_seqlens.dim() == 1 else -1
     if n_seqs < 0:
@@ -153,6 +166,10 @@ def delta_prefill(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Te
     size = workspace.numel()
     _launch(dev, "gdn_delta_prefill", args,
             _on(dev, "workspace", workspace, torch.uint8, (size,)), size)
+    if not made:
+        increment_version(out)
+    if state_out is not None:
+        increment_version(state_out)
     return out
 
 
@@ -163,11 +180,16 @@ def delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tenso
     """gdn_delta_step: one token of every sequence; row i of q, k, v, g, beta
     is sequence i's, its state slot slots[i] of ``state``, updated in place (or
     written to state_out).  Shapes and the rest as delta_prefill's."""
-    if out is None:
+    made = out is None
+    if made:
         out = torch.empty_like(v, memory_format=torch.contiguous_format)
-    dev, args = _delta(q, k, v, g, beta, out, state, state if state_out is None else state_out, slots, q.shape[0], None,
-                       scale, l2norm)
+    into = state if state_out is None else state_out
+    dev, args = _delta(q, k, v, g, beta, out, state, into, slots, q.shape[0], None, scale, l2norm)
     _launch(dev, "gdn_delta_step", args)
+    if not made:
+        increment_version(out)
+    if into is not None:
+        increment_version(into)
     return out
 
 
@@ -205,8 +227,11 @@ def logits_process(logits: torch.Tensor, *, history: Optional[torch.Tensor] = No
     [masks][>= vocab / 32] with a set bit for every allowed token, mask_index
     int32 [rows].  out may be logits itself.  Returns out.
     """
+    offsets, ids, values = (None, None, None) if bias is None else bias
+    _apart_from_gradients(logits, out, repetition, presence, frequency, values)
     dev, dtype, rows, vocab, stride = _logits(logits)
-    if out is None:
+    made = out is None
+    if made:
         out = torch.empty_like(logits, memory_format=torch.contiguous_format)
         into = vocab
     else:
@@ -227,7 +252,6 @@ def logits_process(logits: torch.Tensor, *, history: Optional[torch.Tensor] = No
         _fail("penalties need a history")
     b_at = b_ids = b_values = n_bias = 0
     if bias is not None:
-        offsets, ids, values = bias
         entries = (ids.numel(),)
         b_at = _on(dev, "bias offsets", offsets, _I32, (rows + 1,))
         b_ids, b_values = _on(dev, "bias ids", ids, _I32, entries), _on(dev, "bias values", values, _F32, entries)
@@ -245,6 +269,8 @@ def logits_process(logits: torch.Tensor, *, history: Optional[torch.Tensor] = No
     a = _pack_logits(dtype, rows, vocab, width, n_bias, n_masks, stride, into, h_stride, m_stride, logits.data_ptr(),
                      out.data_ptr(), hist, length, prompt, rep, pres, freq, b_at, b_ids, b_values, m_at, m_index)
     _launch(dev, "gdn_logits_process", a)
+    if not made:
+        increment_version(out)
     return out
 
 
@@ -260,8 +286,9 @@ def sample_tokens(logits: torch.Tensor, uniform: Optional[torch.Tensor] = None, 
     positive: the first of the highest logits.  Returns (tokens int32 [rows],
     logprobs FP32 [rows]); -1 where no logit is above -infinity.
     """
+    _apart_from_gradients(logits, uniform, temperature, top_p, min_p, logprobs)
     dev, dtype, rows, vocab, stride = _logits(logits)
-    one = (rows,)
+    one, given = (rows,), [x for x in (tokens, logprobs) if x is not None]
     if tokens is None:
         tokens = torch.empty(one, dtype=_I32, device=logits.device)
     if logprobs is None:
@@ -273,4 +300,6 @@ def sample_tokens(logits: torch.Tensor, uniform: Optional[torch.Tensor] = None, 
     size = _entry("gdn_sample_workspace")(a)
     ws = torch.empty(size, dtype=torch.uint8, device=logits.device) if size else None
     _launch(dev, "gdn_sample_tokens", a, ws.data_ptr() if size else 0, size)
+    if given:
+        increment_version(given)
     return tokens, logprobs

@@ -274,3 +274,30 @@ def test_delta_refuses_an_output_over_an_input(change, capfd):
 def test_logits_process_refuses_other_rows_of_its_input(change, capfd):
     assert _lib.load().gdn_logits_process(ctypes.byref(logits(**change)), None) == -1
     assert "overlaps logits" in capfd.readouterr().err
+
+
+def test_arguments_that_require_gradients_are_refused():
+    """None is formed: an output cut off from its inputs would train a model
+    wrongly without a word.  Where torch records none they are taken (and
+    refused here for not being on a GPU)."""
+    x, s, cu = torch.zeros((4, 2, 64)), torch.zeros((4, 2)), torch.zeros(2, dtype=torch.int32)
+    S, y, f = torch.zeros((4, 2, 64, 64)), torch.zeros((2, 10)), torch.zeros(2)
+
+    def learnt(t):
+        return t.clone().requires_grad_()
+
+    bias = (torch.zeros(3, dtype=torch.int32), torch.zeros(2, dtype=torch.int32), learnt(f))
+    calls = [lambda: g.sample_tokens(learnt(y)), lambda: g.sample_tokens(y, f, temperature=learnt(f)),
+             lambda: g.logits_process(learnt(y)), lambda: g.logits_process(y, bias=bias),
+             lambda: g.logits_process(y, out=learnt(y)), lambda: g.delta_prefill(x, x, x, s, s, cu, state_in=learnt(S)),
+             lambda: g.delta_prefill(x, x, x, s, s, cu, state_out=learnt(S)), lambda: g.delta_step(x, x, x, s, s, learnt(S))]
+    for i in range(5):
+        a = [x, x, x, s, s]
+        a[i] = learnt(a[i])
+        calls += [lambda a=a: g.delta_prefill(*a, cu), lambda a=a: g.delta_step(*a, S)]
+    for call in calls:
+        with pytest.raises(g.GDNError, match="requires gradients"):
+            call()
+        for off in (torch.no_grad, torch.inference_mode):
+            with off(), pytest.raises(g.GDNError, match="on a GPU"):
+                call()

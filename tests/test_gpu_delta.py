@@ -482,3 +482,32 @@ def test_single_heads_of_transposed_views(hv):
             with pytest.raises(g.GDNError, match="contiguous in a row"):
                 f(q, k, kw.get("v", v), gate, beta, *b, out=kw.get("out", out))
     assert torch.equal(S, T)
+
+
+def test_tensors_written_in_place_count_as_modified():
+    """A value that autograd keeps for a backward pass and an operator then
+    writes over is an error there, as after torch's own in-place operations."""
+    n, hv, d = 3, 2, 64
+    q, k, v, gate, beta = inputs(n, hv, hv, d, d, FP32, 71)
+    cu = torch.tensor([0, n], dtype=torch.int32).cuda()
+    S, out = torch.ones((n, hv, d, d), device="cuda"), torch.empty_like(v)
+    x, y = torch.ones((n, 70), device="cuda"), torch.empty((n, 70), device="cuda")
+    tok, lp = torch.zeros(n, dtype=torch.int32, device="cuda"), torch.zeros(n, device="cuda")
+    calls = [(lambda: g.delta_step(q, k, v, gate, beta, S), [S]),
+             (lambda: g.delta_step(q, k, v, gate, beta, S.clone(), state_out=S, out=out), [S, out]),
+             (lambda: g.delta_prefill(q, k, v, gate, beta, cu, state_out=S, out=out), [S, out]),
+             (lambda: g.logits_process(x, out=y), [y]), (lambda: g.logits_process(x, out=x), [x]),
+             (lambda: g.sample_tokens(x, tokens=tok, logprobs=lp), [tok, lp])]
+    for call, written in calls:
+        before = [t._version for t in written]
+        call()
+        assert all(t._version > b for t, b in zip(written, before))
+    w = torch.ones((n, hv, d, d), device="cuda", requires_grad=True)
+    loss = (w * S).sum()
+    g.delta_step(q, k, v, gate, beta, S)
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        loss.backward()
+    with torch.inference_mode():
+        T = torch.ones((n, hv, d, d), device="cuda")
+        g.delta_step(q, k, v, gate, beta, T)
+    assert g.delta_step(q, k, v, gate, beta, None).shape == v.shape
