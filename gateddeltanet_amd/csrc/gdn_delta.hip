@@ -3,7 +3,6 @@
 // gdn_delta_step (one token of every sequence).
 #include <hip/hip_runtime.h>
 
-#include <cstdio>
 #include <type_traits>
 #include <utility>
 
@@ -93,11 +92,6 @@ __device__ __forceinline__ void for_terms(F &&f) {
 #pragma unroll
         for (int i = NA - 1; i >= 0; --i)
             if (s - i >= 0 && s - i < NB) f(i, s - i);
-}
-template <int NA, int NB>
-__device__ __forceinline__ f32x4 mfma_terms(const u32x4 (&a)[NA], const u32x4 (&b)[NB], f32x4 c) {
-    for_terms<NA, NB>([&](int i, int j) __attribute__((always_inline)) { c = mfma_bf16(a[i], b[j], c); });
-    return c;
 }
 
 // Tokens of a chunk.
@@ -1022,11 +1016,6 @@ size_t plane_bytes(const GDNDelta *a) {
 
 bool dim_ok(uint32_t d) { return d == 64 || d == 128 || d == 256; }
 
-int refuse(const char *who, const char *why) {
-    std::fprintf(stderr, "%s: %s\n", who, why);
-    return -1;
-}
-
 // What the host can see of a call; 1: nothing to do.
 int check(const char *who, const GDNDelta *a, bool packed) {
     if (a == nullptr) return refuse(who, "args is NULL");
@@ -1134,11 +1123,11 @@ extern "C" int gdn_delta_prefill(const GDNDelta *args, void *workspace, size_t w
     // a grid has fewer than 2^32 threads along an axis
     constexpr uint64_t most = (1ull << 32) / (64 * 4) - 8;
     if (places(args) >= most || (uint64_t)args->n_seqs * args->n_v_heads > most / (args->value_dim / 16) - 8)
-        return refuse(who, "too many chunks or heads for one launch");
+        return gdn::refuse(who, "too many chunks or heads for one launch");
     if (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0 ||
         workspace_bytes < gdn_delta_prefill_workspace(args))
-        return refuse(who, "the workspace is missing, misaligned or too small");
-    if (overlaps(*args)) return refuse(who, "o overlaps q, k or v, or state_out a part of state_in");
+        return gdn::refuse(who, "the workspace is missing, misaligned or too small");
+    if (overlaps(*args)) return gdn::refuse(who, "o overlaps q, k or v, or state_out a part of state_in");
     hipStream_t s = static_cast<hipStream_t>(stream);
     return gdn::launched(who, args->dtype == GDN_DTYPE_BF16   ? launch_prefill_dk<Bf16>(*args, workspace, s)
                               : args->dtype == GDN_DTYPE_FP16 ? launch_prefill_dk<Fp16>(*args, workspace, s)
@@ -1150,7 +1139,7 @@ extern "C" int gdn_delta_step(const GDNDelta *args, void *stream) {
     constexpr const char *who = "gdn_delta_step";
     const int rc = check(who, args, false);
     if (rc != 0) return rc < 0 ? -1 : 0;
-    if (overlaps(*args)) return refuse(who, "o overlaps q, k or v, or state_out a part of state_in");
+    if (overlaps(*args)) return gdn::refuse(who, "o overlaps q, k or v, or state_out a part of state_in");
     hipStream_t s = static_cast<hipStream_t>(stream);
     return gdn::launched(who, args->dtype == GDN_DTYPE_BF16   ? launch_step_dk<Bf16>(*args, s)
                               : args->dtype == GDN_DTYPE_FP16 ? launch_step_dk<Fp16>(*args, s)

@@ -36,6 +36,10 @@ hipError_t launch(void (*kernel)(P...), dim3 grid, dim3 block, size_t lds, hipSt
     if (rc != hipSuccess) (void)hipGetLastError();
     return rc;
 }
+inline int refuse(const char *who, const char *why) {
+    std::fprintf(stderr, "%s: %s\n", who, why);
+    return -1;
+}
 inline int launched(const char *who, hipError_t rc) {
     if (rc == hipSuccess) return 0;
     std::fprintf(stderr, "%s: launch failed: %s\n", who, hipGetErrorString(rc));

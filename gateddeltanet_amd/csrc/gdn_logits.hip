@@ -3,7 +3,6 @@
 // gdn_sample_tokens (the draw).
 #include <hip/hip_runtime.h>
 
-#include <cstdio>
 #include <type_traits>
 
 #include "gdn_amd.h"
@@ -1010,7 +1009,7 @@ struct WideRow {
     uint32_t count[kBins];
     Keep keep;
     double log_sum;
-    int done, pad;
+    int done;
     uint64_t cell[];
 };
 template <class T>
@@ -1208,10 +1207,6 @@ __global__ __launch_bounds__(kST) void k_wide_draw(GDNSample p, int shift, void 
     }
 }
 
-int refuse(const char *who, const char *why) {
-    std::fprintf(stderr, "%s: %s\n", who, why);
-    return -1;
-}
 bool misaligned(const void *p, int32_t dtype) {
     return (reinterpret_cast<uintptr_t>(p) & (dtype == GDN_DTYPE_FP32 ? 3 : 1)) != 0;
 }
@@ -1221,6 +1216,7 @@ bool misaligned(const void *p, int32_t dtype) {
 
 extern "C" int gdn_logits_process(const GDNLogits *args, void *stream) {
     using namespace gdn::lg;
+    using gdn::refuse;
     constexpr const char *who = "gdn_logits_process";
     if (args == nullptr) return refuse(who, "args is NULL");
     const GDNLogits &a = *args;
@@ -1288,6 +1284,7 @@ extern "C" size_t gdn_sample_workspace(const GDNSample *args) {
 
 extern "C" int gdn_sample_tokens(const GDNSample *args, void *workspace, size_t workspace_bytes, void *stream) {
     using namespace gdn::lg;
+    using gdn::refuse;
     constexpr const char *who = "gdn_sample_tokens";
     if (args == nullptr) return refuse(who, "args is NULL");
     const GDNSample &a = *args;
