@@ -762,3 +762,60 @@ def test_process_into_columns_beside_the_logits():
     with pytest.raises(g.GDNError):
         g.logits_process(x[:4], out=x[1:])
     assert torch.equal(both, before)
+
+
+def test_run_of_all_captured_is_the_eager_run_of_its_logits():
+    """Two steps of recurrence, projection, processing and draw in a graph: of
+    the logits that it formed, processed rows, tokens and log-probabilities are
+    the eager calls', whatever order its library product took."""
+    from test_gpu_delta import inputs
+
+    n, hv, d, vocab = 3, 2, 64, 900
+    gen = torch.Generator(device="cuda").manual_seed(15)
+    W = torch.randn((hv * d, vocab), generator=gen, device="cuda")
+    prompt = inputs(90, hv, hv, d, d, torch.float32, 40)
+    steps = [inputs(n, hv, hv, d, d, torch.float32, 41 + i) for i in range(2)]
+    us = [torch.rand(n, generator=gen, device="cuda") for _ in range(2)]
+    cu = torch.tensor([0, 37, 37, 90], dtype=torch.int32).cuda()
+    S = torch.zeros((n, hv, d, d), device="cuda")
+    history = torch.zeros((n, 8), dtype=torch.int32, device="cuda")
+    mask = torch.randint(-2**31, 2**31, (n, (vocab + 31) // 32), generator=gen, device="cuda").to(torch.int32)
+    rep, pres, freq, temp, share = (torch.full((n,), v, device="cuda") for v in (1.2, 0.5, 0.25, 0.8, 0.9))
+    lengths = [torch.full((n,), i, dtype=torch.int32, device="cuda") for i in range(2)]
+
+    def token(i, x, ids):
+        y = g.logits_process(x, history=ids, history_len=lengths[i], repetition=rep, presence=pres, frequency=freq, mask=mask)
+        return [y, *g.sample_tokens(y, us[i], temperature=temp, top_p=share)]
+
+    def work():
+        g.delta_prefill(*prompt, cu, state_out=S)
+        got = []
+        for i in range(2):
+            o = g.delta_step(*steps[i], S)
+            x = 4.0 * (o.reshape(n, -1) @ W)
+            got.append([o, x, *token(i, x, history)])
+            history[:, i] = got[i][3]
+        return got
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        work()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        captured = work()
+    for _ in range(4):
+        for u in us:
+            u.copy_(torch.rand(n, generator=gen, device="cuda"))
+        eager = [o.clone() for o, *_ in work()]
+        torch.cuda.synchronize()
+        graph.replay()
+        torch.cuda.synchronize()
+        ids = torch.zeros_like(history)
+        for i, (o, x, y, tok, lp) in enumerate(captured):
+            assert torch.equal(o, eager[i])
+            want = token(i, x, ids)
+            assert all(torch.equal(a, b) for a, b in zip((y, tok, lp), want)), i
+            ids[:, i] = tok
+        assert torch.equal(history, ids)
