@@ -153,6 +153,17 @@ template <int C>
 __device__ __forceinline__ int place_of(int first, int i) {
     return first / C + i;
 }
+// The sequence whose chunk a place is, where starts do not fall.
+template <int C>
+__device__ __forceinline__ int seq_at(const GDNDelta &p, int place) {
+    int lo = 0, hi = (int)p.n_seqs - 1;
+    while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (place_of<C>(span_of(p, mid).first, mid) <= place) lo = mid;
+        else hi = mid - 1;
+    }
+    return lo;
+}
 
 // ------------------------------------------------------------ chunk operands
 
@@ -193,7 +204,8 @@ __device__ __forceinline__ void subst(const float (&row)[16], int li, float (&co
 // while the others write M; then T_21 = -T_22 L_21 T_11 for the 32 x 32 blocks'
 // and for the whole's halves on FP32 MFMAs.
 // The last place's workgroup orders the sequences for k_delta_seq, longest
-// first, by counting their chunks in 256 steps.
+// first, by counting their chunks in 256 steps, and tells it behind them whether
+// a start falls: then places may be shared, and a sequence's searched in vain.
 // Bound by latency: loads, the products, 16 steps of substitution, four stages
 // of the inverse.  BF16, 8 heads of 256: 10.1 us for 70 tokens, 18.9 for 4096 (36
 // MB, 1.9 TB/s), 32.6 for 8111 in 24 sequences; FP32, 2005 tokens, 8 heads of 128:
@@ -214,15 +226,21 @@ __global__ __launch_bounds__(4 * kChunk<T>) void k_delta_prep(GDNDelta p, int *_
     __shared__ __attribute__((aligned(16))) float lm[C][LD];
     __shared__ double glog[C];
     __shared__ float ikn[C], iqn[C], bet[C];
+    __shared__ int falls;
     const int t = threadIdx.x, w = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63, li = lane & 15, kk = lane >> 4;
     const int place = blockIdx.x, hv = blockIdx.y, hk = hv / (int)(p.n_v_heads / p.n_qk_heads);
     if (place == (int)gridDim.x - 1) {
         if (hv != 0) return;
         for (int i = t; i < 256; i += 64 * NW) mem.bucket[i] = 0;
+        if (t == 0) falls = 0;
         __syncthreads();
         auto step = [&](int i) { return 255 - min((span_of(p, i).n + C - 1) / C, 255); };
-        for (int i = t; i < (int)p.n_seqs; i += 64 * NW) atomicAdd(&mem.bucket[step(i)], 1u);
+        for (int i = t; i < (int)p.n_seqs; i += 64 * NW) {
+            atomicAdd(&mem.bucket[step(i)], 1u);
+            if (i > 0 && span_of(p, i).first < span_of(p, i - 1).first) falls = 1;
+        }
         __syncthreads();
+        if (t == 0) order[p.n_seqs] = falls;
         if (w == 0) {
             u32x4 &own = *reinterpret_cast<u32x4 *>(&mem.bucket[4 * lane]);
             const u32x4 n = own;
@@ -239,15 +257,10 @@ __global__ __launch_bounds__(4 * kChunk<T>) void k_delta_prep(GDNDelta p, int *_
         for (int i = t; i < (int)p.n_seqs; i += 64 * NW) order[atomicAdd(&mem.bucket[step(i)], 1u)] = i;
         return;
     }
-    int lo = 0, hi = (int)p.n_seqs - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (place_of<C>(span_of(p, mid).first, mid) <= place) lo = mid;
-        else hi = mid - 1;
-    }
-    const Span sp = span_of(p, lo);
-    const int m0 = (place - place_of<C>(sp.first, lo)) * C;
-    if (m0 < 0 || m0 >= sp.n || slot_of(p, lo) < 0) return;
+    const int seq = seq_at<C>(p, place);
+    const Span sp = span_of(p, seq);
+    const int m0 = (place - place_of<C>(sp.first, seq)) * C;
+    if (m0 < 0 || m0 >= sp.n || slot_of(p, seq) < 0) return;
     const int n = min(C, sp.n - m0), row0 = sp.first + m0;
     ChunkOps<C> &ops = ops_all[(size_t)place * p.n_v_heads + hv];
 
@@ -542,6 +555,10 @@ __global__ __launch_bounds__(64 * KP, (kSeqPerCu<T, DK, KP, CT> == 2 && (CT == 1
     sp.n = __builtin_amdgcn_readfirstlane(sp.n);
     const int chunks = (sp.n + C - 1) / C, col = 16 * CT * cg + li;
     const size_t place = (size_t)place_of<C>(sp.first, seq);
+    // left out unless all its matrices were formed
+    if (order[p.n_seqs])
+        for (int c = 0; c < chunks; ++c)
+            if (seq_at<C>(p, (int)place + c) != seq) return;
     const ChunkOps<C> *ops = ops_all + place * p.n_v_heads + hv;
     // the state's key of tile a, register r of step s: key0 + 32 s + 4 a + r
     const int key0 = ks * (DK / KP) + 8 * kk;
@@ -1002,8 +1019,9 @@ __global__ __launch_bounds__(kT) void k_delta_step(GDNDelta p) {
 
 int chunk_of(const GDNDelta *a) { return a->dtype == GDN_DTYPE_BF16 ? kChunk<Bf16> : kChunk<Fp32>; }
 size_t places(const GDNDelta *a) { return (size_t)a->n_tokens / chunk_of(a) + a->n_seqs; }
-// The workspace: the sequences' order, the chunks' matrices, k and q in terms.
-size_t order_bytes(const GDNDelta *a) { return ((size_t)a->n_seqs * sizeof(int) + 255) / 256 * 256; }
+// The workspace: the sequences' order and whether a start falls, the chunks'
+// matrices, k and q in terms.
+size_t order_bytes(const GDNDelta *a) { return (((size_t)a->n_seqs + 1) * sizeof(int) + 255) / 256 * 256; }
 size_t ops_bytes(const GDNDelta *a) {
     return places(a) * a->n_v_heads *
            (a->dtype == GDN_DTYPE_BF16 ? sizeof(ChunkOps<kChunk<Bf16>>) : sizeof(ChunkOps<kChunk<Fp32>>));

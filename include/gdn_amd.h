@@ -634,7 +634,9 @@ int gdn_test_prefill_gemm(int kind, const float *W, const float *X, uint32_t N, 
  *   n_seqs     sequences.  gdn_delta_prefill: sequence i is the rows
  *              cu_seqlens[i] .. cu_seqlens[i + 1] - 1 (n_seqs + 1 values from
  *              0 up; an empty one keeps its state); rows of no sequence are
- *              not read and their o is left as it was.  gdn_delta_step:
+ *              not read and their o is left as it was.  Ends are held to the
+ *              rows; where they fall, a sequence has its result or is left
+ *              out as one without a slot is.  gdn_delta_step:
  *              n_tokens = n_seqs, row i is sequence i's token, cu_seqlens is
  *              not read.
  *   *_dim      64, 128 or 256, heads contiguous in a row

@@ -511,3 +511,38 @@ def test_tensors_written_in_place_count_as_modified():
         T = torch.ones((n, hv, d, d), device="cuda")
         g.delta_step(q, k, v, gate, beta, T)
     assert g.delta_step(q, k, v, gate, beta, None).shape == v.shape
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32], ids=["bf16", "fp16", "fp32"])
+def test_prefill_ends_that_fall(dtype):
+    """Ends that fall or pass the rows, over a workspace that holds NaN: a
+    sequence that is whole before the fall, and in any case every one whose
+    state is not as it was, has its result."""
+    n, hv, fill = 290, 2, 7.0
+    q, k, v, gate, beta = inputs(n, 1, hv, 64, 64, dtype, 12)
+    gen = torch.Generator().manual_seed(12)
+    calls = [[-5, 140, 290, 1000, 200, 2**31 - 1], [0, 140, 10, 290, 290, 290], [290, 0, 290], [100, 90, 80, 70, 60, 290],
+             [0, 290, 0, 290, 0, 290]]
+    calls += [torch.randint(-20, 320, (m,), generator=gen).tolist() for m in range(2, 14)]
+    for ends in calls:
+        m = len(ends) - 1
+        cu = torch.tensor(ends, dtype=torch.int32).cuda()
+        S = torch.full((m, hv, 64, 64), fill, device="cuda")
+        ws = torch.full((32 << 20,), 255, dtype=torch.uint8, device="cuda")
+        g.delta_prefill(q, k, v, gate, beta, cu, state_out=S, workspace=ws)
+        for i in range(m):
+            first = min(max(ends[i], 0), n)
+            s = slice(first, min(max(ends[i + 1], first), n))
+            if (S[i] == fill).all():
+                assert first != s.stop and any(b < a for a, b in zip(ends, ends[1:])), (ends, i)
+                continue
+            _, want = reference(q[s], k[s], v[s], gate[s], beta[s], torch.zeros_like(S[0]))
+            close(S[i], want, tol(64), f"state {i} of {ends}")
+    cu = torch.tensor(calls[0], dtype=torch.int32).cuda()
+    S = torch.full((5, hv, 64, 64), fill, device="cuda")
+    out = g.delta_prefill(q, k, v, gate, beta, cu, state_out=S)
+    for i, s in ((0, slice(0, 140)), (1, slice(140, 290))):
+        o, want = reference(q[s], k[s], v[s], gate[s], beta[s], torch.zeros_like(S[0]))
+        close(S[i], want, tol(64), f"state {i}")
+        close(out[s][:60], o[:60], tol(64), f"o {i}")  # (rows from 200 on are two sequences')
+    assert (S[2] == 0).all() and (S[3] == 0).all()
