@@ -496,13 +496,15 @@ __global__ __launch_bounds__(4 * kChunk<T>) void k_delta_prep(GDNDelta p, int *_
 // Three barriers a chunk; every operand of the next chunk is on its way into
 // registers meanwhile, in the order of its use.
 // Bound, with few sequences, by a chunk's chain of dependent products: 64 chunks
-// of 8 heads of 256 x 256 in 193 us, 3.0 us each, the matrix unit busy for 1536
+// of 8 heads of 256 x 256 in 194 us, 3.0 us each, the matrix unit busy for 1536
 // of 7200 cycles; with many, by the operands that a head's 16 column tiles read
 // through L2 (8111 tokens in 24 sequences: 199 us, 9 TB/s).  FP32, 2005 tokens in
 // 5 sequences, 8 heads of 128 x 128: 60 us.  Measured against it at 4096 tokens:
 // all keys in one wave 656 us (the products of a tile in a row); two waves and
 // 64 columns 432 (registers spill); 32 columns with K and Q shared by eight waves
 // 259; fragments read from memory 269; two workgroups a CU by force 415 (spills).
+// Two workgroups a CU leave a thread 256 registers: <Bf16, 256, 4, 1> spills 2,
+// <Bf16, 64, 2, 1> 6.
 // A wave takes 32 keys or more, so KP is 2 for 64 keys, else 4.
 template <class T, int DK, int KP, int CT>
 struct SeqLds {

@@ -78,8 +78,8 @@ __device__ __forceinline__ void store_vec(typename T::E *row, int at, int n, con
 // output's occurrences, and a bit for any occurrence.  A bias' entry number
 // goes in by maximum, so the last of equal ids holds.  The tile's logits are on
 // their way meanwhile.
-// 64 rows of 32000 FP32 logits, histories of 2500 tokens, biases and masks: 7.0 us
-// (17 MB, 2.4 TB/s; one row 4.3 us), bound by the steps' latencies: clearing, the
+// 64 rows of 32000 FP32 logits, histories of 2500 tokens, biases and masks: 7.1 us
+// (17 MB, 2.4 TB/s; one row 4.1 us), bound by the steps' latencies: clearing, the
 // ids, the atomics, the row.  256 rows of 99991 BF16 logits: 36 us (2.9 TB/s), 30
 // without histories.  Tiles of 4096 on 512 threads: 35 and 27 us there, but 16.2
 // against 15.0 at 256 x 32000 and 11.6 against 8.7 for histories of 20000, which
@@ -185,7 +185,10 @@ __global__ __launch_bounds__(kPT) void k_process(GDNLogits p) {
 // lies among the threads' highest tokens; 37 us for one that lies among hundreds,
 // of which 13 are the FP64 weights of the whole row; 24 us with neither.  Held rows
 // against slices (below), 64 x 32000: 18 against 30 us for top-k, 37 against 36 for
-// the flat top-p; 1024 x 32000: 76 against 137, 146 against 182.
+// the flat top-p; 1024 x 32000: 76 against 137, 146 against 182.  Few long rows are
+// the rule's cost: one BF16 row of 65536 takes 40 us with neither and 87 with a top-p
+// of 0.99, one of 131072 in slices 19 and 46.  A thread's 128 registers spill 18 for
+// the 16-bit types, 2 for FP32 (in k_wide_border 8 to 14).
 constexpr int kST = 1024, kBins = kST, kWaves = kST / 64;
 constexpr int kList = 512;             // tokens that are ranked against each other
 // A step of more tokens is cut in parts first, 2.4 us; ranking 65 takes 1.9 us, 111
