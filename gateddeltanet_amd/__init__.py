@@ -28,7 +28,8 @@ from .engine import (  # noqa: F401
     synth_uniform,
 )
 
-_DEVICE_OPS = ("delta_prefill", "delta_step", "logits_process", "sample_tokens")
+_DEVICE_OPS = ("conv_prefill", "conv_step", "delta_prefill", "delta_step", "logits_process", "rms_norm", "rms_norm_fp8",
+               "sample_tokens", "scan_prefill", "scan_step")
 
 
 def __getattr__(name: str):

@@ -162,6 +162,44 @@ class GDNDelta(ctypes.Structure):
     ]
 
 
+class GDNConv(ctypes.Structure):
+    """Arguments of gdn_conv_prefill and gdn_conv_step (device pointers)."""
+    _fields_ = [
+        ("dtype", c_int32), ("n_tokens", c_uint32), ("n_seqs", c_uint32), ("channels", c_uint32),
+        ("width", c_uint32), ("silu", c_int32), ("n_slots", c_uint32), ("reserved", c_uint32),
+        ("x_stride", c_int64), ("out_stride", c_int64),
+        ("x", c_void_p), ("out", c_void_p), ("weight", c_void_p), ("bias", c_void_p),
+        ("cu_seqlens", c_void_p), ("slots", c_void_p), ("state_in", c_void_p), ("state_out", c_void_p),
+    ]
+
+
+class GDNScan(ctypes.Structure):
+    """Arguments of gdn_scan_prefill and gdn_scan_step (device pointers)."""
+    _fields_ = [
+        ("dtype", c_int32), ("dt_dtype", c_int32), ("n_tokens", c_uint32), ("n_seqs", c_uint32),
+        ("n_heads", c_uint32), ("n_groups", c_uint32), ("state_dim", c_uint32), ("head_dim", c_uint32),
+        ("softplus", c_int32), ("n_slots", c_uint32),
+        ("x_stride", c_int64), ("b_stride", c_int64), ("c_stride", c_int64), ("dt_stride", c_int64),
+        ("y_stride", c_int64),
+        ("x", c_void_p), ("b", c_void_p), ("c", c_void_p), ("dt", c_void_p), ("y", c_void_p),
+        ("A", c_void_p), ("D", c_void_p), ("dt_bias", c_void_p),
+        ("cu_seqlens", c_void_p), ("slots", c_void_p), ("state_in", c_void_p), ("state_out", c_void_p),
+    ]
+
+
+class GDNNorm(ctypes.Structure):
+    """Arguments of gdn_rms_norm (device pointers)."""
+    _fields_ = [
+        ("dtype", c_int32), ("rows", c_uint32), ("heads", c_uint32), ("dim", c_uint32),
+        ("gate_first", c_int32), ("weight_heads", c_int32), ("fp8", c_int32), ("block", c_uint32),
+        ("eps", c_float), ("reserved", c_uint32),
+        ("x_stride", c_int64), ("residual_stride", c_int64), ("gate_stride", c_int64), ("out_stride", c_int64),
+        ("sum_stride", c_int64),
+        ("x", c_void_p), ("residual", c_void_p), ("gate", c_void_p), ("weight", c_void_p), ("out", c_void_p),
+        ("sum", c_void_p), ("scales", c_void_p),
+    ]
+
+
 class GDNLogits(ctypes.Structure):
     """Arguments of gdn_logits_process (device pointers)."""
     _fields_ = [
@@ -204,6 +242,12 @@ SIGNATURES = {
     "gdn_delta_prefill_workspace": (c_size_t, [POINTER(GDNDelta)]),
     "gdn_delta_prefill": (c_int, [POINTER(GDNDelta), c_void_p, c_size_t, c_void_p]),
     "gdn_delta_step": (c_int, [POINTER(GDNDelta), c_void_p]),
+    "gdn_conv_prefill": (c_int, [POINTER(GDNConv), c_void_p]),
+    "gdn_conv_step": (c_int, [POINTER(GDNConv), c_void_p]),
+    "gdn_scan_prefill_workspace": (c_size_t, [POINTER(GDNScan)]),
+    "gdn_scan_prefill": (c_int, [POINTER(GDNScan), c_void_p, c_size_t, c_void_p]),
+    "gdn_scan_step": (c_int, [POINTER(GDNScan), c_void_p]),
+    "gdn_rms_norm": (c_int, [POINTER(GDNNorm), c_void_p]),
     "gdn_logits_process": (c_int, [POINTER(GDNLogits), c_void_p]),
     "gdn_sample_workspace": (c_size_t, [POINTER(GDNSample)]),
     "gdn_sample_tokens": (c_int, [POINTER(GDNSample), c_void_p, c_size_t, c_void_p]),

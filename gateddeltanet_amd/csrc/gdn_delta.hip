@@ -9,102 +9,17 @@
 #include "gdn_amd.h"
 #include "gdn_device.h"
 #include "gdn_internal.h"
+#include "gdn_packed.h"
 #include "gdn_wy.h"
 
 namespace gdn {
 namespace delta {
 
-// An input type and the BF16 terms its values split into without loss.
-struct Bf16 {
-    static constexpr int kTerms = 1, kWords = 4;  // words of eight values
-    __device__ static void get8(const u32x4 *p, float (&x)[8]) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            x[2 * i] = u2f(p[0][i] << 16);
-            x[2 * i + 1] = u2f(p[0][i] & 0xffff0000u);
-        }
-    }
-    __device__ static float get(const void *p, size_t i) { return u2f((uint32_t) static_cast<const uint16_t *>(p)[i] << 16); }
-    __device__ static void put(void *p, size_t i, float x) {
-        static_cast<uint16_t *>(p)[i] = (uint16_t)cvt_pk(x, 0.0f);
-    }
-};
-struct Fp16 {
-    static constexpr int kTerms = 2, kWords = 4;
-    typedef _Float16 h2 __attribute__((ext_vector_type(2)));
-    __device__ static void get8(const u32x4 *p, float (&x)[8]) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const h2 v = __builtin_bit_cast(h2, (uint32_t)p[0][i]);
-            x[2 * i] = (float)v.x;
-            x[2 * i + 1] = (float)v.y;
-        }
-    }
-    __device__ static float get(const void *p, size_t i) { return (float)static_cast<const _Float16 *>(p)[i]; }
-    __device__ static void put(void *p, size_t i, float x) { static_cast<_Float16 *>(p)[i] = (_Float16)x; }
-};
-struct Fp32 {
-    static constexpr int kTerms = 3, kWords = 8;
-    __device__ static void get8(const u32x4 *p, float (&x)[8]) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = u2f(p[i / 4][i % 4]);
-    }
-    __device__ static float get(const void *p, size_t i) { return static_cast<const float *>(p)[i]; }
-    __device__ static void put(void *p, size_t i, float x) { static_cast<float *>(p)[i] = x; }
-};
-
-// Eight consecutive values as raw words.
-template <class T>
-struct Raw8 {
-    u32x4 w[T::kWords / 4];
-    __device__ __forceinline__ void load(const void *p, size_t i) {
-#pragma unroll
-        for (int j = 0; j < T::kWords / 4; ++j)
-            w[j] = reinterpret_cast<const u32x4 *>(static_cast<const char *>(p) + i * (T::kWords / 2))[j];
-    }
-    __device__ __forceinline__ void zero() {
-#pragma unroll
-        for (int j = 0; j < T::kWords / 4; ++j) w[j] = (u32x4){0u, 0u, 0u, 0u};
-    }
-    // the values' BF16 terms, packed pairs
-    __device__ __forceinline__ void terms(u32x4 (&t)[T::kTerms]) const {
-        if constexpr (T::kTerms == 1) {
-            t[0] = w[0];
-        } else {
-            float x[8];
-            T::get8(w, x);
-            u32x2 a[3], b[3];
-            split3((f32x4){x[0], x[1], x[2], x[3]}, a);
-            split3((f32x4){x[4], x[5], x[6], x[7]}, b);
-#pragma unroll
-            for (int j = 0; j < T::kTerms; ++j) t[j] = (u32x4){a[j].x, a[j].y, b[j].x, b[j].y};
-        }
-    }
-};
-
-// f(a, b) for the terms a, b of two operands, of NA and NB terms, whose
-// products count, smallest first; products below 2^-24 of the whole are left
-// out.
-template <int NA, int NB, class F>
-__device__ __forceinline__ void for_terms(F &&f) {
-#pragma unroll
-    for (int s = 2; s >= 0; --s)
-#pragma unroll
-        for (int i = NA - 1; i >= 0; --i)
-            if (s - i >= 0 && s - i < NB) f(i, s - i);
-}
+using namespace packed;
 
 // Tokens of a chunk.
 template <class T>
 constexpr int kChunk = T::kTerms == 1 ? 64 : 32;
-
-// Four values of 16-bit columns l % 16: of each 16 lanes, lane l names the
-// 8 bytes of row l / 4, columns 4 (l % 4) .. + 3, and gets its column's four rows.
-__device__ __forceinline__ u32x2 read_transposed(const u32x2 *lds) {
-    typedef short s16x4 __attribute__((ext_vector_type(4)));
-    typedef __attribute__((address_space(3))) s16x4 *Ptr;
-    return __builtin_bit_cast(u32x2, __builtin_amdgcn_ds_read_tr16_b64_v4i16((Ptr)(const_cast<u32x2 *>(lds))));
-}
 
 // Where a 16 x 32 tile (row tile i, column step j) of a chunk's lower
 // triangular matrix is kept: tiles above the diagonal are zero and left out.
@@ -133,19 +48,6 @@ struct Planes {
     uint16_t k[T::kTerms][kChunk<T>][DK], q[T::kTerms][kChunk<T>][DK];
 };
 
-// One sequence's rows.
-struct Span {
-    int first, n;
-};
-__device__ __forceinline__ Span span_of(const GDNDelta &p, int i) {
-    const int end = (int)p.n_tokens;
-    const int a = min(max(p.cu_seqlens[i], 0), end), b = min(max(p.cu_seqlens[i + 1], a), end);
-    return {a, b - a};
-}
-__device__ __forceinline__ int slot_of(const GDNDelta &p, int i) {
-    const int s = p.slots ? p.slots[i] : i;
-    return s >= 0 && s < (int)p.n_slots ? s : -1;
-}
 // Chunk c of the sequence that starts at row `first` as number i has place
 // first / C + i + c: places grow with (i, c), none is shared, and there are
 // at most n_tokens / C + n_seqs, so nothing has to be counted first.
@@ -166,13 +68,6 @@ __device__ __forceinline__ int seq_at(const GDNDelta &p, int place) {
 }
 
 // ------------------------------------------------------------ chunk operands
-
-// 2^y, to about 2^-23 of it: the whole powers apart from the rest, which is
-// small enough for FP32.
-__device__ __forceinline__ float exp2_of(double y) {
-    const double n = __builtin_rint(y);
-    return __builtin_ldexpf(__builtin_amdgcn_exp2f((float)(y - n)), (int)n);
-}
 
 // Column `col` of the inverse of a unit lower triangular 16 x 16 block whose
 // row r is lane r's `row`: forward substitution, row M's values broadcast

@@ -1,6 +1,7 @@
 """The operators on the caller's device tensors (include/gdn_amd.h, "operators
-on the caller's device buffers"): the gated delta rule over a batch of
-sequences, and the way from a batch's logits to its tokens.
+on the caller's device buffers"): the recurrences over a batch of sequences (the
+gated delta rule, the selective state space scan), the short convolution in front
+of them, the norm around them, and the way from a batch's logits to its tokens.
 
 Arguments are torch tensors on one GPU; work goes to that GPU's current stream
 and is not waited for, and every call can be captured into a graph.  Where a
@@ -72,6 +73,7 @@ def _packer(cls):
 
 
 _pack_delta, _pack_logits, _pack_sample = _packer(L.GDNDelta), _packer(L.GDNLogits), _packer(L.GDNSample)
+_pack_conv, _pack_scan, _pack_norm = _packer(L.GDNConv), _packer(L.GDNScan), _packer(L.GDNNorm)
 
 
 @functools.lru_cache(maxsize=None)
@@ -191,6 +193,269 @@ def delta_step(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, g: torch.Tenso
     if into is not None:
         increment_version(into)
     return out
+
+
+def _sequences(cu) -> int:
+    if cu.dim() != 1 or cu.shape[0] < 1:
+        _fail("cu_seqlens: expected int32 [sequences + 1]")
+    return cu.shape[0] - 1
+
+
+def _conv(x, weight, bias, silu, out, state_in, state_out, slots, n_seqs, cu):
+    """(GPU, GDNConv) of a call, checked."""
+    _apart_from_gradients(x, weight, bias, out, state_in, state_out)
+    xt, dev = x.dtype, x.get_device()
+    dtype = _DTYPES.get(xt)
+    if dtype is None or dev < 0 or x.dim() != 2:
+        _fail(f"x: expected a bfloat16, float16 or float32 [tokens][channels] on a GPU, got {xt} {tuple(x.shape)} on "
+              f"{x.device}")
+    n, channels = xs = x.shape
+    if out.dtype is not xt or out.shape != xs or out.get_device() != dev:
+        _fail(f"out: expected {xt} {tuple(xs)} on {x.device}, got {out.dtype} {tuple(out.shape)} on {out.device}")
+    sx, so = x.stride(), out.stride()
+    if n and channels > 1 and (sx[1] != 1 or so[1] != 1):
+        _fail(f"channels must be contiguous: strides x {sx}, out {so}")
+    if weight.dim() != 2:
+        _fail(f"weight: expected float32 [channels][width], got {tuple(weight.shape)}")
+    width = weight.shape[1]
+    pool = state_in if state_out is None else state_out
+    n_slots = n_seqs if pool is None else pool.shape[0] if pool.dim() else -1
+    tails = (n_slots, width - 1, channels)
+    at_in = _on(dev, "state_in", state_in, xt, tails)
+    at_out = at_in if state_out is state_in else _on(dev, "state_out", state_out, xt, tails)
+    if slots is None and n_slots < n_seqs:
+        _fail(f"{n_seqs} sequences without slots need as many states, got {n_slots}")
+    return dev, _pack_conv(
+        dtype, n, n_seqs, channels, width, 1 if silu else 0, n_slots, 0, sx[0], so[0], x.data_ptr(), out.data_ptr(),
+        _on(dev, "weight", weight, _F32, (channels, width)), _on(dev, "bias", bias, _F32, (channels,)),
+        _on(dev, "cu_seqlens", cu, _I32, (n_seqs + 1,)), _on(dev, "slots", slots, _I32, (n_seqs,)), at_in, at_out)
+
+
+def conv_prefill(x: torch.Tensor, weight: torch.Tensor, cu_seqlens: torch.Tensor, *, bias: Optional[torch.Tensor] = None,
+                 silu: bool = True, state_in: Optional[torch.Tensor] = None, state_out: Optional[torch.Tensor] = None,
+                 slots: Optional[torch.Tensor] = None, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """gdn_conv_prefill: the short causal convolution over packed sequences.
+
+    x [tokens][channels] (rows may be strided, as slices of a fused projection are);
+    weight FP32 [channels][width], width 2 to 4, its last column the token's own;
+    bias FP32 [channels]; silu: the output through SiLU.  cu_seqlens and slots as
+    delta_prefill's.  state_in (None: zeros) and state_out (None: not kept): the tails,
+    the width - 1 inputs before (behind) the sequence, oldest first, of x's type
+    [slots][width - 1][channels], may be one tensor.  Returns out, [tokens][channels],
+    apart from x; where it is made here, rows of no sequence hold nothing defined.
+    """
+    made = out is None
+    if made:
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
+    dev, args = _conv(x, weight, bias, silu, out, state_in, state_out, slots, _sequences(cu_seqlens), cu_seqlens)
+    _launch(dev, "gdn_conv_prefill", args)
+    if not made:
+        increment_version(out)
+    if state_out is not None:
+        increment_version(state_out)
+    return out
+
+
+def conv_step(x: torch.Tensor, weight: torch.Tensor, state: torch.Tensor, *, bias: Optional[torch.Tensor] = None,
+              silu: bool = True, state_out: Optional[torch.Tensor] = None, slots: Optional[torch.Tensor] = None,
+              out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """gdn_conv_step: one token of every sequence; row i of x is sequence i's, its
+    tail slot slots[i] of ``state``, updated in place (or written to state_out).  out
+    may be x.  Shapes and the rest as conv_prefill's."""
+    made = out is None
+    if made:
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
+    into = state if state_out is None else state_out
+    dev, args = _conv(x, weight, bias, silu, out, state, into, slots, x.shape[0] if x.dim() else 0, None)
+    _launch(dev, "gdn_conv_step", args)
+    if not made:
+        increment_version(out)
+    if into is not None:
+        increment_version(into)
+    return out
+
+
+def _scan(x, dt, A, B, C, D, dt_bias, softplus, out, state_in, state_out, slots, n_seqs, cu):
+    """(GPU, GDNScan) of a call, checked."""
+    _apart_from_gradients(x, dt, A, B, C, D, dt_bias, out, state_in, state_out)
+    xt, dev = x.dtype, x.get_device()
+    dtype = _DTYPES.get(xt)
+    if dtype is None or dev < 0:
+        _fail(f"x: expected a bfloat16, float16 or float32 tensor on a GPU, got {xt} on {x.device}")
+    for name, y in (("x", x), ("B", B), ("C", C), ("out", out)):
+        if y.dtype is not xt or y.dim() != 3 or y.get_device() != dev:
+            _fail(f"{name}: expected {xt} [rows][heads][dim] on {x.device}, got {y.dtype} {tuple(y.shape)} on {y.device}")
+    n, heads, P = xs = x.shape
+    _, groups, N = bs = B.shape
+    if C.shape != bs or bs[0] != n or out.shape != xs:
+        _fail(f"shapes do not agree: x {tuple(xs)}, B {tuple(bs)}, C {tuple(C.shape)}, out {tuple(out.shape)}")
+    sx, sb, sc, so = x.stride(), B.stride(), C.stride(), out.stride()
+    wide, narrow = (P, 1), (N, 1)
+    if n and (sx[1:] != wide or so[1:] != wide or sb[1:] != narrow or sc[1:] != narrow) and not (
+            # (a single head's or group's stride is not used)
+            sx[2] == so[2] == sb[2] == sc[2] == 1 and (heads == 1 or sx[1] == so[1] == P) and (
+                groups == 1 or sb[1] == sc[1] == N)):
+        _fail(f"heads must be contiguous in a row: strides x {sx}, B {sb}, C {sc}, out {so}")
+    sd, of = dt.stride(), dt.dtype
+    if dt.shape != (n, heads) or (of is not xt and of is not _F32) or dt.get_device() != dev or (
+            n > 0 and heads > 1 and sd[1] != 1):
+        _fail(f"dt: expected {xt} or float32 [{n}][{heads}] on {x.device} with contiguous rows, got {of} "
+              f"{tuple(dt.shape)} strides {sd} on {dt.device}")
+    pool = state_in if state_out is None else state_out
+    n_slots = n_seqs if pool is None else pool.shape[0] if pool.dim() else -1
+    states, each = (n_slots, heads, N, P), (heads,)
+    at_in = _on(dev, "state_in", state_in, _F32, states)
+    at_out = at_in if state_out is state_in else _on(dev, "state_out", state_out, _F32, states)
+    if slots is None and n_slots < n_seqs:
+        _fail(f"{n_seqs} sequences without slots need as many states, got {n_slots}")
+    return dev, _pack_scan(
+        dtype, _DTYPES[of], n, n_seqs, heads, groups, N, P, 1 if softplus else 0, n_slots, sx[0], sb[0], sc[0], sd[0],
+        so[0], x.data_ptr(), B.data_ptr(), C.data_ptr(), dt.data_ptr(), out.data_ptr(), _on(dev, "A", A, _F32, each),
+        _on(dev, "D", D, _F32, each), _on(dev, "dt_bias", dt_bias, _F32, each),
+        _on(dev, "cu_seqlens", cu, _I32, (n_seqs + 1,)), _on(dev, "slots", slots, _I32, (n_seqs,)), at_in, at_out)
+
+
+def scan_prefill(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.Tensor, C: torch.Tensor,
+                 cu_seqlens: torch.Tensor, *, D: Optional[torch.Tensor] = None, dt_bias: Optional[torch.Tensor] = None,
+                 softplus: bool = False, state_in: Optional[torch.Tensor] = None,
+                 state_out: Optional[torch.Tensor] = None, slots: Optional[torch.Tensor] = None,
+                 out: Optional[torch.Tensor] = None, workspace: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """gdn_scan_prefill: the selective state space scan over packed sequences.
+
+    x [tokens][heads][head dim], B and C [tokens][groups][state dim] of one type
+    (rows may be strided); dt [tokens][heads] of that type or FP32, the steps, or
+    what dt_bias is added to and (softplus) a softplus makes them of; A (negative in a
+    stable model), D and dt_bias FP32 [heads].  cu_seqlens, state_in, state_out and
+    slots as delta_prefill's, states FP32 [slots][heads][state dim][head dim].
+    Returns out, as x, apart from every input; where it is made here, rows of no
+    sequence hold nothing defined.
+    workspace: uint8, gdn_scan_prefill_workspace bytes (None: allocated).
+    """
+    made = out is None
+    if made:
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
+    dev, args = _scan(x, dt, A, B, C, D, dt_bias, softplus, out, state_in, state_out, slots, _sequences(cu_seqlens),
+                      cu_seqlens)
+    at = size = 0
+    if workspace is None:
+        size = _entry("gdn_scan_prefill_workspace")(args)
+        if size:
+            workspace = torch.empty(size, dtype=torch.uint8, device=x.device)
+            at = workspace.data_ptr()
+    else:
+        size = workspace.numel()
+        at = _on(dev, "workspace", workspace, torch.uint8, (size,))
+    _launch(dev, "gdn_scan_prefill", args, at, size)
+    if not made:
+        increment_version(out)
+    if state_out is not None:
+        increment_version(state_out)
+    return out
+
+
+def scan_step(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.Tensor, C: torch.Tensor, state: torch.Tensor,
+              *, D: Optional[torch.Tensor] = None, dt_bias: Optional[torch.Tensor] = None, softplus: bool = False,
+              state_out: Optional[torch.Tensor] = None, slots: Optional[torch.Tensor] = None,
+              out: Optional[torch.Tensor] = None) -> torch.Tensor:
+    """gdn_scan_step: one token of every sequence; row i of x, dt, B and C is
+    sequence i's, its state slot slots[i] of ``state``, updated in place (or written
+    to state_out).  Shapes and the rest as scan_prefill's."""
+    made = out is None
+    if made:
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
+    into = state if state_out is None else state_out
+    dev, args = _scan(x, dt, A, B, C, D, dt_bias, softplus, out, state, into, slots, x.shape[0] if x.dim() else 0, None)
+    _launch(dev, "gdn_scan_step", args)
+    if not made:
+        increment_version(out)
+    if into is not None:
+        increment_version(into)
+    return out
+
+
+def _rows(dev: int, name: str, x, dtype, shape):
+    """(address, row stride) of rows of this type and shape on GPU dev, the rest of
+    a row contiguous (None: 0)."""
+    if x is None:
+        return 0, 0
+    st = x.stride()
+    if x.dtype is not dtype or x.shape != shape or x.get_device() != dev or (
+            st[-1] != 1 and shape[-1] > 1 and x.numel()) or (
+            len(shape) == 3 and shape[1] > 1 and x.numel() and st[1] != shape[2]):
+        _fail(f"{name}: expected {dtype} {tuple(shape)} on GPU {dev} with contiguous rows, got {x.dtype} "
+              f"{tuple(x.shape)} strides {st} on {x.device}")
+    return x.data_ptr(), st[0]
+
+
+def _norm(x, weight, eps, residual, gate, gate_first, out, out_type, total, scales, block):
+    _apart_from_gradients(x, weight, residual, gate, out, total, scales)
+    xt, dev, shape = x.dtype, x.get_device(), x.shape
+    dtype = _DTYPES.get(xt)
+    if dtype is None or dev < 0 or len(shape) not in (2, 3):
+        _fail(f"x: expected a bfloat16, float16 or float32 [rows][dim] or [rows][heads][dim] on a GPU, got {xt} "
+              f"{tuple(shape)} on {x.device}")
+    rows, dim, heads = shape[0], shape[-1], shape[1] if len(shape) == 3 else 1
+    if total is not None and residual is None:
+        _fail("the sum needs a residual")
+    if gate_first and gate is None:
+        _fail("gate_first needs a gate")
+    shared = weight is None or weight.dim() == 1
+    at_x, sx = _rows(dev, "x", x, xt, shape)
+    at_r, sr = _rows(dev, "residual", residual, xt, shape)
+    at_g, sg = _rows(dev, "gate", gate, xt, shape)
+    at_o, so = _rows(dev, "out", out, out_type, shape)
+    at_s, ss = _rows(dev, "sum", total, xt, shape)
+    _launch(dev, "gdn_rms_norm", _pack_norm(
+        dtype, rows, heads, dim, 1 if gate_first else 0, 0 if shared else 1, 0 if scales is None else 1, block, eps, 0,
+        sx, sr, sg, so, ss, at_x, at_r, at_g, _on(dev, "weight", weight, _F32, (dim,) if shared else (heads, dim)),
+        at_o, at_s, 0 if scales is None else _on(
+            dev, "scales", scales, _F32, (rows, heads * dim // block if block else 1))))
+
+
+def rms_norm(x: torch.Tensor, weight: Optional[torch.Tensor] = None, *, eps: float = 1e-6,
+             residual: Optional[torch.Tensor] = None, gate: Optional[torch.Tensor] = None, gate_first: bool = False,
+             out: Optional[torch.Tensor] = None, sum_out: Optional[torch.Tensor] = None):
+    """gdn_rms_norm: the root-mean-square norm over the last dimension.
+
+    x [rows][dim] or [rows][heads][dim] (rows may be strided); weight FP32 [dim], or
+    [heads][dim]; residual and gate as x.  x + residual is normed; SiLU of the gate
+    multiplies the normed values, or (gate_first) what is normed.  Returns out, as x,
+    or with a residual (out, sum_out), the sum rounded to x's type.  out may be x, residual
+    or gate, sum_out x or residual.
+    """
+    given = [y for y in (out, sum_out) if y is not None]
+    if out is None:
+        out = torch.empty_like(x, memory_format=torch.contiguous_format)
+    if residual is not None and sum_out is None:
+        sum_out = torch.empty_like(x, memory_format=torch.contiguous_format)
+    _norm(x, weight, eps, residual, gate, gate_first, out, x.dtype, sum_out, None, 0)
+    if given:
+        increment_version(given)
+    return out if residual is None else (out, sum_out)
+
+
+def rms_norm_fp8(x: torch.Tensor, weight: Optional[torch.Tensor] = None, *, block: int = 0, eps: float = 1e-6,
+                 residual: Optional[torch.Tensor] = None, gate: Optional[torch.Tensor] = None,
+                 gate_first: bool = False, out: Optional[torch.Tensor] = None, scales: Optional[torch.Tensor] = None,
+                 sum_out: Optional[torch.Tensor] = None):
+    """gdn_rms_norm with an output in 8 bits: (out, scales), or with a residual (out,
+    scales, sum_out).  out, float8_e4m3fn as x, times its scale stands for the normed
+    values; scales FP32 [rows][heads * dim / block], a scale for every 32, 64 or 128
+    values of a row, or [rows][1] (block 0).  The rest as rms_norm's."""
+    given = [y for y in (out, scales, sum_out) if y is not None]
+    if out is None:
+        out = torch.empty_like(x, dtype=torch.float8_e4m3fn, memory_format=torch.contiguous_format)
+    if block not in (0, 32, 64, 128):
+        _fail(f"block: expected 0, 32, 64 or 128, got {block}")
+    if scales is None:
+        wide = x.shape[-1] * (x.shape[1] if x.dim() == 3 else 1) if x.dim() else 0
+        scales = torch.empty((x.shape[0] if x.dim() else 0, wide // block if block else 1), dtype=_F32, device=x.device)
+    if residual is not None and sum_out is None:
+        sum_out = torch.empty_like(x, memory_format=torch.contiguous_format)
+    _norm(x, weight, eps, residual, gate, gate_first, out, torch.float8_e4m3fn, sum_out, scales, block)
+    if given:
+        increment_version(given)
+    return (out, scales) if residual is None else (out, scales, sum_out)
 
 
 def _logits(x: torch.Tensor, name: str = "logits"):

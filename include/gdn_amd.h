@@ -683,6 +683,122 @@ int gdn_delta_prefill(const GDNDelta *args, void *workspace, size_t workspace_by
 /* One token of every sequence. */
 int gdn_delta_step(const GDNDelta *args, void *stream);
 
+/* The short causal convolution over a batch, each channel on its own: with z the
+ * sequence's inputs behind its tail, the width - 1 inputs before them,
+ *   y_t = bias + sum over j of weight[j] z_(t - (width - 1) + j),  out_t = y_t, or
+ *   y_t / (1 + exp(-y_t)) where silu != 0
+ * in FP32, rounded once.  The sequence's tail afterwards is its last width - 1
+ * inputs, of the old tail where it has fewer, as they are.
+ *   n_tokens, n_seqs, cu_seqlens, slots, n_slots   as GDNDelta's, but that ends do
+ *              not fall: where they do, what the rows and tails of the call's
+ *              sequences hold afterwards is not defined
+ *   channels   at most 2^20
+ *   width      2, 3 or 4
+ *   *_stride   elements between rows (with one row not looked at).  Any
+ *              alignment of an element's
+ *   out        gdn_conv_prefill: overlaps no row of x.  gdn_conv_step: may be x, of
+ *              an equal stride
+ *   weight     FP32 [channels][width]; bias FP32 [channels], NULL: 0
+ *   state_in, state_out   [n_slots][width - 1][channels] of the rows' type, oldest
+ *              first; the same buffer, or two that do not overlap.  state_in NULL:
+ *              zeros; state_out NULL: the tails are not kept. */
+typedef struct {
+    int32_t dtype;              /* GDN_DTYPE_* of x, out and the tails */
+    uint32_t n_tokens, n_seqs;
+    uint32_t channels, width;
+    int32_t silu;
+    uint32_t n_slots, reserved;
+    int64_t x_stride, out_stride;
+    const void *x;
+    void *out;
+    const float *weight, *bias;
+    const int32_t *cu_seqlens;
+    const int32_t *slots;
+    const void *state_in;
+    void *state_out;
+} GDNConv;
+/* Packed sequences; one token of every sequence (n_tokens = n_seqs). */
+int gdn_conv_prefill(const GDNConv *args, void *stream);
+int gdn_conv_step(const GDNConv *args, void *stream);
+
+/* The selective state space scan over a batch.  Per head, with the FP32 state S
+ * [state_dim][head_dim] of its sequence and B and C of group
+ * head / (n_heads / n_groups), for each of the sequence's tokens:
+ *   h = dt + dt_bias, where softplus != 0 log(1 + exp(h))
+ *   S = exp(h A) S + h B x^T;  y = S^T C + D x
+ *   n_tokens, n_seqs, cu_seqlens, slots, n_slots   as GDNConv's
+ *   *_dim      64, 128 or 256, heads and groups contiguous in a row
+ *   *_stride   elements between rows (with one row not looked at).  x, b, c and y
+ *              rows start at multiples of 16 bytes and lie less than 16 MB apart;
+ *              y overlaps no input
+ *   dt         [n_tokens][n_heads] of dt_dtype: dtype or GDN_DTYPE_FP32
+ *   A, D, dt_bias   FP32 [n_heads]; D NULL: 0, dt_bias NULL: 0.  h A <= 0 in a
+ *              stable model
+ *   state_in, state_out   [n_slots][n_heads][state_dim][head_dim] FP32, as GDNDelta's
+ * Sums are FP32.  A value that is not finite reaches its own sequence and head
+ * (one of B or C the heads of its group) only, in gdn_scan_prefill there also the
+ * tokens up to 63 before it. */
+typedef struct {
+    int32_t dtype;              /* GDN_DTYPE_* of x, b, c and y */
+    int32_t dt_dtype;
+    uint32_t n_tokens, n_seqs;
+    uint32_t n_heads, n_groups;
+    uint32_t state_dim, head_dim;
+    int32_t softplus;
+    uint32_t n_slots;
+    int64_t x_stride, b_stride, c_stride, dt_stride, y_stride;
+    const void *x, *b, *c, *dt;
+    void *y;
+    const float *A, *D, *dt_bias;
+    const int32_t *cu_seqlens;
+    const int32_t *slots;
+    const float *state_in;
+    float *state_out;
+} GDNScan;
+/* Packed sequences in the chunk-parallel form.  `workspace`:
+ * gdn_scan_prefill_workspace(args) bytes at a multiple of 16 bytes (0 for few
+ * tokens), needed until the work is done. */
+size_t gdn_scan_prefill_workspace(const GDNScan *args);
+int gdn_scan_prefill(const GDNScan *args, void *workspace, size_t workspace_bytes, void *stream);
+/* One token of every sequence (n_tokens = n_seqs, cu_seqlens not read). */
+int gdn_scan_step(const GDNScan *args, void *stream);
+
+/* Root-mean-square norm of a batch's rows, each head on its own, with the
+ * residual in front of it and a gate.  In FP32, with s(z) = z / (1 + exp(-z)):
+ *   h = x + residual;  sum = h, rounded to dtype
+ *   u = h, where gate_first != 0: h s(gate)
+ *   y = u / sqrt(mean of u^2 over the head + eps) weight, where gate_first is 0: times s(gate)
+ *   out = y rounded to dtype, or, where fp8 != 0, y / scale rounded to E4M3 (OCP, no
+ *   infinities), scale the largest |y| of the block / 448 (1 where that is below
+ *   2^-109): of `block` values along the row, or of all the row's where block = 0
+ * The norm is of h as it is, not as sum holds it.
+ *   rows       [rows][heads][dim]; heads * dim at most 2^20, contiguous in a row
+ *   block      0, 32, 64 or 128, a divisor of dim
+ *   *_stride   elements between rows (with one row not looked at).  Any alignment
+ *              of an element's
+ *   weight     FP32 [dim], or [heads][dim] where weight_heads != 0; NULL: 1
+ *   residual, gate   NULL: none; sum NULL: not wanted
+ *   out        may be x, residual or gate of an equal stride where it is of dtype;
+ *   sum        may be x or residual of an equal stride; otherwise neither overlaps an
+ *              input nor the other
+ *   scales     FP32 [rows][heads * dim / block, or 1], where fp8 != 0
+ * A square beyond FP32's range makes its head's y 0.  A block with a value that
+ * is not finite: its scale is an infinity or NaN, its values 0 or NaN. */
+typedef struct {
+    int32_t dtype;              /* GDN_DTYPE_* of x, residual, gate, sum and out */
+    uint32_t rows, heads, dim;
+    int32_t gate_first, weight_heads, fp8;
+    uint32_t block;
+    float eps;
+    uint32_t reserved;
+    int64_t x_stride, residual_stride, gate_stride, out_stride, sum_stride;
+    const void *x, *residual, *gate;
+    const float *weight;
+    void *out, *sum;
+    float *scales;
+} GDNNorm;
+int gdn_rms_norm(const GDNNorm *args, void *stream);
+
 /* Penalties, biases and masks on a batch of logits, each row on its own.  For
  * token t of row r, in FP32, rounded once to dtype:
  *   x = logits[r][t]
