@@ -3,6 +3,8 @@
 // gdn_scan_step (one token of every sequence).
 #include <hip/hip_runtime.h>
 
+#include <type_traits>
+
 #include "gdn_amd.h"
 #include "gdn_device.h"
 #include "gdn_internal.h"
@@ -41,141 +43,166 @@ __device__ __forceinline__ float step_size(const GDNScan &p, float h) {
 // most n_tokens / seg.
 __device__ __forceinline__ int cuts_of(const Span &sp, int seg) { return sp.n > 0 ? (sp.n - 1) / seg : 0; }
 
-template <class T, int N, int NW>
+template <class T, int N, int NW, bool kY>
 struct Lds {
     static constexpr int C = kChunk<T>, NT = T::kTerms, kTri = C == 64 ? 6 : 2;
-    // 16-byte units of a row, the last of them padding: rows four banks apart
-    static constexpr int kRow = N / 8 + 1, kXRow = 2 * NW + 1;
-    u32x4 b[NT][C][kRow], c[NT][C][kRow], x[NT][C][kXRow];
-    u32x4 m[kTri][kOutTerms<T>][64];
-    f32x4 sc[NW][C];
-    float eg[NW][C];
+    // 16-byte units of a row with its padding: B's and C's rows eight banks apart,
+    // which keeps their rows' reads apart and halves the conflicts of B's transposed ones
+    static constexpr int kRow = N / 8 + 2, kXRow = 2 * NW + 1;
+    u32x4 b[NT][C][kRow], c[kY ? NT : 0][C][kRow], x[NT][C][kXRow];
+    u32x4 m[kY ? kTri : 0][kOutTerms<T>][64];
+    // of a block of NW chunks, by token: G's whole powers of two and the rest, the
+    // step h, exp(G), exp(G_last - G) h; with E_j the G in front of 16-token tile j,
+    // exp(G - E) of the token's own tile and exp(E_j - G) h for the tiles behind it
+    struct Steps {
+        int whole[C];
+        float rest[C], step[C], eg[C], left[C], in[C], to[C / 16 - 1][C];
+    } s[NW];
 };
 // Where a 16 x 32 tile of a chunk's lower triangular matrix is kept: row tile j,
 // column step i.
 __device__ __forceinline__ constexpr int tri_tile(int j, int i) { return j < 2 ? j : 2 * j - 2 + i; }
 
+// The workspace: by place, the states behind cut segments, the starts of cut
+// sequences at their first place (NULL where their slots are not written), decays.
+struct Pools {
+    float *states, *starts, *decays;
+};
+
+// Four values as BF16 terms, each the bits the ones before it left, so three are
+// exact.  (An infinity or NaN has a NaN term.)
+template <int K>
+__device__ __forceinline__ void split(const f32x4 x, u32x2 (&p)[K]) {
+    uint32_t u[4];
+    float r[4] = {x.x, x.y, x.z, x.w};
+#pragma unroll
+    for (int k = 0; k < K; ++k) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) u[i] = f2u(r[i]);
+        if (k == K - 1 && K < 3) {  // what is left is rounded
+            p[k].x = cvt_pk(r[0], r[1]);
+            p[k].y = cvt_pk(r[2], r[3]);
+        } else {
+            p[k].x = __builtin_amdgcn_perm(u[1], u[0], 0x07060302u);
+            p[k].y = __builtin_amdgcn_perm(u[3], u[2], 0x07060302u);
+        }
+        if (k < K - 1) {
+#pragma unroll
+            for (int i = 0; i < 4; ++i) r[i] = r[i] - u2f(u[i] & 0xffff0000u);
+        }
+    }
+}
+
+// Waves a SIMD that the LDS leaves room for, at most two.
+template <class T, int N, int NW, bool kY>
+constexpr int kPerSimd = NW == 8 || sizeof(Lds<T, N, NW, kY>) <= (80 << 10) ? 2 : 1;
+
 // A segment's chunks in order, for a head's 16 NW columns, 16 a wave.  With G the
 // running log decay of a chunk (sums in 64 bits) and h the steps:
-//   y = exp(G) C S + M x + D x,  M[m][s] = exp(G_m - G_s) h_s (C_m . B_s), s <= m
-//   S' = exp(G_last) S + B^T (exp(G_last - G) h x)
+//   y = exp(G) C S + M x,  M[m][s] = exp(G_m - G_s) h_s (C_m . B_s), s <= m, and D on
+//   the diagonal;  S' = exp(G_last) S + B^T (exp(G_last - G) h x)
 // Products are BF16 matrix instructions on the terms that the operands split into.
 // A wave's state is the accumulator tiles of its update, and lies so that it is
-// also the B operand of C S: of a 32-row step, lane l holds rows 8 (l / 16) .. + 7 of
-// column l % 16, the first four in one tile, the others in the next.  M's tiles are
-// formed transposed, B C^T, spread over the waves: an accumulator is then half an A
+// also an operand of C S: of a 32-row step, lane l holds rows 8 (l / 16) .. + 7 of
+// column l % 16, the first four in one tile, the others in the next.  y is formed
+// transposed, a lane's token with four columns in a row.  M's tiles are formed
+// transposed too, B C^T, spread over the waves: an accumulator is then half an
 // operand of M x as it is.  x and B^T are read transposed (ds_read_b64_tr_b16).  The
-// steps and decays of NW chunks are formed at a time, a chunk a wave.  The next
-// chunk's rows are on their way into registers meanwhile.
-//   pass 0   the segments with a later one: the first whole, of the others the
-//            state they add to zero and their decay
-//   pass 1   the others whole, from the states behind the segments before them
-// so the slot of a sequence is read before pass 1 writes it, or by the workgroup
-// that does.
-template <class T, int N, int NW>
-__global__ __launch_bounds__(64 * NW, 2) void k_scan_segment(GDNScan p, float *__restrict__ states,
-                                                             float *__restrict__ decays, int seg, int pass, int units) {
-    using L = Lds<T, N, NW>;
+// steps and decays of NW chunks are formed at a time, a chunk a wave.  Two barriers a
+// chunk.  A wave is bound by the latency of what it waits for, so a step's operands
+// are read a step ahead, the next chunk's rows loaded one by one between the
+// products, and the splitting of the state and of x goes between them too.
+// Two kernels of it:
+//   kY false  the segments with a later one: the state that each leaves, the first
+//             of a sequence from its start, the others from zero; their decays; and
+//             the start itself where the sequence's slot is written
+//   kY true   all segments, from the states behind the ones before them
+template <class T, int N, int NW, bool kY>
+__global__ __launch_bounds__(64 * NW, (kPerSimd<T, N, NW, kY>)) void k_scan_segment(GDNScan p, Pools ws, int seg, int units) {
+    using L = Lds<T, N, NW, kY>;
     constexpr int C = L::C, NT = L::NT, MT = C / 16, JT = C / 32, KS = N / 32, OT = kOutTerms<T>, kThreads = 64 * NW;
-    constexpr int kB = C * (N / 8), kX = C * 2 * NW;  // 16-byte units (of 16-bit values) of a chunk's rows
+    constexpr int kCols = 16 * NW, kB = C * (N / 8), kX = C * (kCols / 8);  // 16-byte units (of 16-bit values) of a chunk's rows
     constexpr int kBr = (kB + kThreads - 1) / kThreads, kXr = (kX + kThreads - 1) / kThreads;
     __shared__ L lds;
     const f32x4 zero = {0.0f, 0.0f, 0.0f, 0.0f};
     const int t = threadIdx.x, w = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63, li = lane & 15, kk = lane >> 4;
     // the column groups of a (segment, head) share its rows of B and C: one XCD's
     // (workgroups go to the eight in turn)
-    const int groups = (int)p.head_dim / (16 * NW), bx = blockIdx.x >> 3;
+    const int groups = (int)p.head_dim / kCols, bx = blockIdx.x >> 3;
     const int unit = (bx / groups) * 8 + (blockIdx.x & 7), cg = bx % groups;
     if (unit >= units) return;
     const int head = unit % (int)p.n_heads, place = unit / (int)p.n_heads, group = head / (int)(p.n_heads / p.n_groups);
     const int seq = last_at_most((int)p.n_seqs, place,
-                                 [&](int i) { return span_of(p, i).first / seg + (pass ? i : 0); });
+                                 [&](int i) { return span_of(p, i).first / seg + (kY ? i : 0); });
     Span sp = span_of(p, seq);
     sp.first = __builtin_amdgcn_readfirstlane(sp.first);
     sp.n = __builtin_amdgcn_readfirstlane(sp.n);
     const int slot = __builtin_amdgcn_readfirstlane(slot_of(p, seq));
-    const int cuts = cuts_of(sp, seg), base = sp.first / seg, c0 = place - base - (pass ? seq : 0);
-    if (slot < 0 || c0 < 0 || (pass ? c0 > cuts || (c0 == 0 && cuts > 0) : c0 >= cuts)) return;
-    const bool whole = pass || c0 == 0;
+    const int cuts = cuts_of(sp, seg), base = sp.first / seg, c0 = place - base - (kY ? seq : 0);
+    if (slot < 0 || c0 < 0 || c0 > cuts || (!kY && c0 == cuts)) return;
     const int row0 = sp.first + c0 * seg, n_rows = min(seg, sp.n - c0 * seg), chunks = (n_rows + C - 1) / C;
-    const int col = 16 * (NW * cg + w) + li;
-    const size_t head_at = (size_t)8 * kk * p.head_dim + col, tile = (size_t)N * p.head_dim;
+    const int col0 = kCols * cg + 16 * w;  // the wave's first column
+    const size_t head_at = (size_t)8 * kk * p.head_dim + col0 + li, tile = (size_t)N * p.head_dim;
     auto at_of = [&](int s, int a, int r) { return head_at + (size_t)(32 * s + 4 * a + r) * p.head_dim; };
-    f32x4 S[KS][2];
-    {
-        const float *from = c0 > 0 ? (pass ? states + ((size_t)(base + c0 - 1) * p.n_heads + head) * tile : nullptr)
-                            : p.state_in ? p.state_in + ((size_t)slot * p.n_heads + head) * tile
-                                         : nullptr;
-#pragma unroll
-        for (int s = 0; s < KS; ++s) S[s][0] = S[s][1] = zero;
-        if (from) {
-#pragma unroll
-            for (int s = 0; s < KS; ++s)
-#pragma unroll
-                for (int a = 0; a < 2; ++a)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) S[s][a][r] = from[at_of(s, a, r)];
-        }
-    }
 
     constexpr uint32_t kSize = T::kWords / 2;  // bytes of a value
     Raw8<T> breg[kBr], creg[kBr], xreg[kXr];
     auto rows_at = [&](const void *x, int64_t stride, int row, int first) __attribute__((always_inline)) {
         return static_cast<const char *>(x) + ((size_t)row * stride + first) * kSize;
     };
-    // rows past the segment's end: its last one, in bounds, put as zeros
-    auto fetch = [&](int c) __attribute__((always_inline)) {
-        const int n = n_rows - C * c, row = row0 + C * c;
+    // The part'th of `parts` parts of a chunk's loads.  Rows past the segment's end: its
+    // last one, in bounds, put as zeros.
+    constexpr int kLoads = kBr + kXr + (kY ? kBr : 0);
+    auto fetch = [&](int c, int part, int parts) __attribute__((always_inline)) {
+        const int last_row = n_rows - C * c - 1, row = row0 + C * c;
+        auto load = [&](Raw8<T> &to, const char *from, int64_t stride, int i, int per) __attribute__((always_inline)) {
+            const uint32_t step = (uint32_t)stride * kSize, at = 8 * kSize * (t % per);
+            const uint32_t r = (uint32_t)(i * kThreads + t) / per;
+            to.load(from + min((uint32_t)__umul24(r, step) + at, (uint32_t)__umul24((uint32_t)last_row, step) + at), 0);
+        };
         const char *bp = rows_at(p.b, p.b_stride, row, group * N), *cp = rows_at(p.c, p.c_stride, row, group * N),
-                   *xp = rows_at(p.x, p.x_stride, row, head * (int)p.head_dim + 16 * NW * cg);
-        const uint32_t bs = (uint32_t)p.b_stride * kSize, cs = (uint32_t)p.c_stride * kSize, xs = (uint32_t)p.x_stride * kSize;
+                   *xp = rows_at(p.x, p.x_stride, row, head * (int)p.head_dim + kCols * cg);
 #pragma unroll
-        for (int i = 0; i < kBr; ++i) {
-            const int u = i * kThreads + t, r = min(u / (N / 8), n - 1), at = 8 * kSize * (u % (N / 8));
-            if (kB % kThreads == 0 || u < kB) {
-                breg[i].load(bp + (__umul24(r, bs) + at), 0);
-                if (whole) creg[i].load(cp + (__umul24(r, cs) + at), 0);
+        for (int i = 0; i < kLoads; ++i)
+            if (i * parts / kLoads == part) {
+                if (i < kBr) load(breg[i], bp, p.b_stride, i, N / 8);
+                else if (i < kBr + kXr) load(xreg[i - kBr], xp, p.x_stride, i - kBr, kCols / 8);
+                else if constexpr (kY) load(creg[i - kBr - kXr], cp, p.c_stride, i - kBr - kXr, N / 8);
             }
-        }
-#pragma unroll
-        for (int i = 0; i < kXr; ++i) {
-            const int u = i * kThreads + t, r = min(u / (2 * NW), n - 1), at = 8 * kSize * (u % (2 * NW));
-            if (kX % kThreads == 0 || u < kX) xreg[i].load(xp + (__umul24(r, xs) + at), 0);
-        }
     };
     auto put_rows = [&](int c) __attribute__((always_inline)) {
         const int n = n_rows - C * c;
-        u32x4 e[NT];
+        if (n < C) {
 #pragma unroll
-        for (int i = 0; i < kBr; ++i) {
-            const int u = i * kThreads + t, r = u / (N / 8);
-            if (kB % kThreads != 0 && u >= kB) break;
-            if (r >= n) {
-                breg[i].zero();
-                creg[i].zero();
-            }
-            breg[i].terms(e);
+            for (int i = 0; i < kBr; ++i)
+                if ((i * kThreads + t) / (N / 8) >= n) {
+                    breg[i].zero();
+                    if constexpr (kY) creg[i].zero();
+                }
 #pragma unroll
-            for (int q = 0; q < NT; ++q) lds.b[q][r][u % (N / 8)] = e[q];
-            if (whole) {
-                creg[i].terms(e);
-#pragma unroll
-                for (int q = 0; q < NT; ++q) lds.c[q][r][u % (N / 8)] = e[q];
-            }
+            for (int i = 0; i < kXr; ++i)
+                if ((i * kThreads + t) / (kCols / 8) >= n) xreg[i].zero();
         }
+        auto put = [&](auto &to, const Raw8<T> &from, int i, int per, int total) __attribute__((always_inline)) {
+            const int u = i * kThreads + t;
+            if (total % kThreads != 0 && u >= total) return;
+            u32x4 e[NT];
+            from.terms(e);
 #pragma unroll
-        for (int i = 0; i < kXr; ++i) {
-            const int u = i * kThreads + t, r = u / (2 * NW);
-            if (kX % kThreads != 0 && u >= kX) break;
-            if (r >= n) xreg[i].zero();
-            xreg[i].terms(e);
+            for (int q = 0; q < NT; ++q) to[q][u / per][u % per] = e[q];
+        };
 #pragma unroll
-            for (int q = 0; q < NT; ++q) lds.x[q][r][u % (2 * NW)] = e[q];
+        for (int i = 0; i < kBr; ++i) put(lds.b, breg[i], i, N / 8, kB);
+#pragma unroll
+        for (int i = 0; i < kXr; ++i) put(lds.x, xreg[i], i, kCols / 8, kX);
+        if constexpr (kY) {
+#pragma unroll
+            for (int i = 0; i < kBr; ++i) put(lds.c, creg[i], i, N / 8, kB);
         }
     };
     // wave w's chunk of a block of NW: steps, decays
     const double rate = (double)p.A[head] * 1.44269504088896340736;
-    const float skip = p.D ? p.D[head] : 0.0f;
+    const float skip = kY && p.D ? p.D[head] : 0.0f;
     float dt = 0.0f;
     auto fetch_dt = [&](int c) __attribute__((always_inline)) {
         const int m = C * (c + w) + lane;
@@ -187,19 +214,73 @@ __global__ __launch_bounds__(64 * NW, 2) void k_scan_segment(GDNScan p, float *_
         // held to a size whose differences stay numbers, far beyond FP32's powers
         double g = (double)h * rate;
         g = g < -1e5 ? -1e5 : g > 1e5 ? 1e5 : g;
-        const double sum = wave_scan64(in ? g : 0.0), last = __shfl(sum, 63), n = __builtin_rint(sum);
+        const double sum = wave_scan64(in ? g : 0.0), n = __builtin_rint(sum);
+        auto of_lane = [&](int l) {
+            const uint64_t u = __builtin_bit_cast(uint64_t, sum);
+            const uint32_t lo = (uint32_t)__builtin_amdgcn_readlane((int)u, l),
+                           hi = (uint32_t)__builtin_amdgcn_readlane((int)(u >> 32), l);
+            return __builtin_bit_cast(double, ((uint64_t)hi << 32) | lo);
+        };
+        const double last = of_lane(C - 1);
+        double front = 0.0;
+        if constexpr (kY) {
+#pragma unroll
+            for (int j = 1; j < MT; ++j) {
+                const double e = of_lane(16 * j - 1);
+                if (lane >= 16 * j) front = e;
+                else lds.s[w].to[j - 1][lane] = exp2_of(e - sum) * h;
+            }
+            if (lane < C) lds.s[w].in[lane] = exp2_of(sum - front);
+        }
         if (lane < C) {
-            lds.sc[w][lane] = (f32x4){(float)(sum - n), u2f((uint32_t)(int)n), h, exp2_of(last - sum) * h};
-            lds.eg[w][lane] = exp2_of(sum);
+            lds.s[w].whole[lane] = (int)n;
+            lds.s[w].rest[lane] = (float)(sum - n);
+            lds.s[w].step[lane] = h;
+            lds.s[w].eg[lane] = exp2_of(sum);
+            lds.s[w].left[lane] = exp2_of(last - sum) * h;
         }
     };
 
     if (chunks > 0) {
-        fetch(0);
         fetch_dt(0);
+        fetch(0, 0, 1);
+    }
+    f32x4 S[KS][2];
+    auto each_state = [&](auto &&f) __attribute__((always_inline)) {
+#pragma unroll
+        for (int s = 0; s < KS; ++s)
+#pragma unroll
+            for (int a = 0; a < 2; ++a)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) f(s, a, r);
+    };
+    auto put_state = [&](float *to) __attribute__((always_inline)) {
+        each_state([&](int s, int a, int r) __attribute__((always_inline)) { to[at_of(s, a, r)] = S[s][a][r]; });
+    };
+    // the workspace's states lie as the registers do, a wave's together
+    const size_t kept = (size_t)(col0 / 16) * (16 * N) + 4 * lane;
+    auto keep = [&](float *to) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < 2 * KS; ++i) *reinterpret_cast<f32x4 *>(to + kept + 256 * i) = S[i / 2][i % 2];
+    };
+    {
+        const size_t first = ((size_t)base * p.n_heads + head) * tile;  // in the pools of places
+        const float *ours = !kY          ? nullptr
+                            : c0 > 0     ? ws.states + first + (size_t)(c0 - 1) * p.n_heads * tile
+                            : cuts > 0   ? ws.starts ? ws.starts + first : nullptr
+                                         : nullptr;
+        each_state([&](int s, int a, int r) __attribute__((always_inline)) { S[s][a][r] = 0.0f; });
+        if (ours) {
+#pragma unroll
+            for (int i = 0; i < 2 * KS; ++i) S[i / 2][i % 2] = *reinterpret_cast<const f32x4 *>(ours + kept + 256 * i);
+        } else if (c0 == 0 && p.state_in) {
+            const float *from = p.state_in + ((size_t)slot * p.n_heads + head) * tile;
+            each_state([&](int s, int a, int r) __attribute__((always_inline)) { S[s][a][r] = from[at_of(s, a, r)]; });
+            if (!kY && ws.starts) keep(ws.starts + first);
+        }
     }
     // of M's tiles on the diagonal, the half above it
-    if (w == 0) {
+    if (kY && w == 0) {
 #pragma unroll
         for (int j = 0; j < MT; j += 2)
 #pragma unroll
@@ -207,111 +288,65 @@ __global__ __launch_bounds__(64 * NW, 2) void k_scan_segment(GDNScan p, float *_
                 reinterpret_cast<u32x2 *>(&lds.m[tri_tile(j, j / 2)][q][lane])[1] = (u32x2){0u, 0u};
     }
     float decay = 1.0f;
+    if (chunks > 0) {
+        put_steps(0);
+        put_rows(0);
+        fetch_dt(NW);
+        __syncthreads();
+    }
     for (int c = 0; c < chunks; ++c) {
         const int n = min(C, n_rows - C * c), cb = c % NW;
-        put_rows(c);
-        if (cb == 0) {
-            put_steps(c);
-            fetch_dt(c + NW);
-        }
-        __syncthreads();
-        if (c + 1 < chunks) fetch(c + 1);
-        const f32x4(&sc)[C] = lds.sc[cb];
-        const float(&eg)[C] = lds.eg[cb];
+        const int next = min(c + 1, chunks - 1);  // (the last chunk's rows are loaded again, unused)
+        const typename L::Steps &sc = lds.s[cb];
         f32x4 y[MT];
-        if (whole) {
-            // M's tiles, two halves of a step
-            for (int q = w; q < MT * (MT + 1) / 2; q += NW) {
-                const int j = q < 1 ? 0 : q < 3 ? 1 : q < 6 ? 2 : 3, i = q - j * (j + 1) / 2;
-                f32x4 z[2] = {zero, zero};
+        u32x4 xb[JT][NT], xo[JT][3];
+        // the value of a 16-bit operand's terms
+        auto value = [&](const uint32_t(&u)[NT], int r) __attribute__((always_inline)) {
+            auto term = [&](int q) { return u2f(r % 2 ? u[q] & 0xffff0000u : u[q] << 16); };
+            float v = term(NT - 1);
 #pragma unroll
-                for (int s = 0; s < KS; ++s) {
-                    u32x4 a[NT], b[NT];
+            for (int q = NT - 2; q >= 0; --q) v += term(q);
+            return v;
+        };
+        // x as an operand: of a 32-token step, tokens 4 (l / 16) .. + 3 and those 16 on
+        auto read_x = [&]() __attribute__((always_inline)) {
 #pragma unroll
-                    for (int k = 0; k < NT; ++k) {
-                        a[k] = lds.b[k][16 * i + li][4 * s + kk];
-                        b[k] = lds.c[k][16 * j + li][4 * s + kk];
-                    }
-                    for_terms<NT, NT>([&](int k, int l) __attribute__((always_inline)) { z[s & 1] = mfma_bf16(a[k], b[l], z[s & 1]); });
+            for (int j = 0; j < JT; ++j)
+#pragma unroll
+                for (int q = 0; q < NT; ++q) {
+                    const int m = 32 * j + 4 * kk + (li >> 2), u = 4 * w + (li & 3);
+                    const u32x2 lo = read_transposed(reinterpret_cast<const u32x2 *>(&lds.x[q][m][0]) + u);
+                    const u32x2 hi = read_transposed(reinterpret_cast<const u32x2 *>(&lds.x[q][m + 16][0]) + u);
+                    xb[j][q] = (u32x4){lo.x, lo.y, hi.x, hi.y};
                 }
-                const f32x4 to = sc[16 * j + li];
-                f32x4 v;
+        };
+        // the terms of its values times exp(G_last - G) h, the k'th four
+        auto weigh = [&](int k) __attribute__((always_inline)) {
+            const int j = k / 2, h = k % 2;
+            f32x4 v;
 #pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const f32x4 of = sc[16 * i + 4 * kk + r];
-                    // (above the diagonal a power that makes it zero, not a branch)
-                    const int n2 = i < j || 4 * kk + r <= li ? (int)f2u(to.y) - (int)f2u(of.y) : -1000;
-                    const float e = __builtin_ldexpf(__builtin_amdgcn_exp2f(to.x - of.x), n2) * of.z;
-                    v[r] = e * (z[0][r] + z[1][r]);
-                }
-                u32x2 e[3];
-                split3(v, e);
+            for (int r = 0; r < 4; ++r) {
+                uint32_t u[NT];
 #pragma unroll
-                for (int k = 0; k < OT; ++k) reinterpret_cast<u32x2 *>(&lds.m[tri_tile(j, i / 2)][k][lane])[i & 1] = e[k];
+                for (int q = 0; q < NT; ++q) u[q] = xb[j][q][2 * h + r / 2];
+                v[r] = value(u, r) * sc.left[32 * j + 16 * h + 4 * kk + r];
             }
+            u32x2 e[3];
+            split(v, e);
 #pragma unroll
-            for (int i = 0; i < MT; ++i) y[i] = zero;
-#pragma unroll
-            for (int s = 0; s < KS; ++s) {
-                u32x2 lo[3], hi[3];
-                split3(S[s][0], lo);
-                split3(S[s][1], hi);
-                u32x4 sb[OT], ca[MT][NT];
-#pragma unroll
-                for (int q = 0; q < OT; ++q) sb[q] = (u32x4){lo[q].x, lo[q].y, hi[q].x, hi[q].y};
-#pragma unroll
-                for (int i = 0; i < MT; ++i)
-#pragma unroll
-                    for (int q = 0; q < NT; ++q) ca[i][q] = lds.c[q][16 * i + li][4 * s + kk];
-                for_terms<NT, OT>([&](int a, int b) __attribute__((always_inline)) {
-#pragma unroll
-                    for (int i = 0; i < MT; ++i) y[i] = mfma_bf16(ca[i][a], sb[b], y[i]);
-                });
+            for (int q = 0; q < 3; ++q) {
+                xo[j][q][2 * h] = e[q].x;
+                xo[j][q][2 * h + 1] = e[q].y;
             }
+        };
+        // operands of a 32-row step: C's rows, B^T's, the state's terms
+        auto read_c = [&](int s, u32x4(&ca)[MT][NT]) __attribute__((always_inline)) {
 #pragma unroll
             for (int i = 0; i < MT; ++i)
 #pragma unroll
-                for (int r = 0; r < 4; ++r) y[i][r] *= eg[16 * i + 4 * kk + r];
-            __syncthreads();
-        }
-        // x as a B operand: of a 32-token step, tokens 4 (l / 16) .. + 3 and those 16 on
-        u32x4 xb[JT][NT], xo[JT][3];
-        f32x4 xv[MT];
-#pragma unroll
-        for (int j = 0; j < JT; ++j)
-#pragma unroll
-            for (int q = 0; q < NT; ++q) {
-                const int m = 32 * j + 4 * kk + (li >> 2);
-                const u32x2 lo = read_transposed(reinterpret_cast<const u32x2 *>(&lds.x[q][m][0]) + 4 * w + (li & 3));
-                const u32x2 hi = read_transposed(reinterpret_cast<const u32x2 *>(&lds.x[q][m + 16][0]) + 4 * w + (li & 3));
-                xb[j][q] = (u32x4){lo.x, lo.y, hi.x, hi.y};
-            }
-#pragma unroll
-        for (int j = 0; j < JT; ++j) {
-            u32x2 e[2][3];
-#pragma unroll
-            for (int h = 0; h < 2; ++h) {
-                f32x4 v = zero;
-#pragma unroll
-                for (int q = NT - 1; q >= 0; --q)
-#pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const uint32_t u = xb[j][q][2 * h + r / 2];
-                        v[r] += u2f(r % 2 ? u & 0xffff0000u : u << 16);
-                    }
-                xv[2 * j + h] = v;
-#pragma unroll
-                for (int r = 0; r < 4; ++r) v[r] *= sc[32 * j + 16 * h + 4 * kk + r].w;
-                split3(v, e[h]);
-            }
-#pragma unroll
-            for (int q = 0; q < 3; ++q) xo[j][q] = (u32x4){e[0][q].x, e[0][q].y, e[1][q].x, e[1][q].y};
-        }
-        const float dn = eg[C - 1];
-        decay *= dn;
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-            u32x4 a[2][JT][NT];
+                for (int q = 0; q < NT; ++q) ca[i][q] = lds.c[q][16 * i + li][4 * s + kk];
+        };
+        auto read_b = [&](int s, u32x4(&a)[2][JT][NT]) __attribute__((always_inline)) {
 #pragma unroll
             for (int h = 0; h < 2; ++h)
 #pragma unroll
@@ -323,55 +358,202 @@ __global__ __launch_bounds__(64 * NW, 2) void k_scan_segment(GDNScan p, float *_
                         const u32x2 hi = read_transposed(reinterpret_cast<const u32x2 *>(&lds.b[q][m + 16][0]) + u);
                         a[h][j][q] = (u32x4){lo.x, lo.y, hi.x, hi.y};
                     }
+        };
+        auto terms_of = [&](int s, u32x4(&sb)[OT]) __attribute__((always_inline)) {
+            u32x2 lo[OT], hi[OT];
+            split(S[s][0], lo);
+            split(S[s][1], hi);
+#pragma unroll
+            for (int q = 0; q < OT; ++q) sb[q] = (u32x4){lo[q].x, lo[q].y, hi[q].x, hi[q].y};
+        };
+        // what stands between two of these: the loads first, then products with some
+        // of the rest behind each
+        auto mix = [&](auto products, auto others) __attribute__((always_inline)) {
+#pragma unroll
+            for (int i = 0; i < decltype(products)::value; ++i) {
+                __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+                __builtin_amdgcn_sched_group_barrier(0x002, decltype(others)::value, 0);
+            }
+            __builtin_amdgcn_sched_barrier(0);
+        };
+        using std::integral_constant;
+        constexpr int kParts = kY ? 2 * KS : KS;
+        u32x4 ab[2][2][JT][NT];
+        if constexpr (kY) {
+            // C_m . B_s of row tile j (a lane's token m), column tile i (its four s)
+            struct Operands {
+                u32x4 a[KS][NT], b[KS][NT];
+            };
+            auto read_tile = [&](int j, int i, Operands &o) __attribute__((always_inline)) {
+#pragma unroll
+                for (int s = 0; s < KS; ++s)
+#pragma unroll
+                    for (int k = 0; k < NT; ++k) {
+                        o.a[s][k] = lds.b[k][16 * i + li][4 * s + kk];
+                        o.b[s][k] = lds.c[k][16 * j + li][4 * s + kk];
+                    }
+            };
+            auto products = [&](const Operands &o) __attribute__((always_inline)) {
+                f32x4 z[2] = {zero, zero};
+#pragma unroll
+                for (int s = 0; s < KS; ++s)
+                    for_terms<NT, NT>(
+                        [&](int k, int l) __attribute__((always_inline)) { z[s & 1] = mfma_bf16(o.a[s][k], o.b[s][l], z[s & 1]); });
+                return z[0] + z[1];
+            };
+            auto put_tile = [&](int j, int i, const f32x4 v) __attribute__((always_inline)) {
+                u32x2 e[OT];
+                split(v, e);
+#pragma unroll
+                for (int k = 0; k < OT; ++k) reinterpret_cast<u32x2 *>(&lds.m[tri_tile(j, i / 2)][k][lane])[i & 1] = e[k];
+            };
+            // M's tiles: on the diagonal a power for each value (above it one that
+            // makes it zero, not a branch)
+            auto diagonal = [&](int j, const Operands &o) __attribute__((always_inline)) {
+                const int to = 16 * j + li, of = 16 * j + 4 * kk;
+                const int n_to = sc.whole[to];
+                const float f_to = sc.rest[to];
+                f32x4 e;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int n2 = 4 * kk + r <= li ? n_to - sc.whole[of + r] : -1000;
+                    e[r] = __builtin_ldexpf(__builtin_amdgcn_exp2f(f_to - sc.rest[of + r]), n2) * sc.step[of + r];
+                }
+                f32x4 v = products(o) * e;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) v[r] += 4 * kk + r == li ? skip : 0.0f;
+                put_tile(j, j, v);
+            };
+            // below it what falls in front of the row tile and inside it
+            auto row_of = [](int q) { return q < 1 ? 1 : q < 3 ? 2 : 3; };
+            auto column_of = [&](int q) { return q - row_of(q) * (row_of(q) - 1) / 2; };
+            auto below = [&](int q, const Operands &o) __attribute__((always_inline)) {
+                const int j = row_of(q), i = column_of(q);
+                const float in = sc.in[16 * j + li];
+                f32x4 e;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) e[r] = in * sc.to[j - 1][16 * i + 4 * kk + r];
+                put_tile(j, i, products(o) * e);
+            };
+            // spread over the waves
+            constexpr int kBelow = MT * (MT - 1) / 2;
+            Operands o[2];
+            if constexpr (MT == NW && KS * NT <= 4) {
+                // ten tiles, three a wave (two waves have one of theirs twice), the next
+                // one's operands read ahead
+                const int q = w < kBelow - NW ? NW + w : w;
+                read_tile(row_of(q), column_of(q), o[0]);
+                read_tile(row_of(w), column_of(w), o[1]);
+                below(q, o[0]);
+                read_tile(w, w, o[0]);
+                below(w, o[1]);
+                diagonal(w, o[0]);
+            } else {
+                constexpr int kFirst = MT >= NW ? 0 : MT, kEach = NW - kFirst;
+                if (w < MT) {
+                    read_tile(w, w, o[0]);
+                    diagonal(w, o[0]);
+                }
+#pragma unroll
+                for (int from = 0; from < kBelow; from += kEach) {
+                    const int q = from + w - kFirst;
+                    if (q >= from && q < kBelow) {
+                        read_tile(row_of(q), column_of(q), o[0]);
+                        below(q, o[0]);
+                    }
+                }
+            }
+            __builtin_amdgcn_sched_barrier(0);
+
+            // C S (y's lane l: token l % 16, columns 4 (l / 16) .. + 3) and x's terms
+            u32x4 ca[2][MT][NT], sb[2][OT];
+            read_c(0, ca[0]);
+            read_x();
+            terms_of(0, sb[0]);
+#pragma unroll
+            for (int i = 0; i < MT; ++i) y[i] = zero;
+#pragma unroll
+            for (int s = 0; s < KS; ++s) {
+                if (s + 1 < KS) read_c(s + 1, ca[(s + 1) & 1]);
+                else read_b(0, ab[0]);
+                fetch(next, s, kParts);
+                if (s + 1 < KS) terms_of(s + 1, sb[(s + 1) & 1]);
+#pragma unroll
+                for (int k = 0; k < 2 * JT; ++k)
+                    if (k * KS / (2 * JT) == s) weigh(k);
+                for_terms<OT, NT>([&](int a, int b) __attribute__((always_inline)) {
+#pragma unroll
+                    for (int i = 0; i < MT; ++i) y[i] = mfma_bf16(sb[s & 1][a], ca[s & 1][i][b], y[i]);
+                });
+                mix(integral_constant<int, MT * (OT == 3 ? 6 : NT == 2 ? 4 : 2)>(), integral_constant<int, 5>());
+            }
+        } else {
+            read_x();
+            read_b(0, ab[0]);
+#pragma unroll
+            for (int k = 0; k < 2 * JT; ++k) weigh(k);
+        }
+        const float dn = sc.eg[C - 1];
+        decay *= dn;
+#pragma unroll
+        for (int s = 0; s < KS; ++s) {
+            if (s + 1 < KS) read_b(s + 1, ab[(s + 1) & 1]);
+            fetch(next, kParts - KS + s, kParts);
             S[s][0] *= dn;
             S[s][1] *= dn;
             for_terms<NT, 3>([&](int e, int f) __attribute__((always_inline)) {
 #pragma unroll
                 for (int j = 0; j < JT; ++j)
 #pragma unroll
-                    for (int h = 0; h < 2; ++h) S[s][h] = mfma_bf16(a[h][j][e], xo[j][f], S[s][h]);
+                    for (int h = 0; h < 2; ++h) S[s][h] = mfma_bf16(ab[s & 1][h][j][e], xo[j][f], S[s][h]);
             });
+            __builtin_amdgcn_sched_barrier(0);
         }
-        if (whole) {
-            for_terms<OT, NT>([&](int a, int b) __attribute__((always_inline)) {
+        if constexpr (kY) {
 #pragma unroll
-                for (int j = 0; j < MT; ++j)
+            for (int i = 0; i < MT; ++i) y[i] *= sc.eg[16 * i + li];
+        }
+        __syncthreads();
+        // (B's, C's and x's rows and the steps are free from here, M's tiles from the
+        // next barrier; the rows before the stores, which would be waited for too)
+        if (c + 1 < chunks) {
+            put_rows(c + 1);
+            if (cb == NW - 1) {
+                put_steps(c + 1);
+                fetch_dt(c + 1 + NW);
+            }
+        }
+        if constexpr (kY) {
+            for_terms<NT, OT>([&](int a, int b) __attribute__((always_inline)) {
 #pragma unroll
-                    for (int i = 0; i <= j / 2; ++i) y[j] = mfma_bf16(lds.m[tri_tile(j, i)][a][lane], xb[i][b], y[j]);
+                for (int i = 0; i < JT; ++i)
+#pragma unroll
+                    for (int j = 2 * i; j < MT; ++j) y[j] = mfma_bf16(xb[i][a], lds.m[tri_tile(j, i)][b][lane], y[j]);
             });
-            char *yp = const_cast<char *>(rows_at(p.y, p.y_stride, row0 + C * c, head * (int)p.head_dim));
-            const uint32_t ys = (uint32_t)p.y_stride * kSize;
+            char *yp = const_cast<char *>(rows_at(p.y, p.y_stride, row0 + C * c, head * (int)p.head_dim + col0));
 #pragma unroll
-            for (int j = 0; j < MT; ++j)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) {
-                    const int m = 16 * j + 4 * kk + r;
-                    if (m < n) T::put(yp + (__umul24(m, ys) + col * kSize), 0, __builtin_fmaf(skip, xv[j][r], y[j][r]));
+            for (int j = 0; j < MT; ++j) {
+                const int m = 16 * j + li;
+                char *to = yp + ((uint32_t)__umul24((uint32_t)m, (uint32_t)p.y_stride * kSize) + 4 * kSize * kk);
+                if (m < n) {
+                    if constexpr (kSize == 4) *reinterpret_cast<f32x4 *>(to) = y[j];
+                    else *reinterpret_cast<u32x2 *>(to) = (u32x2){T::pack(y[j].x, y[j].y), T::pack(y[j].z, y[j].w)};
                 }
+            }
         }
         __syncthreads();
     }
-    float *to = nullptr;
-    if (pass) {
-        if (c0 == cuts && p.state_out) to = p.state_out + ((size_t)slot * p.n_heads + head) * tile;
+    if constexpr (kY) {
+        if (c0 == cuts && p.state_out) put_state(p.state_out + ((size_t)slot * p.n_heads + head) * tile);
     } else {
-        to = states + ((size_t)place * p.n_heads + head) * tile;
-        if (cg == 0 && t == 0) decays[(size_t)place * p.n_heads + head] = decay;
-    }
-    if (to) {
-#pragma unroll
-        for (int s = 0; s < KS; ++s)
-#pragma unroll
-            for (int a = 0; a < 2; ++a)
-#pragma unroll
-                for (int r = 0; r < 4; ++r) to[at_of(s, a, r)] = S[s][a][r];
+        keep(ws.states + ((size_t)place * p.n_heads + head) * tile);
+        if (cg == 0 && t == 0) ws.decays[(size_t)place * p.n_heads + head] = decay;
     }
 }
 
-// Between the passes: a sequence's states behind its segments from what each of
+// Between the two: a sequence's states behind its segments from what each of
 // them adds.  Grid (state values / 1024, heads, sequences in turn).
-__global__ __launch_bounds__(kT) void k_scan_join(GDNScan p, float *__restrict__ states, const float *__restrict__ decays,
-                                                  int seg) {
+__global__ __launch_bounds__(kT) void k_scan_join(GDNScan p, Pools ws, int seg) {
     const size_t tile = (size_t)p.state_dim * p.head_dim;
     const int head = blockIdx.y, at = (blockIdx.x * kT + (int)threadIdx.x) * 4;
     for (int seq = blockIdx.z; seq < (int)p.n_seqs; seq += gridDim.z) {
@@ -379,8 +561,8 @@ __global__ __launch_bounds__(kT) void k_scan_join(GDNScan p, float *__restrict__
         const int cuts = cuts_of(sp, seg);
         if (cuts < 2 || slot_of(p, seq) < 0) continue;
         const size_t unit = (size_t)(sp.first / seg) * p.n_heads + head;
-        float *s = states + unit * tile + at;
-        const float *d = decays + unit;
+        float *s = ws.states + unit * tile + at;
+        const float *d = ws.decays + unit;
         const size_t step = p.n_heads * tile;
         f32x4 v = *reinterpret_cast<const f32x4 *>(s);
         constexpr int kAhead = 8;  // segments on their way at once
@@ -463,15 +645,19 @@ __global__ __launch_bounds__(kT) void k_scan_step(GDNScan p) {
 // ------------------------------------------------------------ host
 
 bool dim_ok(uint32_t d) { return d == 64 || d == 128 || d == 256; }
-constexpr int kWaves = 4;
+// Waves of a workgroup, 16 columns each, and workgroups of a segment.
+int waves_of(const GDNScan *a) { return a->head_dim == 64 ? 4 : 8; }
+uint64_t groups_of(const GDNScan *a) { return (uint64_t)a->n_heads * a->head_dim / (16 * waves_of(a)); }
 
-// Tokens of a segment: see k_scan_segment.
+// Tokens of a segment: as many as give eleven waves a CU, in 128s, of which eight run
+// at a time (sequences end inside them), at most 1024.  4096 tokens in one sequence, 32
+// heads of 128 x 64, segments of 192, 256, 384, 512, 1024: 52, 43, 52, 49, 80 us; 8111 in
+// 24, 8 heads of 256 x 256, of 256, 320, 384, 512, 768: 146, 143, 126, 138, 158.  Shorter
+// than the state has rows the states' traffic is more than the rows'.
 int segment_of(const GDNScan *a) {
-    const uint64_t per = (uint64_t)a->n_heads * (a->head_dim / (16 * kWaves));
-    uint64_t seg = (a->n_tokens * per / 768 + 63) / 64 * 64;
-    const uint64_t least = 2 * a->state_dim;
-    seg = seg < least ? least : seg;
-    return (int)(seg > 1024 ? 1024 : seg);
+    const uint64_t even = (a->n_tokens * groups_of(a) * waves_of(a) / (11 * 256) + 127) / 128 * 128;
+    const uint64_t least = a->state_dim > 128 ? a->state_dim : 128;
+    return (int)(even > 1024 ? 1024 : even < least ? least : even);
 }
 size_t places(const GDNScan *a) { return a->n_tokens / (uint32_t)segment_of(a); }
 bool cut(const GDNScan *a) { return a->n_tokens > (uint32_t)segment_of(a); }
@@ -521,31 +707,44 @@ int check(const char *who, const GDNScan *a, bool packed) {
     return 0;
 }
 
-template <class T, int N>
-hipError_t launch_prefill(const GDNScan &a, void *ws, hipStream_t s) {
-    const int seg = segment_of(&a), groups = (int)a.head_dim / (16 * kWaves);
-    float *decays = static_cast<float *>(ws), *states = reinterpret_cast<float *>(static_cast<char *>(ws) + decay_bytes(&a));
-    auto pass = [&](int number, size_t n_places) {
-        const int units = (int)(n_places * a.n_heads);
-        return launch(k_scan_segment<T, N, kWaves>, dim3((unsigned)((units + 7) / 8 * 8 * groups)), dim3(64 * kWaves), 0, s, a,
-                      states, decays, seg, number, units);
-    };
+// The first segments' starts are kept where the slots that they come from are written.
+bool keeps_starts(const GDNScan *a) { return a->state_in && a->state_in == a->state_out; }
+size_t pool_bytes(const GDNScan *a) { return places(a) * a->n_heads * a->state_dim * a->head_dim * sizeof(float); }
+
+template <class T, int N, int NW, bool kY>
+hipError_t launch_segments(const GDNScan &a, const Pools &ws, int seg, size_t n_places, hipStream_t s) {
+    const int units = (int)(n_places * a.n_heads), groups = (int)a.head_dim / (16 * NW);
+    return launch(k_scan_segment<T, N, NW, kY>, dim3((unsigned)((units + 7) / 8 * 8 * groups)), dim3(64 * NW), 0, s, a, ws, seg,
+                  units);
+}
+template <class T, int N, int NW>
+hipError_t launch_prefill(const GDNScan &a, void *mem, hipStream_t s) {
+    const int seg = segment_of(&a);
+    char *at = static_cast<char *>(mem);
+    Pools ws = {nullptr, nullptr, nullptr};
     if (cut(&a)) {
-        hipError_t rc = pass(0, places(&a));
+        ws.decays = reinterpret_cast<float *>(at);
+        ws.states = reinterpret_cast<float *>(at + decay_bytes(&a));
+        if (keeps_starts(&a)) ws.starts = reinterpret_cast<float *>(at + decay_bytes(&a) + pool_bytes(&a));
+        hipError_t rc = launch_segments<T, N, NW, false>(a, ws, seg, places(&a), s);
         if (rc != hipSuccess) return rc;
         if (a.n_tokens > 2u * (uint32_t)seg) {
             rc = launch(k_scan_join, dim3(a.state_dim * a.head_dim / 1024, a.n_heads, a.n_seqs < 1024 ? a.n_seqs : 1024),
-                        dim3(kT), 0, s, a, states, static_cast<const float *>(decays), seg);
+                        dim3(kT), 0, s, a, ws, seg);
             if (rc != hipSuccess) return rc;
         }
     }
-    return pass(1, places(&a) + a.n_seqs);
+    return launch_segments<T, N, NW, true>(a, ws, seg, places(&a) + a.n_seqs, s);
+}
+template <class T, int N>
+hipError_t launch_prefill_w(const GDNScan &a, void *ws, hipStream_t s) {
+    return waves_of(&a) == 4 ? launch_prefill<T, N, 4>(a, ws, s) : launch_prefill<T, N, 8>(a, ws, s);
 }
 template <class T>
 hipError_t launch_prefill_n(const GDNScan &a, void *ws, hipStream_t s) {
-    return a.state_dim == 256   ? launch_prefill<T, 256>(a, ws, s)
-           : a.state_dim == 128 ? launch_prefill<T, 128>(a, ws, s)
-                                : launch_prefill<T, 64>(a, ws, s);
+    return a.state_dim == 256   ? launch_prefill_w<T, 256>(a, ws, s)
+           : a.state_dim == 128 ? launch_prefill_w<T, 128>(a, ws, s)
+                                : launch_prefill_w<T, 64>(a, ws, s);
 }
 template <class T, int N>
 hipError_t launch_step(const GDNScan &a, hipStream_t s) {
@@ -562,7 +761,7 @@ hipError_t launch_step_n(const GDNScan &a, hipStream_t s) {
 extern "C" size_t gdn_scan_prefill_workspace(const GDNScan *args) {
     using namespace gdn::scan;
     if (args == nullptr || !dim_ok(args->state_dim) || !dim_ok(args->head_dim) || !cut(args)) return 0;
-    return decay_bytes(args) + places(args) * args->n_heads * args->state_dim * args->head_dim * sizeof(float);
+    return decay_bytes(args) + pool_bytes(args) * (keeps_starts(args) ? 2 : 1);
 }
 
 extern "C" int gdn_scan_prefill(const GDNScan *args, void *workspace, size_t workspace_bytes, void *stream) {
@@ -571,8 +770,7 @@ extern "C" int gdn_scan_prefill(const GDNScan *args, void *workspace, size_t wor
     const int rc = check(who, args, true);
     if (rc != 0) return rc < 0 ? -1 : 0;
     // a grid has fewer than 2^32 threads along an axis
-    if (((uint64_t)places(args) + args->n_seqs + 8) * args->n_heads * (args->head_dim / (16 * kWaves)) >=
-        (1ull << 32) / (64 * kWaves))
+    if (((uint64_t)places(args) + args->n_seqs + 8) * groups_of(args) >= (1ull << 32) / (64 * (uint64_t)waves_of(args)))
         return gdn::refuse(who, "too many segments or heads for one launch");
     const size_t need = gdn_scan_prefill_workspace(args);
     if (need != 0 && (workspace == nullptr || (reinterpret_cast<uintptr_t>(workspace) & 15) != 0 || workspace_bytes < need))
