@@ -304,10 +304,6 @@ hipError_t launch_norm(const GDNNorm &a, hipStream_t s) {
     if (len <= 128) return launch_units<T, 16, 1, kFp8>(a, units, head_lanes, s);
     if (len <= 256) return launch_units<T, 32, 1, kFp8>(a, units, head_lanes, s);
     if (len <= 512) return launch_units<T, 64, 1, kFp8>(a, units, head_lanes, s);
-    if (units >= 1024) {
-        if (len <= 1024) return launch_units<T, 64, 2, kFp8>(a, units, head_lanes, s);
-        if (len <= 2048) return launch_units<T, 64, 4, kFp8>(a, units, head_lanes, s);
-    }
     if (len <= 2048) return launch_units<T, 256, 1, kFp8>(a, units, head_lanes, s);
     if (len <= 4096) return launch_units<T, 256, 2, kFp8>(a, units, head_lanes, s);
     return launch_units<T, 256, 4, kFp8>(a, units, head_lanes, s);

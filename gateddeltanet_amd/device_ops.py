@@ -28,6 +28,7 @@ _DTYPES = {torch.bfloat16: L.DTYPE_BF16, torch.float16: L.DTYPE_FP16, torch.floa
 
 
 _raw_stream = torch._C._cuda_getCurrentRawStream  # current_stream().cuda_stream without the objects, 2.7 us less
+_current_device = torch._C._cuda_getDevice  # (a tensor on a GPU is there: torch is initialised), 0.2 us less
 _F32, _I32 = torch.float32, torch.int32
 
 
@@ -88,7 +89,7 @@ def _entry(name: str):
 def _launch(dev: int, what: str, *args) -> None:
     """The entry point `what` (*args, stream) with GPU dev as the current one."""
     fn = _entry(what)
-    if torch.cuda.current_device() == dev:
+    if _current_device() == dev:
         rc = fn(*args, _raw_stream(dev))
     else:
         with torch.cuda.device(dev):
