@@ -288,25 +288,38 @@ __global__ __launch_bounds__(kT) void k_norm_long(GDNNorm p) {
 
 // ------------------------------------------------------------ host
 
+// A row with one scale for several heads is a unit where they take whole lanes, else
+// a head is.  Lanes of a unit, 0: k_norm_long's.
+bool joint(const GDNNorm *a) { return a->fp8 && a->block == 0 && a->heads > 1; }
+uint64_t units_of(const GDNNorm *a) { return joint(a) ? a->rows : (uint64_t)a->rows * a->heads; }
+uint64_t length_of(const GDNNorm *a) { return joint(a) ? (uint64_t)a->heads * a->dim : a->dim; }
+int lanes_of(const GDNNorm *a) {
+    const bool whole = !joint(a) || a->dim == 64 || a->dim == 128 || a->dim == 256 || a->dim == 512;
+    const uint64_t len = length_of(a);
+    return !whole || len > 8192 ? 0 : len <= 64 ? 8 : len <= 128 ? 16 : len <= 256 ? 32 : len <= 512 ? 64 : 256;
+}
+
 template <class T, int L, int V, bool kFp8>
 hipError_t launch_units(const GDNNorm &a, int units, int head_lanes, hipStream_t s) {
     return launch(k_norm<T, L, V, kFp8>, dim3((unsigned)((units + kT / L - 1) / (kT / L))), dim3(kT), 0, s, a, units, head_lanes);
 }
 template <class T, bool kFp8>
 hipError_t launch_norm(const GDNNorm &a, hipStream_t s) {
-    // a row with one scale for several heads is a unit where they take whole lanes
-    const bool joint = kFp8 && a.block == 0 && a.heads > 1;
-    const uint64_t len = joint ? (uint64_t)a.heads * a.dim : a.dim;
-    const bool whole = !joint || a.dim == 64 || a.dim == 128 || a.dim == 256 || a.dim == 512;
-    if (len > 8192 || !whole) return launch(k_norm_long<T, kFp8>, dim3(a.rows), dim3(kT), 0, s, a);
-    const int units = (int)(joint ? a.rows : (uint64_t)a.rows * a.heads), head_lanes = joint ? (int)a.dim / 8 : 0;
-    if (len <= 64) return launch_units<T, 8, 1, kFp8>(a, units, head_lanes, s);
-    if (len <= 128) return launch_units<T, 16, 1, kFp8>(a, units, head_lanes, s);
-    if (len <= 256) return launch_units<T, 32, 1, kFp8>(a, units, head_lanes, s);
-    if (len <= 512) return launch_units<T, 64, 1, kFp8>(a, units, head_lanes, s);
-    if (len <= 2048) return launch_units<T, 256, 1, kFp8>(a, units, head_lanes, s);
-    if (len <= 4096) return launch_units<T, 256, 2, kFp8>(a, units, head_lanes, s);
-    return launch_units<T, 256, 4, kFp8>(a, units, head_lanes, s);
+    const int units = (int)units_of(&a), head_lanes = joint(&a) ? (int)a.dim / 8 : 0;
+    const uint64_t len = length_of(&a);
+    switch (lanes_of(&a)) {
+        case 8: return launch_units<T, 8, 1, kFp8>(a, units, head_lanes, s);
+        case 16: return launch_units<T, 16, 1, kFp8>(a, units, head_lanes, s);
+        case 32: return launch_units<T, 32, 1, kFp8>(a, units, head_lanes, s);
+        case 64: return launch_units<T, 64, 1, kFp8>(a, units, head_lanes, s);
+        // 256 threads a row, not a wave with more vectors: 4096 x 2048 BF16 with a
+        // residual 12.6 and 15.0 us, 16384 rows 44.5 and 64, 512 equal
+        case 256:
+            return len <= 2048   ? launch_units<T, 256, 1, kFp8>(a, units, head_lanes, s)
+                   : len <= 4096 ? launch_units<T, 256, 2, kFp8>(a, units, head_lanes, s)
+                                 : launch_units<T, 256, 4, kFp8>(a, units, head_lanes, s);
+        default: return launch(k_norm_long<T, kFp8>, dim3(a.rows), dim3(kT), 0, s, a);
+    }
 }
 template <class T>
 hipError_t launch_out(const GDNNorm &a, hipStream_t s) {
@@ -323,10 +336,12 @@ extern "C" int gdn_rms_norm(const GDNNorm *args, void *stream) {
     const GDNNorm *a = args;
     if (a == nullptr) return refuse(who, "args is NULL");
     if (a->dtype < GDN_DTYPE_BF16 || a->dtype > GDN_DTYPE_FP32) return refuse(who, "unknown dtype");
-    const uint64_t len = (uint64_t)a->heads * a->dim, units = (uint64_t)a->rows * a->heads;
+    const uint64_t len = (uint64_t)a->heads * a->dim;
     if (len == 0 || len > (1u << 20)) return refuse(who, "rows have 1 to 2^20 values");
     // a grid has fewer than 2^32 threads along an axis
-    if (units >= (1u << 24)) return refuse(who, "fewer than 2^24 heads in all");
+    const uint64_t each = lanes_of(a) ? lanes_of(a) : gdn::kT;
+    if (units_of(a) >= 0x7fffff00u || units_of(a) * each >= (1ull << 32) - gdn::kT)
+        return refuse(who, "too many rows for one launch");
     if (a->fp8 && a->block != 0 && ((a->block != 32 && a->block != 64 && a->block != 128) || a->dim % a->block != 0))
         return refuse(who, "a block is 0, 32, 64 or 128 and divides dim");
     if (!(a->eps >= 0.0f) || a->eps > 3.4e38f) return refuse(who, "eps is a finite number from 0 up");

@@ -154,7 +154,7 @@ __global__ __launch_bounds__(64 * NW, (kPerSimd<T, N, NW, kY>)) void k_scan_segm
     // last one, in bounds, put as zeros.
     constexpr int kLoads = kBr + kXr + (kY ? kBr : 0);
     auto fetch = [&](int c, int part, int parts) __attribute__((always_inline)) {
-        const int last_row = n_rows - C * c - 1, row = row0 + C * c;
+        const int last_row = min(n_rows - C * c, C) - 1, row = row0 + C * c;  // (its offset stays in 32 bits)
         auto load = [&](Raw8<T> &to, const char *from, int64_t stride, int i, int per) __attribute__((always_inline)) {
             const uint32_t step = (uint32_t)stride * kSize, at = 8 * kSize * (t % per);
             const uint32_t r = (uint32_t)(i * kThreads + t) / per;
@@ -382,23 +382,37 @@ __global__ __launch_bounds__(64 * NW, (kPerSimd<T, N, NW, kY>)) void k_scan_segm
         if constexpr (kY) {
             // C_m . B_s of row tile j (a lane's token m), column tile i (its four s)
             struct Operands {
-                u32x4 a[KS][NT], b[KS][NT];
+                u32x4 a[NT], b[NT];
             };
-            auto read_tile = [&](int j, int i, Operands &o) __attribute__((always_inline)) {
+            auto read_step = [&](int j, int i, int s, Operands &o) __attribute__((always_inline)) {
 #pragma unroll
-                for (int s = 0; s < KS; ++s)
-#pragma unroll
-                    for (int k = 0; k < NT; ++k) {
-                        o.a[s][k] = lds.b[k][16 * i + li][4 * s + kk];
-                        o.b[s][k] = lds.c[k][16 * j + li][4 * s + kk];
-                    }
+                for (int k = 0; k < NT; ++k) {
+                    o.a[k] = lds.b[k][16 * i + li][4 * s + kk];
+                    o.b[k] = lds.c[k][16 * j + li][4 * s + kk];
+                }
             };
-            auto products = [&](const Operands &o) __attribute__((always_inline)) {
+            auto multiply = [&](const Operands &o, f32x4 z) __attribute__((always_inline)) {
+                for_terms<NT, NT>([&](int k, int l) __attribute__((always_inline)) { z = mfma_bf16(o.a[k], o.b[l], z); });
+                return z;
+            };
+            auto read_tile = [&](int j, int i, Operands(&o)[KS]) __attribute__((always_inline)) {
+#pragma unroll
+                for (int s = 0; s < KS; ++s) read_step(j, i, s, o[s]);
+            };
+            auto products = [&](const Operands(&o)[KS]) __attribute__((always_inline)) {
                 f32x4 z[2] = {zero, zero};
 #pragma unroll
-                for (int s = 0; s < KS; ++s)
-                    for_terms<NT, NT>(
-                        [&](int k, int l) __attribute__((always_inline)) { z[s & 1] = mfma_bf16(o.a[s][k], o.b[s][l], z[s & 1]); });
+                for (int s = 0; s < KS; ++s) z[s & 1] = multiply(o[s], z[s & 1]);
+                return z[0] + z[1];
+            };
+            auto products_at = [&](int j, int i) __attribute__((always_inline)) {
+                f32x4 z[2] = {zero, zero};
+#pragma unroll
+                for (int s = 0; s < KS; ++s) {
+                    Operands o;
+                    read_step(j, i, s, o);
+                    z[s & 1] = multiply(o, z[s & 1]);
+                }
                 return z[0] + z[1];
             };
             auto put_tile = [&](int j, int i, const f32x4 v) __attribute__((always_inline)) {
@@ -409,7 +423,7 @@ __global__ __launch_bounds__(64 * NW, (kPerSimd<T, N, NW, kY>)) void k_scan_segm
             };
             // M's tiles: on the diagonal a power for each value (above it one that
             // makes it zero, not a branch)
-            auto diagonal = [&](int j, const Operands &o) __attribute__((always_inline)) {
+            auto diagonal = [&](int j, const f32x4 z) __attribute__((always_inline)) {
                 const int to = 16 * j + li, of = 16 * j + 4 * kk;
                 const int n_to = sc.whole[to];
                 const float f_to = sc.rest[to];
@@ -419,7 +433,7 @@ __global__ __launch_bounds__(64 * NW, (kPerSimd<T, N, NW, kY>)) void k_scan_segm
                     const int n2 = 4 * kk + r <= li ? n_to - sc.whole[of + r] : -1000;
                     e[r] = __builtin_ldexpf(__builtin_amdgcn_exp2f(f_to - sc.rest[of + r]), n2) * sc.step[of + r];
                 }
-                f32x4 v = products(o) * e;
+                f32x4 v = z * e;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) v[r] += 4 * kk + r == li ? skip : 0.0f;
                 put_tile(j, j, v);
@@ -427,40 +441,34 @@ __global__ __launch_bounds__(64 * NW, (kPerSimd<T, N, NW, kY>)) void k_scan_segm
             // below it what falls in front of the row tile and inside it
             auto row_of = [](int q) { return q < 1 ? 1 : q < 3 ? 2 : 3; };
             auto column_of = [&](int q) { return q - row_of(q) * (row_of(q) - 1) / 2; };
-            auto below = [&](int q, const Operands &o) __attribute__((always_inline)) {
+            auto below = [&](int q, const f32x4 z) __attribute__((always_inline)) {
                 const int j = row_of(q), i = column_of(q);
                 const float in = sc.in[16 * j + li];
                 f32x4 e;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) e[r] = in * sc.to[j - 1][16 * i + 4 * kk + r];
-                put_tile(j, i, products(o) * e);
+                put_tile(j, i, z * e);
             };
             // spread over the waves
             constexpr int kBelow = MT * (MT - 1) / 2;
-            Operands o[2];
             if constexpr (MT == NW && KS * NT <= 4) {
                 // ten tiles, three a wave (two waves have one of theirs twice), the next
                 // one's operands read ahead
                 const int q = w < kBelow - NW ? NW + w : w;
+                Operands o[2][KS];
                 read_tile(row_of(q), column_of(q), o[0]);
                 read_tile(row_of(w), column_of(w), o[1]);
-                below(q, o[0]);
+                below(q, products(o[0]));
                 read_tile(w, w, o[0]);
-                below(w, o[1]);
-                diagonal(w, o[0]);
+                below(w, products(o[1]));
+                diagonal(w, products(o[0]));
             } else {
                 constexpr int kFirst = MT >= NW ? 0 : MT, kEach = NW - kFirst;
-                if (w < MT) {
-                    read_tile(w, w, o[0]);
-                    diagonal(w, o[0]);
-                }
+                if (w < MT) diagonal(w, products_at(w, w));
 #pragma unroll
                 for (int from = 0; from < kBelow; from += kEach) {
                     const int q = from + w - kFirst;
-                    if (q >= from && q < kBelow) {
-                        read_tile(row_of(q), column_of(q), o[0]);
-                        below(q, o[0]);
-                    }
+                    if (q >= from && q < kBelow) below(q, products_at(row_of(q), column_of(q)));
                 }
             }
             __builtin_amdgcn_sched_barrier(0);

@@ -246,6 +246,13 @@ def test_offsets_beyond_32_bits():
     close_fp8(q[-3:], s[-3:], reference(x[-3:], None)[0], 128, "last rows")
 
 
+def test_many_short_heads():
+    x, _, gate, w = inputs((1_200_000, 16, 8), BF16)
+    out = g.rms_norm(x, w[0].contiguous(), gate=gate)
+    for s in (slice(0, 3), slice(599_999, 600_002), slice(1_199_997, 1_200_000)):
+        close(out[s], reference(x[s], w[0], gate=gate[s])[0], s)
+
+
 def test_refusals_of_tensors():
     x, r, gate, w = inputs((4, 2, 64), BF16)
     for bad in (dict(x=x.double()), dict(x=x.cpu()), dict(x=x[0, 0]), dict(x=x[:, :, ::2]), dict(x=x.transpose(0, 1)),

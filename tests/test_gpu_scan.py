@@ -363,6 +363,26 @@ def test_offsets_beyond_32_bits():
         close(pool[s], S, tol(N), s)
 
 
+@TYPES
+def test_rows_nearly_16_mb_apart(dtype):
+    """Rows' offsets in a chunk and the clamped last row's fit their 32 bits."""
+    n, heads, N, P = 150, 2, 64, 64
+    a = inputs(n, heads, 1, N, P, dtype, 7)
+    apart = (1 << 24) // a["x"].element_size() - 8
+    room = torch.zeros(n * apart, dtype=dtype, device="cuda")
+    far = dict(a)
+    for k, at in (("x", 0), ("B", 128), ("C", 192)):
+        far[k] = room[at:].as_strided(a[k].shape, (apart, a[k].shape[2], 1))
+        far[k].copy_(a[k])
+    out = room[512:].as_strided(a["x"].shape, (apart, P, 1))
+    cu = cumulative([100, 1, 49])
+    pool = torch.zeros((3, heads, N, P), device="cuda")
+    call(g.scan_prefill, far, cu, state_out=pool, out=out)
+    want = torch.zeros_like(pool)
+    y = call(g.scan_prefill, a, cu, state_out=want)
+    assert torch.equal(out, y) and torch.equal(pool, want)
+
+
 def test_many_sequences():
     lens = [(i * 7) % 5 for i in range(5000)]
     n = sum(lens)

@@ -118,7 +118,7 @@ def test_scan_places_hold_every_segment():
 NORM = dict(dtype=_lib.DTYPE_BF16, rows=10, heads=2, dim=128, gate_first=0, weight_heads=0, fp8=0, block=0, eps=1e-6,
             x_stride=256, residual_stride=256, gate_stride=256, out_stride=256, sum_stride=256, x=AT, residual=AT + (1 << 16),
             gate=AT + (2 << 16), weight=AT, out=FAR, sum=2 * FAR, scales=3 * FAR)
-BAD_NORM = [dict(dtype=3), dict(dtype=-1), dict(heads=0), dict(dim=0), dict(heads=8193), dict(rows=1 << 23),
+BAD_NORM = [dict(dtype=3), dict(dtype=-1), dict(heads=0), dict(dim=0), dict(heads=8193), dict(rows=1 << 27),
             dict(fp8=1, block=16), dict(fp8=1, block=64, dim=96), dict(fp8=1, block=256), dict(eps=-1.0), dict(eps=float("nan")),
             dict(eps=float("inf")), dict(x=0), dict(out=0), dict(fp8=1, scales=0), dict(x=AT + 1), dict(residual=AT + 65537),
             dict(gate=AT + 65537), dict(out=FAR + 1), dict(sum=2 * FAR + 1), dict(x_stride=255), dict(residual_stride=0),
