@@ -161,9 +161,8 @@ __global__ __launch_bounds__(kT) void k_conv_prefill(GDNConv p, int groups, int 
     const int end = min((tile + 1) * rows, (int)p.n_tokens);
     if (n > 0) taps.load(p, ch, n);
     for (int r = tile * rows; r < end;) {
-        const int seq = last_at_most((int)p.n_seqs, r, [&](int i) { return span_of(p, i).first; });
-        const Span sp = span_of(p, seq);
-        const int to = __builtin_amdgcn_readfirstlane(min(end, sp.first + sp.n)), from = __builtin_amdgcn_readfirstlane(sp.first);
+        const Found found = find(p, r, [](int first, int) { return first; });
+        const int from = found.rows.first, to = min(end, from + found.rows.n);
         if (r >= to) break;  // behind the last sequence
         if (r < from) {      // before the first
             r = min(end, from);
@@ -171,7 +170,7 @@ __global__ __launch_bounds__(kT) void k_conv_prefill(GDNConv p, int groups, int 
         }
         int at = max(r, from + H);
         r = to;
-        if (slot_of(p, seq) < 0 || n <= 0 || at >= to) continue;
+        if (found.slot < 0 || n <= 0 || at >= to) continue;
         Vec<T> z[H + kAhead];
 #pragma unroll
         for (int j = 0; j < H; ++j) z[j].load(p.x, (size_t)(at - H + j) * p.x_stride + ch, n);

@@ -132,6 +132,32 @@ __device__ __forceinline__ int last_at_most(int n, int most, Key &&key) {
     return __builtin_amdgcn_readfirstlane(lo);
 }
 
+// The sequence that last_at_most finds by key(its first row, its number), its rows
+// and its slot.  Of up to 64 every lane holds one's, so that they take one memory
+// latency and not three in a row.
+struct Found {
+    int seq, slot;
+    Span rows;
+};
+template <class A, class Key>
+__device__ __forceinline__ Found find(const A &p, int most, Key &&key) {
+    const int n = (int)p.n_seqs, lane = threadIdx.x & 63;
+    Found f;
+    if (n <= 64) {
+        const int i = min(lane, n - 1), slot = slot_of(p, i);
+        const Span sp = span_of(p, i);
+        f.seq = max(__builtin_popcountll(__ballot(lane < n && key(sp.first, i) <= most)) - 1, 0);
+        f.slot = __builtin_amdgcn_readlane(slot, f.seq);
+        f.rows = {__builtin_amdgcn_readlane(sp.first, f.seq), __builtin_amdgcn_readlane(sp.n, f.seq)};
+    } else {
+        f.seq = last_at_most(n, most, [&](int i) { return key(span_of(p, i).first, i); });
+        const Span sp = span_of(p, f.seq);
+        f.slot = __builtin_amdgcn_readfirstlane(slot_of(p, f.seq));
+        f.rows = {__builtin_amdgcn_readfirstlane(sp.first), __builtin_amdgcn_readfirstlane(sp.n)};
+    }
+    return f;
+}
+
 // 2^y, to about 2^-23 of it: the whole powers apart from the rest, which is
 // small enough for FP32.
 __device__ __forceinline__ float exp2_of(double y) {

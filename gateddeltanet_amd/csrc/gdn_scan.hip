@@ -132,12 +132,9 @@ __global__ __launch_bounds__(64 * NW, (kPerSimd<T, N, NW, kY>)) void k_scan_segm
     const int unit = (bx / groups) * 8 + (blockIdx.x & 7), cg = bx % groups;
     if (unit >= units) return;
     const int head = unit % (int)p.n_heads, place = unit / (int)p.n_heads, group = head / (int)(p.n_heads / p.n_groups);
-    const int seq = last_at_most((int)p.n_seqs, place,
-                                 [&](int i) { return span_of(p, i).first / seg + (kY ? i : 0); });
-    Span sp = span_of(p, seq);
-    sp.first = __builtin_amdgcn_readfirstlane(sp.first);
-    sp.n = __builtin_amdgcn_readfirstlane(sp.n);
-    const int slot = __builtin_amdgcn_readfirstlane(slot_of(p, seq));
+    const Found at = find(p, place, [&](int first, int i) { return first / seg + (kY ? i : 0); });
+    const int seq = at.seq, slot = at.slot;
+    const Span sp = at.rows;
     const int cuts = cuts_of(sp, seg), base = sp.first / seg, c0 = place - base - (kY ? seq : 0);
     if (slot < 0 || c0 < 0 || c0 > cuts || (!kY && c0 == cuts)) return;
     const int row0 = sp.first + c0 * seg, n_rows = min(seg, sp.n - c0 * seg), chunks = (n_rows + C - 1) / C;
@@ -377,7 +374,6 @@ __global__ __launch_bounds__(64 * NW, (kPerSimd<T, N, NW, kY>)) void k_scan_segm
             __builtin_amdgcn_sched_barrier(0);
         };
         using std::integral_constant;
-        constexpr int kParts = kY ? 2 * KS : KS;
         u32x4 ab[2][2][JT][NT];
         if constexpr (kY) {
             // C_m . B_s of row tile j (a lane's token m), column tile i (its four s)
@@ -484,7 +480,6 @@ __global__ __launch_bounds__(64 * NW, (kPerSimd<T, N, NW, kY>)) void k_scan_segm
             for (int s = 0; s < KS; ++s) {
                 if (s + 1 < KS) read_c(s + 1, ca[(s + 1) & 1]);
                 else read_b(0, ab[0]);
-                fetch(next, s, kParts);
                 if (s + 1 < KS) terms_of(s + 1, sb[(s + 1) & 1]);
 #pragma unroll
                 for (int k = 0; k < 2 * JT; ++k)
@@ -506,7 +501,7 @@ __global__ __launch_bounds__(64 * NW, (kPerSimd<T, N, NW, kY>)) void k_scan_segm
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
             if (s + 1 < KS) read_b(s + 1, ab[(s + 1) & 1]);
-            fetch(next, kParts - KS + s, kParts);
+            fetch(next, s, KS);
             S[s][0] *= dn;
             S[s][1] *= dn;
             for_terms<NT, 3>([&](int e, int f) __attribute__((always_inline)) {

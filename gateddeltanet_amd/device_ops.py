@@ -339,10 +339,11 @@ def scan_prefill(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.Te
                       cu_seqlens)
     at = size = 0
     if workspace is None:
-        size = _entry("gdn_scan_prefill_workspace")(args)
-        if size:
-            workspace = torch.empty(size, dtype=torch.uint8, device=x.device)
-            at = workspace.data_ptr()
+        if x.shape[0] > 128:  # (fewer need none)
+            size = _entry("gdn_scan_prefill_workspace")(args)
+            if size:
+                workspace = x.new_empty(size, dtype=torch.uint8)
+                at = workspace.data_ptr()
     else:
         size = workspace.numel()
         at = _on(dev, "workspace", workspace, torch.uint8, (size,))
@@ -450,7 +451,7 @@ def rms_norm_fp8(x: torch.Tensor, weight: Optional[torch.Tensor] = None, *, bloc
         _fail(f"block: expected 0, 32, 64 or 128, got {block}")
     if scales is None:
         wide = x.shape[-1] * (x.shape[1] if x.dim() == 3 else 1) if x.dim() else 0
-        scales = torch.empty((x.shape[0] if x.dim() else 0, wide // block if block else 1), dtype=_F32, device=x.device)
+        scales = x.new_empty((x.shape[0] if x.dim() else 0, wide // block if block else 1), dtype=_F32)
     if residual is not None and sum_out is None:
         sum_out = torch.empty_like(x, memory_format=torch.contiguous_format)
     _norm(x, weight, eps, residual, gate, gate_first, out, torch.float8_e4m3fn, sum_out, scales, block)
