@@ -254,12 +254,15 @@ int check(const char *who, const GDNConv *a, bool packed) {
 }
 
 // Rows a tile: two workgroups of tiles a CU before the tiles grow, since each loads
-// its taps (128 bytes a thread) and looks its sequence up.  8111 tokens of 6144 BF16
-// channels with tiles of 8, 16, 32 rows: 46.6, 42.2, 41.2 us; 4000: 32.5, 26.1, 23.6 (of
-// 16, then); 1000 with tiles of 4 and 32: 11.5, 19.4.
+// its taps (128 bytes a thread) and looks its sequence up, and 16 at most.  6144 BF16
+// channels, tiles of 4, 8, 16, 32 rows: 1000 tokens 11.5 us with 4, 19.4 with 32; 2000
+// 19.5, 16.3; 4000 32.5 with 8, 23.6 with 16; 8111 in 24 sequences 48.3 with 16, 50.5
+// with 32 (46.6 with 8 and 41.2 with 32 where the last-level cache holds what the calls
+// before wrote).  Stores past the caches: 44.6, but the call that reads the rows next is
+// as much slower and more (a copy behind 4000 tokens: 43.5 against 40.0 together).
 int rows_of(const GDNConv *a) {
     const uint64_t want = (uint64_t)a->n_tokens * groups_of(a) / 512;
-    return want >= 32 ? 32 : want >= 16 ? 16 : want >= 8 ? 8 : 4;
+    return want >= 16 ? 16 : want >= 8 ? 8 : 4;
 }
 
 template <class T, int W>
