@@ -554,16 +554,14 @@ __global__ __launch_bounds__(64 * NW, (kPerSimd<T, N, NW, kY>)) void k_scan_segm
     }
 }
 
-// Between the two: a sequence's states behind its segments from what each of
-// them adds.  Grid (state values / 1024, heads, sequences in turn).
+// Between the two: a sequence's states behind its segments from what each of them
+// adds, of 1024 values a workgroup: grid (state values / 1024, heads, sequences of two
+// cuts and more, which up to 64 sequences' lanes tell; of more sequences, these in turn).
 __global__ __launch_bounds__(kT) void k_scan_join(GDNScan p, Pools ws, int seg) {
     const size_t tile = (size_t)p.state_dim * p.head_dim;
     const int head = blockIdx.y, at = (blockIdx.x * kT + (int)threadIdx.x) * 4;
-    for (int seq = blockIdx.z; seq < (int)p.n_seqs; seq += gridDim.z) {
-        const Span sp = span_of(p, seq);
-        const int cuts = cuts_of(sp, seg);
-        if (cuts < 2 || slot_of(p, seq) < 0) continue;
-        const size_t unit = (size_t)(sp.first / seg) * p.n_heads + head;
+    auto join = [&](int first, int cuts) __attribute__((always_inline)) {
+        const size_t unit = (size_t)(first / seg) * p.n_heads + head;
         float *s = ws.states + unit * tile + at;
         const float *d = ws.decays + unit;
         const size_t step = p.n_heads * tile;
@@ -585,6 +583,21 @@ __global__ __launch_bounds__(kT) void k_scan_join(GDNScan p, Pools ws, int seg) 
                     for (int e = 0; e < 4; ++e) v[e] = __builtin_fmaf(a[k], v[e], u[k][e]);
                     *reinterpret_cast<f32x4 *>(s + (c + k) * step) = v;
                 }
+        }
+    };
+    const int n = (int)p.n_seqs, lane = threadIdx.x & 63;
+    if (n <= 64) {
+        const int i = min(lane, n - 1);
+        const Span sp = span_of(p, i);
+        uint64_t mask = __ballot(lane < n && cuts_of(sp, seg) >= 2 && slot_of(p, i) >= 0);
+        for (int z = blockIdx.z; z > 0; --z) mask &= mask - 1;
+        if (mask == 0) return;
+        const int of = __builtin_ctzll(mask), first = __builtin_amdgcn_readlane(sp.first, of);
+        join(first, cuts_of({first, __builtin_amdgcn_readlane(sp.n, of)}, seg));
+    } else {
+        for (int i = blockIdx.z; i < n; i += gridDim.z) {
+            const Span sp = span_of(p, i);
+            if (cuts_of(sp, seg) >= 2 && slot_of(p, i) >= 0) join(sp.first, cuts_of(sp, seg));
         }
     }
 }
@@ -732,8 +745,9 @@ hipError_t launch_prefill(const GDNScan &a, void *mem, hipStream_t s) {
         hipError_t rc = launch_segments<T, N, NW, false>(a, ws, seg, places(&a), s);
         if (rc != hipSuccess) return rc;
         if (a.n_tokens > 2u * (uint32_t)seg) {
-            rc = launch(k_scan_join, dim3(a.state_dim * a.head_dim / 1024, a.n_heads, a.n_seqs < 1024 ? a.n_seqs : 1024),
-                        dim3(kT), 0, s, a, ws, seg);
+            // a sequence of two cuts has two places
+            const unsigned most = a.n_seqs <= 64 ? (unsigned)(places(&a) / 2) : 1024, z = a.n_seqs < most ? a.n_seqs : most;
+            rc = launch(k_scan_join, dim3(a.state_dim * a.head_dim / 1024, a.n_heads, z), dim3(kT), 0, s, a, ws, seg);
             if (rc != hipSuccess) return rc;
         }
     }

@@ -142,6 +142,13 @@ def test_prefill_of_sequences_in_segments(dtype, N, P, lens):
     check_packed(lens, 2, 1, N, P, dtype, shuffle=True, seed=N)
 
 
+@pytest.mark.parametrize("lens", [[0] * 30 + [700] + [1] * 32 + [600], [0] * 30 + [700] + [1] * 33 + [600], [600] * 20],
+                         ids=["64", "65", "20"])
+def test_prefill_of_long_sequences_among_many(lens):
+    """Sequences of several segments, up to 64 of all lengths and more."""
+    check_packed(lens, 2, 1, 64, 64, FP32, shuffle=True, seed=3)
+
+
 @pytest.mark.parametrize("lens", [[5000], [2500, 1, 2600, 1024, 1025]])
 def test_prefill_long(lens):
     check_packed(lens, 1, 1, 64, 64, FP32, seed=9)
