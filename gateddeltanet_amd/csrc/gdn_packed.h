@@ -158,6 +158,27 @@ __device__ __forceinline__ Found find(const A &p, int most, Key &&key) {
     return f;
 }
 
+// The sequence of this rank by size(its rows), the largest first and equal ones in
+// turn, where the wave's lanes hold them all; else of this number.
+template <class A, class Size>
+__device__ __forceinline__ Found ranked(const A &p, int rank, Size &&size) {
+    const int n = (int)p.n_seqs, lane = threadIdx.x & 63, i = n <= 64 ? min(lane, n - 1) : rank;
+    const int slot = slot_of(p, i);
+    const Span sp = span_of(p, i);
+    int of = 0;
+    if (n <= 64) {
+        const int own = size(sp);
+        int before = 0;
+        for (int j = 0; j < n; ++j) {
+            const int other = __builtin_amdgcn_readlane(own, j);
+            before += other > own || (other == own && j < lane);
+        }
+        of = __builtin_ctzll(__ballot(lane < n && before == rank) | (1ull << 63));
+    }
+    return {n <= 64 ? of : rank, __builtin_amdgcn_readlane(slot, of),
+            {__builtin_amdgcn_readlane(sp.first, of), __builtin_amdgcn_readlane(sp.n, of)}};
+}
+
 // 2^y, to about 2^-23 of it: the whole powers apart from the rest, which is
 // small enough for FP32.
 __device__ __forceinline__ float exp2_of(double y) {

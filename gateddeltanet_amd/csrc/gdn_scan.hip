@@ -109,16 +109,27 @@ constexpr int kPerSimd = NW == 8 || sizeof(Lds<T, N, NW, kY>) <= (80 << 10) ? 2 
 // transposed too, B C^T, spread over the waves: an accumulator is then half an
 // operand of M x as it is.  x and B^T are read transposed (ds_read_b64_tr_b16).  The
 // steps and decays of NW chunks are formed at a time, a chunk a wave.  Two barriers a
-// chunk.  A wave is bound by the latency of what it waits for, so a step's operands
-// are read a step ahead, the next chunk's rows loaded one by one between the
-// products, and the splitting of the state and of x goes between them too.
+// chunk.  A step's operands are read a step ahead, the next chunk's rows loaded one by
+// one between the products of the update, and the splitting of the state and of x goes
+// between those of C S.
 // Two kernels of it:
 //   kY false  the segments with a later one: the state that each leaves, the first
 //             of a sequence from its start, the others from zero; their decays; and
 //             the start itself where the sequence's slot is written
 //   kY true   all segments, from the states behind the ones before them
+// Bound by the instructions that a wave can issue: two waves a SIMD (registers, LDS),
+// each with 600 vector instructions a chunk of 64 tokens, 100 products and 140 LDS
+// instructions, one in five cycles or so; 512 workgroups of four chunks, 33 us, 17.7 of
+// them launch, lookup, first loads and states, 3.85 a chunk of the two on a CU (4096
+// tokens, 32 heads of 128 x 64: kY 26.6 us, not kY 14.4, matrix unit 26 % busy, vector
+// units 40, LDS 36).  8111 tokens in 24 sequences, 8 heads of 256 x 256, 100 MB of states:
+// 94 and 28.6 us.  Measured against it at 4096 tokens: M's weights as exponentials for
+// each value, loads in one piece, three barriers 28.8; two column tiles in each of four
+// waves (one wave a SIMD) 34.5; two heads a workgroup of eight waves equal; chunks of 32
+// tokens 49 against 45 in all.  Conflict-free reads of B^T (the state's rows in another
+// order, C read by 8 bytes) halve the LDS's busy cycles and change no time.
 template <class T, int N, int NW, bool kY>
-__global__ __launch_bounds__(64 * NW, (kPerSimd<T, N, NW, kY>)) void k_scan_segment(GDNScan p, Pools ws, int seg, int units) {
+__global__ __launch_bounds__(64 * NW, (kPerSimd<T, N, NW, kY>)) void k_scan_segment(GDNScan p, Pools ws, int seg, int n_places, int units) {
     using L = Lds<T, N, NW, kY>;
     constexpr int C = L::C, NT = L::NT, MT = C / 16, JT = C / 32, KS = N / 32, OT = kOutTerms<T>, kThreads = 64 * NW;
     constexpr int kCols = 16 * NW, kB = C * (N / 8), kX = C * (kCols / 8);  // 16-byte units (of 16-bit values) of a chunk's rows
@@ -132,11 +143,14 @@ __global__ __launch_bounds__(64 * NW, (kPerSimd<T, N, NW, kY>)) void k_scan_segm
     const int unit = (bx / groups) * 8 + (blockIdx.x & 7), cg = bx % groups;
     if (unit >= units) return;
     const int head = unit % (int)p.n_heads, place = unit / (int)p.n_heads, group = head / (int)(p.n_heads / p.n_groups);
-    const Found at = find(p, place, [&](int first, int i) { return first / seg + (kY ? i : 0); });
-    const int seq = at.seq, slot = at.slot;
+    // cut segments by place; behind them, shorter, the sequences' last ones
+    const bool last = kY && place >= n_places;
+    const Found at = last ? ranked(p, place - n_places, [&](const Span &sp) { return sp.n - cuts_of(sp, seg) * seg; })
+                          : find(p, place, [&](int first, int) { return first / seg; });
+    const int slot = at.slot;
     const Span sp = at.rows;
-    const int cuts = cuts_of(sp, seg), base = sp.first / seg, c0 = place - base - (kY ? seq : 0);
-    if (slot < 0 || c0 < 0 || c0 > cuts || (!kY && c0 == cuts)) return;
+    const int cuts = cuts_of(sp, seg), base = sp.first / seg, c0 = last ? cuts : place - base;
+    if (slot < 0 || c0 < 0 || (!last && c0 >= cuts)) return;
     const int row0 = sp.first + c0 * seg, n_rows = min(seg, sp.n - c0 * seg), chunks = (n_rows + C - 1) / C;
     const int col0 = kCols * cg + 16 * w;  // the wave's first column
     const size_t head_at = (size_t)8 * kk * p.head_dim + col0 + li, tile = (size_t)N * p.head_dim;
@@ -555,7 +569,8 @@ __global__ __launch_bounds__(64 * NW, (kPerSimd<T, N, NW, kY>)) void k_scan_segm
 }
 
 // Between the two: a sequence's states behind its segments from what each of them
-// adds, of 1024 values a workgroup: grid (state values / 1024, heads, sequences of two
+// adds, their bytes once in and out (4096 tokens, 32 heads of 128 x 64, 15 states of 1 MB:
+// 7.3 us, 4.3 TB/s), of 1024 values a workgroup: grid (state values / 1024, heads, sequences of two
 // cuts and more, which up to 64 sequences' lanes tell; of more sequences, these in turn).
 __global__ __launch_bounds__(kT) void k_scan_join(GDNScan p, Pools ws, int seg) {
     const size_t tile = (size_t)p.state_dim * p.head_dim;
@@ -605,7 +620,9 @@ __global__ __launch_bounds__(kT) void k_scan_join(GDNScan p, Pools ws, int seg) 
 // ------------------------------------------------------------ a single token
 
 // A (sequence, head)'s token for 64 columns: grid (head_dim / 64, heads,
-// sequences).  The state's tile goes through registers once.
+// sequences).  The state's tile goes through registers once, y's sums formed as it is
+// written, so its bytes bound the kernel: 64 sequences of 32 heads of 128 x 64, 134 MB, in
+// 21 us (6.3 TB/s, partly from the last-level cache), one of 16 heads of 128 x 128 in 4.3.
 template <class T, int N>
 __global__ __launch_bounds__(kT) void k_scan_step(GDNScan p) {
     constexpr int L = 16, RP = kT / L, NR = N / RP;  // lanes a row, rows a pass, passes
@@ -728,10 +745,10 @@ bool keeps_starts(const GDNScan *a) { return a->state_in && a->state_in == a->st
 size_t pool_bytes(const GDNScan *a) { return places(a) * a->n_heads * a->state_dim * a->head_dim * sizeof(float); }
 
 template <class T, int N, int NW, bool kY>
-hipError_t launch_segments(const GDNScan &a, const Pools &ws, int seg, size_t n_places, hipStream_t s) {
-    const int units = (int)(n_places * a.n_heads), groups = (int)a.head_dim / (16 * NW);
+hipError_t launch_segments(const GDNScan &a, const Pools &ws, int seg, int n_places, hipStream_t s) {
+    const int units = (int)((n_places + (kY ? a.n_seqs : 0)) * a.n_heads), groups = (int)a.head_dim / (16 * NW);
     return launch(k_scan_segment<T, N, NW, kY>, dim3((unsigned)((units + 7) / 8 * 8 * groups)), dim3(64 * NW), 0, s, a, ws, seg,
-                  units);
+                  n_places, units);
 }
 template <class T, int N, int NW>
 hipError_t launch_prefill(const GDNScan &a, void *mem, hipStream_t s) {
@@ -742,7 +759,7 @@ hipError_t launch_prefill(const GDNScan &a, void *mem, hipStream_t s) {
         ws.decays = reinterpret_cast<float *>(at);
         ws.states = reinterpret_cast<float *>(at + decay_bytes(&a));
         if (keeps_starts(&a)) ws.starts = reinterpret_cast<float *>(at + decay_bytes(&a) + pool_bytes(&a));
-        hipError_t rc = launch_segments<T, N, NW, false>(a, ws, seg, places(&a), s);
+        hipError_t rc = launch_segments<T, N, NW, false>(a, ws, seg, (int)places(&a), s);
         if (rc != hipSuccess) return rc;
         if (a.n_tokens > 2u * (uint32_t)seg) {
             // a sequence of two cuts has two places
@@ -751,7 +768,7 @@ hipError_t launch_prefill(const GDNScan &a, void *mem, hipStream_t s) {
             if (rc != hipSuccess) return rc;
         }
     }
-    return launch_segments<T, N, NW, true>(a, ws, seg, places(&a) + a.n_seqs, s);
+    return launch_segments<T, N, NW, true>(a, ws, seg, cut(&a) ? (int)places(&a) : 0, s);
 }
 template <class T, int N>
 hipError_t launch_prefill_w(const GDNScan &a, void *ws, hipStream_t s) {

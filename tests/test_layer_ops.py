@@ -96,23 +96,21 @@ def test_scan_null_workspace_and_nothing_to_do():
 
 
 def test_scan_places_hold_every_segment():
-    """States behind all segments of a sequence but the last have places first /
-    seg + segment, none shared, all inside the workspace; segments have places first
-    / seg + number + segment (the kernels' indexing, restated)."""
+    """Segments of a sequence but the last, and the states behind them, have places
+    first / seg + segment, none shared, all inside the workspace (the kernels'
+    indexing, restated)."""
     rng = random.Random(5)
     for _ in range(300):
         seg = rng.choice([64, 128, 256, 1024])
         lens = [rng.choice([0, 1, seg - 1, seg, seg + 1, 2 * seg, rng.randint(0, 6 * seg)]) for _ in range(rng.randint(1, 9))]
         start = rng.randint(0, 2 * seg)
         total = start + sum(lens) + rng.randint(0, 70)
-        kept, whole, first = [], [], start
-        for i, n in enumerate(lens):
+        kept, first = [], start
+        for n in lens:
             cuts = (n - 1) // seg if n else 0
             kept += [first // seg + c for c in range(cuts)]
-            whole += [first // seg + i + c for c in range(cuts + 1)]
             first += n
         assert len(set(kept)) == len(kept) and all(0 <= p < total // seg for p in kept)
-        assert len(set(whole)) == len(whole) and all(0 <= p < total // seg + len(lens) for p in whole)
 
 
 NORM = dict(dtype=_lib.DTYPE_BF16, rows=10, heads=2, dim=128, gate_first=0, weight_heads=0, fp8=0, block=0, eps=1e-6,
