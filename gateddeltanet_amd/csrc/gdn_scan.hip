@@ -19,9 +19,9 @@ using namespace packed;
 // Tokens of a chunk.
 template <class T>
 constexpr int kChunk = T::kTerms == 1 ? 64 : 32;
-// BF16 terms of the FP32 operands that only y is formed from: two leave 2^-17 of a
-// product out, which a y of 8 or 11 significand bits does not show; the state's
-// have three throughout.
+// BF16 terms of the FP32 operands that only y is formed from: two leave out 2^-16 of an
+// operand at most (the first is cut, the second rounded), which a y of 8 or 11
+// significand bits does not show; the state's have three throughout.
 template <class T>
 constexpr int kOutTerms = T::kTerms == 3 ? 3 : 2;
 

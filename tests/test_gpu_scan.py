@@ -6,8 +6,9 @@ update one, each of at most state_dim + 64 products rounded to FP32; n roundings
 roundings of its own, and with them a decay exp(G) |G| exp(G) 4 2^-24, at most 1.5 2^-24 of
 what it decays.  Relative to the norm of a sequence's whole result that is
 TOL = 4 sqrt(state_dim + 64) 2^-24 (4.3e-6 at 256).  A y of 16 bits is formed from
-operands of two BF16 terms: 2^-17 of a product more for each of two, taken as 2^-16 of the
-root mean square, and half a step of the type, eps / 2 of the value.  LEAST: what FP32
+operands of two BF16 terms, off by 2^-16 at most and by 2^-16 / sqrt(12) in the mean, one in
+each of its two sums: taken as 2^-16 of the root mean square; and half a step of the
+type, eps / 2 of the value.  LEAST: what FP32
 has no normal number for, below 2^-126 a product, of up to 2^16 products of factors
 below 2^6 (a step of 200 below zero is e^-200).
 """
