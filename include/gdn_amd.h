@@ -735,7 +735,9 @@ int gdn_conv_step(const GDNConv *args, void *stream);
  *   A, D, dt_bias   FP32 [n_heads]; D NULL: 0, dt_bias NULL: 0.  h A <= 0 in a
  *              stable model
  *   state_in, state_out   [n_slots][n_heads][state_dim][head_dim] FP32, as GDNDelta's
- * Sums are FP32.  A value that is not finite reaches its own sequence and head
+ * Sums are FP32.  gdn_scan_prefill forms the product of up to 1024 tokens' exp(h A)
+ * by itself: with growth (h A > 0) beyond FP32's range in it, 2^127, states are infinities
+ * or NaN.  A value that is not finite reaches its own sequence and head
  * (one of B or C the heads of its group) only, in gdn_scan_prefill there also the
  * tokens up to 63 before it. */
 typedef struct {
