@@ -236,6 +236,41 @@ def test_captured_and_replayed():
             assert torch.equal(t, u)
 
 
+def test_replayed_with_other_sequences():
+    """A graph of the most rows and sequences, replayed with other ends and slots: padded
+    sequences are empty or have a slot of -1, rows behind the last are left."""
+    n, channels, width = 150, 264, 4
+    x, w, b = inputs(n, channels, width, FP32)
+    cu, slots = torch.zeros(6, dtype=torch.int32, device="cuda"), torch.zeros(5, dtype=torch.int32, device="cuda")
+    pool, out = torch.zeros((7, width - 1, channels), device="cuda"), torch.zeros_like(x)
+    g.conv_prefill(x, w, cu, bias=b, state_in=pool, state_out=pool, slots=slots, out=out)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        g.conv_prefill(x, w, cu, bias=b, state_in=pool, state_out=pool, slots=slots, out=out)
+    first = torch.randn(pool.shape, generator=torch.Generator(device="cuda").manual_seed(2), device="cuda")
+    for lens, where in [([150, 0, 0, 0, 0], [3, -1, -1, -1, -1]), ([1, 70, 0, 30, 2], [0, 6, 1, 2, 5]),
+                        ([0, 0, 0, 0, 0], [4, 3, 2, 1, 0]), ([17, 15, 60, 16, 3], [6, 5, 4, 3, 7])]:
+        cu.copy_(cumulative(lens))
+        slots.copy_(torch.tensor(where, dtype=torch.int32))
+        pool.copy_(first)
+        out.fill_(5.0)
+        torch.cuda.synchronize()
+        graph.replay()
+        at, used = 0, []
+        for m, slot in zip(lens, where):
+            part = slice(at, at + m)
+            at += m
+            if not 0 <= slot < 7:
+                assert (out[part] == 5).all()
+                continue
+            used.append(slot)
+            y, tol, end = reference(x[part], w, b, first[slot], True)
+            close(out[part], y, tol, f"{m} tokens")
+            assert torch.equal(pool[slot], end), m
+        rest = [i for i in range(7) if i not in used]
+        assert (out[at:] == 5).all() and torch.equal(pool[rest], first[rest])
+
+
 def test_on_a_stream_of_its_own():
     x, w, b = inputs(64, 2048, 4, BF16)
     want = g.conv_prefill(x, w, cumulative([64]), bias=b)

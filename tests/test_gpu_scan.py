@@ -143,6 +143,43 @@ def test_prefill_of_sequences_in_segments(dtype, N, P, lens):
     check_packed(lens, 2, 1, N, P, dtype, shuffle=True, seed=N)
 
 
+@pytest.mark.parametrize("kept", ["same", "apart", "read", "written", "neither"])
+@pytest.mark.parametrize("P", [64, 256])
+def test_pools_of_sequences_in_segments(kept, P):
+    """One pool read and written, two, one that is only read or written, none; a padded
+    sequence (slot -1) among the sequences."""
+    lens, N = [300, 520, 0, 129, 128], 64
+    a = inputs(sum(lens), 2, 1, N, P, FP32, seed=21)
+    gen = torch.Generator(device="cuda").manual_seed(22)
+    first = 0.3 * torch.randn((6, 2, N, P), generator=gen, device="cuda")
+    source, sink = first.clone(), 0.3 * torch.randn(first.shape, generator=gen, device="cuda")
+    before = sink.clone()
+    where = [5, 0, 3, -1, 1]
+    state_in = source if kept in ("same", "apart", "read") else None
+    state_out = source if kept == "same" else sink if kept in ("apart", "written") else None
+    slots = torch.tensor(where, dtype=torch.int32).cuda()
+    if kept == "neither":  # (as many slots as sequences: the numbers are held to them)
+        where = [4, 0, 3, -1, 1]
+        slots = torch.tensor(where, dtype=torch.int32).cuda()
+    out = torch.full_like(a["x"], 5.0)
+    call(g.scan_prefill, a, cumulative(lens), state_in=state_in, state_out=state_out, slots=slots, out=out)
+    at = 0
+    for i, m in enumerate(lens):
+        part, slot = slice(at, at + m), where[i]
+        at += m
+        if slot < 0:
+            assert (out[part] == 5).all()
+            continue
+        y, S = reference(rows(a, part), torch.zeros_like(first[0]) if state_in is None else first[slot])
+        close(out[part], y, tol(N), f"y of sequence {i}")
+        if state_out is not None:
+            close(state_out[slot], S, tol(N), f"state of sequence {i}")
+    if kept != "same":
+        assert torch.equal(source, first)
+    rest = [i for i in range(6) if i not in where] if state_out is sink else list(range(6))
+    assert torch.equal(sink[rest], before[rest])
+
+
 @pytest.mark.parametrize("lens", [[0] * 30 + [700] + [1] * 32 + [600], [0] * 30 + [700] + [1] * 33 + [600], [600] * 20],
                          ids=["64", "65", "20"])
 def test_prefill_of_long_sequences_among_many(lens):
@@ -332,6 +369,41 @@ def test_captured_and_replayed():
         graph.replay()
         for t, u in zip((out, pool, after), want):
             assert torch.equal(t, u)
+
+
+def test_replayed_with_other_sequences():
+    """A graph of the most rows and sequences, replayed with other ends and slots: padded
+    sequences are empty or have a slot of -1, rows behind the last are left."""
+    n, heads, N, P = 1500, 2, 64, 64
+    a = inputs(n, heads, 1, N, P, FP32, 1)
+    cu, slots = torch.zeros(6, dtype=torch.int32, device="cuda"), torch.zeros(5, dtype=torch.int32, device="cuda")
+    pool, out = torch.zeros((7, heads, N, P), device="cuda"), torch.zeros_like(a["x"])
+    call(g.scan_prefill, a, cu, state_in=pool, state_out=pool, slots=slots, out=out)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call(g.scan_prefill, a, cu, state_in=pool, state_out=pool, slots=slots, out=out)
+    first = 0.3 * torch.randn(pool.shape, generator=torch.Generator(device="cuda").manual_seed(2), device="cuda")
+    for lens, where in [([1500, 0, 0, 0, 0], [3, -1, -1, -1, -1]), ([1, 700, 0, 300, 2], [0, 6, 1, 2, 5]),
+                        ([0, 0, 0, 0, 0], [4, 3, 2, 1, 0]), ([129, 128, 600, 257, 300], [6, 5, 4, 3, 7])]:
+        cu.copy_(cumulative(lens))
+        slots.copy_(torch.tensor(where, dtype=torch.int32))
+        pool.copy_(first)
+        out.fill_(5.0)
+        torch.cuda.synchronize()
+        graph.replay()
+        at, used = 0, []
+        for m, slot in zip(lens, where):
+            part = slice(at, at + m)
+            at += m
+            if not 0 <= slot < 7:
+                assert (out[part] == 5).all()
+                continue
+            used.append(slot)
+            y, S = reference(rows(a, part), first[slot])
+            close(out[part], y, tol(N), f"y of {m} tokens")
+            close(pool[slot], S, tol(N), f"state of {m} tokens")
+        rest = [i for i in range(7) if i not in used]
+        assert (out[at:] == 5).all() and torch.equal(pool[rest], first[rest])
 
 
 def test_two_streams_at_once():
