@@ -84,11 +84,12 @@ __device__ __forceinline__ float lanes_sum(float v, int n) {
 __device__ __forceinline__ uint32_t lanes_max(uint32_t v, int n) {
     return lanes(v, n, [](uint32_t a, uint32_t b) { return a > b ? a : b; });
 }
-__device__ __forceinline__ uint32_t largest(const float (&y)[8]) {
+// (0 of no values: behind a row's heads there is no root, with an eps of 0 a NaN)
+__device__ __forceinline__ uint32_t largest(const float (&y)[8], int n) {
     uint32_t m = 0;
 #pragma unroll
     for (int i = 0; i < 8; ++i) m = max(m, f2u(y[i]) & 0x7fffffffu);
-    return m;
+    return n > 0 ? m : 0;
 }
 // 1 for a block whose largest magnitude is too small to be divided by
 __device__ __forceinline__ float scale_of(uint32_t magnitude) {
@@ -186,7 +187,7 @@ __global__ __launch_bounds__(kT) void k_norm(GDNNorm p, int units, int head_lane
             if constexpr (!kFp8) store8<T>(p.out, row * p.out_stride + first + at, n, u[v]);
         }
         if constexpr (kFp8) {
-            uint32_t m = largest(u[v]);
+            uint32_t m = largest(u[v], n);
             if (p.block == 0) {
                 top = max(top, m);
             } else {
@@ -255,7 +256,7 @@ __global__ __launch_bounds__(kT) void k_norm_long(GDNNorm p) {
                 const int at = 8 * (s * kT + t);
                 inputs<T>(p, row, head * dim + at, dim - at, h, u, g);
                 normed(p, root, weights_at(head, at), dim - at, u, g);
-                top = max(top, largest(u));
+                top = max(top, largest(u, dim - at));
             }
         }
         top = lanes_max(top, 64);
@@ -273,7 +274,7 @@ __global__ __launch_bounds__(kT) void k_norm_long(GDNNorm p) {
             if (p.sum) store8<T>(p.sum, row * p.sum_stride + head * dim + at, n, h);
             if constexpr (kFp8) {
                 if (p.block != 0) {
-                    scale = scale_of(lanes_max(largest(u), (int)p.block / 8));
+                    scale = scale_of(lanes_max(largest(u, n), (int)p.block / 8));
                     if (n > 0 && at % (int)p.block == 0)
                         p.scales[(row * p.heads * p.dim + (size_t)head * dim + at) / p.block] = scale;
                 }

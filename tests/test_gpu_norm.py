@@ -108,6 +108,15 @@ def test_heads(dtype, heads, dim):
             close(total, h, (heads, dim), 2.0**-24)
 
 
+@pytest.mark.parametrize("heads,dim", [(3, 64), (5, 128), (3, 256), (9, 512), (4, 100)])
+def test_rows_of_heads_without_an_eps(heads, dim):
+    """Heads that do not fill a layout's lanes: nothing of what is not there."""
+    x, r, gate, w = inputs((6, heads, dim), FP32, heads * dim)
+    q, s = g.rms_norm_fp8(x, w, gate=gate, eps=0.0)
+    y, _ = reference(x, w, gate=gate, eps=0.0)
+    close_fp8(q, s, y, 0, (heads, dim))
+
+
 @TYPES
 @pytest.mark.parametrize("block", [32, 64, 128])
 @pytest.mark.parametrize("shape", [(3, 128), (70, 2048), (4, 384), (5, 8, 256), (2, 3, 8320), (1100, 1024), (9, 6400)])
