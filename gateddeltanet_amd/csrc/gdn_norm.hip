@@ -140,27 +140,38 @@ __device__ __forceinline__ void normed(const GDNNorm &p, float root, int w_at, i
     }
 }
 
-// Rows (`heads_of` heads of a row each, or one) whose values stay in registers: L
-// lanes of V vectors of eight a unit.  `head_lanes`: lanes that a head of several in
-// a unit has, 0 for one head.  Memory-bound, each value read and written once: 4096 x
-// 2048 BF16 with a residual into 8 bits, 59 MB, in 14 us (4.2 TB/s); 64 x 8 heads of 256
-// with a gate 3.2 us, two memory latencies and a reduction.
+// Units, a head or a row of several, whose values stay in registers: L lanes of V
+// vectors of eight a unit.  `head_lanes`: the lanes of each of a unit's heads (a power of
+// two; those behind its values idle), 0 where the unit is a head.  Memory-bound, each
+// value read and written once: 4096 x 2048 BF16 with a residual into 8 bits, 59 MB, in
+// 14 us (4.2 TB/s); 64 x 8 heads of 256 with a gate 3.2 us, two memory latencies and a
+// reduction.
 template <class T, int L, int V, bool kFp8>
-__global__ __launch_bounds__(kT) void k_norm(GDNNorm p, int units, int head_lanes) {
+__global__ __launch_bounds__((L > kT ? L : kT)) void k_norm(GDNNorm p, int units, int head_lanes) {
     constexpr int W = L > 64 ? L / 64 : 1, LW = L > 64 ? 64 : L;  // waves a unit, lanes of each
-    __shared__ float sums[4];
-    __shared__ uint32_t tops[4];
-    const int t = threadIdx.x, l = t % L, w = t >> 6, per_row = head_lanes ? 1 : (int)p.heads;
-    const int unit = min((int)(blockIdx.x * (kT / L)) + t / L, units - 1);
-    const bool own = (int)(blockIdx.x * (kT / L)) + t / L < units;
+    constexpr int kUnits = L > kT ? 1 : kT / L;  // of a workgroup
+    __shared__ float sums[W];
+    __shared__ uint32_t tops[W];
+    const int t = threadIdx.x, l = t % L, w = t >> 6, per_row = head_lanes ? 1 : (int)p.heads, dim = (int)p.dim;
+    const int unit = min((int)(blockIdx.x * kUnits) + t / L, units - 1), own_head = unit % per_row;
+    const bool own = (int)(blockIdx.x * kUnits) + t / L < units;
     const size_t row = unit / per_row;
-    const int len = head_lanes ? (int)(p.heads * p.dim) : (int)p.dim, first = (unit % per_row) * (int)p.dim;
+    const int turn = head_lanes ? __builtin_ctz(head_lanes) : 0;
+    // of vector v: its head, its place in it, its values that there are
+    auto head_of = [&](int v) { return head_lanes ? (v * L + l) >> turn : own_head; };
+    auto place_of = [&](int v) { return head_lanes ? 8 * (l & (head_lanes - 1)) : 8 * (v * L + l); };
+    auto left_of = [&](int v) { return head_of(v) < (int)p.heads ? dim - place_of(v) : 0; };
     float h[V][8], u[V][8], g[V][8], sum[V];
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-        const int at = 8 * (v * L + l);
-        inputs<T>(p, row, first + at, len - at, h[v], u[v], g[v]);
+        inputs<T>(p, row, head_of(v) * dim + place_of(v), left_of(v), h[v], u[v], g[v]);
         sum[v] = squares(u[v]);
+    }
+    // (at once: 4096 rows of 8192 BF16 values into 8 bits 41.5 us, 48 with the outputs)
+    if (own && p.sum) {
+#pragma unroll
+        for (int v = 0; v < V; ++v)
+            store8<T>(p.sum, row * p.sum_stride + head_of(v) * dim + place_of(v), left_of(v), h[v]);
     }
     if (head_lanes) {
 #pragma unroll
@@ -172,19 +183,20 @@ __global__ __launch_bounds__(kT) void k_norm(GDNNorm p, int units, int head_lane
         if constexpr (W > 1) {
             if ((t & 63) == 0) sums[w] = sum[0];
             __syncthreads();
-            sum[0] = (sums[0] + sums[1]) + (sums[2] + sums[3]);
+            sum[0] = 0.0f;
+#pragma unroll
+            for (int i = 0; i < W; i += 4) sum[0] += (sums[i] + sums[i + 1]) + (sums[i + 2] + sums[i + 3]);
         }
     }
     float root = root_of(p, sum[0]);
     uint32_t top = 0;
 #pragma unroll
     for (int v = 0; v < V; ++v) {
-        const int at = 8 * (v * L + l), n = len - at;
+        const int place = place_of(v), at = head_of(v) * dim + place, n = left_of(v);
         if (head_lanes && v > 0) root = root_of(p, sum[v]);
-        normed(p, root, p.weight_heads ? first + at : head_lanes ? at % (int)p.dim : at, n, u[v], g[v]);
-        if (own) {
-            if (p.sum) store8<T>(p.sum, row * p.sum_stride + first + at, n, h[v]);
-            if constexpr (!kFp8) store8<T>(p.out, row * p.out_stride + first + at, n, u[v]);
+        normed(p, root, p.weight_heads ? at : place, n, u[v], g[v]);
+        if constexpr (!kFp8) {
+            if (own) store8<T>(p.out, row * p.out_stride + at, n, u[v]);
         }
         if constexpr (kFp8) {
             uint32_t m = largest(u[v], n);
@@ -195,8 +207,8 @@ __global__ __launch_bounds__(kT) void k_norm(GDNNorm p, int units, int head_lane
 #pragma unroll
                 for (int i = 0; i < 8; ++i) u[v][i] *= inv;
                 if (own && n > 0) {
-                    store8_fp8(p.out, row * p.out_stride + first + at, n, u[v]);
-                    if (at % (int)p.block == 0) p.scales[(row * p.heads * p.dim + first + at) / p.block] = scale;
+                    store8_fp8(p.out, row * p.out_stride + at, n, u[v]);
+                    if (place % (int)p.block == 0) p.scales[(row * p.heads * dim + at) / p.block] = scale;
                 }
             }
         }
@@ -207,15 +219,15 @@ __global__ __launch_bounds__(kT) void k_norm(GDNNorm p, int units, int head_lane
             if constexpr (W > 1) {
                 if ((t & 63) == 0) tops[w] = top;
                 __syncthreads();
-                top = max(max(tops[0], tops[1]), max(tops[2], tops[3]));
+#pragma unroll
+                for (int i = 0; i < W; ++i) top = max(top, tops[i]);
             }
             const float scale = scale_of(top), inv = 1.0f / scale;
 #pragma unroll
             for (int v = 0; v < V; ++v) {
-                const int at = 8 * (v * L + l);
 #pragma unroll
                 for (int i = 0; i < 8; ++i) u[v][i] *= inv;
-                if (own) store8_fp8(p.out, row * p.out_stride + first + at, len - at, u[v]);
+                if (own) store8_fp8(p.out, row * p.out_stride + head_of(v) * dim + place_of(v), left_of(v), u[v]);
             }
             if (own && l == 0) p.scales[row] = scale;
         }
@@ -224,39 +236,48 @@ __global__ __launch_bounds__(kT) void k_norm(GDNNorm p, int units, int head_lane
 
 // Rows of any length and number of heads, a workgroup each, read again for every
 // pass: the squares, the largest magnitude of the row's y where it has one scale,
-// the outputs.  A value is read and written by one thread throughout.
+// the outputs.  Heads of `head_lanes` lanes (a power of two up to 64) side by side, or of
+// all 256 in turn.  A value is read and written by one thread throughout.
 template <class T, bool kFp8>
-__global__ __launch_bounds__(kT) void k_norm_long(GDNNorm p) {
+__global__ __launch_bounds__(kT) void k_norm_long(GDNNorm p, int head_lanes) {
     __shared__ float sums[2][4];
     __shared__ uint32_t tops[4];
-    const int t = threadIdx.x, w = t >> 6, dim = (int)p.dim, steps = (dim + 8 * kT - 1) / (8 * kT);
+    const int t = threadIdx.x, w = t >> 6, l = t & (head_lanes - 1), own = t / head_lanes, per = kT / head_lanes;
+    const int dim = (int)p.dim, heads = (int)p.heads, steps = (dim + 8 * head_lanes - 1) / (8 * head_lanes);
     const size_t row = blockIdx.x;
     float h[8], u[8], g[8];
     int turn = 0;
+    auto place_of = [&](int s) { return 8 * (s * head_lanes + l); };
+    auto left_of = [&](int head, int s) { return head < heads ? dim - place_of(s) : 0; };
+    auto read = [&](int head, int s) { inputs<T>(p, row, head * dim + place_of(s), left_of(head, s), h, u, g); };
     auto root_at = [&](int head) {
         float sum = 0.0f;
         for (int s = 0; s < steps; ++s) {
-            const int at = 8 * (s * kT + t);
-            inputs<T>(p, row, head * dim + at, dim - at, h, u, g);
+            read(head, s);
             sum += squares(u);
         }
-        sum = lanes_sum(sum, 64);
-        turn ^= 1;  // (a turn's readers are done before the one after next)
-        if ((t & 63) == 0) sums[turn][w] = sum;
-        __syncthreads();
-        return root_of(p, (sums[turn][0] + sums[turn][1]) + (sums[turn][2] + sums[turn][3]));
+        sum = lanes_sum(sum, min(head_lanes, 64));
+        if (head_lanes > 64) {
+            turn ^= 1;  // (a turn's readers are done before the one after next)
+            if ((t & 63) == 0) sums[turn][w] = sum;
+            __syncthreads();
+            sum = (sums[turn][0] + sums[turn][1]) + (sums[turn][2] + sums[turn][3]);
+        }
+        return root_of(p, sum);
     };
-    auto weights_at = [&](int head, int at) { return p.weight_heads ? head * dim + at : at; };
+    auto finish = [&](int head, int s, float root) {
+        read(head, s);
+        normed(p, root, (p.weight_heads ? head * dim : 0) + place_of(s), left_of(head, s), u, g);
+    };
     float scale = 1.0f;
     if (kFp8 && p.block == 0) {
         uint32_t top = 0;
-        for (int head = 0; head < (int)p.heads; ++head) {
+        for (int from = 0; from < heads; from += per) {
+            const int head = from + own;
             const float root = root_at(head);
             for (int s = 0; s < steps; ++s) {
-                const int at = 8 * (s * kT + t);
-                inputs<T>(p, row, head * dim + at, dim - at, h, u, g);
-                normed(p, root, weights_at(head, at), dim - at, u, g);
-                top = max(top, largest(u, dim - at));
+                finish(head, s, root);
+                top = max(top, largest(u, left_of(head, s)));
             }
         }
         top = lanes_max(top, 64);
@@ -265,25 +286,24 @@ __global__ __launch_bounds__(kT) void k_norm_long(GDNNorm p) {
         scale = scale_of(max(max(tops[0], tops[1]), max(tops[2], tops[3])));
         if (t == 0) p.scales[row] = scale;
     }
-    for (int head = 0; head < (int)p.heads; ++head) {
+    for (int from = 0; from < heads; from += per) {
+        const int head = from + own;
         const float root = root_at(head);
         for (int s = 0; s < steps; ++s) {
-            const int at = 8 * (s * kT + t), n = dim - at;
-            inputs<T>(p, row, head * dim + at, n, h, u, g);
-            normed(p, root, weights_at(head, at), n, u, g);
-            if (p.sum) store8<T>(p.sum, row * p.sum_stride + head * dim + at, n, h);
+            const int place = place_of(s), at = head * dim + place, n = left_of(head, s);
+            finish(head, s, root);
+            if (p.sum) store8<T>(p.sum, row * p.sum_stride + at, n, h);
             if constexpr (kFp8) {
                 if (p.block != 0) {
                     scale = scale_of(lanes_max(largest(u, n), (int)p.block / 8));
-                    if (n > 0 && at % (int)p.block == 0)
-                        p.scales[(row * p.heads * p.dim + (size_t)head * dim + at) / p.block] = scale;
+                    if (n > 0 && place % (int)p.block == 0) p.scales[(row * heads * dim + at) / p.block] = scale;
                 }
                 const float inv = 1.0f / scale;
 #pragma unroll
                 for (int i = 0; i < 8; ++i) u[i] *= inv;
-                store8_fp8(p.out, row * p.out_stride + head * dim + at, n, u);
+                store8_fp8(p.out, row * p.out_stride + at, n, u);
             } else {
-                store8<T>(p.out, row * p.out_stride + head * dim + at, n, u);
+                store8<T>(p.out, row * p.out_stride + at, n, u);
             }
         }
     }
@@ -291,24 +311,30 @@ __global__ __launch_bounds__(kT) void k_norm_long(GDNNorm p) {
 
 // ------------------------------------------------------------ host
 
-// A row with one scale for several heads is a unit where they take whole lanes, else
-// a head is.  Lanes of a unit, 0: k_norm_long's.
+// A row with one scale for several heads is a unit, each head in lanes of its own (all
+// of k_norm_long's above 2048 values), else a head is.  Lanes of a unit, 0: k_norm_long's.
 bool joint(const GDNNorm *a) { return a->fp8 && a->block == 0 && a->heads > 1; }
 uint64_t units_of(const GDNNorm *a) { return joint(a) ? a->rows : (uint64_t)a->rows * a->heads; }
-uint64_t length_of(const GDNNorm *a) { return joint(a) ? (uint64_t)a->heads * a->dim : a->dim; }
+int head_lanes_of(const GDNNorm *a) {
+    int n = 4;
+    while (n < 64 && 8u * n < a->dim) n *= 2;
+    return a->dim > 2048 ? kT : n;
+}
+uint64_t length_of(const GDNNorm *a) { return joint(a) ? (uint64_t)a->heads * head_lanes_of(a) * 8 : a->dim; }
 int lanes_of(const GDNNorm *a) {
-    const bool whole = !joint(a) || a->dim == 64 || a->dim == 128 || a->dim == 256 || a->dim == 512;
     const uint64_t len = length_of(a);
-    return !whole || len > 8192 ? 0 : len <= 64 ? 8 : len <= 128 ? 16 : len <= 256 ? 32 : len <= 512 ? 64 : 256;
+    if (len > 16384 || (joint(a) && a->dim > 512)) return 0;
+    return len <= 64 ? 8 : len <= 128 ? 16 : len <= 256 ? 32 : len <= 512 ? 64 : len <= 8192 ? 256 : a->fp8 ? 512 : 1024;
 }
 
 template <class T, int L, int V, bool kFp8>
 hipError_t launch_units(const GDNNorm &a, int units, int head_lanes, hipStream_t s) {
-    return launch(k_norm<T, L, V, kFp8>, dim3((unsigned)((units + kT / L - 1) / (kT / L))), dim3(kT), 0, s, a, units, head_lanes);
+    return launch(k_norm<T, L, V, kFp8>, dim3((unsigned)(L > kT ? units : (units + kT / L - 1) / (kT / L))), dim3(L > kT ? L : kT),
+                  0, s, a, units, head_lanes);
 }
 template <class T, bool kFp8>
 hipError_t launch_norm(const GDNNorm &a, hipStream_t s) {
-    const int units = (int)units_of(&a), head_lanes = joint(&a) ? (int)a.dim / 8 : 0;
+    const int units = (int)units_of(&a), head_lanes = joint(&a) ? head_lanes_of(&a) : 0;
     const uint64_t len = length_of(&a);
     switch (lanes_of(&a)) {
         case 8: return launch_units<T, 8, 1, kFp8>(a, units, head_lanes, s);
@@ -316,12 +342,17 @@ hipError_t launch_norm(const GDNNorm &a, hipStream_t s) {
         case 32: return launch_units<T, 32, 1, kFp8>(a, units, head_lanes, s);
         case 64: return launch_units<T, 64, 1, kFp8>(a, units, head_lanes, s);
         // 256 threads a row, not a wave with more vectors: 4096 x 2048 BF16 with a
-        // residual 12.6 and 15.0 us, 16384 rows 44.5 and 64, 512 equal
+        // residual 12.6 and 15.0 us, 16384 rows 44.5 and 64, 512 equal.  Above 8192 values
+        // more threads: with 256, 512, 1024 of them and in k_norm_long, 4096 x 12288 BF16
+        // with a residual take 138, 92, 80 and 99 us, into 8 bits, which holds the values
+        // across a second barrier, 135, 90, 102 and 133
         case 256:
             return len <= 2048   ? launch_units<T, 256, 1, kFp8>(a, units, head_lanes, s)
                    : len <= 4096 ? launch_units<T, 256, 2, kFp8>(a, units, head_lanes, s)
                                  : launch_units<T, 256, 4, kFp8>(a, units, head_lanes, s);
-        default: return launch(k_norm_long<T, kFp8>, dim3(a.rows), dim3(kT), 0, s, a);
+        case 512:
+        case 1024: return launch_units<T, kFp8 ? 512 : 1024, kFp8 ? 4 : 2, kFp8>(a, units, head_lanes, s);
+        default: return launch(k_norm_long<T, kFp8>, dim3(a.rows), dim3(kT), 0, s, a, joint(&a) ? head_lanes_of(&a) : kT);
     }
 }
 template <class T>

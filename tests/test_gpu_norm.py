@@ -62,7 +62,7 @@ def inputs(shape, dtype, seed=0):
     return (1.5 * normal[0]).to(dtype), (4 * normal[1]).to(dtype), (2 * normal[2]).to(dtype), w
 
 
-DIMS = [1, 2, 7, 8, 9, 63, 64, 65, 128, 200, 256, 257, 512, 513, 1000, 1024, 1500, 2048, 2049, 4096, 5000, 8192, 8193, 20000]
+DIMS = [1, 2, 7, 8, 9, 63, 64, 65, 128, 200, 256, 257, 512, 513, 1000, 1024, 1500, 2048, 2049, 4096, 5000, 8192, 8193, 12000, 16384, 16385, 20000]
 
 
 @TYPES
@@ -94,7 +94,8 @@ def test_rows_either_side_of_a_change_of_layout(rows, dim):
 
 @TYPES
 @pytest.mark.parametrize("heads,dim", [(8, 256), (3, 64), (5, 128), (2, 512), (4, 100), (16, 512), (32, 512), (7, 33), (2, 9000),
-                                       (1, 128)])
+                                       (1, 128), (3, 96), (48, 100), (40, 48), (2000, 1), (300, 33), (9, 1000), (3, 2048),
+                                       (2, 2049), (64, 200)])
 def test_heads(dtype, heads, dim):
     x, r, gate, w = inputs((6, heads, dim), dtype, heads * dim)
     for weight in (w, w[0].contiguous()):
