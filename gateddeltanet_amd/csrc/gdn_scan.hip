@@ -685,12 +685,18 @@ uint64_t groups_of(const GDNScan *a) { return (uint64_t)a->n_heads * a->head_dim
 // Tokens of a segment: as many as give eleven waves a CU, in 128s, of which eight run
 // at a time (sequences end inside them), at most 1024.  4096 tokens in one sequence, 32
 // heads of 128 x 64, segments of 192, 256, 384, 512, 1024: 52, 43, 52, 49, 80 us; 8111 in
-// 24, 8 heads of 256 x 256, of 256, 320, 384, 512, 768: 146, 143, 126, 138, 158.  Shorter
-// than the state has rows the states' traffic is more than the rows'.
+// 24, 8 heads of 256 x 256, of 256, 320, 384, 512, 768: 146, 143, 126, 138, 158; 512 in
+// one, of 128, 256: 36, 42.  64 tokens where that leaves half of the eight or so idle, for
+// the chunks that follow each other are what takes the time: 300 tokens of 8 heads of 128
+// x 128, segments of 128 and 64, BF16 22.6, 18.9, FP32 33.9, 24.3; 1000 25.2, 25.2 and
+// 36.6, 30.8; (more: the states' traffic, 4 x 500 of 256 x 128 38, 48).  Up to 256
+// tokens are not cut (one launch in place of two or three): 150 of 32 heads of 128 x 64
+// 13.3 us, 16.9 in two segments; 256, 16.4 and 17.1.
 int segment_of(const GDNScan *a) {
-    const uint64_t even = (a->n_tokens * groups_of(a) * waves_of(a) / (11 * 256) + 127) / 128 * 128;
-    const uint64_t least = a->state_dim > 128 ? a->state_dim : 128;
-    return (int)(even > 1024 ? 1024 : even < least ? least : even);
+    if (a->n_tokens <= 256) return 256;
+    const uint64_t waves = a->n_tokens * groups_of(a) * waves_of(a);  // times tokens of a segment
+    const uint64_t even = (waves / (11 * 256) + 127) / 128 * 128;
+    return waves <= 32 * 11 * 256 ? 64 : even > 1024 ? 1024 : (int)even;
 }
 size_t places(const GDNScan *a) { return a->n_tokens / (uint32_t)segment_of(a); }
 bool cut(const GDNScan *a) { return a->n_tokens > (uint32_t)segment_of(a); }

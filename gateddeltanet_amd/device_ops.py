@@ -339,7 +339,7 @@ def scan_prefill(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.Te
                       cu_seqlens)
     at = size = 0
     if workspace is None:
-        if x.shape[0] > 128:  # (fewer need none)
+        if x.shape[0] > 256:  # (fewer need none)
             size = _entry("gdn_scan_prefill_workspace")(args)
             if size:
                 workspace = x.new_empty(size, dtype=torch.uint8)

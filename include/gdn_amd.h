@@ -759,7 +759,7 @@ typedef struct {
 } GDNScan;
 /* Packed sequences in the chunk-parallel form.  `workspace`:
  * gdn_scan_prefill_workspace(args) bytes at a multiple of 16 bytes (0 for few
- * tokens, up to 128 at least), needed until the work is done. */
+ * tokens, up to 256 at least), needed until the work is done. */
 size_t gdn_scan_prefill_workspace(const GDNScan *args);
 int gdn_scan_prefill(const GDNScan *args, void *workspace, size_t workspace_bytes, void *stream);
 /* One token of every sequence (n_tokens = n_seqs, cu_seqlens not read). */

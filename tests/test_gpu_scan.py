@@ -143,6 +143,13 @@ def test_prefill_of_sequences_in_segments(dtype, N, P, lens):
     check_packed(lens, 2, 1, N, P, dtype, shuffle=True, seed=N)
 
 
+@TYPES
+@pytest.mark.parametrize("N,P,heads,n", [(64, 64, 4, 257), (128, 128, 8, 1409), (128, 128, 8, 1407), (256, 256, 3, 2600),
+                                         (64, 128, 2, 256)])
+def test_prefill_either_side_of_a_change_of_segments(dtype, N, P, heads, n):
+    check_packed([n // 2 + 11, 0, n - n // 2 - 11], heads, 1, N, P, dtype, shuffle=True, seed=n)
+
+
 @pytest.mark.parametrize("kept", ["same", "apart", "read", "written", "neither"])
 @pytest.mark.parametrize("P", [64, 256])
 def test_pools_of_sequences_in_segments(kept, P):
