@@ -19,11 +19,6 @@ using namespace packed;
 // Tokens of a chunk.
 template <class T>
 constexpr int kChunk = T::kTerms == 1 ? 64 : 32;
-// BF16 terms of the FP32 operands that only y is formed from: two leave out 2^-16 of an
-// operand at most (the first is cut, the second rounded), which a y of 8 or 11
-// significand bits does not show; the state's have three throughout.
-template <class T>
-constexpr int kOutTerms = T::kTerms == 3 ? 3 : 2;
 
 // A token's step: dt + dt_bias, softplus of it where asked for.
 template <class T>
@@ -50,7 +45,7 @@ struct Lds {
     // which keeps their rows' reads apart and halves the conflicts of B's transposed ones
     static constexpr int kRow = N / 8 + 2, kXRow = 2 * NW + 1;
     u32x4 b[NT][C][kRow], c[kY ? NT : 0][C][kRow], x[NT][C][kXRow];
-    u32x4 m[kY ? kTri : 0][kOutTerms<T>][64];
+    u32x4 m[kY ? kTri : 0][3][64];
     // of a block of NW chunks, by token: G's whole powers of two and the rest, the
     // step h, exp(G), exp(G_last - G) h; with E_j the G in front of 16-token tile j,
     // exp(G - E) of the token's own tile and exp(E_j - G) h for the tiles behind it
@@ -69,24 +64,18 @@ struct Pools {
     float *states, *starts, *decays;
 };
 
-// Four values as BF16 terms, each the bits the ones before it left, so three are
-// exact.  (An infinity or NaN has a NaN term.)
-template <int K>
-__device__ __forceinline__ void split(const f32x4 x, u32x2 (&p)[K]) {
+// Four values as three BF16 terms, each the bits the ones before it left, so they
+// are exact.  (An infinity or NaN has a NaN term.)
+__device__ __forceinline__ void split(const f32x4 x, u32x2 (&p)[3]) {
     uint32_t u[4];
     float r[4] = {x.x, x.y, x.z, x.w};
 #pragma unroll
-    for (int k = 0; k < K; ++k) {
+    for (int k = 0; k < 3; ++k) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) u[i] = f2u(r[i]);
-        if (k == K - 1 && K < 3) {  // what is left is rounded
-            p[k].x = cvt_pk(r[0], r[1]);
-            p[k].y = cvt_pk(r[2], r[3]);
-        } else {
-            p[k].x = __builtin_amdgcn_perm(u[1], u[0], 0x07060302u);
-            p[k].y = __builtin_amdgcn_perm(u[3], u[2], 0x07060302u);
-        }
-        if (k < K - 1) {
+        p[k].x = __builtin_amdgcn_perm(u[1], u[0], 0x07060302u);
+        p[k].y = __builtin_amdgcn_perm(u[3], u[2], 0x07060302u);
+        if (k < 2) {
 #pragma unroll
             for (int i = 0; i < 4; ++i) r[i] = r[i] - u2f(u[i] & 0xffff0000u);
         }
@@ -131,7 +120,7 @@ constexpr int kPerSimd = NW == 8 || sizeof(Lds<T, N, NW, kY>) <= (80 << 10) ? 2 
 template <class T, int N, int NW, bool kY>
 __global__ __launch_bounds__(64 * NW, (kPerSimd<T, N, NW, kY>)) void k_scan_segment(GDNScan p, Pools ws, int seg, int n_places, int units) {
     using L = Lds<T, N, NW, kY>;
-    constexpr int C = L::C, NT = L::NT, MT = C / 16, JT = C / 32, KS = N / 32, OT = kOutTerms<T>, kThreads = 64 * NW;
+    constexpr int C = L::C, NT = L::NT, MT = C / 16, JT = C / 32, KS = N / 32, kThreads = 64 * NW;
     constexpr int kCols = 16 * NW, kB = C * (N / 8), kX = C * (kCols / 8);  // 16-byte units (of 16-bit values) of a chunk's rows
     constexpr int kBr = (kB + kThreads - 1) / kThreads, kXr = (kX + kThreads - 1) / kThreads;
     __shared__ L lds;
@@ -295,7 +284,7 @@ __global__ __launch_bounds__(64 * NW, (kPerSimd<T, N, NW, kY>)) void k_scan_segm
 #pragma unroll
         for (int j = 0; j < MT; j += 2)
 #pragma unroll
-            for (int q = 0; q < OT; ++q)
+            for (int q = 0; q < 3; ++q)
                 reinterpret_cast<u32x2 *>(&lds.m[tri_tile(j, j / 2)][q][lane])[1] = (u32x2){0u, 0u};
     }
     float decay = 1.0f;
@@ -370,12 +359,12 @@ __global__ __launch_bounds__(64 * NW, (kPerSimd<T, N, NW, kY>)) void k_scan_segm
                         a[h][j][q] = (u32x4){lo.x, lo.y, hi.x, hi.y};
                     }
         };
-        auto terms_of = [&](int s, u32x4(&sb)[OT]) __attribute__((always_inline)) {
-            u32x2 lo[OT], hi[OT];
+        auto terms_of = [&](int s, u32x4(&sb)[3]) __attribute__((always_inline)) {
+            u32x2 lo[3], hi[3];
             split(S[s][0], lo);
             split(S[s][1], hi);
 #pragma unroll
-            for (int q = 0; q < OT; ++q) sb[q] = (u32x4){lo[q].x, lo[q].y, hi[q].x, hi[q].y};
+            for (int q = 0; q < 3; ++q) sb[q] = (u32x4){lo[q].x, lo[q].y, hi[q].x, hi[q].y};
         };
         // what stands between two of these: the loads first, then products with some
         // of the rest behind each
@@ -426,10 +415,10 @@ __global__ __launch_bounds__(64 * NW, (kPerSimd<T, N, NW, kY>)) void k_scan_segm
                 return z[0] + z[1];
             };
             auto put_tile = [&](int j, int i, const f32x4 v) __attribute__((always_inline)) {
-                u32x2 e[OT];
+                u32x2 e[3];
                 split(v, e);
 #pragma unroll
-                for (int k = 0; k < OT; ++k) reinterpret_cast<u32x2 *>(&lds.m[tri_tile(j, i / 2)][k][lane])[i & 1] = e[k];
+                for (int k = 0; k < 3; ++k) reinterpret_cast<u32x2 *>(&lds.m[tri_tile(j, i / 2)][k][lane])[i & 1] = e[k];
             };
             // M's tiles: on the diagonal a power for each value (above it one that
             // makes it zero, not a branch)
@@ -484,7 +473,7 @@ __global__ __launch_bounds__(64 * NW, (kPerSimd<T, N, NW, kY>)) void k_scan_segm
             __builtin_amdgcn_sched_barrier(0);
 
             // C S (y's lane l: token l % 16, columns 4 (l / 16) .. + 3) and x's terms
-            u32x4 ca[2][MT][NT], sb[2][OT];
+            u32x4 ca[2][MT][NT], sb[2][3];
             read_c(0, ca[0]);
             read_x();
             terms_of(0, sb[0]);
@@ -498,11 +487,11 @@ __global__ __launch_bounds__(64 * NW, (kPerSimd<T, N, NW, kY>)) void k_scan_segm
 #pragma unroll
                 for (int k = 0; k < 2 * JT; ++k)
                     if (k * KS / (2 * JT) == s) weigh(k);
-                for_terms<OT, NT>([&](int a, int b) __attribute__((always_inline)) {
+                for_terms<3, NT>([&](int a, int b) __attribute__((always_inline)) {
 #pragma unroll
                     for (int i = 0; i < MT; ++i) y[i] = mfma_bf16(sb[s & 1][a], ca[s & 1][i][b], y[i]);
                 });
-                mix(integral_constant<int, MT * (OT == 3 ? 6 : NT == 2 ? 4 : 2)>(), integral_constant<int, 5>());
+                mix(integral_constant<int, MT * (NT == 3 ? 6 : NT == 2 ? 5 : 3)>(), integral_constant<int, 5>());
             }
         } else {
             read_x();
@@ -541,7 +530,7 @@ __global__ __launch_bounds__(64 * NW, (kPerSimd<T, N, NW, kY>)) void k_scan_segm
             }
         }
         if constexpr (kY) {
-            for_terms<NT, OT>([&](int a, int b) __attribute__((always_inline)) {
+            for_terms<NT, 3>([&](int a, int b) __attribute__((always_inline)) {
 #pragma unroll
                 for (int i = 0; i < JT; ++i)
 #pragma unroll
