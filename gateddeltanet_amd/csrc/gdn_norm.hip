@@ -96,6 +96,19 @@ __device__ __forceinline__ float scale_of(uint32_t magnitude) {
     const float m = u2f(magnitude);
     return m < 0x1p-100f ? 1.0f : m / 448.0f;
 }
+// y / scale: the product with the reciprocal, corrected by what it leaves of y, so that a
+// quotient that FP32 holds, as one halfway between two E4M3 values, is exact, and others
+// are a division's but within 2^-23 of a step of halfway between two FP32 values.  (4096
+// x 8192 BF16 with a residual 42.8 us, with divisions 47.)  Of an infinite scale 0, or NaN
+// of an infinity.
+struct Quotient {
+    float inv, by;
+    __device__ __forceinline__ explicit Quotient(float scale) : inv(1.0f / scale), by(inv == 0.0f ? 0.0f : scale) {}
+    __device__ __forceinline__ float operator()(float y) const {
+        const float q = y * inv;
+        return __builtin_fmaf(__builtin_fmaf(-q, by, y), inv, q);
+    }
+};
 
 // u (and h) of eight values at `at` of row `row`; s(gate) where it comes behind.
 template <class T>
@@ -203,9 +216,10 @@ __global__ __launch_bounds__((L > kT ? L : kT)) void k_norm(GDNNorm p, int units
             if (p.block == 0) {
                 top = max(top, m);
             } else {
-                const float scale = scale_of(lanes_max(m, (int)p.block / 8)), inv = 1.0f / scale;
+                const float scale = scale_of(lanes_max(m, (int)p.block / 8));
+                const Quotient over(scale);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) u[v][i] *= inv;
+                for (int i = 0; i < 8; ++i) u[v][i] = over(u[v][i]);
                 if (own && n > 0) {
                     store8_fp8(p.out, row * p.out_stride + at, n, u[v]);
                     if (place % (int)p.block == 0) p.scales[(row * p.heads * dim + at) / p.block] = scale;
@@ -222,11 +236,12 @@ __global__ __launch_bounds__((L > kT ? L : kT)) void k_norm(GDNNorm p, int units
 #pragma unroll
                 for (int i = 0; i < W; ++i) top = max(top, tops[i]);
             }
-            const float scale = scale_of(top), inv = 1.0f / scale;
+            const float scale = scale_of(top);
+            const Quotient over(scale);
 #pragma unroll
             for (int v = 0; v < V; ++v) {
 #pragma unroll
-                for (int i = 0; i < 8; ++i) u[v][i] *= inv;
+                for (int i = 0; i < 8; ++i) u[v][i] = over(u[v][i]);
                 if (own) store8_fp8(p.out, row * p.out_stride + head_of(v) * dim + place_of(v), left_of(v), u[v]);
             }
             if (own && l == 0) p.scales[row] = scale;
@@ -298,9 +313,9 @@ __global__ __launch_bounds__(kT) void k_norm_long(GDNNorm p, int head_lanes) {
                     scale = scale_of(lanes_max(largest(u, n), (int)p.block / 8));
                     if (n > 0 && place % (int)p.block == 0) p.scales[(row * heads * dim + at) / p.block] = scale;
                 }
-                const float inv = 1.0f / scale;
+                const Quotient over(scale);
 #pragma unroll
-                for (int i = 0; i < 8; ++i) u[i] *= inv;
+                for (int i = 0; i < 8; ++i) u[i] = over(u[i]);
                 store8_fp8(p.out, row * p.out_stride + at, n, u);
             } else {
                 store8<T>(p.out, row * p.out_stride + at, n, u);
