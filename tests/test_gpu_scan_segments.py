@@ -1,0 +1,51 @@
+"""gdn_scan_prefill where it cuts sequences, against the scan token by token in 64 bits
+(gpu): many sequences.  Tolerances: test_gpu_scan's.
+"""
+import pytest
+import torch
+
+import gateddeltanet_amd as g
+from test_gpu_scan import BF16, FP32, call, check_packed, close, cumulative, inputs, reference, rows, tol
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("lens", [[1] * 600 + [700, 0, 513, 130] + [2] * 500 + [900, 257],  # more sequences than places
+                                  [0] * 1030 + [400, 1, 0, 700, 3, 300], [1, 200] * 40, [5000] + [0] * 64 + [5000]],
+                         ids=["places", "past-1024", "two-cuts", "sequences"])
+def test_long_sequences_among_more_than_64(lens):
+    """Those of several segments, by number or by place, some past the 1024th."""
+    a = inputs(sum(lens), 1, 1, 64, 64, FP32, seed=4)
+    gen = torch.Generator(device="cuda").manual_seed(5)
+    first = 0.3 * torch.randn((len(lens) + 2, 1, 64, 64), generator=gen, device="cuda")
+    where = torch.randperm(len(lens) + 2, generator=torch.Generator().manual_seed(6))[:len(lens)].tolist()
+    left_out = [i for i in range(len(lens)) if i % 97 == 3]
+    slots = [-1 if i in left_out else s for i, s in enumerate(where)]
+    pool, out = first.clone(), torch.full_like(a["x"], 5.0)
+    call(g.scan_prefill, a, cumulative(lens), state_in=pool, state_out=pool, out=out,
+         slots=torch.tensor(slots, dtype=torch.int32).cuda())
+    cu = cumulative(lens).tolist()
+    for i, n in enumerate(lens):
+        part = slice(cu[i], cu[i + 1])
+        if i in left_out:
+            assert (out[part] == 5).all() and torch.equal(pool[where[i]], first[where[i]])
+        elif n > 2 or i % 50 == 0:
+            y, S = reference(rows(a, part), first[where[i]])
+            close(out[part], y, tol(64), f"y of sequence {i}, {n} tokens")
+            close(pool[where[i]], S, tol(64), f"state of sequence {i}, {n} tokens")
+
+
+@pytest.mark.parametrize("most", [900, 1100], ids=["places", "sequences"])
+def test_more_than_1024_sequences_and_places(most):
+    """More than a join's grid has workgroups for, more or fewer sequences than places (of
+    1024 tokens)."""
+    lens = [most] * 1000 + [2100, 2049, 1] * 40
+    n = sum(lens)
+    a = inputs(n, 1, 1, 64, 64, BF16, seed=7)
+    pool = torch.zeros((len(lens), 1, 64, 64), device="cuda")
+    out = call(g.scan_prefill, a, cumulative(lens), state_out=pool)
+    cu = cumulative(lens).tolist()
+    for i in (0, 999, 1000, 1022, 1023, 1024, 1027, 1117):
+        y, S = reference(rows(a, slice(cu[i], cu[i + 1])), torch.zeros((1, 64, 64), device="cuda"))
+        close(out[cu[i]:cu[i + 1]], y, tol(64), i)
+        close(pool[i], S, tol(64), i)
