@@ -1,11 +1,14 @@
 """gdn_scan_prefill where it cuts sequences, against the scan token by token in 64 bits
-(gpu): many sequences.  Tolerances: test_gpu_scan's.
+(gpu): many sequences, and segments of every length.  Tolerances: test_gpu_scan's.
 """
+import ctypes
+
 import pytest
 import torch
 
 import gateddeltanet_amd as g
-from test_gpu_scan import BF16, FP32, call, check_packed, close, cumulative, inputs, reference, rows, tol
+from gateddeltanet_amd import _lib
+from test_gpu_scan import BF16, FP16, FP32, call, close, cumulative, inputs, reference, rows, tol
 
 pytestmark = pytest.mark.gpu
 
@@ -49,3 +52,39 @@ def test_more_than_1024_sequences_and_places(most):
         y, S = reference(rows(a, slice(cu[i], cu[i + 1])), torch.zeros((1, 64, 64), device="cuda"))
         close(out[cu[i]:cu[i + 1]], y, tol(64), i)
         close(pool[i], S, tol(64), i)
+
+
+def places(n, heads, N, P, dtype):
+    """Segments of a batch's rows that have a state in the workspace: n // their length."""
+    a = _lib.GDNScan(dtype={BF16: _lib.DTYPE_BF16, FP16: _lib.DTYPE_FP16, FP32: _lib.DTYPE_FP32}[dtype], n_tokens=n, n_seqs=1,
+                     n_heads=heads, n_groups=1, state_dim=N, head_dim=P, n_slots=1)
+    return _lib.load().gdn_scan_prefill_workspace(ctypes.byref(a)) // (heads * N * P * 4)
+
+
+SEGMENTS = [(128, 64, 32, 1900), (256, 64, 32, 3000), (384, 64, 64, 4000), (768, 64, 64, 8000), (1024, 64, 128, 8000),
+            (256, 128, 32, 2000), (384, 128, 32, 3000), (768, 128, 64, 4000), (1024, 128, 64, 6000),
+            (256, 256, 16, 2000), (384, 256, 16, 3000), (768, 256, 32, 4000), (1024, 256, 32, 6000)]
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP16, FP32], ids=["bf16", "fp16", "fp32"])
+@pytest.mark.parametrize("seg,P,heads,n", SEGMENTS)
+def test_segments_of_every_length(dtype, seg, P, heads, n):
+    """Steps, decays and operands refilled over all of a segment's chunks; a sequence of
+    three cuts and more, one that ends with a segment, short ones; three of the heads."""
+    N = 64 if seg < 1024 else 128
+    assert places(n, heads, N, P, dtype) == n // seg
+    lens = [n - 2 * seg // 3 - 70, 0, 1, 2 * seg // 3, 69]
+    assert lens[0] > 3 * seg or seg == 1024
+    lens = lens if seg < 1024 else [3 * seg + 1, 0, n - 3 * seg - 71, 1, 69]
+    a = inputs(n, heads, 1, N, P, dtype, seed=seg + P)
+    gen = torch.Generator(device="cuda").manual_seed(seg)
+    pool = 0.3 * torch.randn((len(lens), heads, N, P), generator=gen, device="cuda")
+    some = torch.tensor([0, heads // 2 + 1, heads - 1], device="cuda")
+    few = {k: v if k in "BC" else v[:, some] if k in ("x", "dt") else v[some] for k, v in a.items()}
+    first = pool[:, some]
+    out = call(g.scan_prefill, a, cumulative(lens), state_in=pool, state_out=pool)
+    cu = cumulative(lens).tolist()
+    for i, m in enumerate(lens):
+        y, S = reference(rows(few, slice(cu[i], cu[i + 1])), first[i])
+        close(out[cu[i]:cu[i + 1], some], y, tol(N), f"y of sequence {i}, {m} tokens")
+        close(pool[i, some], S, tol(N), f"state of sequence {i}, {m} tokens")
