@@ -88,3 +88,31 @@ def test_segments_of_every_length(dtype, seg, P, heads, n):
         y, S = reference(rows(few, slice(cu[i], cu[i + 1])), first[i])
         close(out[cu[i]:cu[i + 1], some], y, tol(N), f"y of sequence {i}, {m} tokens")
         close(pool[i, some], S, tol(N), f"state of sequence {i}, {m} tokens")
+
+
+@pytest.mark.parametrize("N,P,heads", [(64, 64, 2), (128, 128, 8), (64, 256, 3)])
+def test_a_workspace_of_its_size_between_guards(N, P, heads):
+    """Every state and decay lies in it, of batches whose ends lie around those of segments,
+    before and behind rows of no sequence; and what was there is not read."""
+    edge = [1, 63, 64, 65, 127, 128, 129, 255, 256, 257, 300]
+    batches = [([n], 0, 0) for n in (257, 319, 320, 321, 383, 384, 385, 512, 513, 640, 641, 1025)]
+    batches += [([n, 0, m, 1], first, 20) for n, m, first in zip(edge, edge[3:] + edge[:3], [250, 0, 63, 1, 64, 129, 0, 37, 65, 3, 128])]
+    batches += [([1000, 1, 1], 0, 0), ([1, 1000, 1], 62, 0), ([1, 1, 1000], 0, 0), ([130] * 66, 5, 3)]
+    for lens, first, behind in batches:
+        n = max(first + sum(lens) + behind, 300)
+        a = inputs(n, heads, 1, N, P, BF16, seed=n)
+        cu = cumulative(lens, first)
+        for start in (False, True):  # (slots that are read and written have their starts in it)
+            pool = [0.3 * torch.ones((len(lens), heads, N, P), device="cuda") for _ in range(2)]
+            args = _lib.GDNScan(dtype=_lib.DTYPE_BF16, n_tokens=n, n_seqs=len(lens), n_heads=heads, n_groups=1, state_dim=N,
+                                head_dim=P, n_slots=len(lens), state_in=pool[0].data_ptr() if start else None,
+                                state_out=pool[0].data_ptr())
+            need = _lib.load().gdn_scan_prefill_workspace(ctypes.byref(args))
+            out, got = [torch.zeros_like(a["x"]) for _ in pool], []
+            for p, o, fill in zip(pool, out, (0xFF, 0x3C)):  # NaN; small numbers
+                room = torch.full((need + 8192,), fill, dtype=torch.uint8, device="cuda")
+                call(g.scan_prefill, a, cu, state_in=p if start else None, state_out=p, out=o, workspace=room[4096:4096 + need])
+                assert (room[:4096] == fill).all() and (room[4096 + need:] == fill).all(), (lens, first)
+                got.append((o, p))
+            assert torch.equal(got[0][0], got[1][0]) and torch.equal(got[0][1], got[1][1]), (lens, first)
+            assert torch.isfinite(got[0][0]).all() and torch.isfinite(got[0][1]).all(), (lens, first)

@@ -152,3 +152,14 @@ def test_tensors_on_the_cpu_are_refused():
         g.scan_prefill(y, torch.zeros((4, 1)), torch.zeros(1), b, b, cu)
     with pytest.raises(g.GDNError):
         g.scan_step(y, torch.zeros((4, 1)), torch.zeros(1), b, b, torch.zeros((4, 1, 64, 64)))
+
+
+def test_a_scan_of_up_to_256_tokens_needs_no_workspace():
+    """Of every shape, as the header says."""
+    lib = _lib.load()
+    for n_heads, state_dim, head_dim, n_seqs in ((1, 64, 64, 1), (128, 128, 64, 1), (65535, 256, 256, 65535), (8, 256, 128, 256)):
+        for dtype in (_lib.DTYPE_BF16, _lib.DTYPE_FP16, _lib.DTYPE_FP32):
+            for n_tokens in (0, 1, 64, 65, 128, 255, 256):
+                a = struct(_lib.GDNScan, SCAN, dict(dtype=dtype, n_heads=n_heads, n_groups=1, state_dim=state_dim,
+                                                    head_dim=head_dim, n_seqs=n_seqs, n_tokens=n_tokens))
+                assert lib.gdn_scan_prefill_workspace(ctypes.byref(a)) == 0
