@@ -246,7 +246,7 @@ int check(const char *who, const GDNConv *a, bool packed) {
                             a->x_stride > most || a->out_stride > most))
         return refuse(who, "a row stride is smaller than the row, or above 2^40");
     const uint64_t row = (uint64_t)a->channels * size;
-    if (!(a->x == a->out && a->x_stride == a->out_stride && !packed) &&
+    if (!(a->x == a->out && (a->n_tokens == 1 || a->x_stride == a->out_stride) && !packed) &&
         rows_overlap(a->out, row, a->out_stride * size, a->x, row, a->x_stride * size, a->n_tokens))
         return refuse(who, "out overlaps x");
     if (a->state_in && a->state_out && a->state_in != a->state_out) {

@@ -342,3 +342,17 @@ def test_nothing_to_do():
     into = torch.zeros_like(pool)
     g.conv_prefill(none, w, cumulative([0, 0]), state_in=pool, state_out=into)
     assert torch.equal(into, pool)
+
+
+def test_one_row_over_its_input_whatever_its_strides():
+    """A single row's stride is not looked at, in place neither."""
+    x, w, b = inputs(1, 200, 4, BF16)
+    pool = torch.randn((1, 3, 200), device="cuda").to(BF16)
+    a, c = pool.clone(), pool.clone()
+    want = g.conv_step(x, w, a, bias=b)
+    y = x.clone()
+    g.conv_step(y.as_strided((1, 200), (999, 1)), w, c, bias=b, out=y)
+    assert torch.equal(y, want) and torch.equal(a, c)
+    y = x.clone()
+    with pytest.raises(g.GDNError):  # a row of its own, but not the same one
+        g.conv_step(y[:, 1:], w[1:].contiguous(), torch.zeros((1, 3, 199), dtype=BF16, device="cuda"), out=y[:, :199])
