@@ -337,13 +337,12 @@ def scan_prefill(x: torch.Tensor, dt: torch.Tensor, A: torch.Tensor, B: torch.Te
         out = torch.empty_like(x, memory_format=torch.contiguous_format)
     dev, args = _scan(x, dt, A, B, C, D, dt_bias, softplus, out, state_in, state_out, slots, _sequences(cu_seqlens),
                       cu_seqlens)
-    at = size = 0
+    at = 0
     if workspace is None:
-        if x.shape[0] > 256:  # (fewer need none)
-            size = _entry("gdn_scan_prefill_workspace")(args)
-            if size:
-                workspace = x.new_empty(size, dtype=torch.uint8)
-                at = workspace.data_ptr()
+        size = _entry("gdn_scan_prefill_workspace")(args)
+        if size:
+            workspace = x.new_empty(size, dtype=torch.uint8)
+            at = workspace.data_ptr()
     else:
         size = workspace.numel()
         at = _on(dev, "workspace", workspace, torch.uint8, (size,))
