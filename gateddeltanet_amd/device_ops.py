@@ -8,8 +8,8 @@ and is not waited for, and every call can be captured into a graph.  Where a
 function makes its output or workspace, it takes them from torch's allocator on
 that stream.  Errors raise ``GDNError``, before anything is enqueued.  Nothing
 here is recorded for gradients, so where torch records them a floating-point
-argument that requires one is an error; a tensor written in place counts as
-modified, as after torch's own in-place operations.
+argument that requires one is an error, and so is one with a tangent; a tensor
+written in place counts as modified, as after torch's own in-place operations.
 """
 from __future__ import annotations
 
@@ -19,6 +19,7 @@ import struct
 from typing import Optional, Tuple
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.graph import increment_version
 
 from . import _lib as L
@@ -42,6 +43,10 @@ def _apart_from_gradients(*tensors) -> None:
             if x is not None and x.requires_grad:
                 _fail("an argument requires gradients, which these operators do not form: detach it, or call under "
                       "torch.no_grad()")
+    if forward_ad._current_level >= 0:  # (a level is open, which no_grad() does not close)
+        for x in tensors:
+            if x is not None and forward_ad.unpack_dual(x).tangent is not None:
+                _fail("an argument carries a tangent, which these operators do not pass on: unpack it first")
 
 
 def _on(dev: int, name: str, x, dtype, shape) -> int:

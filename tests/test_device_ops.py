@@ -5,6 +5,7 @@ import ctypes
 
 import pytest
 import torch
+from torch.autograd import forward_ad
 
 import gateddeltanet_amd as g
 from gateddeltanet_amd import _lib
@@ -301,3 +302,37 @@ def test_arguments_that_require_gradients_are_refused():
         for off in (torch.no_grad, torch.inference_mode):
             with off(), pytest.raises(g.GDNError, match="on a GPU"):
                 call()
+
+
+def _calls(f):
+    """Every operator on tensors, f applied to one floating-point argument (on the CPU:
+    the first thing that is looked at is whether gradients are asked for)."""
+    def z(*shape):
+        return torch.zeros(shape)
+
+    cu, slots = torch.tensor([0, 4], dtype=torch.int32), torch.zeros(4, dtype=torch.int32)
+    head, state, gates = z(4, 1, 64), z(4, 1, 64, 64), z(4, 1)
+    return {
+        "conv_prefill": lambda: g.conv_prefill(z(4, 16), f(z(16, 4)), cu),
+        "conv_step": lambda: g.conv_step(z(4, 16), z(16, 4), f(z(4, 3, 16))),
+        "delta_prefill": lambda: g.delta_prefill(head, head, f(z(4, 1, 64)), gates, gates, cu),
+        "delta_step": lambda: g.delta_step(head, head, head, gates, f(gates), state, slots=slots),
+        "logits_process": lambda: g.logits_process(f(z(2, 9))),
+        "rms_norm": lambda: g.rms_norm(f(z(2, 9))),
+        "rms_norm_fp8": lambda: g.rms_norm_fp8(z(2, 9), residual=f(z(2, 9))),
+        "sample_tokens": lambda: g.sample_tokens(z(2, 9), f(z(2))),
+        "scan_prefill": lambda: g.scan_prefill(head, gates, f(z(1)), head, head, cu),
+        "scan_step": lambda: g.scan_step(head, gates, z(1), head, head, f(state)),
+    }
+
+
+@pytest.mark.parametrize("op", _calls(lambda x: x))
+def test_tangents_are_refused(op):
+    with forward_ad.dual_level():
+        call = _calls(lambda x: forward_ad.make_dual(x, torch.ones_like(x)))[op]
+        with pytest.raises(g.GDNError, match="tangent"):
+            call()
+        with torch.no_grad(), pytest.raises(g.GDNError, match="tangent"):
+            call()
+        with pytest.raises(g.GDNError, match="GPU"):  # none of them has one
+            _calls(lambda x: x)[op]()
