@@ -784,8 +784,10 @@ int gdn_scan_step(const GDNScan *args, void *stream);
  *   sum        may be x or residual of an equal stride; otherwise neither overlaps an
  *              input nor the other
  *   scales     FP32 [rows][heads * dim / block, or 1], where fp8 != 0
- * A square beyond FP32's range makes its head's y 0.  A block with a value that
- * is not finite: its scale is an infinity or NaN, its values 0 or NaN. */
+ * Squares are FP32.  One beyond its range makes its head's y 0.  With an eps below
+ * 2^-126, a head whose root mean square is below 2^-63 has fewer bits, and with an eps
+ * of 0 one whose values are all below 2^-75 has infinities and NaN.  A block with a
+ * value that is not finite: its scale is an infinity or NaN, its values 0 or NaN. */
 typedef struct {
     int32_t dtype;              /* GDN_DTYPE_* of x, residual, gate, sum and out */
     uint32_t rows, heads, dim;

@@ -296,3 +296,22 @@ def test_nothing_to_do():
     assert g.rms_norm(none).shape == (0, 64)
     q, s = g.rms_norm_fp8(none, block=32)
     assert q.shape == (0, 64) and s.shape[0] == 0
+
+
+@pytest.mark.parametrize("dtype", [BF16, FP32], ids=["bf16", "fp32"])
+@pytest.mark.parametrize("dim", [100, 2048, 20000])
+def test_tiny_heads_with_and_without_an_eps(dtype, dim):
+    """As the header says: FP32's squares hold heads of 2^-63 and more, or any with an eps
+    of 2^-126; with less, infinities and NaN."""
+    x, _, _, w = inputs((4, dim), FP32, dim)
+    x = x.sign() * x.abs().clamp(0.25, 4)
+    y = (x * 2.0**-61).to(dtype)
+    close(g.rms_norm(y, w, eps=0.0), reference(y, w, 0.0)[0], "2^-63 and more")
+    for size in (2.0**-64, 2.0**-70, 2.0**-90):
+        y = (x * size).to(dtype)
+        close(g.rms_norm(y, w, eps=2.0**-126), reference(y, w, 2.0**-126)[0], size)
+    y[:, 3] = 0
+    out = g.rms_norm(y, w, eps=0.0)
+    assert torch.isnan(out[:, 3]).all() and torch.isinf(out[:, 4:]).all()
+    q, s = g.rms_norm_fp8(y, w, eps=0.0)
+    assert not torch.isfinite(s).any()
