@@ -771,8 +771,8 @@ int gdn_scan_step(const GDNScan *args, void *stream);
  *   u = h, where gate_first != 0: h s(gate)
  *   y = u / sqrt(mean of u^2 over the head + eps) weight, where gate_first is 0: times s(gate)
  *   out = y rounded to dtype, or, where fp8 != 0, y / scale rounded to E4M3 (OCP, no
- *   infinities), scale the largest |y| of the block / 448 (1 where that is below
- *   2^-109): of `block` values along the row, or of all the row's where block = 0
+ *   infinities), scale the largest |y| of the block / 448 (1 where that |y| is below
+ *   2^-100): of `block` values along the row, or of all the row's where block = 0
  * The norm is of h as it is, not as sum holds it.
  *   rows       [rows][heads][dim]; heads * dim at most 2^20, contiguous in a row
  *   block      0, 32, 64 or 128, a divisor of dim

@@ -315,3 +315,13 @@ def test_tiny_heads_with_and_without_an_eps(dtype, dim):
     assert torch.isnan(out[:, 3]).all() and torch.isinf(out[:, 4:]).all()
     q, s = g.rms_norm_fp8(y, w, eps=0.0)
     assert not torch.isfinite(s).any()
+
+
+def test_scales_of_tiny_blocks():
+    """1 for a block whose largest value is below 2^-100, the value over 448 from there up."""
+    w = torch.ones(96, device="cuda")
+    w[:32] *= 2.0**-100
+    w[32:64] *= torch.nextafter(torch.tensor(2.0**-100), torch.tensor(0.0)).item()
+    q, s = g.rms_norm_fp8(torch.ones((1, 96), device="cuda"), w, block=32, eps=0.0)
+    assert s[0].tolist() == [torch.tensor(2.0**-100).div(torch.tensor(448.0)).item(), 1.0, torch.tensor(1.0).div(torch.tensor(448.0)).item()]
+    assert (q[0, :32].float() == 448).all() and (q[0, 32:64].float() == 0).all() and (q[0, 64:].float() == 448).all()
