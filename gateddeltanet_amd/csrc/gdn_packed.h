@@ -81,8 +81,8 @@ struct Raw8 {
 };
 
 // f(a, b) for the terms a, b of two operands, of NA and NB terms, whose
-// products count, smallest first; products below 2^-24 of the whole are left
-// out.
+// products count, smallest first.  Left out are products of 2^-24 of the whole at
+// most where both operands' terms are rounded, of 2^-23 where one's first is cut.
 template <int NA, int NB, class F>
 __device__ __forceinline__ void for_terms(F &&f) {
 #pragma unroll

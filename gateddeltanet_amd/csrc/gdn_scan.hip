@@ -64,22 +64,27 @@ struct Pools {
     float *states, *starts, *decays;
 };
 
-// Four values as three BF16 terms, each the bits the ones before it left, so they
-// are exact.  (An infinity or NaN has a NaN term.)
+// Four values as three BF16 terms, which are exact: the first cut, so that none is
+// rounded up to an infinity, the second rounded.  (An infinity or NaN has a NaN term.)
 __device__ __forceinline__ void split(const f32x4 x, u32x2 (&p)[3]) {
     uint32_t u[4];
     float r[4] = {x.x, x.y, x.z, x.w};
-#pragma unroll
-    for (int k = 0; k < 3; ++k) {
+    auto cut = [&](u32x2 &to) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < 4; ++i) u[i] = f2u(r[i]);
-        p[k].x = __builtin_amdgcn_perm(u[1], u[0], 0x07060302u);
-        p[k].y = __builtin_amdgcn_perm(u[3], u[2], 0x07060302u);
-        if (k < 2) {
+        to.x = __builtin_amdgcn_perm(u[1], u[0], 0x07060302u);
+        to.y = __builtin_amdgcn_perm(u[3], u[2], 0x07060302u);
+    };
+    cut(p[0]);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) r[i] = r[i] - u2f(u[i] & 0xffff0000u);
-        }
-    }
+    for (int i = 0; i < 4; ++i) r[i] -= u2f(u[i] & 0xffff0000u);
+    p[1].x = cvt_pk(r[0], r[1]);
+    p[1].y = cvt_pk(r[2], r[3]);
+    r[0] -= u2f(p[1].x << 16);
+    r[1] -= u2f(p[1].x & 0xffff0000u);
+    r[2] -= u2f(p[1].y << 16);
+    r[3] -= u2f(p[1].y & 0xffff0000u);
+    cut(p[2]);
 }
 
 // Waves a SIMD that the LDS leaves room for, at most two.

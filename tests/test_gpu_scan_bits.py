@@ -67,3 +67,32 @@ def test_the_tokens_in_y(dtype, N, P):
     out = g.scan_prefill(x, h, torch.zeros(heads, device="cuda"), B, B, ends.to(torch.int32).cuda(), D=D)
     want = h[first].double() - h[second].double() - D.double()
     close(out[second], want[..., None].expand(-1, -1, P), "M x")
+
+
+def test_products_of_fp32_values():
+    """B x^T and C S, each (a - 1) b from a b - b, for which six of nine products of three
+    terms are formed.  In 2^-24 of a b: left out is at most 2 (a and b of 24 bits that come
+    next to that).  A matrix instruction cuts what it adds 2^-24 below its largest operand:
+    1 in the one whose operands are b's first term, 2^-7 and less in the other five (their
+    operands are a's or b's later terms), and rounds six sums of 2^-7 and less: 3 + 11 2^-7
+    in all.  Of C S's two rows it adds one before the other: their sum in between, between
+    1 and 2, is cut and rounded once more, 2."""
+    step = 2.0**-23
+    k = torch.arange(64, device="cuda").double()
+    a = (1 + step * (0x7FBF - 0x11 * k)).float()
+    b = (1 + step * (0xFFFF - 0x105 * k)).float()
+    want = (a.double() - 1)[:, None] * b.double()
+    size = 2.0**-24 * a.double()[:, None] * b.double()
+    bound = (3 + 11 / 128) * size
+    N, P = 64, 64
+    x, B = b.expand(2, 1, P).contiguous(), torch.stack([a, -torch.ones_like(a)])[:, None]
+    cu, pool = torch.tensor([0, 2], dtype=torch.int32).cuda(), torch.zeros((1, 1, N, P), device="cuda")
+    h, A = torch.ones((2, 1), device="cuda"), torch.zeros(1, device="cuda")
+    g.scan_prefill(x, h, A, B, torch.zeros_like(B), cu, state_out=pool)
+    assert ((pool[0, 0].double() - want).abs() <= bound).all(), float(((pool[0, 0].double() - want) / bound).abs().max())
+    S, C = torch.zeros((1, 1, N, P), device="cuda"), torch.zeros((64, 1, N), device="cuda")
+    S[0, 0, 3] = S[0, 0, 9] = b
+    C[:, 0, 3], C[:, 0, 9] = a, -1
+    none = torch.zeros((64, 1, P), device="cuda")
+    y = g.scan_prefill(none, torch.zeros((64, 1), device="cuda"), A, torch.zeros_like(C), C, cu * 32, state_in=S)
+    assert ((y[:, 0].double() - want).abs() <= bound + 2 * size).all(), float(((y[:, 0].double() - want) / bound).abs().max())
