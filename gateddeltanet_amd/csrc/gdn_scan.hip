@@ -425,8 +425,8 @@ __global__ __launch_bounds__(64 * NW, (kPerSimd<T, N, NW, kY>)) void k_scan_segm
 #pragma unroll
                 for (int k = 0; k < 3; ++k) reinterpret_cast<u32x2 *>(&lds.m[tri_tile(j, i / 2)][k][lane])[i & 1] = e[k];
             };
-            // M's tiles: on the diagonal a power for each value (above it one that
-            // makes it zero, not a branch)
+            // M's tiles: on the diagonal a power for each value, above it zeros whatever the
+            // tokens hold
             auto diagonal = [&](int j, const f32x4 z) __attribute__((always_inline)) {
                 const int to = 16 * j + li, of = 16 * j + 4 * kk;
                 const int n_to = sc.whole[to];
@@ -434,12 +434,12 @@ __global__ __launch_bounds__(64 * NW, (kPerSimd<T, N, NW, kY>)) void k_scan_segm
                 f32x4 e;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
-                    const int n2 = 4 * kk + r <= li ? n_to - sc.whole[of + r] : -1000;
+                    const int n2 = n_to - sc.whole[of + r];
                     e[r] = __builtin_ldexpf(__builtin_amdgcn_exp2f(f_to - sc.rest[of + r]), n2) * sc.step[of + r];
                 }
                 f32x4 v = z * e;
 #pragma unroll
-                for (int r = 0; r < 4; ++r) v[r] += 4 * kk + r == li ? skip : 0.0f;
+                for (int r = 0; r < 4; ++r) v[r] = 4 * kk + r <= li ? v[r] + (4 * kk + r == li ? skip : 0.0f) : 0.0f;
                 put_tile(j, j, v);
             };
             // below it what falls in front of the row tile and inside it
@@ -535,6 +535,38 @@ __global__ __launch_bounds__(64 * NW, (kPerSimd<T, N, NW, kY>)) void k_scan_segm
             }
         }
         if constexpr (kY) {
+            // a value of x that is not finite, times M's zeros, would reach the tokens before it:
+            // its column's outputs from it on are made NaN instead, and it 0
+            auto word = [&](int j, int i) __attribute__((always_inline)) { return xb[j][NT == 1 ? 0 : 1][i] & 0x7fff7fffu; };
+            typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+            u16x2 top = {0, 0};
+#pragma unroll
+            for (int j = 0; j < JT; ++j)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) top = __builtin_elementwise_max(top, __builtin_bit_cast(u16x2, word(j, i)));
+            if (__ballot(top.x >= 0x7f80 || top.y >= 0x7f80) != 0) {
+                int first = C;  // (the terms behind the first show it, of values of several)
+#pragma unroll
+                for (int j = 0; j < JT; ++j)
+#pragma unroll
+                    for (int r = 7; r >= 0; --r) {
+                        const uint32_t half = r % 2 ? 0xffff0000u : 0xffffu;
+                        if ((word(j, r / 2) & half) >= (0x7f807f80u & half)) {
+                            first = min(first, 32 * j + 16 * (r / 4) + 4 * kk + r % 4);
+#pragma unroll
+                            for (int q = 0; q < NT; ++q) xb[j][q][r / 2] &= ~half;
+                        }
+                    }
+                first = min(first, __shfl_xor(first, 16));
+                first = min(first, __shfl_xor(first, 32));
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int from = __shfl(first, 4 * kk + r);
+#pragma unroll
+                    for (int j = 0; j < MT; ++j)
+                        if (16 * j + li >= from) y[j][r] = __builtin_nanf("");
+                }
+            }
             for_terms<NT, 3>([&](int a, int b) __attribute__((always_inline)) {
 #pragma unroll
                 for (int i = 0; i < JT; ++i)

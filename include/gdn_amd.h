@@ -738,8 +738,8 @@ int gdn_conv_step(const GDNConv *args, void *stream);
  * Sums are FP32.  gdn_scan_prefill forms the product of up to 1024 tokens' exp(h A)
  * by itself: with growth (h A > 0) beyond FP32's range in it, 2^127, states are infinities
  * or NaN.  A value that is not finite reaches its own sequence and head
- * (one of B or C the heads of its group) only, in gdn_scan_prefill there also the
- * tokens up to 63 before it. */
+ * (one of B or C the heads of its group) only, from its token on; the outputs that an
+ * infinite x reaches may be NaN. */
 typedef struct {
     int32_t dtype;              /* GDN_DTYPE_* of x, b, c and y */
     int32_t dt_dtype;

@@ -524,3 +524,31 @@ def test_writes_count_as_modifications():
     versions = out._version, pool._version
     call(g.scan_prefill, a, cumulative([8]), state_out=pool, out=out)
     assert out._version > versions[0] and pool._version > versions[1]
+
+
+@TYPES
+@pytest.mark.parametrize("N,P", [(64, 64), (128, 64), (256, 64), (64, 128), (256, 256)])
+def test_tokens_before_a_value_that_is_not_finite(dtype, N, P):
+    """They are as if it were not there, in its 16 tokens, chunk and segment too; its own
+    and, of the state, those behind it are not finite."""
+    heads, lens, at = 2, [150, 700], 150
+    n = sum(lens)
+    a = inputs(n, heads, 2, N, P, dtype, seed=N + P)
+    clean, S0 = torch.empty_like(a["x"]), torch.empty((2, heads, N, P), device="cuda")
+    call(g.scan_prefill, a, cumulative(lens), state_out=S0, out=clean)
+    for k, (name, value) in enumerate([(name, v) for name in ("x", "B", "C", "dt") for v in ("nan", "inf", "-inf")]):
+        if name == "dt" and value == "-inf":
+            continue  # (its softplus is 0)
+        for t in (k % 3, 15 + k % 2, 31 + k % 3, 63 + k % 2, 90 + k, 470 + 17 * k):
+            b = {**a, name: a[name].clone()}
+            b[name][(at + t, 1, 5) if name in ("x", "B", "C") else (at + t, 1)] = float(value)
+            S = torch.empty_like(S0)
+            out = call(g.scan_prefill, b, cumulative(lens), state_out=S)
+            assert torch.equal(out[:at + t], clean[:at + t]), (name, value, t)
+            assert torch.equal(out[:, 0], clean[:, 0]) and torch.equal(S[:, 0], S0[:, 0]) and torch.equal(S[0], S0[0])
+            own = out[at + t:, 1, 5] if name == "x" else out[at + t:at + t + 1, 1] if name == "C" else out[at + t:, 1]
+            assert not torch.isfinite(own[0]).any(), (name, value, t)
+            if name == "C":
+                assert torch.equal(out[at + t + 1:], clean[at + t + 1:]) and torch.equal(S, S0)
+            else:
+                assert not torch.isfinite(S[1, 1]).all(), (name, value, t)
