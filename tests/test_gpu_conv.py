@@ -356,3 +356,25 @@ def test_one_row_over_its_input_whatever_its_strides():
     y = x.clone()
     with pytest.raises(g.GDNError):  # a row of its own, but not the same one
         g.conv_step(y[:, 1:], w[1:].contiguous(), torch.zeros((1, 3, 199), dtype=BF16, device="cuda"), out=y[:, :199])
+
+
+@TYPES
+@pytest.mark.parametrize("width", [2, 3])
+@pytest.mark.parametrize("channels", [5, 136, 2051])
+def test_step_of_every_width(dtype, width, channels):
+    n, slots, where = 5, 6, [4, 0, -1, 5, 2]
+    x, w, b = inputs(n, channels, width, dtype, channels + width)
+    tails = torch.randn((slots, width - 1, channels), device="cuda").to(dtype)
+    for bias, silu, start in ((b, True, True), (None, False, True), (b, True, False)):
+        pool, out = tails.clone(), torch.full_like(x, 5.0)
+        into = pool if start else None
+        g.conv_step(x, w, into, bias=bias, silu=silu, slots=torch.tensor(where, dtype=torch.int32).cuda(), out=out)
+        for i, s in enumerate(where):
+            if s < 0 or (not start and s >= n):  # (without tails there are as many slots as sequences)
+                assert (out[i] == 5).all()
+                continue
+            y, tol, end = reference(x[i:i + 1], w, bias, tails[s] if start else torch.zeros_like(tails[s]), silu)
+            close(out[i:i + 1], y, tol, i)
+            assert torch.equal(pool[s], end if start else tails[s])
+        rest = [s for s in range(slots) if s not in where]
+        assert torch.equal(pool[rest], tails[rest])
