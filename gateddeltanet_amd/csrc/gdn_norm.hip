@@ -157,7 +157,7 @@ __device__ __forceinline__ void normed(const GDNNorm &p, float root, int w_at, i
 // vectors of eight a unit.  `head_lanes`: the lanes of each of a unit's heads (a power of
 // two; those behind its values idle), 0 where the unit is a head.  Memory-bound, each
 // value read and written once: 4096 x 2048 BF16 with a residual into 8 bits, 59 MB, in
-// 14 us (4.2 TB/s); 64 x 8 heads of 256 with a gate 3.2 us, two memory latencies and a
+// 14.3 us (4.1 TB/s); 64 x 8 heads of 256 with a gate 3.2 us, two memory latencies and a
 // reduction.
 template <class T, int L, int V, bool kFp8>
 __global__ __launch_bounds__((L > kT ? L : kT)) void k_norm(GDNNorm p, int units, int head_lanes) {
@@ -180,7 +180,7 @@ __global__ __launch_bounds__((L > kT ? L : kT)) void k_norm(GDNNorm p, int units
         inputs<T>(p, row, head_of(v) * dim + place_of(v), left_of(v), h[v], u[v], g[v]);
         sum[v] = squares(u[v]);
     }
-    // (at once: 4096 rows of 8192 BF16 values into 8 bits 41.5 us, 48 with the outputs)
+    // (at once: 4096 rows of 8192 BF16 values into 8 bits 42.4 us, with the outputs 6 more)
     if (own && p.sum) {
 #pragma unroll
         for (int v = 0; v < V; ++v)
@@ -360,7 +360,7 @@ hipError_t launch_norm(const GDNNorm &a, hipStream_t s) {
         // residual 12.6 and 15.0 us, 16384 rows 44.5 and 64, 512 equal.  Above 8192 values
         // more threads: with 256, 512, 1024 of them and in k_norm_long, 4096 x 12288 BF16
         // with a residual take 138, 92, 80 and 99 us, into 8 bits, which holds the values
-        // across a second barrier, 135, 90, 102 and 133
+        // across a second barrier, 135, 90, 102 and 133 (512 now 91, its quotients exact)
         case 256:
             return len <= 2048   ? launch_units<T, 256, 1, kFp8>(a, units, head_lanes, s)
                    : len <= 4096 ? launch_units<T, 256, 2, kFp8>(a, units, head_lanes, s)

@@ -187,7 +187,8 @@ __device__ __forceinline__ float exp2_of(double y) {
 }
 
 // x / (1 + exp(-x)), to a few 2^-24 of it (0 below -88): the exponential's whole
-// powers of two apart from the rest, which is small enough for FP32.
+// powers of two apart from the rest, which is small enough for FP32, with log2(e) in two
+// parts for it (Cody and Waite's reduction).
 __device__ __forceinline__ float silu_of(float x) {
     const float y = __builtin_amdgcn_fmed3f(-x, -200.0f, 200.0f), n = __builtin_rintf(y * 1.44269504f);
     const float f = __builtin_fmaf(y, 1.925963033e-8f, __builtin_fmaf(y, 1.44269502f, -n));  // log2(e) in two parts

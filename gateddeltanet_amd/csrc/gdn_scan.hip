@@ -111,13 +111,14 @@ constexpr int kPerSimd = NW == 8 || sizeof(Lds<T, N, NW, kY>) <= (80 << 10) ? 2 
 //             of a sequence from its start, the others from zero; their decays; and
 //             the start itself where the sequence's slot is written
 //   kY true   all segments, from the states behind the ones before them
-// Bound by the instructions that a wave can issue: two waves a SIMD (registers, LDS),
-// each with 600 vector instructions a chunk of 64 tokens, 100 products and 140 LDS
-// instructions, one in five cycles or so; 512 workgroups of four chunks, 33 us, 17.7 of
-// them launch, lookup, first loads and states, 3.85 a chunk of the two on a CU (4096
-// tokens, 32 heads of 128 x 64: kY 26.6 us, not kY 14.4, matrix unit 26 % busy, vector
-// units 40, LDS 36).  8111 tokens in 24 sequences, 8 heads of 256 x 256, 100 MB of states:
-// 94 and 28.6 us.  Measured against it at 4096 tokens: M's weights as exponentials for
+// Bound by the instructions that a wave can issue: two waves a SIMD, each with 650
+// vector instructions a chunk of 64 tokens, 126 products and 130 LDS instructions, one in
+// seven cycles or so.  512 workgroups of one to four chunks, two on a CU, from zero states
+// 12.3, 18.6, 24.5, 29.7 us: 5.8 a chunk, 6.5 for launch, lookup and first loads; with
+// states in and out 2.5 to 3 more.  4096 tokens, 32 heads of 128 x 64: kY 29.8 us, not kY
+// 14.1; matrix unit 29 % busy, vector units 45, LDS 34.  8111 tokens in 24 sequences, 8
+// heads of 256 x 256, 100 MB of states: 105 and 28.8 us.  Measured at 4096 tokens against
+// 26.6, when y's operands of a 16-bit type had two terms: M's weights as exponentials for
 // each value, loads in one piece, three barriers 28.8; two column tiles in each of four
 // waves (one wave a SIMD) 34.5; two heads a workgroup of eight waves equal; chunks of 32
 // tokens 49 against 45 in all.  Conflict-free reads of B^T (the state's rows in another
@@ -713,12 +714,15 @@ __global__ __launch_bounds__(kT) void k_scan_step(GDNScan p) {
 // ------------------------------------------------------------ host
 
 bool dim_ok(uint32_t d) { return d == 64 || d == 128 || d == 256; }
-// Waves of a workgroup, 16 columns each, and workgroups of a segment.
+// Waves of a workgroup, 16 columns each, and workgroups of a segment: the eight share
+// their rows of B and C, which four would stage twice as often (not measured).
 int waves_of(const GDNScan *a) { return a->head_dim == 64 ? 4 : 8; }
 uint64_t groups_of(const GDNScan *a) { return (uint64_t)a->n_heads * a->head_dim / (16 * waves_of(a)); }
 
 // Tokens of a segment: as many as give eleven waves a CU, in 128s, of which eight run
-// at a time (sequences end inside them), at most 1024.  4096 tokens in one sequence, 32
+// at a time (sequences end inside them; of BF16 256 x 64 only four run, which the rule
+// does not look at), at most 1024.  Measured when y's operands of a 16-bit type had two
+// terms: 4096 tokens in one sequence, 32
 // heads of 128 x 64, segments of 192, 256, 384, 512, 1024: 52, 43, 52, 49, 80 us; 8111 in
 // 24, 8 heads of 256 x 256, of 256, 320, 384, 512, 768: 146, 143, 126, 138, 158; 512 in
 // one, of 128, 256: 36, 42.  64 tokens where that leaves half of the eight or so idle, for

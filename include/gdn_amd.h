@@ -616,7 +616,7 @@ int gdn_test_prefill_gemm(int kind, const float *W, const float *X, uint32_t N, 
  * can be captured into a graph.  What the host can see is checked (-1 and one
  * line on stderr, nothing enqueued); indices that only the device sees
  * (sequence ends, slots, token ids, lengths) are held to the buffers' sizes by
- * the kernels.  Calls that may run at the same time need workspaces of their
+ * the kernels.  A call of more rows than one launch's 2^32 threads hold is refused.  Calls that may run at the same time need workspaces of their
  * own.  Clear a struct before filling it. */
 
 /* Types of the activations and logits. */
